@@ -13,10 +13,12 @@ tree so that they travel with it; nothing is installed into site-packages.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -42,6 +44,17 @@ def _stale(target: Path, sources: list[Path]) -> bool:
     return any(s.stat().st_mtime > t for s in sources)
 
 
+def _unit_sources(unit: Path) -> list[Path]:
+    """A translation unit, the csrc headers it includes (transitively) and the public header."""
+    seen, todo = set(), [unit]
+    while todo:
+        f = todo.pop()
+        if f not in seen and f.is_file():
+            seen.add(f)
+            todo += [CSRC / n for n in re.findall(r'#include "([^"/]+)"', f.read_text())]
+    return [*seen, INCLUDE / "nvfp4_decoder_attention.h"]
+
+
 def _run(cmd: list[str]) -> None:
     print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
@@ -52,11 +65,15 @@ def build_capi(force: bool = False, verbose_ptxas: bool = False) -> Path:
     if not force and not _stale(CAPI_SO, sources):
         return CAPI_SO
     LIB.mkdir(exist_ok=True)
-    cmd = [_nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
-           "-cudart", "static", "-o", str(CAPI_SO), str(CSRC / "capi.cu"), str(CSRC / "noalloc.cu")]
+    flags = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
     if verbose_ptxas:
-        cmd.insert(1, "-Xptxas=-v")
-    _run(cmd)
+        flags.append("-Xptxas=-v")
+    # One object per translation unit, compiled side by side, then one link.
+    objects = [LIB / f"{u.stem}.o" for u in sorted(CSRC.glob("*.cu"))]
+    units = [u for u, o in zip(sorted(CSRC.glob("*.cu")), objects) if force or _stale(o, _unit_sources(u))]
+    with ThreadPoolExecutor() as pool:
+        list(pool.map(lambda u: _run([_nvcc(), *flags, "-c", str(u), "-o", str(LIB / f"{u.stem}.o")]), units))
+    _run([_nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", str(CAPI_SO), *map(str, objects)])
     return CAPI_SO
 
 

@@ -1,0 +1,318 @@
+// C ABI of drafted-token verification: rotary positions of q and k, the
+// quantised KV cache and the attention of a tree of drafted tokens.
+// Declarations: include/nvfp4_decoder_attention.h.
+#include <algorithm>
+#include <cmath>
+#include <limits>
+
+#include "host_util.cuh"
+#include "kv_quant.cuh"
+#include "rope_positions.cuh"
+#include "tree_attention.cuh"
+
+namespace nvfp4da {
+namespace {
+
+constexpr int64_t kI32Max = std::numeric_limits<int32_t>::max();
+
+// a * b <= limit for nonnegative a, b without overflow.
+bool product_within(int64_t a, int64_t b, int64_t limit) { return a == 0 || b <= limit / a; }
+
+int lanes_per_row(int64_t head_dim) {
+  int lanes = 2;
+  while (lanes * 8 < head_dim) lanes *= 2;
+  return lanes;
+}
+
+// Elements per access that a strided BF16 tensor's rows allow.
+int row_vector(const void* base, const int64_t* strides) {
+  int v = 8;
+  for (int i = 0; i < 3; ++i)
+    while (v > 1 && strides[i] % v != 0) v /= 2;
+  while (v > 1 && !aligned(base, 2 * v)) v /= 2;
+  return v;
+}
+
+int check_cache(const nvfp4da_kv_cache* c) {
+  if (!c) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "cache is NULL");
+  if (c->format != NVFP4DA_KV_BF16 && c->format != NVFP4DA_KV_E4M3 && c->format != NVFP4DA_KV_NVFP4)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "unknown cache format %d", c->format);
+  if (c->batch <= 0 || c->kv_heads <= 0 || c->capacity <= 0 || c->head_dim <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "cache dimensions must all be positive");
+  if (c->head_dim % 16 != 0 || c->head_dim > 256)
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 and at most 256, got %lld",
+                static_cast<long long>(c->head_dim));
+  if (!product_within(c->batch, c->kv_heads, 65535))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "B*Hkv must be at most 65535");
+  if (!product_within(c->batch * c->kv_heads, c->capacity, kI32Max))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "the cache must have at most 2^31 - 1 rows");
+  const void* fields[6] = {c->k_codes, c->v_codes, c->k_row_scales, c->v_row_scales, c->k_block_scales,
+                           c->v_block_scales};
+  const int used = c->format == NVFP4DA_KV_BF16 ? 2 : (c->format == NVFP4DA_KV_E4M3 ? 4 : 6);
+  for (int i = 0; i < used; ++i) {
+    if (!fields[i]) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "a field of the cache is NULL");
+    if (!aligned(fields[i], 16))
+      return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "every field of the cache must be 16-byte aligned");
+  }
+  if (c->format != NVFP4DA_KV_BF16 && c->capacity % NVFP4DA_KV_CAPACITY_MULTIPLE != 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "a quantised cache's capacity must be a multiple of %d, got %lld",
+                NVFP4DA_KV_CAPACITY_MULTIPLE, static_cast<long long>(c->capacity));
+  return NVFP4DA_OK;
+}
+
+KvStore k_store(const nvfp4da_kv_cache& c) {
+  return {static_cast<uint8_t*>(c.k_codes), c.k_block_scales, c.k_row_scales};
+}
+KvStore v_store(const nvfp4da_kv_cache& c) {
+  return {static_cast<uint8_t*>(c.v_codes), c.v_block_scales, c.v_row_scales};
+}
+
+// ---------------------------------------------------------------- rotary positions
+template <int V, bool ADJACENT>
+cudaError_t launch_rope(RopeQkParams p, cudaStream_t s) {
+  const int pairs = p.rotary_dim / 2;
+  const int64_t per_token = static_cast<int64_t>(p.q_heads + p.kv_heads) * (p.head_dim / V);
+  // Tokens per block: enough items for every thread to have one, as far as the
+  // (cos, sin) table holds them.
+  int64_t tpb = std::max<int64_t>(1, kRopeThreads / per_token);
+  if (pairs > 0) tpb = std::min<int64_t>(tpb, kRopeMaxPairs / pairs);
+  p.tokens_per_block = static_cast<int>(tpb);
+  rope_qk_kernel<V, ADJACENT><<<static_cast<unsigned>(ceil_div(p.rows, tpb)), kRopeThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------- tree attention
+struct TreePlan {
+  int splits;
+  int64_t split_len;
+  size_t bytes;
+};
+
+int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_t max_past, TreePlan& pl) {
+  int r = check_cache(c);
+  if (r) return r;
+  if (tokens <= 0 || q_heads <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "token and query head counts must be positive");
+  if (q_heads % c->kv_heads != 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "number of query heads must be divisible by number of KV heads");
+  if (max_past < 0) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "past_length must be nonnegative");
+  if (tokens > c->capacity || max_past > c->capacity - tokens)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "past_length + drafted token count exceeds cache capacity (%lld + %lld > %lld)",
+                static_cast<long long>(max_past), static_cast<long long>(tokens), static_cast<long long>(c->capacity));
+  const int64_t group = q_heads / c->kv_heads;
+  if (!product_within(group, tokens, 65535) || !product_within(c->batch * q_heads, tokens, kI32Max))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "too many query rows: (Hq/Hkv)*T must be at most 65535 and B*T*Hq below 2^31");
+  const int64_t visible = max_past + tokens;
+  const int64_t base = c->batch * c->kv_heads * ceil_div(group * tokens, kTreeWarps);
+  int64_t splits = std::min(ceil_div(8LL * sm_count(), base), ceil_div(visible, 128));
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, 1024));
+  pl.split_len = ceil_div(ceil_div(visible, splits), 32) * 32;
+  pl.splits = static_cast<int>(ceil_div(visible, pl.split_len));
+  const size_t rows = static_cast<size_t>(c->batch * tokens * q_heads);
+  pl.bytes = align_up(pl.splits > 1 ? rows * pl.splits * (c->head_dim + 2) * 4 : 16, 256);
+  return NVFP4DA_OK;
+}
+
+}  // namespace
+}  // namespace nvfp4da
+
+using namespace nvfp4da;
+
+extern "C" {
+
+int nvfp4da_apply_rope_qk(const uint16_t* q, const int64_t* q_strides, uint16_t* q_out, const uint16_t* k,
+                          const int64_t* k_strides, uint16_t* k_out, int64_t batch, int64_t tokens, int64_t q_heads,
+                          int64_t kv_heads, int64_t head_dim, const int64_t* positions, int64_t position_stride,
+                          const float* inv_freq, int64_t rotary_dim, int interleaved, float attention_factor,
+                          void* stream) {
+  if (!q || !q_out || !q_strides || batch <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads < 0 || head_dim <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "apply_rope_qk: invalid arguments");
+  if (kv_heads > 0 && (!k || !k_out || !k_strides))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "apply_rope_qk: NULL k, k_out or k_strides");
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "rotary_dim must be even, at least 2 and at most head_dim, got %lld",
+                static_cast<long long>(rotary_dim));
+  if (!positions || !inv_freq) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "apply_rope_qk: NULL positions or inv_freq");
+  if (!std::isfinite(attention_factor))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "attention_factor must be finite");
+  if (rotary_dim / 2 > kRopeMaxPairs)
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "rotary_dim must be at most %d", 2 * kRopeMaxPairs);
+  if (!product_within(batch, tokens, kI32Max) || !product_within(q_heads + kv_heads, head_dim, kI32Max / kRopeThreads))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "apply_rope_qk: tensors too large for a one-dimensional grid");
+  RopeQkParams p{};
+  p.q = q;
+  p.k = k;
+  p.q_out = q_out;
+  p.k_out = k_out;
+  int v = row_vector(q, q_strides);
+  if (kv_heads > 0) v = std::min(v, row_vector(k, k_strides));
+  for (int i = 0; i < 3; ++i) {
+    p.q_stride[i] = q_strides[i];
+    p.k_stride[i] = kv_heads > 0 ? k_strides[i] : 0;
+  }
+  while (v > 1 && (!aligned(q_out, 2 * v) || (kv_heads > 0 && !aligned(k_out, 2 * v)) || head_dim % v != 0)) v /= 2;
+  const int64_t unit = interleaved ? rotary_dim : rotary_dim / 2;
+  while (v > 1 && unit % v != 0) v /= 2;
+  p.positions = positions;
+  p.pos_stride = position_stride;
+  p.inv_freq = inv_freq;
+  p.factor = attention_factor;
+  p.rows = batch * tokens;
+  p.tokens = static_cast<int>(tokens);
+  p.q_heads = static_cast<int>(q_heads);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.head_dim = static_cast<int>(head_dim);
+  p.rotary_dim = static_cast<int>(rotary_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (interleaved)
+    e = v == 8 ? launch_rope<8, true>(p, s) : v == 4 ? launch_rope<4, true>(p, s) : v == 2 ? launch_rope<2, true>(p, s) : launch_rope<1, true>(p, s);
+  else
+    e = v == 8 ? launch_rope<8, false>(p, s) : v == 4 ? launch_rope<4, false>(p, s) : v == 2 ? launch_rope<2, false>(p, s) : launch_rope<1, false>(p, s);
+  if (e != cudaSuccess) return cuda_fail(e, "apply_rope_qk launch");
+  return NVFP4DA_OK;
+}
+
+int nvfp4da_kv_quant_append(const nvfp4da_kv_cache* c, const uint16_t* new_k, const int64_t* k_strides,
+                            const uint16_t* new_v, const int64_t* v_strides, int64_t tokens, int64_t past_length,
+                            const int64_t* past_lengths, const int64_t* counts, void* stream) {
+  int r = check_cache(c);
+  if (r) return r;
+  if (c->format == NVFP4DA_KV_BF16)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "kv_quant_append needs a quantised cache (nvfp4da_kv_cache_append takes BF16)");
+  if (!new_k || !new_v || !k_strides || !v_strides || tokens <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "kv_quant_append: invalid arguments");
+  if (!past_lengths) {
+    if (past_length < 0) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "past_length must be nonnegative");
+    if (tokens > c->capacity || past_length > c->capacity - tokens)
+      return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "past_length + current token count exceeds cache capacity");
+  }
+  KvAppendParams p{};
+  p.lanes = lanes_per_row(c->head_dim);
+  if (!product_within(c->batch * c->kv_heads, tokens, kI32Max / p.lanes))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "kv_quant_append: too many rows for a one-dimensional grid");
+  p.k = k_store(*c);
+  p.v = v_store(*c);
+  p.new_k = new_k;
+  p.new_v = new_v;
+  for (int i = 0; i < 3; ++i) {
+    p.k_stride[i] = k_strides[i];
+    p.v_stride[i] = v_strides[i];
+  }
+  p.vec_k = row_vector(new_k, k_strides) == 8;
+  p.vec_v = row_vector(new_v, v_strides) == 8;
+  p.batch = static_cast<int>(c->batch);
+  p.tokens = static_cast<int>(tokens);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.head_dim = static_cast<int>(c->head_dim);
+  p.capacity = c->capacity;
+  p.past_length = past_length;
+  p.past_lengths = past_lengths;
+  p.counts = counts;
+  const int64_t threads = c->batch * c->kv_heads * tokens * p.lanes;
+  const unsigned grid = static_cast<unsigned>(ceil_div(threads, kKvThreads));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c->format == NVFP4DA_KV_E4M3) kv_quant_append_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p);
+  else kv_quant_append_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p);
+  NVFP4DA_CHECK_LAUNCH("kv_quant_append launch");
+  return NVFP4DA_OK;
+}
+
+int nvfp4da_kv_quant_read(const nvfp4da_kv_cache* c, int64_t start, const int64_t* starts, int64_t length,
+                          uint16_t* k_out, uint16_t* v_out, void* stream) {
+  int r = check_cache(c);
+  if (r) return r;
+  if (c->format == NVFP4DA_KV_BF16)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "kv_quant_read needs a quantised cache");
+  if (!k_out || !v_out || length <= 0) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "kv_quant_read: invalid arguments");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "kv_quant_read outputs must be 16-byte aligned");
+  if (!starts && (start < 0 || length > c->capacity || start > c->capacity - length))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "rows [%lld, %lld + %lld) are not inside the cache capacity %lld",
+                static_cast<long long>(start), static_cast<long long>(start), static_cast<long long>(length),
+                static_cast<long long>(c->capacity));
+  KvReadParams p{};
+  p.lanes = lanes_per_row(c->head_dim);
+  if (!product_within(c->batch * c->kv_heads, length, (int64_t(1) << 32) / p.lanes - kKvThreads))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "kv_quant_read: too many rows for a one-dimensional grid");
+  p.k = k_store(*c);
+  p.v = v_store(*c);
+  p.out_k = k_out;
+  p.out_v = v_out;
+  p.batch = static_cast<int>(c->batch);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.head_dim = static_cast<int>(c->head_dim);
+  p.capacity = c->capacity;
+  p.length = length;
+  p.start = start;
+  p.starts = starts;
+  const int64_t threads = c->batch * c->kv_heads * length * p.lanes;
+  const unsigned grid = static_cast<unsigned>(ceil_div(threads, kKvThreads));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c->format == NVFP4DA_KV_E4M3) kv_quant_read_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p);
+  else kv_quant_read_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p);
+  NVFP4DA_CHECK_LAUNCH("kv_quant_read launch");
+  return NVFP4DA_OK;
+}
+
+size_t nvfp4da_tree_attention_workspace_size(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads,
+                                             int64_t max_past_length) {
+  TreePlan pl;
+  return plan_tree(c, tokens, q_heads, max_past_length, pl) ? 0 : pl.bytes;
+}
+
+int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const uint8_t* tree_mask,
+                           int64_t mask_batch_stride, uint16_t* context, int64_t tokens, int64_t q_heads,
+                           int64_t past_length, const int64_t* past_lengths, int64_t max_past_length, void* ws,
+                           size_t ws_bytes, void* stream) {
+  if (!past_lengths) max_past_length = past_length;
+  TreePlan pl;
+  int r = plan_tree(c, tokens, q_heads, max_past_length, pl);
+  if (r) return r;
+  if (!q || !context) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "tree attention: NULL pointer");
+  if (!aligned(q, 16) || !aligned(context, 16))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
+  if (pl.splits > 1 && (!ws || ws_bytes < pl.bytes))
+    return fail(NVFP4DA_ERR_WORKSPACE, "tree attention workspace too small (%zu < %zu bytes)", ws ? ws_bytes : size_t(0),
+                pl.bytes);
+  if (pl.splits > 1 && !aligned(ws, 16))
+    return fail(NVFP4DA_ERR_WORKSPACE, "the tree attention workspace must be 16-byte aligned");
+  TreeAttnParams p{};
+  p.q = q;
+  p.k = k_store(*c);
+  p.v = v_store(*c);
+  p.mask = tree_mask;
+  p.mask_stride = mask_batch_stride;
+  p.ctx = context;
+  p.partials = static_cast<float*>(ws);
+  p.batch = static_cast<int>(c->batch);
+  p.tokens = static_cast<int>(tokens);
+  p.q_heads = static_cast<int>(q_heads);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.head_dim = static_cast<int>(c->head_dim);
+  p.capacity = c->capacity;
+  p.past_length = past_length;
+  p.past_lengths = past_lengths;
+  p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c->head_dim)));
+  p.splits = pl.splits;
+  p.split_len = pl.split_len;
+  p.lanes = lanes_per_row(c->head_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t group = q_heads / c->kv_heads;
+  const dim3 grid(static_cast<unsigned>(pl.splits), static_cast<unsigned>(ceil_div(group * tokens, kTreeWarps)),
+                  static_cast<unsigned>(c->batch * c->kv_heads));
+  switch (c->format) {
+    case NVFP4DA_KV_BF16: tree_attn_general_kernel<kKvFmtBf16><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
+    case NVFP4DA_KV_E4M3: tree_attn_general_kernel<kKvFmtE4m3><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
+    default: tree_attn_general_kernel<kKvFmtNvfp4><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
+  }
+  NVFP4DA_CHECK_LAUNCH("tree attention launch");
+  if (pl.splits > 1) {
+    const int64_t rows = c->batch * tokens * q_heads;
+    tree_combine_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, s>>>(p);
+    NVFP4DA_CHECK_LAUNCH("tree attention combine launch");
+  }
+  return NVFP4DA_OK;
+}
+
+}  // extern "C"

@@ -2,7 +2,8 @@
 //
 // Registers the reference's nine schemas in its namespace
 // (src/bindings.cpp:888-916) so that its Python loader, wrappers and tests bind
-// to this library unchanged, plus the fused forward and the device quantizer.
+// to this library unchanged, plus the fused forward, the device quantizer and
+// the operators that verify drafted tokens over a quantised KV cache.
 // Structural checks raise RuntimeError with the reference's messages (its tests
 // match on them); outputs are fresh contiguous tensors on the input's device;
 // everything runs on the current CUDA stream with no host synchronisation.
@@ -15,6 +16,7 @@
 #include <cmath>
 #include <cstdint>
 #include <limits>
+#include <optional>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -381,6 +383,195 @@ std::tuple<Tensor, Tensor, Tensor> quantize_nvfp4(const Tensor& source) {
   return {packed, scales, gamma};
 }
 
+// ---------------------------------------------------------------- drafted-token verification
+using OptTensor = std::optional<Tensor>;
+
+// [B, T, H, D] BF16 rows by strides: only the last dimension has to be contiguous.
+void expect_rows(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must have dtype torch.bfloat16");
+  TORCH_CHECK(t.dim() == 4, name, " must have rank 4, got rank ", t.dim());
+  TORCH_CHECK(t.size(0) > 0 && t.size(1) > 0 && t.size(2) > 0 && t.size(3) > 0, name,
+              " dimensions must all be positive");
+  TORCH_CHECK(t.stride(3) == 1 || t.size(3) == 1, name, " must be contiguous in its last dimension");
+}
+
+struct RowStrides {
+  int64_t v[3];
+};
+RowStrides row_strides(const Tensor& t) {
+  RowStrides s;
+  for (int i = 0; i < 3; ++i) s.v[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  return s;
+}
+
+const int64_t* lengths(const OptTensor& t, const char* name, int64_t batch, const Tensor& ref, const char* ref_name) {
+  if (!t.has_value()) return nullptr;
+  expect(*t, name, at::kLong);
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == batch, name, " must have shape [B]");
+  expect_same_device(*t, name, ref, ref_name);
+  return t->data_ptr<int64_t>();
+}
+
+// The C view of a cache: BF16 codes without scales, or E4M3 / NVFP4 codes with theirs.
+nvfp4da_kv_cache kv_cache(const Tensor& kc, const Tensor& vc, const OptTensor& kr, const OptTensor& vr,
+                          const OptTensor& kb, const OptTensor& vb) {
+  TORCH_CHECK(kr.has_value() == vr.has_value() && kb.has_value() == vb.has_value() && (kr.has_value() || !kb.has_value()),
+              "a cache has row scales (and, NVFP4, block scales) for both K and V");
+  nvfp4da_kv_cache c{};
+  c.format = !kr.has_value() ? NVFP4DA_KV_BF16 : (kb.has_value() ? NVFP4DA_KV_NVFP4 : NVFP4DA_KV_E4M3);
+  const at::ScalarType type = c.format == NVFP4DA_KV_BF16 ? at::kBFloat16 : at::kByte;
+  const char* kn = c.format == NVFP4DA_KV_BF16 ? "k_cache" : "k_codes";
+  const char* vn = c.format == NVFP4DA_KV_BF16 ? "v_cache" : "v_codes";
+  expect(kc, kn, type);
+  expect(vc, vn, type);
+  TORCH_CHECK(kc.dim() == 4, kn, " must have rank 4, got rank ", kc.dim());
+  TORCH_CHECK(vc.sizes() == kc.sizes(), vn, " must have the same shape as ", kn, "; got ", vc.sizes(), " and ",
+              kc.sizes());
+  expect_same_device(vc, vn, kc, kn);
+  c.k_codes = kc.data_ptr();
+  c.v_codes = vc.data_ptr();
+  c.batch = kc.size(0);
+  c.kv_heads = kc.size(1);
+  c.capacity = kc.size(2);
+  c.head_dim = c.format == NVFP4DA_KV_NVFP4 ? 2 * kc.size(3) : kc.size(3);
+  if (c.format == NVFP4DA_KV_BF16) return c;
+  const Tensor* rows[2] = {&*kr, &*vr};
+  const char* row_names[2] = {"k_row_scales", "v_row_scales"};
+  for (int i = 0; i < 2; ++i) {
+    expect(*rows[i], row_names[i], at::kFloat);
+    TORCH_CHECK(rows[i]->dim() == 3 && rows[i]->sizes() == kc.sizes().slice(0, 3), row_names[i],
+                " must have shape [B, Hkv, C]");
+    expect_same_device(*rows[i], row_names[i], kc, kn);
+  }
+  c.k_row_scales = kr->data_ptr<float>();
+  c.v_row_scales = vr->data_ptr<float>();
+  if (c.format == NVFP4DA_KV_E4M3) return c;
+  const Tensor* blocks[2] = {&*kb, &*vb};
+  const char* block_names[2] = {"k_block_scales", "v_block_scales"};
+  for (int i = 0; i < 2; ++i) {
+    expect(*blocks[i], block_names[i], at::kByte);
+    TORCH_CHECK(blocks[i]->dim() == 4 && blocks[i]->sizes().slice(0, 3) == kc.sizes().slice(0, 3) &&
+                    blocks[i]->size(3) * 16 == c.head_dim,
+                block_names[i], " must have shape [B, Hkv, C, D/16]");
+    expect_same_device(*blocks[i], block_names[i], kc, kn);
+  }
+  c.k_block_scales = kb->data_ptr<uint8_t>();
+  c.v_block_scales = vb->data_ptr<uint8_t>();
+  return c;
+}
+
+std::tuple<Tensor, Tensor> apply_rope_qk(const Tensor& q, const Tensor& k, const Tensor& positions,
+                                         const Tensor& inv_freq, bool interleaved, double factor) {
+  expect_rows(q, "q");
+  expect_rows(k, "k");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3),
+              "q and k must agree in batch, tokens and head dimension; got ", q.sizes(), " and ", k.sizes());
+  const int64_t b = q.size(0), t = q.size(1), d = q.size(3);
+  expect(positions, "positions", at::kLong);
+  const bool shared = positions.dim() == 1;
+  TORCH_CHECK(shared ? positions.size(0) == t : (positions.dim() == 2 && positions.size(0) == b && positions.size(1) == t),
+              "positions must have shape [T] or [B, T]; got ", positions.sizes());
+  expect(inv_freq, "inv_freq", at::kFloat);
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.size(0) >= 1, "inv_freq must have shape [rotary_dim / 2]");
+  TORCH_CHECK(2 * inv_freq.size(0) <= d, "rotary_dim (twice the length of inv_freq) must be at most the head dimension (",
+              2 * inv_freq.size(0), " > ", d, ")");
+  expect_same_device(k, "k", q, "q");
+  expect_same_device(positions, "positions", q, "q");
+  expect_same_device(inv_freq, "inv_freq", q, "q");
+  const float factor32 = static_cast<float>(factor);
+  TORCH_CHECK(std::isfinite(factor32), "attention_factor must be finite");
+  const c10::cuda::CUDAGuard g(q.device());
+  Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  const RowStrides qs = row_strides(q), ks = row_strides(k);
+  check_status(nvfp4da_apply_rope_qk(bits(q), qs.v, mbits(qo), bits(k), ks.v, mbits(ko), b, t, q.size(2), k.size(2), d,
+                                     positions.data_ptr<int64_t>(), shared ? 0 : t, inv_freq.data_ptr<float>(),
+                                     2 * inv_freq.size(0), interleaved ? 1 : 0, factor32, cur_stream(q)),
+               "cuda_apply_rope_qk");
+  return {qo, ko};
+}
+
+void quantized_kv_append_(Tensor& kc, Tensor& vc, Tensor& kr, Tensor& vr, const OptTensor& kb, const OptTensor& vb,
+                          const Tensor& nk, const Tensor& nv, int64_t past_length, const OptTensor& past_lengths,
+                          const OptTensor& counts) {
+  const nvfp4da_kv_cache c = kv_cache(kc, vc, kr, vr, kb, vb);
+  expect_rows(nk, "new_k");
+  expect_rows(nv, "new_v");
+  TORCH_CHECK(nv.sizes() == nk.sizes(), "new_v must have the same shape as new_k; got ", nv.sizes(), " and ",
+              nk.sizes());
+  expect_same_device(nk, "new_k", kc, "the cache");
+  expect_same_device(nv, "new_v", kc, "the cache");
+  TORCH_CHECK(nk.size(0) == c.batch && nk.size(2) == c.kv_heads && nk.size(3) == c.head_dim,
+              "new K/V must have shape [B, T, Hkv, D] matching the cache; got ", nk.sizes());
+  const int64_t* pl = lengths(past_lengths, "past_lengths", c.batch, kc, "the cache");
+  const int64_t* n = lengths(counts, "counts", c.batch, kc, "the cache");
+  TORCH_CHECK(pl || past_length >= 0, "past_length must be nonnegative");
+  TORCH_CHECK(pl || past_length <= c.capacity - nk.size(1),
+              "past_length + current token count exceeds cache capacity (", past_length, " + ", nk.size(1), " > ",
+              c.capacity, ")");
+  const c10::cuda::CUDAGuard g(kc.device());
+  const RowStrides ks = row_strides(nk), vs = row_strides(nv);
+  check_status(nvfp4da_kv_quant_append(&c, bits(nk), ks.v, bits(nv), vs.v, nk.size(1), past_length, pl, n,
+                                       cur_stream(kc)),
+               "cuda_quantized_kv_append_");
+}
+
+std::tuple<Tensor, Tensor> quantized_kv_read(const Tensor& kc, const Tensor& vc, const Tensor& kr, const Tensor& vr,
+                                             const OptTensor& kb, const OptTensor& vb, int64_t start, int64_t length,
+                                             const OptTensor& starts) {
+  const nvfp4da_kv_cache c = kv_cache(kc, vc, kr, vr, kb, vb);
+  const int64_t* st = lengths(starts, "starts", c.batch, kc, "the cache");
+  TORCH_CHECK(length > 0 && length <= c.capacity, "length must be in [1, ", c.capacity, "], got ", length);
+  TORCH_CHECK(st || (start >= 0 && start <= c.capacity - length), "rows [", start, ", ", start, " + ", length,
+              ") are not inside the cache capacity ", c.capacity);
+  const c10::cuda::CUDAGuard g(kc.device());
+  const auto options = kc.options().dtype(at::kBFloat16);
+  Tensor k = at::empty({c.batch, c.kv_heads, length, c.head_dim}, options), v = at::empty(k.sizes(), options);
+  check_status(nvfp4da_kv_quant_read(&c, start, st, length, mbits(k), mbits(v), cur_stream(kc)),
+               "cuda_quantized_kv_read");
+  return {k, v};
+}
+
+Tensor tree_attention_cached(const Tensor& q, const Tensor& kc, const Tensor& vc, const OptTensor& kr,
+                             const OptTensor& vr, const OptTensor& kb, const OptTensor& vb, const OptTensor& tree_mask,
+                             int64_t past_length, const OptTensor& past_lengths, int64_t max_past_length) {
+  expect_rank4(q, "q");
+  const nvfp4da_kv_cache c = kv_cache(kc, vc, kr, vr, kb, vb);
+  expect_same_device(kc, "the cache", q, "q");
+  const int64_t b = q.size(0), t = q.size(1), hq = q.size(2);
+  TORCH_CHECK(b == c.batch, "q and cache batch sizes must match (", b, " != ", c.batch, ")");
+  TORCH_CHECK(q.size(3) == c.head_dim, "q and cache head dimensions must match (", q.size(3), " != ", c.head_dim, ")");
+  TORCH_CHECK(c.kv_heads > 0 && hq % c.kv_heads == 0, "number of query heads must be divisible by number of KV heads (",
+              hq, " % ", c.kv_heads, " != 0)");
+  const int64_t* pl = lengths(past_lengths, "past_lengths", b, q, "q");
+  const int64_t max_past = pl ? max_past_length : past_length;
+  TORCH_CHECK(max_past >= 0, pl ? "max_past_length" : "past_length", " must be nonnegative");
+  TORCH_CHECK(max_past <= c.capacity - t, pl ? "max_past_length" : "past_length",
+              " + drafted token count exceeds cache capacity (", max_past, " + ", t, " > ", c.capacity, ")");
+  const uint8_t* mask = nullptr;
+  int64_t mask_stride = 0;
+  if (tree_mask.has_value()) {
+    expect(*tree_mask, "tree_mask", at::kBool);
+    const bool shared = tree_mask->dim() == 2;
+    const int64_t o = shared ? 0 : 1;
+    TORCH_CHECK((shared || (tree_mask->dim() == 3 && tree_mask->size(0) == b)) && tree_mask->size(o) == t &&
+                    tree_mask->size(o + 1) == t,
+                "tree_mask must have shape [T, T] or [B, T, T]; got ", tree_mask->sizes());
+    expect_same_device(*tree_mask, "tree_mask", q, "q");
+    mask = static_cast<const uint8_t*>(tree_mask->data_ptr());
+    mask_stride = shared ? 0 : t * t;
+  }
+  const c10::cuda::CUDAGuard g(q.device());
+  Tensor ctx = at::empty(q.sizes(), q.options());
+  const size_t wsb = nvfp4da_tree_attention_workspace_size(&c, t, hq, max_past);
+  TORCH_CHECK(wsb > 0, "cuda_tree_attention_cached rejected its arguments: ", nvfp4da_last_error());
+  Tensor ws = workspace(q, wsb);
+  check_status(nvfp4da_tree_attention(bits(q), &c, mask, mask_stride, mbits(ctx), t, hq, past_length, pl, max_past,
+                                      ws.data_ptr(), wsb, cur_stream(q)),
+               "cuda_tree_attention_cached");
+  return ctx;
+}
+
 }  // namespace
 }  // namespace nvfp4da_ops
 
@@ -422,4 +613,25 @@ TORCH_LIBRARY(cuda_nvfp4_decoder_attention, m) {
       "rope_theta=10000.0) -> Tensor",
       TORCH_FN(forward_varlen_));
   m.def("cuda_quantize_nvfp4(Tensor source) -> (Tensor, Tensor, Tensor)", TORCH_FN(quantize_nvfp4));
+  // Drafted-token verification: rotary positions, the quantised KV cache, tree
+  // attention.  A cache without scales is BF16, with row scales E4M3, with block
+  // scales too NVFP4.
+  m.def(
+      "cuda_apply_rope_qk(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, bool interleaved=True, float "
+      "attention_factor=1.0) -> (Tensor, Tensor)",
+      TORCH_FN(apply_rope_qk));
+  m.def(
+      "cuda_quantized_kv_append_(Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_row_scales, Tensor(d!) "
+      "v_row_scales, Tensor(e!)? k_block_scales, Tensor(f!)? v_block_scales, Tensor new_k, Tensor new_v, int "
+      "past_length=0, Tensor? past_lengths=None, Tensor? counts=None) -> ()",
+      TORCH_FN(quantized_kv_append_));
+  m.def(
+      "cuda_quantized_kv_read(Tensor k_codes, Tensor v_codes, Tensor k_row_scales, Tensor v_row_scales, Tensor? "
+      "k_block_scales, Tensor? v_block_scales, int start, int length, Tensor? starts=None) -> (Tensor, Tensor)",
+      TORCH_FN(quantized_kv_read));
+  m.def(
+      "cuda_tree_attention_cached(Tensor q, Tensor k, Tensor v, Tensor? k_row_scales, Tensor? v_row_scales, Tensor? "
+      "k_block_scales, Tensor? v_block_scales, Tensor? tree_mask=None, int past_length=0, Tensor? past_lengths=None, "
+      "int max_past_length=0) -> Tensor",
+      TORCH_FN(tree_attention_cached));
 }

@@ -29,9 +29,12 @@ EXPORTED = (
     "nvfp4da_debug_wait_timeout", "nvfp4da_qkv_rope_append_shard", "nvfp4da_qkv_rope_append_shard_workspace_size",
     "nvfp4da_gqa_attention_partials_workspace_size", "nvfp4da_gqa_attention_partials",
     "nvfp4da_attention_combine", "nvfp4da_w4a16_gemm", "nvfp4da_decoder_attention_forward_hostio",
+    "nvfp4da_apply_rope_qk", "nvfp4da_kv_quant_append", "nvfp4da_kv_quant_read",
+    "nvfp4da_tree_attention_workspace_size", "nvfp4da_tree_attention",
 )
 
 PATH_AUTO, PATH_CHAIN, PATH_STEP = 0, 1, 2
+KV_BF16, KV_E4M3, KV_NVFP4 = 0, 1, 2
 
 
 class CapiError(RuntimeError):
@@ -59,6 +62,13 @@ class ForwardArgs(C.Structure):
                 ("capacity", C.c_int64), ("past_length", C.c_int64), ("past_lengths", C.c_void_p),
                 ("max_past_length", C.c_int64), ("rms_eps", C.c_float), ("rope_theta", C.c_float),
                 ("stages", C.POINTER(Stages))]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("format", C.c_int), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p),
+                ("k_block_scales", C.c_void_p), ("v_block_scales", C.c_void_p), ("k_row_scales", C.c_void_p),
+                ("v_row_scales", C.c_void_p), ("batch", C.c_int64), ("kv_heads", C.c_int64),
+                ("capacity", C.c_int64), ("head_dim", C.c_int64)]
 
 
 _lib: C.CDLL | None = None
@@ -102,6 +112,14 @@ def load() -> C.CDLL:
                                                      i64, vp, sz, vp]),
         "nvfp4da_attention_combine": (C.c_int, [vp, C.c_int, i64, i64, vp, vp]),
         "nvfp4da_w4a16_gemm": (C.c_int, [vp, i64, C.POINTER(Weight), vp, vp]),
+        "nvfp4da_apply_rope_qk": (C.c_int, [vp, C.POINTER(i64), vp, vp, C.POINTER(i64), vp, i64, i64, i64, i64, i64,
+                                            vp, i64, vp, i64, C.c_int, C.c_float, vp]),
+        "nvfp4da_kv_quant_append": (C.c_int, [C.POINTER(KvCache), vp, C.POINTER(i64), vp, C.POINTER(i64), i64, i64,
+                                              vp, vp, vp]),
+        "nvfp4da_kv_quant_read": (C.c_int, [C.POINTER(KvCache), i64, vp, i64, vp, vp, vp]),
+        "nvfp4da_tree_attention_workspace_size": (sz, [C.POINTER(KvCache), i64, i64, i64]),
+        "nvfp4da_tree_attention": (C.c_int, [vp, C.POINTER(KvCache), vp, i64, vp, i64, i64, i64, vp, i64, vp, sz,
+                                             vp]),
         "nvfp4da_decoder_attention_forward_hostio": (C.c_int, [C.POINTER(ForwardArgs), vp, vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
@@ -216,6 +234,33 @@ def quantize(source: torch.Tensor, stream=None):
     _check(lib.nvfp4da_quantize_nvfp4(_p(source), 1 if source.dtype == torch.bfloat16 else 0, n, k, _p(packed),
                                       _p(scales), _p(gamma), _p(ws), wsb, _stream(stream)))
     return packed, scales, gamma
+
+
+def kv_cache(cache) -> KvCache:
+    """C view of a QuantizedKVCache-like object, or of a pair of BF16 caches (device tensors)."""
+    if isinstance(cache, (tuple, list)):
+        k, v = cache
+        return KvCache(KV_BF16, k.data_ptr(), v.data_ptr(), None, None, None, None, *k.shape)
+    blocks = [None if t is None else t.data_ptr() for t in (cache.k_block_scales, cache.v_block_scales)]
+    b, hkv, c = cache.k_row_scales.shape
+    return KvCache(KV_E4M3 if blocks[0] is None else KV_NVFP4, cache.k_codes.data_ptr(), cache.v_codes.data_ptr(),
+                   *blocks, cache.k_row_scales.data_ptr(), cache.v_row_scales.data_ptr(), b, hkv, c, cache.head_dim)
+
+
+def tree_attention(q, cache, past_length: int = 0, tree_mask=None, past_lengths=None, max_past_length=None,
+                   stream=None) -> torch.Tensor:
+    b, t, hq, _ = q.shape
+    maxp = past_length if past_lengths is None else max_past_length
+    kv, lib = kv_cache(cache), load()
+    wsb = lib.nvfp4da_tree_attention_workspace_size(C.byref(kv), t, hq, maxp)
+    if wsb == 0:
+        raise CapiError(ERR_INVALID_ARGUMENT, lib.nvfp4da_last_error().decode())
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
+    ctx = torch.empty_like(q)
+    stride = 0 if tree_mask is None or tree_mask.ndim == 2 else t * t
+    _check(lib.nvfp4da_tree_attention(_p(q), C.byref(kv), _p(tree_mask), stride, _p(ctx), t, hq, past_length,
+                                      _p(past_lengths), maxp, _p(ws), wsb, _stream(stream)))
+    return ctx
 
 
 def sync_status(stream=None, clear: bool = True) -> int:

@@ -272,6 +272,77 @@ int nvfp4da_attention_combine(const float* partials, int shards, int64_t rows, i
 #define NVFP4DA_NOALLOC_SCRATCH_BYTES (8u * 1024u * 1024u)
 int nvfp4da_decoder_attention_forward_noalloc(const nvfp4da_forward_args* args, void* stream);
 
+/* ---- Verifying drafted tokens over a quantised KV cache (no counterpart in
+ * the reference, which decodes causally over a BF16 cache).  One step:
+ * projections, nvfp4da_apply_rope_qk at the drafted tokens' positions
+ * (P_b + depth in the tree), nvfp4da_kv_quant_append into slots P_b ..,
+ * nvfp4da_tree_attention, the O projection; accepted tokens' K/V rows are
+ * appended again in order, at P_b, with their per-sequence counts. */
+#define NVFP4DA_KV_BF16 0
+#define NVFP4DA_KV_E4M3 1
+#define NVFP4DA_KV_NVFP4 2
+/* Capacities of quantised caches are multiples of this. */
+#define NVFP4DA_KV_CAPACITY_MULTIPLE 64
+/* A KV cache of B sequences, Hkv heads, C slots.  A row is the D elements of
+ * one (sequence, head, slot); head_dim a multiple of 16, at most 256.
+ *   BF16   codes uint16 [B, Hkv, C, D]; no scales
+ *   E4M3   codes uint8 [B, Hkv, C, D]; row_scales float32 [B, Hkv, C];
+ *          value = e4m3(code) * row_scale
+ *   NVFP4  codes uint8 [B, Hkv, C, D/2] (even element in the low nibble),
+ *          block_scales uint8 [B, Hkv, C, D/16] (UE4M3), row_scales float32:
+ *          every row is one [1, D] matrix of nvfp4da_weight's format. */
+typedef struct nvfp4da_kv_cache {
+  int format;
+  void* k_codes;
+  void* v_codes;
+  uint8_t* k_block_scales;
+  uint8_t* v_block_scales;
+  float* k_row_scales;
+  float* v_row_scales;
+  int64_t batch, kv_heads, capacity, head_dim;
+} nvfp4da_kv_cache;
+
+/* Rotary positions of q [B, T, Hq, D] and k [B, T, Hkv, D] (kv_heads 0: q
+ * alone) into contiguous q_out, k_out.  *_strides: element strides (host) of
+ * batch, token and head, the last dimension contiguous.  positions: device
+ * int64, positions[b * position_stride + t] (position_stride 0: one row for
+ * all).  inv_freq: device float32 [rotary_dim / 2]; the first rotary_dim
+ * elements of a head turn by position * inv_freq, in adjacent pairs
+ * (interleaved != 0) or as halves (m, m + rotary_dim / 2), sine and cosine
+ * times attention_factor; the others are copied. */
+int nvfp4da_apply_rope_qk(const uint16_t* q, const int64_t* q_strides, uint16_t* q_out, const uint16_t* k,
+                          const int64_t* k_strides, uint16_t* k_out, int64_t batch, int64_t tokens, int64_t q_heads,
+                          int64_t kv_heads, int64_t head_dim, const int64_t* positions, int64_t position_stride,
+                          const float* inv_freq, int64_t rotary_dim, int interleaved, float attention_factor,
+                          void* stream);
+
+/* Quantise new_k, new_v [B, T, Hkv, D] (BF16, by strides as above) into slots
+ * P_b + t of an E4M3 or NVFP4 cache.  counts (device int64 [B], optional):
+ * tokens t >= counts[b] are not written; neither is a slot outside the cache.
+ * Row scale: max |x| / 448 (E4M3) or / 2688 (NVFP4); a row that holds an
+ * infinity or NaN reads back as NaN throughout. */
+int nvfp4da_kv_quant_append(const nvfp4da_kv_cache* cache, const uint16_t* new_k, const int64_t* k_strides,
+                            const uint16_t* new_v, const int64_t* v_strides, int64_t tokens, int64_t past_length,
+                            const int64_t* past_lengths, const int64_t* counts, void* stream);
+
+/* Rows [S_b, S_b + length) of a quantised cache as BF16 [B, Hkv, length, D];
+ * S_b = starts[b] (device int64 [B]) when given, else start.  Rows outside the
+ * cache read as zeros. */
+int nvfp4da_kv_quant_read(const nvfp4da_kv_cache* cache, int64_t start, const int64_t* starts, int64_t length,
+                          uint16_t* k_out, uint16_t* v_out, void* stream);
+
+/* Attention of T drafted tokens, q and context [B, T, Hq, D], over a cache that
+ * holds them in slots P_b .. P_b + T - 1: token t sees slots below P_b and
+ * slot P_b + u where tree_mask[b * mask_batch_stride + t * T + u] is not 0
+ * (NULL: u <= t).  A query that sees nothing gets zeros.  T = 1 is decode.
+ * max_past_length >= every P_b (== past_length without past_lengths). */
+size_t nvfp4da_tree_attention_workspace_size(const nvfp4da_kv_cache* cache, int64_t tokens, int64_t q_heads,
+                                             int64_t max_past_length);
+int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* cache, const uint8_t* tree_mask,
+                           int64_t mask_batch_stride, uint16_t* context, int64_t tokens, int64_t q_heads,
+                           int64_t past_length, const int64_t* past_lengths, int64_t max_past_length,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
