@@ -9,6 +9,7 @@
 #include "kv_quant.cuh"
 #include "rope_positions.cuh"
 #include "tree_attention.cuh"
+#include "tree_stream.cuh"
 
 namespace nvfp4da {
 namespace {
@@ -83,10 +84,51 @@ cudaError_t launch_rope(RopeQkParams p, cudaStream_t s) {
 
 // ---------------------------------------------------------------- tree attention
 struct TreePlan {
-  int splits;
+  bool stream;  // tree_stream_kernel, else the general kernel
+  int wide;     // NG: 8-row groups of queries per warp
+  int row_chunks, rows_per_pass, passes;
+  int splits;   // general kernel
   int64_t split_len;
   size_t bytes;
 };
+
+constexpr int kTsWarps = 8;
+
+template <int D, int FMT, int NG>
+cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p,
+                               cudaStream_t s) {
+  auto* kern = tree_stream_kernel<D, FMT, NG, kTsWarps>;
+  const uint32_t smem = TsCfg<D, FMT, NG, kTsWarps>::bytes(p.batch);
+  cudaError_t e = ensure_smem(kern, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<p.grid, (kTsWarps + 1) * 32, smem, s>>>(tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>(p.batch * p.kv_heads * p.passes),
+                  static_cast<unsigned>(std::min(p.rows_per_pass, p.group * p.tokens)));
+  return launch(tree_stream_combine_kernel<D>, grid, dim3(128), 0, s, true, p);
+}
+
+template <int FMT>
+cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& tk, const CUtensorMap& tv,
+                                 const TreeStreamParams& p, cudaStream_t s) {
+  switch (head_dim) {
+    case 64: return wide == 2 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
+    case 128: return wide == 2 ? launch_tree_stream<128, FMT, 2>(tk, tv, p, s) : launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
+    default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
+  }
+}
+
+// The tensor map of K or V: BF16 rows in 64-element boxes, codes as 128-byte lines.
+bool tree_map(CUtensorMap* map, const nvfp4da_kv_cache& c, const void* base) {
+  const uint64_t rows = static_cast<uint64_t>(c.batch * c.kv_heads * c.capacity), d = c.head_dim;
+  if (c.format == NVFP4DA_KV_BF16)
+    return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, d, rows, d * 2, 64, kTsTile,
+                       CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t bytes = c.format == NVFP4DA_KV_E4M3 ? d : d / 2;
+  return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 128, rows * bytes / 128, 128, 128,
+                     static_cast<uint32_t>(kTsTile * bytes / 128), CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_t max_past, TreePlan& pl) {
   int r = check_cache(c);
@@ -102,7 +144,23 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
   const int64_t group = q_heads / c->kv_heads;
   if (!product_within(group, tokens, 65535) || !product_within(c->batch * q_heads, tokens, kI32Max))
     return fail(NVFP4DA_ERR_UNSUPPORTED, "too many query rows: (Hq/Hkv)*T must be at most 65535 and B*T*Hq below 2^31");
-  const int64_t visible = max_past + tokens;
+  const int64_t visible = max_past + tokens, nq = group * tokens;
+  const int64_t d = c->head_dim;
+  // The streaming kernel: tensor-core tiles for these head dimensions; the
+  // tile line of 128-byte lines and the prefix of the batch have to fit.
+  pl.stream = (d == 64 || d == 128 || d == 256) && c->batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
+              product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
+  if (pl.stream) {
+    pl.wide = nq > 8 && d <= 128 ? 2 : 1;
+    pl.row_chunks = 1;
+    while (pl.row_chunks < kTsWarps && 8 * pl.wide * pl.row_chunks < nq) pl.row_chunks *= 2;
+    pl.rows_per_pass = 8 * pl.wide * pl.row_chunks;
+    pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
+    pl.splits = 1;
+    pl.split_len = visible;
+    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * pl.rows_per_pass * (d * 4 + 8), 256);
+    return NVFP4DA_OK;
+  }
   const int64_t base = c->batch * c->kv_heads * ceil_div(group * tokens, kTreeWarps);
   int64_t splits = std::min(ceil_div(8LL * sm_count(), base), ceil_div(visible, 128));
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, 1024));
@@ -272,11 +330,46 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
   if (!q || !context) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "tree attention: NULL pointer");
   if (!aligned(q, 16) || !aligned(context, 16))
     return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
-  if (pl.splits > 1 && (!ws || ws_bytes < pl.bytes))
+  const bool needs_ws = pl.stream || pl.splits > 1;
+  if (needs_ws && (!ws || ws_bytes < pl.bytes))
     return fail(NVFP4DA_ERR_WORKSPACE, "tree attention workspace too small (%zu < %zu bytes)", ws ? ws_bytes : size_t(0),
                 pl.bytes);
-  if (pl.splits > 1 && !aligned(ws, 16))
+  if (needs_ws && !aligned(ws, 16))
     return fail(NVFP4DA_ERR_WORKSPACE, "the tree attention workspace must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (pl.stream) {
+    CUtensorMap tk, tv;
+    if (!tree_map(&tk, *c, c->k_codes) || !tree_map(&tv, *c, c->v_codes))
+      return fail(NVFP4DA_ERR_CUDA, "tensor map encoding failed for the tree attention");
+    TreeStreamParams t{};
+    t.q = q;
+    t.k = k_store(*c);
+    t.v = v_store(*c);
+    t.mask = tree_mask;
+    t.mask_stride = mask_batch_stride;
+    t.ctx = context;
+    t.batch = static_cast<int>(c->batch);
+    t.tokens = static_cast<int>(tokens);
+    t.q_heads = static_cast<int>(q_heads);
+    t.kv_heads = static_cast<int>(c->kv_heads);
+    t.group = static_cast<int>(q_heads / c->kv_heads);
+    t.capacity = c->capacity;
+    t.past_length = past_length;
+    t.past_lengths = past_lengths;
+    t.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c->head_dim)));
+    t.row_chunks = pl.row_chunks;
+    t.rows_per_pass = pl.rows_per_pass;
+    t.passes = pl.passes;
+    t.grid = sm_count();
+    t.part_o = static_cast<float*>(ws);
+    t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
+    cudaError_t e = c->format == NVFP4DA_KV_BF16 ? launch_tree_stream_d<kKvFmtBf16>(c->head_dim, pl.wide, tk, tv, t, s)
+                    : c->format == NVFP4DA_KV_E4M3
+                        ? launch_tree_stream_d<kKvFmtE4m3>(c->head_dim, pl.wide, tk, tv, t, s)
+                        : launch_tree_stream_d<kKvFmtNvfp4>(c->head_dim, pl.wide, tk, tv, t, s);
+    if (e != cudaSuccess) return cuda_fail(e, "streaming tree attention launch");
+    return NVFP4DA_OK;
+  }
   TreeAttnParams p{};
   p.q = q;
   p.k = k_store(*c);
@@ -297,7 +390,6 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
   p.splits = pl.splits;
   p.split_len = pl.split_len;
   p.lanes = lanes_per_row(c->head_dim);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t group = q_heads / c->kv_heads;
   const dim3 grid(static_cast<unsigned>(pl.splits), static_cast<unsigned>(ceil_div(group * tokens, kTreeWarps)),
                   static_cast<unsigned>(c->batch * c->kv_heads));

@@ -1,0 +1,955 @@
+// Tree attention at HBM rate: a persistent, TMA-fed tensor-core kernel that
+// reads a BF16, E4M3 or NVFP4 cache in its own format (head_dim 64, 128, 256).
+// Semantics: tree_attention.cuh.
+//
+// Work decomposition.  The group * T query rows of one (sequence, KV head) are
+// cut into passes of RP rows (nearly always one pass).  Every (sequence, KV
+// head, pass) owns the ceil((P_b + T) / 64) tiles of 64 positions its keys
+// fill; all of them are laid end to end and one CTA per SM takes an equal
+// contiguous range of that line, so every SM streams the same bytes whatever
+// the lengths.  A CTA's part of one unit either is the whole unit (the result
+// is written) or leaves a partial (o, m, l): only a CTA's first and last parts
+// can be partial, so it has two slots.  tree_stream_combine_kernel joins a
+// unit's partials in CTA order.
+//
+// Per CTA: a producer lane moves K and V tiles (TMA, 128-byte swizzle) and
+// their scales (bulk copies) into a ring of stages.  NW consumer warps: RC row
+// chunks of 8 NG query rows, NW / RC position warps per chunk; a warp takes
+// 16-position slices, whole tiles alternating between groups of four position
+// warps.  With x^T for a fragment that holds positions or head elements in its
+// 16 rows and queries in its 8 columns:
+//   S^T[pos, q] = K[pos, :] . Q^T      mma.m16n8k16, FP32 accumulators
+//   O^T[d, q]  += V^T[d, pos] P^T
+// The element k of an MMA step may be any element of the head as long as K and
+// Q agree, and a row of O^T any element d: a lane of K takes D/4 consecutive
+// elements of its row, a lane of V takes D/8 consecutive elements of its four
+// positions, so codes are read 8 or 16 bytes at a time and decoded in
+// registers; nothing is written back to shared memory.
+//
+// Numerics.  Codes (times the NVFP4 block scale) are exact in FP16; the query
+// row is scaled by a power of two to FP16 (exact down to 2^-39 of its largest
+// element); the row scale of K multiplies the FP32 score.  P goes to FP16 as
+// p_j gamma_j / G 2^11, G the largest row scale of V that the query has seen so
+// far (>= 2^-126): 11 significant bits down to 2^-25 of the largest.  Over BF16 caches Q and V stay
+// BF16 and P is split into two BF16 terms.  The softmax runs in base 2; its
+// reference m moves only when a score passes m + 4 (p <= 16), so most slices
+// need neither a reduction nor a rescale.  m, l, o and all sums are FP32.
+//
+// Slices that reach P_b (drafted tokens, the sequence's end) take a second
+// instantiation that applies the mask, drops positions past the end and zeroes
+// infinities and NaN in V before the MMA (0 * NaN would reach queries that do
+// not see the row); queries that do see such an element get it added after.
+//
+// Waits are bounded: a barrier that does not complete within 2^22 tries records
+// kErrBarrierTimeout in g_tree_errors and the CTA stops waiting (its results
+// are then garbage; the GPU stays usable).
+#pragma once
+
+#include <cuda.h>
+#include <math.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "kv_quant.cuh"
+#include "tree_attention.cuh"
+
+namespace nvfp4da {
+
+__device__ unsigned g_tree_errors;
+
+constexpr int kTsTile = 64;        // positions per stage
+constexpr int kTsMaxBatch = 1024;  // sequences whose prefix shared memory holds
+constexpr float kTsSlack = 4.0f;   // a score may pass the reference m by this (log2)
+constexpr float kTsPScale = 2048.0f;
+constexpr float kTsMinUnit = 1.17549435e-38f;  // 2^-126
+
+template <int D, int FMT, int NG, int NW>
+struct TsCfg {
+  static_assert(D == 64 || D == 128 || D == 256, "head_dim 64, 128 or 256");
+  static constexpr int kThreads = (NW + 1) * 32;
+  static constexpr int kRowBytes = FMT == kKvFmtBf16 ? 2 * D : (FMT == kKvFmtE4m3 ? D : D / 2);
+  static constexpr uint32_t kCodes = kTsTile * kRowBytes;  // one of K, V
+  static constexpr uint32_t kBlockScales = FMT == kKvFmtNvfp4 ? kTsTile * (D / 16) : 0;
+  static constexpr uint32_t kRowScales = FMT == kKvFmtBf16 ? 0 : kTsTile * 4;
+  static constexpr uint32_t kOffV = kCodes, kOffKb = 2 * kCodes, kOffVb = kOffKb + kBlockScales,
+                            kOffKr = kOffVb + kBlockScales, kOffVr = kOffKr + kRowScales;
+  static constexpr uint32_t kTx = kOffVr + kRowScales;  // bytes a stage receives
+  static constexpr uint32_t kStage = (kTx + 1023) / 1024 * 1024;
+  static constexpr int kRows = 8 * NG;                               // query rows per warp
+  static constexpr uint32_t kComb = NW * kRows * D * 4;              // per-warp O for the join
+  static constexpr uint32_t kMl = 3 * NW * kRows * 4 + NW * kRows * 8;  // m, l, factor; joined (m, l)
+  static constexpr int kGroups = NW / 4;                             // most tile groups
+  static constexpr int kFit = static_cast<int>((217u * 1024 - kComb - kMl) / kStage);
+  // A whole number of groups: the CTA's n-th tile goes to stage n % kStages and
+  // group n % groups, so every stage serves one group only.
+  static constexpr int kStages = (kFit > 12 ? 12 : kFit) / kGroups * kGroups;
+  static_assert(kStages >= 2, "two stages at least");
+  static constexpr uint32_t kOffComb = kStages * kStage;
+  static constexpr uint32_t kOffMl = kOffComb + kComb;
+  static constexpr uint32_t kOffBar = kOffMl + kMl;
+  static constexpr uint32_t kOffPrefix = kOffBar + 2 * kStages * 8;
+  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 8u * (batch + 1) + 1024; }
+};
+
+struct TreeStreamParams {
+  const uint16_t* q;
+  KvStore k, v;  // scales; the codes come through the tensor maps
+  const uint8_t* mask;
+  int64_t mask_stride;
+  uint16_t* ctx;
+  int batch, tokens, q_heads, kv_heads, group;
+  int64_t capacity;
+  int64_t past_length;
+  const int64_t* past_lengths;
+  float scale_log2;    // log2(e) / sqrt(D)
+  int row_chunks;      // RC: power of two, <= NW
+  int rows_per_pass;   // RP = 8 NG RC
+  int passes;
+  int grid;            // CTAs of the streaming kernel
+  float* part_o;       // [2 grid][RP][D]: slots 2 CTA (its first segment) and 2 CTA + 1 (its last)
+  float2* part_ml;     // [2 grid][RP]
+};
+
+// ---------------------------------------------------------------- PTX
+__device__ __forceinline__ void ts_tma_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void ts_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ts_bar_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
+__device__ __forceinline__ uint32_t ts_transpose(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ float ts_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int FMT>
+__device__ __forceinline__ void ts_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (FMT == kKvFmtBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ts_ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ts_ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t ts_pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t ts_pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t ts_hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two packed pairs of E4M3 -> two f16x2.
+__device__ __forceinline__ void ts_e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+}
+
+// Byte offset o of a tile of 128-byte lines, 16-byte chunks swizzled by line.
+__device__ __forceinline__ uint32_t ts_swz(uint32_t o) { return o ^ ((o >> 3) & 0x70u); }
+
+// The 16-bit halves of w whose exponent is all ones (FP16 or BF16) become 0;
+// `bad` collects them (bit 0: low half, bit 1: high half).
+template <int FMT>
+__device__ __forceinline__ uint32_t ts_finite(uint32_t w, uint32_t& bad) {
+  constexpr uint32_t e = FMT == kKvFmtBf16 ? 0x7f80u : 0x7c00u;
+  if ((w & e) == e) {
+    bad |= 1u;
+    w &= 0xffff0000u;
+  }
+  if (((w >> 16) & e) == e) {
+    bad |= 2u;
+    w &= 0x0000ffffu;
+  }
+  return w;
+}
+
+// ---------------------------------------------------------------- the walk over one CTA's range
+struct TsWalk {
+  const long long* prefix;  // [B + 1]: tiles before sequence b (all its units)
+  int units;                // per sequence
+  long long x, x_end;
+  int b, u;
+  int t0, t1, nt;  // this segment's tiles [t0, t1) of nt in the unit
+  __device__ bool begin(const long long* pre, int batch, int per_seq, long long x0, long long x1) {
+    prefix = pre;
+    units = per_seq;
+    x = x0;
+    x_end = x1;
+    if (x >= x_end) return false;
+    int lo = 0, hi = batch - 1;  // the last b with prefix[b] <= x (every sequence has a tile)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= x) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    nt = static_cast<int>((prefix[b + 1] - prefix[b]) / units);
+    const long long within = x - prefix[b];
+    u = static_cast<int>(within / nt);
+    t0 = static_cast<int>(within % nt);
+    t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (x_end - x)));
+    return true;
+  }
+  __device__ bool next() {
+    x += t1 - t0;
+    if (x >= x_end) return false;
+    if (++u == units) {
+      u = 0;
+      ++b;
+      nt = static_cast<int>((prefix[b + 1] - prefix[b]) / units);
+    }
+    t0 = 0;
+    t1 = static_cast<int>(min(static_cast<long long>(nt), x_end - x));
+    return true;
+  }
+};
+
+// Positions of sequence b that any of its drafted tokens may see.
+__device__ __forceinline__ int64_t ts_visible(const TreeStreamParams& p, int b) {
+  return min(tree_past(p.past_lengths, p.past_length, b, p.capacity) + p.tokens, p.capacity);
+}
+
+// CTA (of g over n tiles, CTA c owning [c n / g, (c + 1) n / g)) that holds tile x.
+__device__ __forceinline__ int ts_cta_of(long long x, long long n, int g) {
+  return static_cast<int>(((x + 1) * g - 1) / n);
+}
+
+// Element d of position r (in the tile) of V as the MMA saw it, before ts_finite.
+template <int D, int FMT>
+__device__ __forceinline__ float ts_v_element(const uint8_t* vt, const uint8_t* vb, int r, int d) {
+  if (FMT == kKvFmtBf16) {
+    const uint32_t o = (d >> 6) * (kTsTile * 128) + ts_swz(r * 128 + (d & 63) * 2);
+    return bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(vt + o));
+  }
+  if (FMT == kKvFmtE4m3) return f16x2_to_f32x2(e4m3x2_to_f16x2(vt[ts_swz(r * D + d)])).x;
+  const uint32_t byte = vt[ts_swz(r * (D / 2) + d / 2)];
+  const float2 pair = f16x2_to_f32x2(e2m1x2_to_f16x2(byte));
+  return ((d & 1) ? pair.y : pair.x) * f16x2_to_f32x2(e4m3x2_to_f16x2(vb[r * (D / 16) + d / 16])).x;
+}
+
+// ---------------------------------------------------------------- the streaming kernel
+template <int D, int FMT, int NG, int NW>
+__global__ void __launch_bounds__((NW + 1) * 32, 1)
+    tree_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                       const TreeStreamParams p) {
+  using Cfg = TsCfg<D, FMT, NG, NW>;
+  constexpr int KS = D / 16;  // MMA steps of K Q^T, 16-element row blocks of O^T
+  constexpr bool kQuant = FMT != kKvFmtBf16;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* so = reinterpret_cast<float*>(smem + Cfg::kOffComb);  // [warp][row][D]
+  float* sm_m = reinterpret_cast<float*>(smem + Cfg::kOffMl);  // [warp][row]
+  float* sm_l = sm_m + NW * Cfg::kRows;
+  float* sm_f = sm_l + NW * Cfg::kRows;
+  float2* sm_ml = reinterpret_cast<float2*>(sm_f + NW * Cfg::kRows);  // [row of the pass]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
+  uint64_t* empty = full + Cfg::kStages;
+  long long* prefix = reinterpret_cast<long long*>(smem + Cfg::kOffPrefix);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x;
+  const int rc_n = p.row_chunks, pw_n = NW / rc_n;       // row chunks, position warps per chunk
+  const int groups = pw_n >= 4 ? pw_n / 4 : 1;           // tiles alternate between groups
+  const int units = p.kv_heads * p.passes;
+  const int nq = p.group * p.tokens;                     // query rows per KV head
+
+  pdl_launch_dependents();  // the join waits for this kernel's memory itself
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], pw_n >= 4 ? 4 * rc_n : NW);
+    }
+    fence_mbar_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+  }
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x)
+    prefix[b + 1] = (ts_visible(p, b) + kTsTile - 1) / kTsTile * units;
+  __syncthreads();
+  if (warp == 0) {
+    long long carry = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      const int b = base + lane;
+      long long v = b < p.batch ? prefix[b + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(kFull, v, o);
+        if (lane >= o) v += u;
+      }
+      if (b < p.batch) prefix[b + 1] = carry + v;
+      carry += __shfl_sync(kFull, v, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  const long long n_tiles = prefix[p.batch];
+  // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
+  // every CTA between a unit's first and last holds one of its tiles.
+  const int G = n_tiles < p.grid ? static_cast<int>(n_tiles) : p.grid;
+  if (cta >= G) return;
+  const long long x0 = n_tiles * cta / G, x1 = n_tiles * (cta + 1) / G;
+
+  if (warp == NW) {
+    // ---------------------------------------------------------------- producer
+    if (lane != 0) return;
+    TsWalk w;
+    bool more = w.begin(prefix, p.batch, units, x0, x1);
+    int stage = 0;
+    uint32_t phase = 0;
+    long long it = 0;
+    while (more) {
+      const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
+      for (int t = w.t0; t < w.t1; ++t, ++it) {
+        if (it >= Cfg::kStages && !mbar_wait_bounded(&empty[stage], phase ^ 1u, &g_tree_errors)) return;
+        uint8_t* st = smem + stage * Cfg::kStage;
+        mbar_arrive_expect_tx(&full[stage], Cfg::kTx);
+        const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile;
+        if constexpr (!kQuant) {
+#pragma unroll
+          for (int bx = 0; bx < D / 64; ++bx) {
+            ts_tma_2d(st + bx * (kTsTile * 128), &tm_k, bx * 64, static_cast<int>(row), &full[stage]);
+            ts_tma_2d(st + Cfg::kOffV + bx * (kTsTile * 128), &tm_v, bx * 64, static_cast<int>(row), &full[stage]);
+          }
+        } else {  // the codes as a matrix of 128-byte lines
+          const int line = static_cast<int>(row * Cfg::kRowBytes / 128);
+          ts_tma_2d(st, &tm_k, 0, line, &full[stage]);
+          ts_tma_2d(st + Cfg::kOffV, &tm_v, 0, line, &full[stage]);
+          if constexpr (FMT == kKvFmtNvfp4) {
+            bulk_g2s(st + Cfg::kOffKb, p.k.block_scales + row * (D / 16), Cfg::kBlockScales, &full[stage]);
+            bulk_g2s(st + Cfg::kOffVb, p.v.block_scales + row * (D / 16), Cfg::kBlockScales, &full[stage]);
+          }
+          bulk_g2s(st + Cfg::kOffKr, p.k.row_scales + row, Cfg::kRowScales, &full[stage]);
+          bulk_g2s(st + Cfg::kOffVr, p.v.row_scales + row, Cfg::kRowScales, &full[stage]);
+        }
+        if (++stage == Cfg::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      more = w.next();
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int g = lane >> 2, tq = lane & 3;  // fragment row / column pair
+  const int rc = warp % rc_n, pw = warp / rc_n;
+  const int slices = pw_n >= 4 ? 1 : 4 / pw_n;  // per tile and warp
+  const int slice0 = pw_n >= 4 ? pw % 4 : pw * slices;
+  TsWalk w;
+  bool more = w.begin(prefix, p.batch, units, x0, x1);
+  bool dead = false;
+  long long it = 0;
+  int stage = 0, turn = 0;  // it % kStages, it % groups
+  uint32_t phase = 0;
+  while (more) {
+    const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes;
+    const int64_t past = tree_past(p.past_lengths, p.past_length, b, p.capacity);
+    const int64_t vis = min(past + p.tokens, p.capacity);
+    const int n0 = pass * p.rows_per_pass + rc * Cfg::kRows;  // this warp's first query row
+    // Query row n = t * group + j; global row of q and ctx:
+    auto q_row = [&](int n) {
+      return (static_cast<int64_t>(b) * p.tokens + n / p.group) * p.q_heads + static_cast<int64_t>(kvh) * p.group +
+             n % p.group;
+    };
+
+    // ---- Q^T fragments: this lane's column is n0 + 8 j + g; q_scale: of its score columns 2 tq, 2 tq + 1
+    uint32_t qb[NG][KS][2];
+    float q_scale[NG][2];
+    int tok[NG][2];  // drafted token of the score columns (-1: no such row)
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int n = n0 + 8 * j + g;
+      const uint16_t* src = p.q + q_row(n < nq ? n : 0) * D;
+      float own = 1.0f;
+      if constexpr (!kQuant) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          qb[j][ks][0] = n < nq ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * tq) : 0u;
+          qb[j][ks][1] = n < nq ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + 2 * tq) : 0u;
+        }
+      } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint2 e = n < nq ? *reinterpret_cast<const uint2*>(src + (D / 4) * tq + 4 * ks) : make_uint2(0u, 0u);
+          qb[j][ks][0] = e.x;
+          qb[j][ks][1] = e.y;
+          top = max(top, max(max(e.x & 0x7fffu, (e.x >> 16) & 0x7fffu), max(e.y & 0x7fffu, (e.y >> 16) & 0x7fffu)));
+        }
+        top = max(top, __shfl_xor_sync(kFull, top, 1));
+        top = max(top, __shfl_xor_sync(kFull, top, 2));
+        // 2^e that brings the row's largest element to [2^14, 2^15)
+        const int ex = static_cast<int>(top >> 7);
+        const int e = (ex == 0 || ex == 255) ? 0 : min(14 - (ex - 127), 100);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        own = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t e2 = qb[j][ks][i];
+            qb[j][ks][i] = ts_pack_f16(__uint_as_float(e2 << 16) * up, __uint_as_float(e2 & 0xffff0000u) * up);
+          }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        q_scale[j][c] = __shfl_sync(kFull, own, (2 * tq + c) * 4) * p.scale_log2;
+        const int col = n0 + 8 * j + 2 * tq + c;
+        tok[j][c] = col < nq ? col / p.group : -1;
+      }
+    }
+
+    float m_run[NG][2], l_run[NG][2], acc[NG][KS][4];
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      m_run[j][0] = m_run[j][1] = -INFINITY;
+      l_run[j][0] = l_run[j][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.0f;
+    }
+    float g_run[NG][2], p_unit[NG][2];  // G of the score columns, 2^11 / G (0: no row with a scale above 2^-126 yet)
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      g_run[j][0] = g_run[j][1] = kTsMinUnit;
+      p_unit[j][0] = p_unit[j][1] = 0.0f;
+    }
+
+    // One slice of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
+    auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int64_t pos0) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      const uint8_t *kt = st, *vt = st + Cfg::kOffV;
+      float s[NG][2][4];  // two accumulators, alternate steps
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[j][h][0] = s[j][h][1] = s[j][h][2] = s[j][h][3] = 0.0f;
+      // ---- S^T = K Q^T; score rows: positions pos0 + g and pos0 + 8 + g
+      if constexpr (FMT == kKvFmtBf16) {
+        const int mat = lane >> 3, r = r0 + (mat & 1) * 8 + (lane & 7);
+        const uint32_t base = smem_u32(kt) + r * 128;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int c = (ks & 3) * 2 + (mat >> 1);
+          uint32_t a[4];
+          ts_ldsm4(base + (ks >> 2) * (kTsTile * 128) + ((c ^ (lane & 7)) << 4), a);
+#pragma unroll
+          for (int j = 0; j < NG; ++j) ts_mma<FMT>(s[j][ks & 1], a[0], a[1], a[2], a[3], qb[j][ks][0], qb[j][ks][1]);
+        }
+      } else if constexpr (FMT == kKvFmtE4m3) {
+        // D / 4 codes per row and lane, four per MMA step
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const uint32_t o = (D / 4) * tq + 16 * i;
+          const uint4 w0 = *reinterpret_cast<const uint4*>(kt + ts_swz((r0 + g) * D + o));
+          const uint4 w1 = *reinterpret_cast<const uint4*>(kt + ts_swz((r0 + 8 + g) * D + o));
+          const uint32_t c0[4] = {w0.x, w0.y, w0.z, w0.w}, c1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t a0, a1, a2, a3;
+            ts_e4m3x4(c0[e], a0, a2);
+            ts_e4m3x4(c1[e], a1, a3);
+            const int ks = 4 * i + e;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) ts_mma<FMT>(s[j][ks & 1], a0, a1, a2, a3, qb[j][ks][0], qb[j][ks][1]);
+          }
+        }
+      } else {
+        // D / 4 codes per row and lane: words of eight, two MMA steps each; a block scale per two words
+        constexpr int NWORD = D / 32, NB = D / 64;
+        const uint8_t* kb = st + Cfg::kOffKb;
+        uint32_t c[2][NWORD], bs[2][NB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = r0 + 8 * h + g;
+          if constexpr (D == 64) {
+            const uint2 v = *reinterpret_cast<const uint2*>(kt + ts_swz(r * (D / 2) + (D / 8) * tq));
+            c[h][0] = v.x;
+            c[h][1] = v.y;
+            bs[h][0] = kb[r * (D / 16) + tq];
+          } else {
+#pragma unroll
+            for (int i = 0; i < NWORD / 4; ++i) {
+              const uint4 v = *reinterpret_cast<const uint4*>(kt + ts_swz(r * (D / 2) + (D / 8) * tq + 16 * i));
+              c[h][4 * i] = v.x;
+              c[h][4 * i + 1] = v.y;
+              c[h][4 * i + 2] = v.z;
+              c[h][4 * i + 3] = v.w;
+              const uint32_t two = *reinterpret_cast<const uint16_t*>(kb + r * (D / 16) + NB * tq + 2 * i);
+              bs[h][2 * i] = two & 0xffu;
+              bs[h][2 * i + 1] = two >> 8;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < NB; ++i) bs[h][i] = e4m3x2_to_f16x2(bs[h][i] * 0x101u);  // in both halves
+        }
+#pragma unroll
+        for (int i = 0; i < NWORD; ++i) {
+          uint32_t d0[4], d1[4];
+          e2m1x8_to_f16x2x4(c[0][i], d0);
+          e2m1x8_to_f16x2x4(c[1][i], d1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            d0[e] = ts_hmul2(d0[e], bs[0][i / 2]);
+            d1[e] = ts_hmul2(d1[e], bs[1][i / 2]);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int ks = 2 * i + e;
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+              ts_mma<FMT>(s[j][e], d0[2 * e], d1[2 * e], d0[2 * e + 1], d1[2 * e + 1], qb[j][ks][0], qb[j][ks][1]);
+          }
+        }
+      }
+
+      // ---- scores in log2 units; sc[j][i]: position pos0 + g (+ 8 for i >= 2), column 2 tq + (i & 1)
+      [[maybe_unused]] float k_unit[2] = {1.0f, 1.0f}, v_unit[2] = {1.0f, 1.0f};
+      if constexpr (kQuant) {
+        const float* kr = reinterpret_cast<const float*>(st + Cfg::kOffKr) + r0 + g;
+        const float* vr = reinterpret_cast<const float*>(st + Cfg::kOffVr) + r0 + g;
+        k_unit[0] = kr[0];
+        k_unit[1] = kr[8];
+        v_unit[0] = vr[0];
+        v_unit[1] = vr[8];
+      }
+      float sc[NG][4];
+      bool sees[NG][4];
+      bool above = false;
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = (s[j][0][i] + s[j][1][i]) * q_scale[j][i & 1];
+          if constexpr (kQuant) x *= k_unit[i >> 1];
+          if constexpr (EDGE) {
+            const int64_t pos = pos0 + g + (i >> 1) * 8, u = pos - past;
+            const int t = tok[j][i & 1];
+            bool ok = t >= 0 && pos < vis;
+            if (ok && u >= 0)
+              ok = p.mask ? p.mask[b * p.mask_stride + static_cast<int64_t>(t) * p.tokens + u] != 0 : u <= t;
+            sees[j][i] = ok;
+            if (!ok) x = -INFINITY;
+          } else {
+            sees[j][i] = true;
+          }
+          sc[j][i] = x;
+          above |= x > m_run[j][i & 1] + kTsSlack;
+        }
+      // ---- the reference moves (for every column) when a score passes it by the slack
+      if (__any_sync(kFull, above)) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          float alpha[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(sc[j][c], sc[j][c + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
+            const float m_new = fmaxf(m_run[j][c], mx);
+            alpha[c] = m_run[j][c] == -INFINITY ? 0.0f : ts_exp2(m_run[j][c] - m_new);
+            m_run[j][c] = m_new;
+            l_run[j][c] *= alpha[c];
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            acc[j][i][0] *= alpha[0];
+            acc[j][i][1] *= alpha[1];
+            acc[j][i][2] *= alpha[0];
+            acc[j][i][3] *= alpha[1];
+          }
+        }
+      }
+      if constexpr (kQuant) {  // the largest finite row scale of V that each column has seen
+        bool up = false;
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            up |= sees[j][i] && v_unit[i >> 1] > g_run[j][i & 1] && v_unit[i >> 1] < INFINITY;
+        if (__any_sync(kFull, up)) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = g_run[j][c];
+              if (sees[j][c] && v_unit[0] < INFINITY) mx = fmaxf(mx, v_unit[0]);
+              if (sees[j][c + 2] && v_unit[1] < INFINITY) mx = fmaxf(mx, v_unit[1]);
+              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
+              f[c] = __fdiv_rn(g_run[j][c], mx);
+              g_run[j][c] = mx;
+              p_unit[j][c] = __fdiv_rn(kTsPScale, mx);
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              acc[j][i][0] *= f[0];
+              acc[j][i][1] *= f[1];
+              acc[j][i][2] *= f[0];
+              acc[j][i][3] *= f[1];
+            }
+          }
+        }
+      }
+      // ---- P^T as B fragments
+      uint32_t ph[NG][2];
+      [[maybe_unused]] uint32_t pl[NG][2];  // second term, BF16 only
+      float pr[NG][4];
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        float wt[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // -inf only stands for a key that is not seen, or one that weighs nothing
+          pr[j][i] = sc[j][i] == -INFINITY ? 0.0f : ts_exp2(sc[j][i] - m_run[j][i & 1]);
+          wt[i] = pr[j][i];
+          if constexpr (kQuant) wt[i] *= v_unit[i >> 1] * p_unit[j][i & 1];
+          if constexpr (EDGE) wt[i] = sees[j][i] ? wt[i] : 0.0f;
+        }
+        l_run[j][0] += pr[j][0] + pr[j][2];
+        l_run[j][1] += pr[j][1] + pr[j][3];
+        if constexpr (kQuant) {
+          ph[j][0] = ts_transpose(ts_pack_f16(wt[0], wt[1]));
+          ph[j][1] = ts_transpose(ts_pack_f16(wt[2], wt[3]));
+        } else {
+          const uint32_t h0 = ts_pack_bf16(wt[0], wt[1]), h1 = ts_pack_bf16(wt[2], wt[3]);
+          ph[j][0] = ts_transpose(h0);
+          ph[j][1] = ts_transpose(h1);
+          pl[j][0] = ts_transpose(ts_pack_bf16(wt[0] - __uint_as_float(h0 << 16), wt[1] - __uint_as_float(h0 & 0xffff0000u)));
+          pl[j][1] = ts_transpose(ts_pack_bf16(wt[2] - __uint_as_float(h1 << 16), wt[3] - __uint_as_float(h1 & 0xffff0000u)));
+        }
+      }
+      // ---- O^T += V^T P^T
+      uint32_t bad = 0;  // positions (bits) whose V holds an infinity or NaN somewhere in this lane's part
+      // Positions of the fragments' halves: 2 tq, 2 tq + 1 (registers 0, 1) and + 8 (registers 2, 3).
+      auto clean = [&](uint32_t (&a)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t pos = pos0 + 2 * tq + (i >> 1) * 8;
+          if (pos >= vis) a[i] = 0u;
+          else if (pos + 1 >= vis) a[i] &= 0x0000ffffu;
+          uint32_t two = 0;
+          a[i] = ts_finite<FMT>(a[i], two);
+          bad |= two << (2 * tq + (i >> 1) * 8);
+        }
+      };
+      auto pv = [&](int mt, uint32_t (&a)[4]) {
+        if constexpr (EDGE) clean(a);
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          ts_mma<FMT>(acc[j][mt], a[0], a[1], a[2], a[3], ph[j][0], ph[j][1]);
+          if constexpr (!kQuant) ts_mma<FMT>(acc[j][mt], a[0], a[1], a[2], a[3], pl[j][0], pl[j][1]);
+        }
+      };
+      if constexpr (FMT == kKvFmtBf16) {
+        const int mat = lane >> 3, r = r0 + (mat >> 1) * 8 + (lane & 7);
+        const uint32_t base = smem_u32(vt) + r * 128;
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) {
+          const int c = (mt & 3) * 2 + (mat & 1);
+          uint32_t a[4];
+          ts_ldsm4_trans(base + (mt >> 2) * (kTsTile * 128) + ((c ^ (lane & 7)) << 4), a);
+          pv(mt, a);
+        }
+      } else {
+        // D / 8 codes of four positions per lane; row g of block mt is element D/8 g + 2 mt, row g + 8 the next
+        constexpr int BYTES = Cfg::kRowBytes / 8;  // 4 to 32
+        uint32_t c[4][BYTES / 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = r0 + 2 * tq + (e & 1) + (e >> 1) * 8;
+          const uint32_t o = r * Cfg::kRowBytes + BYTES * g;
+          if constexpr (BYTES == 4) {
+            c[e][0] = *reinterpret_cast<const uint32_t*>(vt + ts_swz(o));
+          } else if constexpr (BYTES == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(vt + ts_swz(o));
+            c[e][0] = v.x;
+            c[e][1] = v.y;
+          } else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+              const uint4 v = *reinterpret_cast<const uint4*>(vt + ts_swz(o + 16 * i));
+              c[e][4 * i] = v.x;
+              c[e][4 * i + 1] = v.y;
+              c[e][4 * i + 2] = v.z;
+              c[e][4 * i + 3] = v.w;
+            }
+          }
+        }
+        if constexpr (FMT == kKvFmtE4m3) {
+#pragma unroll
+          for (int i = 0; i < BYTES / 4; ++i) {
+            uint32_t d[4][2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ts_e4m3x4(c[e][i], d[e][0], d[e][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t a[4] = {__byte_perm(d[0][h], d[1][h], 0x5410), __byte_perm(d[0][h], d[1][h], 0x7632),
+                               __byte_perm(d[2][h], d[3][h], 0x5410), __byte_perm(d[2][h], d[3][h], 0x7632)};
+              pv(2 * i + h, a);
+            }
+          }
+        } else {
+          constexpr int NB = D == 256 ? 2 : 1;  // block scales per lane and position
+          const uint8_t* vb = st + Cfg::kOffVb;
+          uint32_t bs[NB][2];  // [block][positions 2 tq and + 1, + 8 and + 9]
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint8_t* at = vb + (r0 + 2 * tq + 8 * h) * (D / 16) + (D / 8 * g + 16 * i) / 16;
+              bs[i][h] = e4m3x2_to_f16x2(at[0] | (static_cast<uint32_t>(at[D / 16]) << 8));
+            }
+#pragma unroll
+          for (int i = 0; i < BYTES / 4; ++i) {
+            uint32_t d[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) e2m1x8_to_f16x2x4(c[e][i], d[e]);
+            const uint32_t b0 = bs[i * NB / (BYTES / 4)][0], b1 = bs[i * NB / (BYTES / 4)][1];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              uint32_t a[4] = {ts_hmul2(__byte_perm(d[0][h], d[1][h], 0x5410), b0),
+                               ts_hmul2(__byte_perm(d[0][h], d[1][h], 0x7632), b0),
+                               ts_hmul2(__byte_perm(d[2][h], d[3][h], 0x5410), b1),
+                               ts_hmul2(__byte_perm(d[2][h], d[3][h], 0x7632), b1)};
+              pv(4 * i + h, a);
+            }
+          }
+        }
+      }
+      if constexpr (EDGE) {
+        // Infinities and NaN of V that were zeroed: added for the queries that see the row.
+        bad = __reduce_or_sync(kFull, bad);
+        while (bad) {
+          const int r = __ffs(bad) - 1;
+          bad &= bad - 1;
+          const int from = (r & 7) * 4 + tq;
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float lo = __shfl_sync(kFull, sees[j][c] ? pr[j][c] : -1.0f, from);
+              const float hi = __shfl_sync(kFull, sees[j][c + 2] ? pr[j][c + 2] : -1.0f, from);
+              const float pj = r < 8 ? lo : hi;
+              if (!(pj < 0.0f)) {
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int d = FMT == kKvFmtBf16 ? 16 * mt + 8 * h + g : D / 8 * g + 2 * mt + h;
+                    const float x = ts_v_element<D, FMT>(vt, st + Cfg::kOffVb, r0 + r, d);
+                    if (!isfinite(x)) acc[j][mt][2 * h + c] += pj * x;
+                  }
+              }
+            }
+        }
+      }
+    };
+
+    for (int t = w.t0; t < w.t1; ++t, ++it) {
+      const bool mine = pw_n < 4 || turn == (pw >> 2);
+      if (mine) {
+        if (!dead && !mbar_wait_bounded(&full[stage], phase, &g_tree_errors)) dead = true;
+        const uint8_t* st = smem + stage * Cfg::kStage;
+        for (int i = 0; i < slices; ++i) {
+          const int r0 = (slice0 + i) * 16;
+          const int64_t pos0 = static_cast<int64_t>(t) * kTsTile + r0;
+          if (dead || pos0 >= vis) break;
+          if (pos0 + 16 <= past) slice(std::false_type{}, st, r0, pos0);
+          else slice(std::true_type{}, st, r0, pos0);
+        }
+        __syncwarp();
+        if (lane == 0) ts_arrive(&empty[stage]);
+      }
+      if (++turn == groups) turn = 0;
+      if (++stage == Cfg::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+
+    // ---- this segment's (m, l, o): join the position warps of each row chunk
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float unit = kQuant ? g_run[j][c] * (1.0f / kTsPScale) : 1.0f;
+        float l = l_run[j][c];
+        l += __shfl_xor_sync(kFull, l, 4);
+        l += __shfl_xor_sync(kFull, l, 8);
+        l += __shfl_xor_sync(kFull, l, 16);
+        const int row = warp * Cfg::kRows + 8 * j + 2 * tq + c;
+        if (g == 0) {
+          sm_m[row] = m_run[j][c];
+          sm_l[row] = l;
+        }
+        float* o = so + row * D;
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) {
+          if constexpr (kQuant) {
+            *reinterpret_cast<float2*>(o + D / 8 * g + 2 * mt) =
+                make_float2(acc[j][mt][c] * unit, acc[j][mt][2 + c] * unit);
+          } else {
+            o[16 * mt + g] = acc[j][mt][c];
+            o[16 * mt + 8 + g] = acc[j][mt][2 + c];
+          }
+        }
+      }
+    }
+    ts_bar_sync(NW * 32);
+    const int n_first = pass * p.rows_per_pass;
+    const int rows = min(p.rows_per_pass, nq - n_first);
+    for (int r = threadIdx.x; r < rows; r += NW * 32) {
+      const int chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
+      float mx = -INFINITY, l = 0.0f;
+      for (int u = 0; u < pw_n; ++u) mx = fmaxf(mx, sm_m[(u * rc_n + chunk) * Cfg::kRows + rr]);
+      for (int u = 0; u < pw_n; ++u) {
+        const int i = (u * rc_n + chunk) * Cfg::kRows + rr;
+        const float f = sm_m[i] == -INFINITY ? (sm_l[i] == 0.0f ? 0.0f : 1.0f) : ts_exp2(sm_m[i] - mx);
+        sm_f[i] = f;
+        l = fmaf(sm_l[i], f, l);
+      }
+      sm_ml[r] = make_float2(mx, l);
+    }
+    ts_bar_sync(NW * 32);
+    const bool whole = w.t0 == 0 && w.t1 == w.nt;
+    const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 32) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4, chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int u = 0; u < pw_n; ++u) {
+        const int k = (u * rc_n + chunk) * Cfg::kRows + rr;
+        const float f = sm_f[k];
+        if (f == 0.0f) continue;
+        const float4 v = *reinterpret_cast<const float4*>(so + k * D + d);
+        o.x = fmaf(v.x, f, o.x);
+        o.y = fmaf(v.y, f, o.y);
+        o.z = fmaf(v.z, f, o.z);
+        o.w = fmaf(v.w, f, o.w);
+      }
+      if (whole) {
+        const float l = sm_ml[r].y;
+        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        if (l == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<uint2*>(p.ctx + q_row(n_first + r) * D + d) =
+            make_uint2(ts_pack_bf16(o.x * inv, o.y * inv), ts_pack_bf16(o.z * inv, o.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (slot * p.rows_per_pass + r) * D + d) = o;
+        if (d == 0) p.part_ml[slot * p.rows_per_pass + r] = sm_ml[r];
+      }
+    }
+    ts_bar_sync(NW * 32);  // the join's shared memory is reused by the next segment
+    more = w.next();
+  }
+}
+
+// ---------------------------------------------------------------- joining partials
+// Grid (unit, row of the pass): a block joins one query row of a unit that
+// several CTAs share, in CTA order; four warps take every fourth partial.
+template <int D>
+__global__ void __launch_bounds__(128) tree_stream_combine_kernel(const TreeStreamParams p) {
+  __shared__ long long red[2][4];
+  __shared__ float s_m[4], s_l[4];
+  __shared__ float s_o[4][D];
+  const int units = p.kv_heads * p.passes;
+  const int b = blockIdx.x / units, u = blockIdx.x % units, pass = u % p.passes, kvh = u / p.passes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = pass * p.rows_per_pass + blockIdx.y;
+  if (n >= p.group * p.tokens) return;
+  long long before = 0, all = 0;
+  for (int i = threadIdx.x; i < p.batch; i += 128) {
+    const long long t = (ts_visible(p, i) + kTsTile - 1) / kTsTile * units;
+    all += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(kFull, before, o);
+    all += __shfl_xor_sync(kFull, all, o);
+  }
+  if (lane == 0) {
+    red[0][warp] = before;
+    red[1][warp] = all;
+  }
+  __syncthreads();
+  before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+  all = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  const long long nt = (ts_visible(p, b) + kTsTile - 1) / kTsTile;
+  const long long first = before + u * nt;
+  const int G = all < p.grid ? static_cast<int>(all) : p.grid;
+  const int c0 = ts_cta_of(first, all, G), c1 = ts_cta_of(first + nt - 1, all, G);
+  pdl_wait();
+  if (c0 == c1) return;  // one CTA held the unit and wrote its result
+  constexpr int V = D / 32;  // elements per lane
+  const bool starts_c0 = all * c0 / G == first;  // the unit begins its first CTA's range
+  auto at = [&](int c) {
+    return (2 * static_cast<int64_t>(c) + (c == c0 && !starts_c0 ? 1 : 0)) * p.rows_per_pass + blockIdx.y;
+  };
+  float mx = -INFINITY;
+  for (int c = c0 + static_cast<int>(threadIdx.x); c <= c1; c += 128) mx = fmaxf(mx, __ldcg(&p.part_ml[at(c)]).x);
+  mx = warp_max_f32(mx);
+  if (lane == 0) s_m[warp] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  float o[V] = {}, l = 0.0f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += 4) {
+    const float2 ml = __ldcg(&p.part_ml[at(c)]);
+    const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(ml.x - mx);
+    l = fmaf(ml.y, f, l);
+    const float* src = p.part_o + at(c) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = __ldcg(src + i);
+      o[i] = f == 0.0f ? o[i] : fmaf(x, f, o[i]);
+    }
+  }
+  if (lane == 0) s_l[warp] = l;
+#pragma unroll
+  for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
+  __syncthreads();
+  l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+  const int64_t row = (static_cast<int64_t>(b) * p.tokens + n / p.group) * p.q_heads +
+                      static_cast<int64_t>(kvh) * p.group + n % p.group;
+  for (int d = threadIdx.x; d < D; d += 128) {
+    const float x = s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d];
+    p.ctx[row * D + d] = f32_to_bf16_bits(l == 0.0f ? 0.0f : x * inv);
+  }
+}
+
+}  // namespace nvfp4da
