@@ -10,6 +10,7 @@
 #include "rope_positions.cuh"
 #include "tree_attention.cuh"
 #include "tree_stream.cuh"
+#include "tree_tc.cuh"
 
 namespace nvfp4da {
 namespace {
@@ -84,7 +85,8 @@ cudaError_t launch_rope(RopeQkParams p, cudaStream_t s) {
 
 // ---------------------------------------------------------------- tree attention
 struct TreePlan {
-  bool stream;  // tree_stream_kernel, else the general kernel
+  bool stream;  // tree_stream_kernel (or tc: tree_tc_kernel), else the general kernel
+  bool tc;
   int wide;     // NG: 8-row groups of queries per warp
   int row_chunks, rows_per_pass, passes;
   int splits;   // general kernel
@@ -93,6 +95,25 @@ struct TreePlan {
 };
 
 constexpr int kTsWarps = 8;
+constexpr int64_t kTcMinRows = 17;  // query rows per KV head from which tree_tc_kernel runs
+
+template <int D>
+cudaError_t launch_tree_combine(const TreeStreamParams& p, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.batch * p.kv_heads * p.passes),
+                  static_cast<unsigned>(std::min(p.rows_per_pass, p.group * p.tokens)));
+  return launch(tree_stream_combine_kernel<D>, grid, dim3(128), 0, s, true, p);
+}
+
+template <int D, int FMT, bool SPLIT>
+cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p, cudaStream_t s) {
+  auto* kern = tree_tc_kernel<D, FMT, SPLIT>;
+  const uint32_t smem = TtCfg<D, FMT, SPLIT>::bytes(p.batch);
+  cudaError_t e = ensure_smem(kern, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<p.grid, kTtThreads, smem, s>>>(tk, tv, p);
+  e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_tree_combine<D>(p, s);
+}
 
 template <int D, int FMT, int NG>
 cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p,
@@ -103,10 +124,15 @@ cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, con
   if (e != cudaSuccess) return e;
   kern<<<p.grid, (kTsWarps + 1) * 32, smem, s>>>(tk, tv, p);
   e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(p.batch * p.kv_heads * p.passes),
-                  static_cast<unsigned>(std::min(p.rows_per_pass, p.group * p.tokens)));
-  return launch(tree_stream_combine_kernel<D>, grid, dim3(128), 0, s, true, p);
+  return e != cudaSuccess ? e : launch_tree_combine<D>(p, s);
+}
+
+template <int FMT>
+cudaError_t launch_tree_tc_d(int64_t head_dim, bool split, const CUtensorMap& tk, const CUtensorMap& tv,
+                             const TreeStreamParams& p, cudaStream_t s) {
+  if (head_dim == 64)
+    return split ? launch_tree_tc<64, FMT, true>(tk, tv, p, s) : launch_tree_tc<64, FMT, false>(tk, tv, p, s);
+  return split ? launch_tree_tc<128, FMT, true>(tk, tv, p, s) : launch_tree_tc<128, FMT, false>(tk, tv, p, s);
 }
 
 template <int FMT>
@@ -150,6 +176,15 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
   // tile line of 128-byte lines and the prefix of the batch have to fit.
   pl.stream = (d == 64 || d == 128 || d == 256) && c->batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
               product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
+  pl.tc = pl.stream && d <= 128 && nq >= kTcMinRows;
+  if (pl.tc) {
+    pl.passes = static_cast<int>(ceil_div(nq, 2 * kTtRows));
+    pl.rows_per_pass = static_cast<int>(ceil_div(nq, pl.passes));
+    pl.splits = 1;
+    pl.split_len = visible;
+    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * pl.rows_per_pass * (d * 4 + 8), 256);
+    return NVFP4DA_OK;
+  }
   if (pl.stream) {
     pl.wide = nq > 8 && d <= 128 ? 2 : 1;
     pl.row_chunks = 1;
@@ -363,6 +398,14 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
     t.grid = sm_count();
     t.part_o = static_cast<float*>(ws);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
+    if (pl.tc) {
+      const bool split = pl.rows_per_pass > kTtRows;
+      cudaError_t e = c->format == NVFP4DA_KV_BF16   ? launch_tree_tc_d<kKvFmtBf16>(c->head_dim, split, tk, tv, t, s)
+                      : c->format == NVFP4DA_KV_E4M3 ? launch_tree_tc_d<kKvFmtE4m3>(c->head_dim, split, tk, tv, t, s)
+                                                     : launch_tree_tc_d<kKvFmtNvfp4>(c->head_dim, split, tk, tv, t, s);
+      if (e != cudaSuccess) return cuda_fail(e, "tensor-core tree attention launch");
+      return NVFP4DA_OK;
+    }
     cudaError_t e = c->format == NVFP4DA_KV_BF16 ? launch_tree_stream_d<kKvFmtBf16>(c->head_dim, pl.wide, tk, tv, t, s)
                     : c->format == NVFP4DA_KV_E4M3
                         ? launch_tree_stream_d<kKvFmtE4m3>(c->head_dim, pl.wide, tk, tv, t, s)

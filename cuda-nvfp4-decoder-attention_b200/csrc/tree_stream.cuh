@@ -30,7 +30,7 @@
 // row is scaled by a power of two to FP16 (exact down to 2^-39 of its largest
 // element); the row scale of K multiplies the FP32 score.  P goes to FP16 as
 // p_j gamma_j / G 2^11, G the largest row scale of V that the query has seen so
-// far (>= 2^-126): 11 significant bits down to 2^-25 of the largest.  Over BF16 caches Q and V stay
+// far (>= 2^-100): 11 significant bits down to 2^-25 of the largest.  Over BF16 caches Q and V stay
 // BF16 and P is split into two BF16 terms.  The softmax runs in base 2; its
 // reference m moves only when a score passes m + 4 (p <= 16), so most slices
 // need neither a reduction nor a rescale.  m, l, o and all sums are FP32.
@@ -62,7 +62,7 @@ constexpr int kTsTile = 64;        // positions per stage
 constexpr int kTsMaxBatch = 1024;  // sequences whose prefix shared memory holds
 constexpr float kTsSlack = 4.0f;   // a score may pass the reference m by this (log2)
 constexpr float kTsPScale = 2048.0f;
-constexpr float kTsMinUnit = 1.17549435e-38f;  // 2^-126
+constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 
 template <int D, int FMT, int NG, int NW>
 struct TsCfg {
@@ -439,11 +439,11 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
 #pragma unroll
       for (int i = 0; i < KS; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.0f;
     }
-    float g_run[NG][2], p_unit[NG][2];  // G of the score columns, 2^11 / G (0: no row with a scale above 2^-126 yet)
+    float g_run[NG][2], p_unit[NG][2];  // G of the score columns, 2^11 / G
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       g_run[j][0] = g_run[j][1] = kTsMinUnit;
-      p_unit[j][0] = p_unit[j][1] = 0.0f;
+      p_unit[j][0] = p_unit[j][1] = kTsPScale / kTsMinUnit;
     }
 
     // One slice of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
