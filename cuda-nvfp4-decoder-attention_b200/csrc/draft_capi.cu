@@ -99,15 +99,22 @@ constexpr int64_t kTcMinRows = 17;  // query rows per KV head from which tree_tc
 
 template <int D>
 cudaError_t launch_tree_combine(const TreeStreamParams& p, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(p.batch * p.kv_heads * p.passes),
-                  static_cast<unsigned>(std::min(p.rows_per_pass, p.group * p.tokens)));
-  return launch(tree_stream_combine_kernel<D>, grid, dim3(128), 0, s, true, p);
+  const dim3 grid(static_cast<unsigned>(2 * p.grid),
+                  static_cast<unsigned>(ceil_div(std::min(p.rows_per_pass, p.group * p.tokens), kTsJoinWarps)));
+  return launch(tree_stream_combine_kernel<D>, grid, dim3(kTsJoinWarps * 32), 0, s, true, p);
 }
 
 template <int D, int FMT, bool SPLIT>
 cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p, cudaStream_t s) {
   auto* kern = tree_tc_kernel<D, FMT, SPLIT>;
   const uint32_t smem = TtCfg<D, FMT, SPLIT>::bytes(p.batch);
+  // The warps' register shares are drawn from what the block is launched with.
+  static const int regs = [&] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs * kTtThreads < (kTtSoftmaxRegs * kTtSoftmaxWarps + kTtOtherRegs * (kTtThreads / 32 - kTtSoftmaxWarps)) * 32)
+    return cudaErrorLaunchOutOfResources;
   cudaError_t e = ensure_smem(kern, smem);
   if (e != cudaSuccess) return e;
   kern<<<p.grid, kTtThreads, smem, s>>>(tk, tv, p);
@@ -182,7 +189,7 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
     pl.rows_per_pass = static_cast<int>(ceil_div(nq, pl.passes));
     pl.splits = 1;
     pl.split_len = visible;
-    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * pl.rows_per_pass * (d * 4 + 8), 256);
+    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * (pl.rows_per_pass * (d * 4 + 8) + 16), 256);
     return NVFP4DA_OK;
   }
   if (pl.stream) {
@@ -193,7 +200,7 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
     pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
     pl.splits = 1;
     pl.split_len = visible;
-    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * pl.rows_per_pass * (d * 4 + 8), 256);
+    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * (pl.rows_per_pass * (d * 4 + 8) + 16), 256);
     return NVFP4DA_OK;
   }
   const int64_t base = c->batch * c->kv_heads * ceil_div(group * tokens, kTreeWarps);
@@ -396,7 +403,8 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
     t.rows_per_pass = pl.rows_per_pass;
     t.passes = pl.passes;
     t.grid = sm_count();
-    t.part_o = static_cast<float*>(ws);
+    t.part_slots = static_cast<int4*>(ws);
+    t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
     if (pl.tc) {
       const bool split = pl.rows_per_pass > kTtRows;

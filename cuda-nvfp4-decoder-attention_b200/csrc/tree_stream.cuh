@@ -109,6 +109,7 @@ struct TreeStreamParams {
   int grid;            // CTAs of the streaming kernel
   float* part_o;       // [2 grid][RP][D]: slots 2 CTA (its first segment) and 2 CTA + 1 (its last)
   float2* part_ml;     // [2 grid][RP]
+  int4* part_slots;    // [2 grid]: see ts_write_slot
 };
 
 // ---------------------------------------------------------------- PTX
@@ -245,6 +246,17 @@ __device__ __forceinline__ int ts_cta_of(long long x, long long n, int g) {
   return static_cast<int>(((x + 1) * g - 1) / n);
 }
 
+// What a slot of partials holds: the unit and its CTAs, where the slot is the
+// first part of a unit that several CTAs share; unit -1 otherwise.
+__device__ __forceinline__ void ts_write_slot(const TreeStreamParams& p, long long n_tiles, int G, int cta, long long x0,
+                                              const TsWalk& w) {
+  const bool first = w.x == x0;
+  const bool starts = w.t0 == 0 && w.t1 < w.nt;  // the unit's first part, more to come
+  const int last = static_cast<int>(ts_cta_of(w.x - w.t0 + w.nt - 1, n_tiles, G));
+  p.part_slots[2 * cta + (first ? 0 : 1)] =
+      starts ? make_int4(w.b, w.u, cta, last) : make_int4(-1, 0, 0, 0);
+}
+
 // Element d of position r (in the tile) of V as the MMA saw it, before ts_finite.
 template <int D, int FMT>
 __device__ __forceinline__ float ts_v_element(const uint8_t* vt, const uint8_t* vb, int r, int d) {
@@ -267,7 +279,9 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
   constexpr int KS = D / 16;  // MMA steps of K Q^T, 16-element row blocks of O^T
   constexpr bool kQuant = FMT != kKvFmtBf16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // Pointer arithmetic, not an integer round trip: the compiler then knows that
+  // what it points to is shared memory.
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* so = reinterpret_cast<float*>(smem + Cfg::kOffComb);  // [warp][row][D]
   float* sm_m = reinterpret_cast<float*>(smem + Cfg::kOffMl);  // [warp][row]
   float* sm_l = sm_m + NW * Cfg::kRows;
@@ -317,8 +331,10 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
   // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
   // every CTA between a unit's first and last holds one of its tiles.
   const int G = n_tiles < p.grid ? static_cast<int>(n_tiles) : p.grid;
+  if (threadIdx.x < 2) p.part_slots[2 * cta + threadIdx.x] = make_int4(-1, 0, 0, 0);
   if (cta >= G) return;
   const long long x0 = n_tiles * cta / G, x1 = n_tiles * (cta + 1) / G;
+  __syncthreads();
 
   if (warp == NW) {
     // ---------------------------------------------------------------- producer
@@ -848,6 +864,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
     ts_bar_sync(NW * 32);
     const bool whole = w.t0 == 0 && w.t1 == w.nt;
     const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
+    if (!whole && threadIdx.x == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
     for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 32) {
       const int r = i / (D / 4), d = i % (D / 4) * 4, chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -878,78 +895,56 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
 }
 
 // ---------------------------------------------------------------- joining partials
-// Grid (unit, row of the pass): a block joins one query row of a unit that
-// several CTAs share, in CTA order; four warps take every fourth partial.
+// Grid (slot, group of rows): a warp joins one query row of a unit that several
+// CTAs share, in CTA order.  Only the slot of the unit's first part has work.
+constexpr int kTsJoinWarps = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) tree_stream_combine_kernel(const TreeStreamParams p) {
-  __shared__ long long red[2][4];
-  __shared__ float s_m[4], s_l[4];
-  __shared__ float s_o[4][D];
-  const int units = p.kv_heads * p.passes;
-  const int b = blockIdx.x / units, u = blockIdx.x % units, pass = u % p.passes, kvh = u / p.passes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = pass * p.rows_per_pass + blockIdx.y;
-  if (n >= p.group * p.tokens) return;
-  long long before = 0, all = 0;
-  for (int i = threadIdx.x; i < p.batch; i += 128) {
-    const long long t = (ts_visible(p, i) + kTsTile - 1) / kTsTile * units;
-    all += t;
-    if (i < b) before += t;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(kFull, before, o);
-    all += __shfl_xor_sync(kFull, all, o);
-  }
-  if (lane == 0) {
-    red[0][warp] = before;
-    red[1][warp] = all;
-  }
-  __syncthreads();
-  before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-  all = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  const long long nt = (ts_visible(p, b) + kTsTile - 1) / kTsTile;
-  const long long first = before + u * nt;
-  const int G = all < p.grid ? static_cast<int>(all) : p.grid;
-  const int c0 = ts_cta_of(first, all, G), c1 = ts_cta_of(first + nt - 1, all, G);
+__global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(const TreeStreamParams p) {
   pdl_wait();
-  if (c0 == c1) return;  // one CTA held the unit and wrote its result
-  constexpr int V = D / 32;  // elements per lane
-  const bool starts_c0 = all * c0 / G == first;  // the unit begins its first CTA's range
+  const int4 unit = __ldcg(&p.part_slots[blockIdx.x]);
+  if (unit.x < 0) return;
+  const int b = unit.x, u = unit.y, c0 = unit.z, c1 = unit.w;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * kTsJoinWarps + (threadIdx.x >> 5);
+  const int pass = u % p.passes, kvh = u / p.passes, n = pass * p.rows_per_pass + r;
+  if (r >= p.rows_per_pass || n >= p.group * p.tokens) return;
+  // The unit's part in its first CTA is in this slot, in the others in their first.
   auto at = [&](int c) {
-    return (2 * static_cast<int64_t>(c) + (c == c0 && !starts_c0 ? 1 : 0)) * p.rows_per_pass + blockIdx.y;
+    return (c == c0 ? static_cast<int64_t>(blockIdx.x) : 2 * static_cast<int64_t>(c)) * p.rows_per_pass + r;
   };
   float mx = -INFINITY;
-  for (int c = c0 + static_cast<int>(threadIdx.x); c <= c1; c += 128) mx = fmaxf(mx, __ldcg(&p.part_ml[at(c)]).x);
+  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[at(c)]).x);
   mx = warp_max_f32(mx);
-  if (lane == 0) s_m[warp] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  constexpr int V = D / 32;  // elements per lane
   float o[V] = {}, l = 0.0f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += 4) {
-    const float2 ml = __ldcg(&p.part_ml[at(c)]);
+  for (int base = c0; base <= c1; base += 32) {
+    const float2 ml = base + lane <= c1 ? __ldcg(&p.part_ml[at(base + lane)]) : make_float2(-INFINITY, 0.0f);
     const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(ml.x - mx);
     l = fmaf(ml.y, f, l);
-    const float* src = p.part_o + at(c) * D + lane * V;
+    const int count = min(32, c1 - base + 1);
+#pragma unroll 4
+    for (int c = 0; c < count; ++c) {
+      const float fc = __shfl_sync(kFull, f, c);
+      const float* src = p.part_o + at(base + c) * D + lane * V;
+      float x[V];
+      if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(src));
+      } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float x = __ldcg(src + i);
-      o[i] = f == 0.0f ? o[i] : fmaf(x, f, o[i]);
+        for (int i = 0; i < V / 4; ++i) reinterpret_cast<float4*>(x)[i] = __ldcg(reinterpret_cast<const float4*>(src) + i);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = fc == 0.0f ? o[i] : fmaf(x[i], fc, o[i]);
     }
   }
-  if (lane == 0) s_l[warp] = l;
-#pragma unroll
-  for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
-  __syncthreads();
-  l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  l = warp_sum_f32(l);
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
   const int64_t row = (static_cast<int64_t>(b) * p.tokens + n / p.group) * p.q_heads +
                       static_cast<int64_t>(kvh) * p.group + n % p.group;
-  for (int d = threadIdx.x; d < D; d += 128) {
-    const float x = s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d];
-    p.ctx[row * D + d] = f32_to_bf16_bits(l == 0.0f ? 0.0f : x * inv);
-  }
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.ctx + row * D + lane * V);
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i)
+    dst[i] = l == 0.0f ? 0u : ts_pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
 }
 
 }  // namespace nvfp4da

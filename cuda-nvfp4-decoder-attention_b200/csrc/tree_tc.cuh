@@ -15,8 +15,9 @@
 //   129 to 256 rows  each stream holds half of the rows and takes every tile.
 //
 // Roles: warps 0-3 and 4-7 softmax of streams 0 and 1 (one query row per
-// thread); warps 8-13 prepare operands; warp 14 issues the MMAs; warp 15 the
-// loads.  Per tile of 64 keys:
+// thread); warps 8-15 prepare operands; warps 16 and 18 issue the MMAs of a
+// stream each (one warp for both could not issue them fast enough beside the
+// others on its scheduler); warp 17 the loads.  Per tile of 64 keys:
 //   load     codes and scales (TMA, bulk copies) into a ring; BF16 K and V
 //            straight into operand tiles;
 //   prepare  codes (times the NVFP4 block scale) to FP16, exact, as [key][d]
@@ -25,11 +26,15 @@
 //            V rows past the end and infinities or NaN in V become 0;
 //   S = Q K^T   M 128, N 64, into one of the stream's two score buffers;
 //   softmax  scores times the row scale of K (FP32), mask, P = 2^(s - m) times
-//            the row scale of V over G, to FP16 (BF16 caches: two BF16 terms);
-//            the reference m and the scale G move only when passed by a slack
-//            of 2^4 and 2^3, and only then the accumulator is rescaled;
-//   O += P V  M 128, N = D, accumulated in tensor memory.
-// The numerics are those of tree_stream.cuh (P 2^7 p_j gamma_j / G here).
+//            the row scale of V over G, to FP16 (BF16 caches: two BF16 terms),
+//            written over the scores in tensor memory; the reference m and the
+//            scale G move only when passed by a slack of 2^4 and 2^3, and only
+//            then the accumulator is rescaled;
+//   O += P V  M 128, N = D, P read from tensor memory, accumulated there.
+// Shared memory feeds the MMAs, so P stays out of it: with P as a
+// shared-memory operand its reads and writes took a third of the bandwidth and
+// the kernel 1.6 times as long.
+// The numerics are those of tree_stream.cuh (P is 2^7 p_j gamma_j / G here).
 //
 // Waits are bounded (one second, shared give-up flag, recorded in
 // g_tree_errors); tensor memory is freed on every path.
@@ -42,8 +47,12 @@ namespace nvfp4da {
 constexpr int kTtRows = 128;
 constexpr int kTtKeys = 64;
 constexpr int kTtSoftmaxWarps = 8;
-constexpr int kTtPrepWarps = 6;
-constexpr int kTtThreads = (kTtSoftmaxWarps + kTtPrepWarps + 2) * 32;
+constexpr int kTtPrepWarps = 8;
+constexpr int kTtMmaWarp = kTtSoftmaxWarps + kTtPrepWarps, kTtLoadWarp = kTtMmaWarp + 1;
+constexpr int kTtThreads = (kTtSoftmaxWarps + kTtPrepWarps + 4) * 32;  // whole warpgroups; warp 19 idles
+// Registers: 96 a thread at launch (640 threads); the softmax warps take what
+// the others give: 256 * 144 + 384 * 64 = 640 * 96.
+constexpr int kTtSoftmaxRegs = 144, kTtOtherRegs = 64;
 constexpr int kTtUnitSlots = 8;  // tiles whose row scales are kept
 constexpr float kTtPScale = 128.0f;
 constexpr float kTtUnitSlack = 8.0f;
@@ -55,19 +64,19 @@ struct TtCfg {
   static constexpr bool kQuant = FMT != kKvFmtBf16;
   static constexpr int kPanels = D / 64;                      // 64-element panels of a row
   static constexpr uint32_t kOperand = kPanels * kTtKeys * 128;  // a K or V tile, 16-bit
-  static constexpr int kK = kQuant ? 2 : 3, kV = SPLIT ? 2 : 3;  // tiles of each in flight
+  static constexpr int kK = kQuant ? (SPLIT ? 2 : 3) : 4;   // K and V tiles in flight
+  static constexpr int kV = kQuant ? 3 : 4;
   static constexpr int kStages = kQuant ? (FMT == kKvFmtNvfp4 ? 4 : 3) : 0;  // ring of codes
   static constexpr int kQRows = SPLIT ? 256 : 192;
   static constexpr uint32_t kQPanel = kQRows * 128;
-  static constexpr int kTerms = kQuant ? 1 : 2;
-  static constexpr uint32_t kP = kTerms * kTtRows * 128;  // per stream
   static constexpr uint32_t kOffK = 0, kOffV = kOffK + kK * kOperand, kOffRing = kOffV + kV * kOperand,
-                            kOffQ = kOffRing + kStages * Codes::kStage, kOffP = kOffQ + kPanels * kQPanel,
-                            kOffUnits = kOffP + 2 * kP;
-  static constexpr uint32_t kUnits = kQuant ? kTtUnitSlots * kTtKeys * 8 : 0;
+                            kOffQ = kOffRing + kStages * Codes::kStage, kOffUnits = kOffQ + kPanels * kQPanel;
+  // Row scales of a tile's keys: K (times log2(e) / sqrt(D)), V, and V's largest finite one.
+  static constexpr uint32_t kUnitFloats = 2 * kTtKeys + 4;
+  static constexpr uint32_t kUnits = kQuant ? kTtUnitSlots * kUnitFloats * 4 : 0;
   static constexpr uint32_t kOffPrefix = kOffUnits + kUnits;
-  // The joining area (stream 1's o) overlays Q and P.
-  static_assert(kPanels * kQPanel + 2 * kP >= kTtRows * D * 4, "room to join the streams");
+  // Stream 1's o of up to 64 rows overlays Q when the streams are joined.
+  static_assert(kPanels * kQPanel >= 64u * D * 4, "room to join the streams");
   static constexpr uint32_t bytes(int batch) { return kOffPrefix + 8u * (batch + 1) + 1024; }
 };
 
@@ -77,9 +86,10 @@ struct TtCfg {
 // (46), swizzle mode 2 (61-63).  K-major: stride = 1024 between 8-row groups.
 // MN-major: stride = 1024 between groups of 8 k, leading = the distance between
 // 64-element panels.
-__device__ __forceinline__ uint64_t tt_desc(uint32_t saddr, uint32_t leading) {
-  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(leading >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+// Only the start address varies: the low words are added up in 32 bits.
+constexpr uint32_t kTtDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t tt_desc_low(uint32_t saddr, uint32_t leading) {
+  return ((saddr & 0x3FFFFu) >> 4) | ((leading >> 4) << 16);
 }
 // Instruction descriptor, kind::f16: FP32 D, A and B FP16 or BF16, A K-major,
 // B K-major or MN-major (bit 16), N >> 3 at 17, M >> 4 at 24.
@@ -89,13 +99,28 @@ __host__ __device__ constexpr uint32_t tt_idesc(int n, bool mn_major) {
   return (1u << 4) | (type << 7) | (type << 10) | (mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(kTtRows >> 4) << 24);
 }
-__device__ __forceinline__ void tt_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+__device__ __forceinline__ void tt_mma(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc,
                                        uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}" ::"r"(tmem_d),
+      "r"(a_low), "r"(b_low), "r"(kTtDescHigh), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// The same with A in tensor memory.
+__device__ __forceinline__ void tt_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_low, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_low), "r"(kTtDescHigh), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool tt_elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
 }
 __device__ __forceinline__ void tt_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -104,37 +129,76 @@ __device__ __forceinline__ void tt_commit(uint64_t* bar) {
 __device__ __forceinline__ void tt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tt_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tt_ld32(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 columns of this warp's lanes, without waiting for them.
+__device__ __forceinline__ void tt_ld32_async(uint32_t taddr, float* v) {
   __syncwarp();
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tt_st32(uint32_t taddr, const float (&v)[32]) {
+__device__ __forceinline__ void tt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// After tt_wait_ld: nothing may use v[0 .. N) earlier.
+template <int N>
+__device__ __forceinline__ void tt_loaded(float* v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void tt_ld32(uint32_t taddr, float (&v)[32]) {
+  tt_ld32_async(taddr, v);
+  tt_wait_ld();
+  tt_loaded<32>(v);
+}
+__device__ __forceinline__ void tt_ld16(uint32_t taddr, float (&v)[16]) {
   __syncwarp();
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
-      "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
-      "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
-      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])),
-      "r"(__float_as_uint(v[15])), "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])),
-      "r"(__float_as_uint(v[18])), "r"(__float_as_uint(v[19])), "r"(__float_as_uint(v[20])),
-      "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])), "r"(__float_as_uint(v[23])),
-      "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])),
-      "r"(__float_as_uint(v[27])), "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])),
-      "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr));
+  tt_wait_ld();
+  tt_loaded<16>(v);
+}
+__device__ __forceinline__ void tt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  __syncwarp();
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+// Column of P, in its score buffer, of the MMA step of keys 16 ks ..: FP16
+// pairs, or per 32 keys the first BF16 terms and then the second (the scores of
+// the other 32 keys stay whole until they are read).
+template <int FMT>
+__host__ __device__ constexpr uint32_t tt_p_col(int ks) {
+  return FMT == kKvFmtBf16 ? (ks >> 1) * 32 + (ks & 1) * 8 : ks * 8;
+}
+// Two FP32 operations in one instruction.
+__device__ __forceinline__ float2 tt_mul2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}" : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 tt_add2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}" : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 tt_fma2(float2 a, float2 b, float2 d) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 w, {%6, %7};\n"
+      " fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(d.x), "f"(d.y));
+  return c;
 }
 
 // Bounded wait; gives up when another role has (`bad`) or after one second.
@@ -190,15 +254,17 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   using Codes = typename C::Codes;
   constexpr bool kQuant = C::kQuant;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t ring_full[4], ring_free[4], k_full[3], k_free[3], v_raw[3], v_full[3], v_free[3], q_full,
-      s_full[2][2], s_free[2][2], p_full[2], o_done[2], seg_done, join_ready, join_read;
+  // Pointer arithmetic, not an integer round trip: the compiler then knows that
+  // what it points to is shared memory.
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  __shared__ uint64_t ring_full[4], ring_free[4], k_full[4], k_free[4], v_raw[4], v_full[4], v_free[4], q_full,
+      s_full[2][2], p_full[2][2], o_done[2], o_end[2], seg_done, join_ready, join_read;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile unsigned s_bad;    // a wait gave up
   __shared__ volatile unsigned s_wild;   // an infinity or NaN was taken out of V
-  __shared__ float2 join_ml[kTtRows];
+  __shared__ float4 join[kTtRows];       // stream 1's m, l and the unit of its o
   long long* prefix = reinterpret_cast<long long*>(smem + C::kOffPrefix);
-  float2* units_kv = reinterpret_cast<float2*>(smem + C::kOffUnits);  // [slot][key]: row scales of K (scaled) and V
+  float* units_kv = reinterpret_cast<float*>(smem + C::kOffUnits);  // [slot][kUnitFloats]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
@@ -206,7 +272,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const int nq = p.group * p.tokens;
 
   pdl_launch_dependents();
-  if (warp == 14) {
+  if (warp == kTtMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                  "r"(512)
                  : "memory");
@@ -216,22 +282,20 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(&ring_full[i], 1);
       mbar_init(&ring_free[i], kTtPrepWarps);
-    }
-    for (int i = 0; i < 3; ++i) {
       mbar_init(&k_full[i], kQuant ? kTtPrepWarps : 1);
-      mbar_init(&k_free[i], 1);
+      mbar_init(&k_free[i], SPLIT ? 2 : 1);  // each stream that reads the tile
       mbar_init(&v_raw[i], 1);
       mbar_init(&v_full[i], kTtPrepWarps);
-      mbar_init(&v_free[i], 1);
+      mbar_init(&v_free[i], SPLIT ? 2 : 1);
     }
     mbar_init(&q_full, kTtSoftmaxWarps);
     for (int s = 0; s < 2; ++s) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[s][i], 1);
-        mbar_init(&s_free[s][i], 4);
+        mbar_init(&p_full[s][i], 4);  // per buffer: a warp may be one job ahead of another
       }
-      mbar_init(&p_full[s], 4);
       mbar_init(&o_done[s], 1);
+      mbar_init(&o_end[s], 1);
     }
     mbar_init(&seg_done, kTtSoftmaxWarps);
     mbar_init(&join_ready, kTtSoftmaxWarps);
@@ -259,6 +323,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     }
     if (lane == 0) prefix[0] = 0;
   }
+  if (tid < 2) p.part_slots[2 * cta + tid] = make_int4(-1, 0, 0, 0);
   __syncthreads();
   const uint32_t tmem = tmem_slot;
   const long long n_tiles = prefix[p.batch];
@@ -270,7 +335,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   auto s_col = [&](int s, int buf) { return tmem + static_cast<uint32_t>((2 * s + buf) * kTtKeys); };
   auto o_col = [&](int s) { return tmem + 256u + static_cast<uint32_t>(s * D); };
 
-  if (warp == 15) {
+  if (warp >= kTtSoftmaxWarps) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtOtherRegs));
+  if (warp == kTtLoadWarp) {
     // ---------------------------------------------------------------- loads
     if (lane == 0) {
       TtRing<kQuant ? (C::kStages ? C::kStages : 1) : C::kK> rk;
@@ -316,75 +383,91 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 14) {
-    // ---------------------------------------------------------------- MMAs
-    if (lane == 0) {
-      constexpr uint32_t kIdescS = tt_idesc<FMT>(kTtKeys, false), kIdescO = tt_idesc<FMT>(D, true);
-      TtRing<C::kK> rk;
-      TtRing<C::kV> rv;
-      uint32_t q_phase = 0, s_count[2] = {0, 0}, p_count[2] = {0, 0};
-      bool ok = true;
-      for (; more && ok; more = w.next()) {
-        const int tiles = w.t1 - w.t0, jobs = SPLIT ? 2 * tiles : tiles;
-        const int rows = min(p.rows_per_pass, nq - (w.u % p.passes) * p.rows_per_pass);
-        const bool shifted = !SPLIT && rows <= 64;
-        ok = tt_wait(&q_full, q_phase, &s_bad);
-        q_phase ^= 1u;
-        bool begun[2] = {false, false};
-        for (int k = 0; k < jobs + 2 && ok; ++k) {
-          if (k < jobs) {
-            const int s = k & 1, buf = s_count[s] & 1;
-            const bool last_use = !SPLIT || s == 1;
-            ok = tt_wait(&k_full[rk.i], rk.phase, &s_bad) &&
-                 tt_wait(&s_free[s][buf], ((s_count[s] >> 1) & 1) ^ 1u, &s_bad);
-            if (!ok) break;
-            tt_fence_after();
-            // query rows of this stream in the Q tile
-            const int q0 = SPLIT ? s * kTtRows : (shifted && s == 0 ? 64 : 0);
+  } else if (warp == kTtMmaWarp || warp == kTtMmaWarp + 2) {
+    // ---------------------------------------------------------------- MMAs, a warp per stream
+    // The whole warp walks the line, one lane issues.  The stream's P takes the
+    // place of its scores: the scores of job n + 2 go into the buffer that held
+    // P of job n, after that job's P V in issue order.
+    constexpr uint32_t kIdescS = tt_idesc<FMT>(kTtKeys, false), kIdescO = tt_idesc<FMT>(D, true);
+    const int s = (warp - kTtMmaWarp) / 2;
+    const bool issuer = tt_elect();
+    const uint32_t base = smem_u32(smem), o_at = o_col(s);
+    TtRing<C::kK> rk;
+    TtRing<C::kV> rv;
+    uint32_t q_phase = 0, nth = 0, nth_s = 0;  // P V and scores issued, over all segments
+    bool ok = true;
+    for (; more && ok; more = w.next()) {
+      const int tiles = w.t1 - w.t0;
+      const int rows = min(p.rows_per_pass, nq - (w.u % p.passes) * p.rows_per_pass);
+      const bool shifted = !SPLIT && rows <= 64;
+      // query rows of this stream in the Q tile
+      const uint32_t q0 = SPLIT ? s * kTtRows : (shifted && s == 0 ? 64 : 0);
+      const uint32_t qa = tt_desc_low(base + C::kOffQ + q0 * 128, 16);
+      ok = __all_sync(kFull, tt_wait(&q_full, q_phase, &s_bad));
+      q_phase ^= 1u;
+      auto scores = [&] {
+        ok = __all_sync(kFull, tt_wait(&k_full[rk.i], rk.phase, &s_bad));
+        if (!ok) return;
+        tt_fence_after();
+        const uint32_t ka = tt_desc_low(base + C::kOffK + rk.i * C::kOperand, 16);
+        const uint32_t d = s_col(s, nth_s & 1);
+        if (issuer) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t qa = smem_u32(smem + C::kOffQ + (ks >> 2) * C::kQPanel + q0 * 128) + (ks & 3) * 32;
-              const uint32_t ka = smem_u32(smem + C::kOffK + rk.i * C::kOperand + (ks >> 2) * (kTtKeys * 128)) + (ks & 3) * 32;
-              tt_mma(s_col(s, buf), tt_desc(qa, 16), tt_desc(ka, 16), kIdescS, ks ? 1u : 0u);
-            }
-            tt_commit(&s_full[s][buf]);
-            ++s_count[s];
-            if (last_use) {
-              tt_commit(&k_free[rk.i]);
-              rk.next();
-            }
-          }
-          if (k >= 2) {
-            const int s = k & 1;
-            const bool last_use = !SPLIT || s == 1;
-            ok = tt_wait(&p_full[s], p_count[s] & 1, &s_bad) && tt_wait(&v_full[rv.i], rv.phase, &s_bad);
-            if (!ok) break;
-            tt_fence_after();
+          for (int ks = 0; ks < D / 16; ++ks)
+            tt_mma(d, qa + ((ks >> 2) * C::kQPanel + (ks & 3) * 32) / 16,
+                   ka + ((ks >> 2) * (kTtKeys * 128) + (ks & 3) * 32) / 16, kIdescS, ks ? 1u : 0u);
+          tt_commit(&s_full[s][nth_s & 1]);
+          tt_commit(&k_free[rk.i]);
+        }
+        __syncwarp();
+        ++nth_s;
+      };
+      // Tiles in order; without SPLIT every other one is this stream's.
+      int next_s = 0;  // tile whose scores come next
+      auto advance_scores = [&] {
+        while (next_s < tiles) {
+          const bool mine = SPLIT || (next_s & 1) == s;
+          if (mine) scores();
+          rk.next();
+          ++next_s;
+          if (mine) break;
+        }
+      };
+      advance_scores();
+      if (ok) advance_scores();
+      for (int t = 0; t < tiles && ok; ++t) {
+        if (SPLIT || (t & 1) == s) {
+          ok = tt_wait(&p_full[s][nth & 1], (nth >> 1) & 1, &s_bad) && tt_wait(&v_full[rv.i], rv.phase, &s_bad);
+          if (!(ok = __all_sync(kFull, ok))) break;
+          tt_fence_after();
+          const uint32_t va = tt_desc_low(base + C::kOffV + rv.i * C::kOperand, kTtKeys * 128);
+          const uint32_t pa = s_col(s, nth & 1);
+          const uint32_t begun = t >= (SPLIT ? 1 : 2) ? 1u : 0u;  // not the stream's first tile of the segment
+          if (issuer) {
 #pragma unroll
             for (int ks = 0; ks < kTtKeys / 16; ++ks) {
-              const uint32_t va = smem_u32(smem + C::kOffV + rv.i * C::kOperand) + ks * 2048;
-#pragma unroll
-              for (int term = 0; term < C::kTerms; ++term) {
-                const uint32_t pa = smem_u32(smem + C::kOffP + s * C::kP + term * (kTtRows * 128)) + ks * 32;
-                tt_mma(o_col(s), tt_desc(pa, 16), tt_desc(va, kTtKeys * 128), kIdescO,
-                       (begun[s] || ks || term) ? 1u : 0u);
-              }
+              tt_mma_ts(o_at, pa + tt_p_col<FMT>(ks), va + ks * 2048 / 16, kIdescO, ks ? 1u : begun);
+              if constexpr (!kQuant) tt_mma_ts(o_at, pa + tt_p_col<FMT>(ks) + 16, va + ks * 2048 / 16, kIdescO, 1u);
             }
-            begun[s] = true;
             tt_commit(&o_done[s]);
-            ++p_count[s];
-            if (last_use) {
-              tt_commit(&v_free[rv.i]);
-              rv.next();
-            }
+            tt_commit(&v_free[rv.i]);
           }
+          __syncwarp();
+          ++nth;
+          advance_scores();
         }
+        rv.next();
       }
+      while (next_s < tiles) {  // the other stream's last tile
+        rk.next();
+        ++next_s;
+      }
+      if (ok && issuer) tt_commit(&o_end[s]);
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp >= kTtSoftmaxWarps) {
+  } else if (warp >= kTtSoftmaxWarps && warp < kTtMmaWarp) {
     // ---------------------------------------------------------------- operands
-    const int pt = tid - kTtSoftmaxWarps * 32;  // 0 .. 191
+    const int pt = tid - kTtSoftmaxWarps * 32;  // 0 .. 255
     constexpr int kN = kTtPrepWarps * 32;
     TtRing<C::kStages ? C::kStages : 1> rr;
     TtRing<C::kK> rk;
@@ -399,68 +482,93 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         const bool edge = key0 + kTtKeys > past;
         const int live = static_cast<int>(min(static_cast<int64_t>(kTtKeys), vis - key0));  // keys before the end
         if constexpr (kQuant) {
-          ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad) && tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+          // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16), eight keys side by side;
+          // K's and V's are read together, before either is converted.
+          constexpr int kItems = Codes::kRowBytes / 16;
+          constexpr int kRounds = (kTtKeys * kItems + kN - 1) / kN;
+          ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad);
           if (!(ok = __all_sync(kFull, ok))) break;
           const uint8_t* st = smem + C::kOffRing + rr.i * Codes::kStage;
-          if (pt < kTtKeys) {
-            const float kr = reinterpret_cast<const float*>(st + Codes::kOffKr)[pt];
-            const float vr = reinterpret_cast<const float*>(st + Codes::kOffVr)[pt];
-            units_kv[slot * kTtKeys + pt] = make_float2(kr * p.scale_log2, vr);
+          uint4 raw[2][kRounds];
+          [[maybe_unused]] uint32_t scales[2][kRounds];
+#pragma unroll
+          for (int x = 0; x < kRounds; ++x) {
+            const int i = pt + x * kN, c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
+            if (i < kTtKeys * kItems) {
+              const uint32_t at = ts_swz(r * Codes::kRowBytes + 16 * c);
+              raw[0][x] = *reinterpret_cast<const uint4*>(st + at);
+              raw[1][x] = *reinterpret_cast<const uint4*>(st + Codes::kOffV + at);
+              if constexpr (FMT == kKvFmtNvfp4) {
+                scales[0][x] = *reinterpret_cast<const uint16_t*>(st + Codes::kOffKb + r * (D / 16) + 2 * c);
+                scales[1][x] = *reinterpret_cast<const uint16_t*>(st + Codes::kOffVb + r * (D / 16) + 2 * c);
+              }
+            }
+          }
+          if (warp == kTtSoftmaxWarps) {  // the first of these warps: the row scales
+            float* un = units_kv + slot * C::kUnitFloats;
+            const float2 kr = reinterpret_cast<const float2*>(st + Codes::kOffKr)[lane];
+            const float2 vr = reinterpret_cast<const float2*>(st + Codes::kOffVr)[lane];
+            reinterpret_cast<float2*>(un)[lane] = make_float2(kr.x * p.scale_log2, kr.y * p.scale_log2);
+            reinterpret_cast<float2*>(un + kTtKeys)[lane] = vr;
+            const float top = warp_max_f32(fmaxf(vr.x < INFINITY ? vr.x : 0.0f, vr.y < INFINITY ? vr.y : 0.0f));
+            if (lane == 0) un[2 * kTtKeys] = top;
           }
           slot = slot + 1 == kTtUnitSlots ? 0 : slot + 1;
-          // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16), eight keys side by side.
-          constexpr int kItems = Codes::kRowBytes / 16;
-          auto prepare = [&](const uint8_t* codes, const uint8_t* blocks, uint8_t* out, bool clean) {
-            for (int i = pt; i < kTtKeys * kItems; i += kN) {
-              const int c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
-              const uint4 raw = *reinterpret_cast<const uint4*>(codes + ts_swz(r * Codes::kRowBytes + 16 * c));
-              const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
-              uint32_t h[FMT == kKvFmtNvfp4 ? 16 : 8];
+          __syncwarp();
+          if (lane == 0) ts_arrive(&ring_free[rr.i]);
+          rr.next();
+          auto prepare = [&](int which, uint8_t* out, bool clean) {
+#pragma unroll
+            for (int x = 0; x < kRounds; ++x) {
+              const int i = pt + x * kN, c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
+              if (i >= kTtKeys * kItems) break;
+              const uint32_t word[4] = {raw[which][x].x, raw[which][x].y, raw[which][x].z, raw[which][x].w};
+              uint32_t b0 = 0, b1 = 0;
               if constexpr (FMT == kKvFmtNvfp4) {
-                const uint32_t two = *reinterpret_cast<const uint16_t*>(blocks + r * (D / 16) + 2 * c);
-                const uint32_t b0 = e4m3x2_to_f16x2((two & 0xffu) * 0x101u), b1 = e4m3x2_to_f16x2((two >> 8) * 0x101u);
+                const uint32_t both = e4m3x2_to_f16x2(scales[which][x]);
+                b0 = __byte_perm(both, both, 0x1010);
+                b1 = __byte_perm(both, both, 0x3232);
+              }
+              // 16-byte chunks of 8 elements
+              constexpr int kChunks = FMT == kKvFmtNvfp4 ? 4 : 2;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  uint32_t d[4];
-                  e2m1x8_to_f16x2x4(word[e], d);
+              for (int y = 0; y < kChunks; ++y) {
+                uint32_t h[4];
+                if constexpr (FMT == kKvFmtNvfp4) {
+                  e2m1x8_to_f16x2x4(word[y], h);
 #pragma unroll
-                  for (int x = 0; x < 4; ++x) h[4 * e + x] = ts_hmul2(d[x], e < 2 ? b0 : b1);
+                  for (int z = 0; z < 4; ++z) h[z] = ts_hmul2(h[z], y < 2 ? b0 : b1);
+                } else {
+                  ts_e4m3x4(word[2 * y], h[0], h[1]);
+                  ts_e4m3x4(word[2 * y + 1], h[2], h[3]);
                 }
-              } else {
+                if (clean) {
+                  uint32_t bad = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ts_e4m3x4(word[e], h[2 * e], h[2 * e + 1]);
-              }
-              constexpr int kChunks = FMT == kKvFmtNvfp4 ? 4 : 2;  // 8 elements each
-              if (clean) {
-                uint32_t bad = 0;
-#pragma unroll
-                for (int x = 0; x < 4 * kChunks; ++x) h[x] = r < live ? ts_finite<FMT>(h[x], bad) : 0u;
-                if (bad) s_wild = 1u;
-              }
-#pragma unroll
-              for (int x = 0; x < kChunks; ++x) {
-                const int ch = c * kChunks + x;  // chunk of the whole row
+                  for (int z = 0; z < 4; ++z) h[z] = r < live ? ts_finite<FMT>(h[z], bad) : 0u;
+                  if (bad) s_wild = 1u;
+                }
+                const int ch = c * kChunks + y;  // chunk of the whole row
                 *reinterpret_cast<uint4*>(out + (ch >> 3) * (kTtKeys * 128) + tt_chunk(r, ch & 7)) =
-                    make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
+                    make_uint4(h[0], h[1], h[2], h[3]);
               }
             }
           };
-          prepare(st, st + Codes::kOffKb, smem + C::kOffK + rk.i * C::kOperand, false);
+          ok = tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+          if (!(ok = __all_sync(kFull, ok))) break;
+          prepare(0, smem + C::kOffK + rk.i * C::kOperand, false);
           tt_fence_async();
           __syncwarp();
           if (lane == 0) ts_arrive(&k_full[rk.i]);
           rk.next();
           ok = tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad);
           if (!(ok = __all_sync(kFull, ok))) break;
-          prepare(st + Codes::kOffV, st + Codes::kOffVb, smem + C::kOffV + rv.i * C::kOperand, edge);
+          if (edge) prepare(1, smem + C::kOffV + rv.i * C::kOperand, true);
+          else prepare(1, smem + C::kOffV + rv.i * C::kOperand, false);
           tt_fence_async();
           __syncwarp();
-          if (lane == 0) {
-            ts_arrive(&v_full[rv.i]);
-            ts_arrive(&ring_free[rr.i]);
-          }
+          if (lane == 0) ts_arrive(&v_full[rv.i]);
           rv.next();
-          rr.next();
         } else {
           ok = tt_wait(&v_raw[rv.i], rv.phase, &s_bad);
           if (!(ok = __all_sync(kFull, ok))) break;
@@ -490,11 +598,13 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         }
       }
     }
+  }
   } else {
     // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTtSoftmaxRegs));
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;  // stream, row of its tile
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    uint32_t s_count = 0, o_phase = 0, end_phase = 0;
+    uint32_t s_count = 0, o_count = 0, end_phase = 0, o_end_phase = 0;  // scores seen, P tiles given, segments ended
     bool first_segment = true;
     int slot0 = 0;  // unit slot of the segment's first tile
     bool ok = true;
@@ -557,7 +667,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 
       float m = -INFINITY, l = 0.0f, g_run = kTsMinUnit, p_unit = kTtPScale / kTsMinUnit;
       const uint8_t* mask_row = p.mask ? p.mask + b * p.mask_stride + static_cast<int64_t>(tok) * p.tokens : nullptr;
-      uint8_t* pt_base = smem + C::kOffP + s * C::kP;
       int done = 0;  // jobs of this stream in the segment
       for (int i = SPLIT ? 0 : s; i < tiles && ok; i += SPLIT ? 1 : 2, ++done) {
         const int buf = s_count & 1;
@@ -566,204 +675,219 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         if (!(ok = __all_sync(kFull, ok))) break;
         tt_fence_after();
         ++s_count;
-        const float2* unit = units_kv + ((slot0 + i) & (kTtUnitSlots - 1)) * kTtKeys;
+        const uint32_t s_at = s_col(s, buf) + lanes;
+        const float* unit = units_kv + ((slot0 + i) & (kTtUnitSlots - 1)) * C::kUnitFloats;
         auto tile = [&](auto edge_tag) {
           constexpr bool EDGE = decltype(edge_tag)::value;
           // Keys of the tile this row sees, one bit each.
-          unsigned long long seen = ~0ull;
+          [[maybe_unused]] unsigned long long seen = ~0ull;
           if constexpr (EDGE) {
-            seen = 0;
-            for (int e = 0; e < kTtKeys; ++e) {
-              const int64_t pos = key0 + e;
-              if (has && pos < vis && tree_sees(mask_row, tok, pos - past)) seen |= 1ull << e;
-            }
+            const int64_t old = past - key0;  // committed keys of the tile
+            seen = old <= 0 ? 0ull : (1ull << old) - 1;  // fewer than 64 in such a tile
+            const int64_t first = max(past, key0), last = min(vis, key0 + kTtKeys);
+            if (has)
+              for (int64_t pos = first; pos < last; ++pos)
+                if (tree_sees(mask_row, tok, pos - past)) seen |= 1ull << (pos - key0);
           }
-          // ---- maxima: scores (in units of own) and row scales of V
-          float mx = -INFINITY;
-          [[maybe_unused]] float vx = 0.0f;
+          // 32 scores in units of own; unseen keys -inf.
+          auto scores = [&](int h, float (&x)[32]) {
+            tt_ld32(s_at + 32 * h, x);
+            if constexpr (kQuant) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 u = *reinterpret_cast<const float4*>(unit + 32 * h + e);
+                const float2 a = tt_mul2(make_float2(x[e], x[e + 1]), make_float2(u.x, u.y));
+                const float2 c = tt_mul2(make_float2(x[e + 2], x[e + 3]), make_float2(u.z, u.w));
+                x[e] = a.x;
+                x[e + 1] = a.y;
+                x[e + 2] = c.x;
+                x[e + 3] = c.y;
+              }
+            }
+            if constexpr (EDGE) {
+              const uint32_t bits = static_cast<uint32_t>(seen >> (32 * h));
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1)) x[e] = -INFINITY;
+            }
+          };
+          float f = 1.0f;  // what the accumulator is to be scaled by
           if (warp_has) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float x[32];
-              tt_ld32(s_col(s, buf) + lanes + 32 * h, x);
+              scores(h, x);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const bool sees = !EDGE || ((seen >> (32 * h + e)) & 1);
-                if constexpr (kQuant) {
-                  const float2 uu = unit[32 * h + e];
-                  x[e] *= uu.x;
-                  if (sees && uu.y < INFINITY) vx = fmaxf(vx, uu.y);
+              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+            }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * own;
+            if (has && top > m + kTsSlack) {
+              f = m == -INFINITY ? 0.0f : ts_exp2(m - top);
+              l *= f;
+              m = top;
+            }
+            if constexpr (kQuant) {
+              float vx = unit[2 * kTtKeys];
+              if constexpr (EDGE) {
+                vx = 0.0f;
+#pragma unroll 1
+                for (int e = 0; e < kTtKeys; ++e) {
+                  const float u = unit[kTtKeys + e];
+                  if (((seen >> e) & 1) && u < INFINITY) vx = fmaxf(vx, u);
                 }
-                if (sees) mx = fmaxf(mx, x[e]);
+              }
+              if (has && vx > g_run * kTtUnitSlack) {
+                f *= __fdiv_rn(g_run, vx);
+                g_run = vx;
+                p_unit = __fdiv_rn(kTtPScale, vx);
               }
             }
           }
-          mx *= own;
-          float f = 1.0f;  // what the accumulator is to be scaled by
-          if (has && mx > m + kTsSlack) {
-            f = m == -INFINITY ? 0.0f : ts_exp2(m - mx);
-            l *= f;
-            m = mx;
-          }
-          if constexpr (kQuant) {
-            if (has && vx > g_run * kTtUnitSlack) {
-              f *= __fdiv_rn(g_run, vx);
-              g_run = vx;
-              p_unit = __fdiv_rn(kTtPScale, vx);
-            }
-          }
-          // ---- P V of the tile before is done: its P tile is free, its accumulator settled
-          if (done > 0) {
-            ok = tt_wait(&o_done[s], o_phase, &s_bad);
-            o_phase ^= 1u;
+          // ---- the accumulator, once P V of the tile before is done
+          if (done > 0 && __any_sync(kFull, f != 1.0f)) {
+            // The scores of this job were issued after the P V of the job before last: one phase is in question.
+            ok = tt_wait(&o_done[s], (o_count - 1) & 1, &s_bad);
             if (!(ok = __all_sync(kFull, ok))) return;
             tt_fence_after();
-            if (__any_sync(kFull, f != 1.0f)) {
 #pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                float o[32];
-                tt_ld32(o_col(s) + lanes + c, o);
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tt_ld16(o_col(s) + lanes + c, o);
+              uint32_t y[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= f;
-                tt_st32(o_col(s) + lanes + c, o);
-              }
-              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(o[e] * f);
+              tt_st16(o_col(s) + lanes + c, y);
             }
           }
-          // ---- P
+          // ---- P over the scores; scores of -inf (unseen among them) weigh 0 against the finite m_ref
           if (warp_has) {
-            float sum = 0.0f;
+            const float m_ref = m == -INFINITY ? 0.0f : m;
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float x[32];
-              tt_ld32(s_col(s, buf) + lanes + 32 * h, x);
+              scores(h, x);
+              uint32_t out[16];
+              [[maybe_unused]] uint32_t out2[16];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                [[maybe_unused]] float2 uu = make_float2(1.0f, 1.0f);
+              for (int e = 0; e < 32; e += 2) {
+                float2 y = tt_fma2(make_float2(x[e], x[e + 1]), make_float2(own, own), make_float2(-m_ref, -m_ref));
+                y.x = ts_exp2(y.x);
+                y.y = ts_exp2(y.y);
+                sum[(e >> 1) & 1] = tt_add2(sum[(e >> 1) & 1], y);
                 if constexpr (kQuant) {
-                  uu = unit[32 * h + e];
-                  x[e] *= uu.x;
-                }
-                float pj = ts_exp2(fmaf(x[e], own, -m));
-                if (EDGE || m == -INFINITY) {
-                  const bool sees = !EDGE || ((seen >> (32 * h + e)) & 1);
-                  if (!sees || x[e] == -INFINITY) pj = 0.0f;
-                  sum += pj;
-                  if constexpr (kQuant) pj = sees ? pj * (uu.y * p_unit) : 0.0f;
-                } else {
-                  sum += pj;
-                  if constexpr (kQuant) pj *= uu.y * p_unit;
-                }
-                x[e] = pj;
-              }
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint32_t hi[4];
-                [[maybe_unused]] uint32_t lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float a = x[8 * c + 2 * e], d = x[8 * c + 2 * e + 1];
-                  if constexpr (kQuant) {
-                    hi[e] = ts_pack_f16(a, d);
-                  } else {
-                    hi[e] = ts_pack_bf16(a, d);
-                    lo[e] = ts_pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
+                  const float2 u = *reinterpret_cast<const float2*>(unit + kTtKeys + 32 * h + e);
+                  y = tt_mul2(y, tt_mul2(u, make_float2(p_unit, p_unit)));
+                  if constexpr (EDGE) {  // a row that is not seen may have any scale
+                    if (!((seen >> (32 * h + e)) & 1)) y.x = 0.0f;
+                    if (!((seen >> (32 * h + e)) & 2)) y.y = 0.0f;
                   }
+                  out[e / 2] = ts_pack_f16(y.x, y.y);
+                } else {
+                  out[e / 2] = ts_pack_bf16(y.x, y.y);
+                  out2[e / 2] = ts_pack_bf16(y.x - __uint_as_float(out[e / 2] << 16),
+                                             y.y - __uint_as_float(out[e / 2] & 0xffff0000u));
                 }
-                uint8_t* at = pt_base + tt_chunk(r, 4 * h + c);
-                *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if constexpr (!kQuant) *reinterpret_cast<uint4*>(at + kTtRows * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
               }
+              tt_st16(s_at + tt_p_col<FMT>(2 * h), out);
+              if constexpr (!kQuant) tt_st16(s_at + tt_p_col<FMT>(2 * h) + 16, out2);
             }
-            l += sum;
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           }
+          tt_wait_st();
           tt_fence_before();
-          tt_fence_async();
           __syncwarp();
-          if (lane == 0) {
-            ts_arrive(&s_free[s][buf]);
-            ts_arrive(&p_full[s]);
-          }
+          if (lane == 0) ts_arrive(&p_full[s][buf]);
+          ++o_count;
         };
         if (key0 + kTtKeys > past) tile(std::true_type{});
         else tile(std::false_type{});
       }
       slot0 = (slot0 + tiles) & (kTtUnitSlots - 1);
-      if (ok && done > 0) {
-        ok = tt_wait(&o_done[s], o_phase, &s_bad);
-        o_phase ^= 1u;
-        ok = __all_sync(kFull, ok);
-        tt_fence_after();
-      }
+      // Every P V of the segment.  (Waiting on o_done here could miss it: it may be one or two phases on.)
+      ok = ok && tt_wait(&o_end[s], o_end_phase, &s_bad);
+      ok = __all_sync(kFull, ok);
+      o_end_phase ^= 1u;
+      tt_fence_after();
       // ---- the segment's (m, l, o)
       const float unit_o = kQuant ? g_run * (1.0f / kTtPScale) : 1.0f;
-      float4* area = reinterpret_cast<float4*>(smem + C::kOffQ);  // [D / 4][row]
+      float4* area = reinterpret_cast<float4*>(smem + C::kOffQ);  // [D / 4][64 rows]
       if (!SPLIT) {
-        // Every MMA of the segment has read its Q and P: stream 1 leaves its part in their place.
+        // Every MMA of the segment has read its Q.  Stream 0 reads stream 1's accumulator in tensor memory,
+        // or, where its rows lie in other lanes, in the place of Q.
         __syncwarp();
         if (lane == 0) ts_arrive(&seg_done);
         ok = ok && tt_wait(&seg_done, end_phase, &s_bad);
         ok = __all_sync(kFull, ok);
         if (ok && s == 1 && warp_has) {
-          if (done > 0) {
+          if (done > 0 && shifted) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              float o[32];
-              tt_ld32(o_col(1) + lanes + c, o);
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tt_ld16(o_col(1) + lanes + c, o);
               if (has)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  area[(c / 4 + e) * kTtRows + n] = make_float4(o[4 * e] * unit_o, o[4 * e + 1] * unit_o,
-                                                                o[4 * e + 2] * unit_o, o[4 * e + 3] * unit_o);
+                for (int e = 0; e < 4; ++e)
+                  area[(c / 4 + e) * 64 + n] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
           }
-          if (has) join_ml[n] = make_float2(m, l);
+          if (has) join[n] = make_float4(m, l, unit_o, 0.0f);
         }
         tt_fence_before();
         __syncwarp();
         if (lane == 0) ts_arrive(&join_ready);
         ok = ok && tt_wait(&join_ready, end_phase, &s_bad);
         ok = __all_sync(kFull, ok);
+        tt_fence_after();
         end_phase ^= 1u;
       }
       if (ok && warp_has && (SPLIT || s == 0)) {
         float f0 = unit_o, f1 = 0.0f, mj = m, lj = l;
         if (!SPLIT && tiles > 1) {
-          const float2 ml = has ? join_ml[n] : make_float2(-INFINITY, 0.0f);
-          mj = fmaxf(m, ml.x);
+          const float4 other = has ? join[n] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+          mj = fmaxf(m, other.x);
           const float a0 = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ts_exp2(m - mj);
-          f1 = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(ml.x - mj);
-          lj = l * a0 + ml.y * f1;
+          const float a1 = other.x == -INFINITY ? (other.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(other.x - mj);
+          lj = l * a0 + other.y * a1;
           f0 *= a0;
+          f1 = other.z * a1;
         }
         const bool whole = w.t0 == 0 && w.t1 == w.nt;
         const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
+        if (!whole && tid == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
         const float inv = lj == 0.0f ? 0.0f : __fdiv_rn(1.0f, lj);
         const int64_t v_row = (static_cast<int64_t>(b) * p.kv_heads + kvh) * p.capacity;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          tt_ld32(o_col(s) + lanes + c, o);
-          if (!has) continue;  // tt_ld32 brings the lanes together again
+        for (int c = 0; c < D; c += 16) {
+          float o[16], o1[16];
+          tt_ld16(o_col(s) + lanes + c, o);
+          if (!SPLIT && !shifted && tiles > 1) {
+            tt_ld16(o_col(1) + lanes + c, o1);
+          } else if (!SPLIT && tiles > 1 && has) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = f0 == 0.0f ? 0.0f : o[e] * f0;
-          if (f1 != 0.0f) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 x = area[(c / 4 + e) * kTtRows + n];
-              o[4 * e] = fmaf(x.x, f1, o[4 * e]);
-              o[4 * e + 1] = fmaf(x.y, f1, o[4 * e + 1]);
-              o[4 * e + 2] = fmaf(x.z, f1, o[4 * e + 2]);
-              o[4 * e + 3] = fmaf(x.w, f1, o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) {
+              const float4 x = area[(c / 4 + e) * 64 + n];
+              o1[4 * e] = x.x;
+              o1[4 * e + 1] = x.y;
+              o1[4 * e + 2] = x.z;
+              o1[4 * e + 3] = x.w;
             }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o1[e] = 0.0f;
           }
+          if (!has) continue;  // the next tt_ld16 brings the lanes together again
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            o[e] = (f0 == 0.0f ? 0.0f : o[e] * f0) + (f1 == 0.0f ? 0.0f : o1[e] * f1);
           if (s_wild) {  // infinities and NaN of V that were taken out, for the rows that see them
             const int64_t first = max(past, static_cast<int64_t>(w.t0) * kTtKeys);
             const int64_t last = min(vis, static_cast<int64_t>(w.t1) * kTtKeys);
             for (int64_t pos = first; pos < last; ++pos) {
               if (!tree_sees(mask_row, tok, pos - past)) continue;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
+              for (int e = 0; e < 16; ++e) {
                 const float x = tt_v_global<D, FMT>(p.v, v_row + pos, c + e);
                 if (!isfinite(x)) o[e] += x;
               }
@@ -772,7 +896,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           if (whole) {
             uint4* dst = reinterpret_cast<uint4*>(p.ctx + q_row * D + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 2; ++e) {
               uint32_t x[4];
 #pragma unroll
               for (int y = 0; y < 4; ++y)
@@ -782,7 +906,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           } else {
             float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * p.rows_per_pass + n) * D + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
         if (has && !whole) p.part_ml[slot * p.rows_per_pass + n] = make_float2(mj, lj);
@@ -794,7 +918,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   tt_fence_before();
   __syncthreads();
-  if (warp == 14) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == kTtMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 }  // namespace nvfp4da
