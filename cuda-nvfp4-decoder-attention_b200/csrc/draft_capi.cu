@@ -184,6 +184,10 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
   pl.stream = (d == 64 || d == 128 || d == 256) && c->batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
               product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
   pl.tc = pl.stream && d <= 128 && nq >= kTcMinRows;
+  // Tiles and their order are 32-bit in the kernels.
+  const int64_t most_passes = ceil_div(nq, 8);
+  if (!product_within(c->batch * c->kv_heads * ceil_div(c->capacity, kTsTile), most_passes, kI32Max))
+    pl.stream = pl.tc = false;
   if (pl.tc) {
     pl.passes = static_cast<int>(ceil_div(nq, 2 * kTtRows));
     pl.rows_per_pass = static_cast<int>(ceil_div(nq, pl.passes));

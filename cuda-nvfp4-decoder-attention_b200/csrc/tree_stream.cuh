@@ -29,10 +29,11 @@
 // Numerics.  Codes (times the NVFP4 block scale) are exact in FP16; the query
 // row is scaled by a power of two to FP16 (exact down to 2^-39 of its largest
 // element); the row scale of K multiplies the FP32 score.  P goes to FP16 as
-// p_j gamma_j / G 2^11, G the largest row scale of V that the query has seen so
-// far (>= 2^-100): 11 significant bits down to 2^-25 of the largest.  Over BF16 caches Q and V stay
+// p_j gamma_j / G 2^5, G the largest row scale of V that the query has seen so
+// far (>= 2^-100): 11 significant bits down to 2^-19 of the reference, and
+// absolute steps of 2^-29 of it below.  Over BF16 caches Q and V stay
 // BF16 and P is split into two BF16 terms.  The softmax runs in base 2; its
-// reference m moves only when a score passes m + 4 (p <= 16), so most slices
+// reference m moves only when a score passes it by the slack, so most slices
 // need neither a reduction nor a rescale.  m, l, o and all sums are FP32.
 //
 // Slices that reach P_b (drafted tokens, the sequence's end) take a second
@@ -60,8 +61,11 @@ __device__ unsigned g_tree_errors;
 
 constexpr int kTsTile = 64;        // positions per stage
 constexpr int kTsMaxBatch = 1024;  // sequences whose prefix shared memory holds
-constexpr float kTsSlack = 4.0f;   // a score may pass the reference m by this (log2)
-constexpr float kTsPScale = 2048.0f;
+// A score may pass the reference m by 2^kTsSlack: P in FP16 then stays below
+// kTsPScale 2^10 = 2^15; BF16 terms have the range of FP32.
+template <int FMT>
+constexpr float kTsSlack = FMT == kKvFmtBf16 ? 20.0f : 10.0f;
+constexpr float kTsPScale = 32.0f;
 constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 
 template <int D, int FMT, int NG, int NW>
@@ -89,7 +93,7 @@ struct TsCfg {
   static constexpr uint32_t kOffMl = kOffComb + kComb;
   static constexpr uint32_t kOffBar = kOffMl + kMl;
   static constexpr uint32_t kOffPrefix = kOffBar + 2 * kStages * 8;
-  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 8u * (batch + 1) + 1024; }
+  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 4u * (batch + 1) + 1024; }
 };
 
 struct TreeStreamParams {
@@ -197,12 +201,12 @@ __device__ __forceinline__ uint32_t ts_finite(uint32_t w, uint32_t& bad) {
 
 // ---------------------------------------------------------------- the walk over one CTA's range
 struct TsWalk {
-  const long long* prefix;  // [B + 1]: tiles before sequence b (all its units)
-  int units;                // per sequence
-  long long x, x_end;
+  const int* prefix;  // [B + 1]: tiles before sequence b (all its units)
+  int units;          // per sequence
+  int x, x_end;
   int b, u;
   int t0, t1, nt;  // this segment's tiles [t0, t1) of nt in the unit
-  __device__ bool begin(const long long* pre, int batch, int per_seq, long long x0, long long x1) {
+  __device__ bool begin(const int* pre, int batch, int per_seq, int x0, int x1) {
     prefix = pre;
     units = per_seq;
     x = x0;
@@ -215,11 +219,11 @@ struct TsWalk {
       else hi = mid - 1;
     }
     b = lo;
-    nt = static_cast<int>((prefix[b + 1] - prefix[b]) / units);
-    const long long within = x - prefix[b];
-    u = static_cast<int>(within / nt);
-    t0 = static_cast<int>(within % nt);
-    t1 = static_cast<int>(min(static_cast<long long>(nt), t0 + (x_end - x)));
+    nt = (prefix[b + 1] - prefix[b]) / units;
+    const int within = x - prefix[b];
+    u = within / nt;
+    t0 = within % nt;
+    t1 = min(nt, t0 + (x_end - x));
     return true;
   }
   __device__ bool next() {
@@ -228,31 +232,64 @@ struct TsWalk {
     if (++u == units) {
       u = 0;
       ++b;
-      nt = static_cast<int>((prefix[b + 1] - prefix[b]) / units);
+      nt = (prefix[b + 1] - prefix[b]) / units;
     }
     t0 = 0;
-    t1 = static_cast<int>(min(static_cast<long long>(nt), x_end - x));
+    t1 = min(nt, x_end - x);
     return true;
   }
 };
 
-// Positions of sequence b that any of its drafted tokens may see.
-__device__ __forceinline__ int64_t ts_visible(const TreeStreamParams& p, int b) {
-  return min(tree_past(p.past_lengths, p.past_length, b, p.capacity) + p.tokens, p.capacity);
+// P_b and the positions of sequence b that any of its drafted tokens may see
+// (both fit 32 bits: a cache has fewer than 2^31 rows).
+__device__ __forceinline__ int ts_past(const TreeStreamParams& p, int b) {
+  return static_cast<int>(tree_past(p.past_lengths, p.past_length, b, p.capacity));
+}
+__device__ __forceinline__ int ts_visible(const TreeStreamParams& p, int b) {
+  return static_cast<int>(min(static_cast<int64_t>(ts_past(p, b)) + p.tokens, p.capacity));
+}
+
+// First tile of CTA c of g over n tiles.
+__device__ __forceinline__ int ts_first_tile(int n, int c, int g) {
+  return static_cast<int>(static_cast<long long>(n) * c / g);
+}
+
+// The tiles before every sequence, into prefix[0 .. B]; all threads of the block.
+__device__ __forceinline__ void ts_prefix(const TreeStreamParams& p, int units, int* prefix) {
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x)
+    prefix[b + 1] = (ts_visible(p, b) + kTsTile - 1) / kTsTile * units;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    int carry = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      const int b = base + lane;
+      int v = b < p.batch ? prefix[b + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFull, v, o);
+        if (lane >= o) v += u;
+      }
+      if (b < p.batch) prefix[b + 1] = carry + v;
+      carry += __shfl_sync(kFull, v, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
 }
 
 // CTA (of g over n tiles, CTA c owning [c n / g, (c + 1) n / g)) that holds tile x.
-__device__ __forceinline__ int ts_cta_of(long long x, long long n, int g) {
-  return static_cast<int>(((x + 1) * g - 1) / n);
+__device__ __forceinline__ int ts_cta_of(int x, int n, int g) {
+  return static_cast<int>(((static_cast<long long>(x) + 1) * g - 1) / n);
 }
 
 // What a slot of partials holds: the unit and its CTAs, where the slot is the
 // first part of a unit that several CTAs share; unit -1 otherwise.
-__device__ __forceinline__ void ts_write_slot(const TreeStreamParams& p, long long n_tiles, int G, int cta, long long x0,
+__device__ __forceinline__ void ts_write_slot(const TreeStreamParams& p, int n_tiles, int G, int cta, int x0,
                                               const TsWalk& w) {
   const bool first = w.x == x0;
   const bool starts = w.t0 == 0 && w.t1 < w.nt;  // the unit's first part, more to come
-  const int last = static_cast<int>(ts_cta_of(w.x - w.t0 + w.nt - 1, n_tiles, G));
+  const int last = ts_cta_of(w.x - w.t0 + w.nt - 1, n_tiles, G);
   p.part_slots[2 * cta + (first ? 0 : 1)] =
       starts ? make_int4(w.b, w.u, cta, last) : make_int4(-1, 0, 0, 0);
 }
@@ -289,7 +326,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
   float2* sm_ml = reinterpret_cast<float2*>(sm_f + NW * Cfg::kRows);  // [row of the pass]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t* empty = full + Cfg::kStages;
-  long long* prefix = reinterpret_cast<long long*>(smem + Cfg::kOffPrefix);
+  int* prefix = reinterpret_cast<int*>(smem + Cfg::kOffPrefix);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
@@ -308,32 +345,14 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
   }
-  for (int b = threadIdx.x; b < p.batch; b += blockDim.x)
-    prefix[b + 1] = (ts_visible(p, b) + kTsTile - 1) / kTsTile * units;
-  __syncthreads();
-  if (warp == 0) {
-    long long carry = 0;
-    for (int base = 0; base < p.batch; base += 32) {
-      const int b = base + lane;
-      long long v = b < p.batch ? prefix[b + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(kFull, v, o);
-        if (lane >= o) v += u;
-      }
-      if (b < p.batch) prefix[b + 1] = carry + v;
-      carry += __shfl_sync(kFull, v, 31);
-    }
-    if (lane == 0) prefix[0] = 0;
-  }
-  __syncthreads();
-  const long long n_tiles = prefix[p.batch];
+  ts_prefix(p, units, prefix);
+  const int n_tiles = prefix[p.batch];
   // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
   // every CTA between a unit's first and last holds one of its tiles.
-  const int G = n_tiles < p.grid ? static_cast<int>(n_tiles) : p.grid;
+  const int G = min(n_tiles, p.grid);
   if (threadIdx.x < 2) p.part_slots[2 * cta + threadIdx.x] = make_int4(-1, 0, 0, 0);
   if (cta >= G) return;
-  const long long x0 = n_tiles * cta / G, x1 = n_tiles * (cta + 1) / G;
+  const int x0 = ts_first_tile(n_tiles, cta, G), x1 = ts_first_tile(n_tiles, cta + 1, G);
   __syncthreads();
 
   if (warp == NW) {
@@ -343,11 +362,11 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
     bool more = w.begin(prefix, p.batch, units, x0, x1);
     int stage = 0;
     uint32_t phase = 0;
-    long long it = 0;
+    bool lapped = false;  // every stage has been filled once
     while (more) {
       const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
-      for (int t = w.t0; t < w.t1; ++t, ++it) {
-        if (it >= Cfg::kStages && !mbar_wait_bounded(&empty[stage], phase ^ 1u, &g_tree_errors)) return;
+      for (int t = w.t0; t < w.t1; ++t) {
+        if (lapped && !mbar_wait_bounded(&empty[stage], phase ^ 1u, &g_tree_errors)) return;
         uint8_t* st = smem + stage * Cfg::kStage;
         mbar_arrive_expect_tx(&full[stage], Cfg::kTx);
         const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile;
@@ -371,6 +390,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
         if (++stage == Cfg::kStages) {
           stage = 0;
           phase ^= 1u;
+          lapped = true;
         }
       }
       more = w.next();
@@ -386,18 +406,15 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
   TsWalk w;
   bool more = w.begin(prefix, p.batch, units, x0, x1);
   bool dead = false;
-  long long it = 0;
-  int stage = 0, turn = 0;  // it % kStages, it % groups
+  int stage = 0, turn = 0;  // the CTA's tile counter modulo kStages, modulo groups
   uint32_t phase = 0;
   while (more) {
     const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes;
-    const int64_t past = tree_past(p.past_lengths, p.past_length, b, p.capacity);
-    const int64_t vis = min(past + p.tokens, p.capacity);
+    const int past = ts_past(p, b), vis = ts_visible(p, b);
     const int n0 = pass * p.rows_per_pass + rc * Cfg::kRows;  // this warp's first query row
     // Query row n = t * group + j; global row of q and ctx:
-    auto q_row = [&](int n) {
-      return (static_cast<int64_t>(b) * p.tokens + n / p.group) * p.q_heads + static_cast<int64_t>(kvh) * p.group +
-             n % p.group;
+    auto q_row = [&](int n) -> int64_t {
+      return (b * p.tokens + n / p.group) * p.q_heads + kvh * p.group + n % p.group;
     };
 
     // ---- Q^T fragments: this lane's column is n0 + 8 j + g; q_scale: of its score columns 2 tq, 2 tq + 1
@@ -455,7 +472,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
 #pragma unroll
       for (int i = 0; i < KS; ++i) acc[j][i][0] = acc[j][i][1] = acc[j][i][2] = acc[j][i][3] = 0.0f;
     }
-    float g_run[NG][2], p_unit[NG][2];  // G of the score columns, 2^11 / G
+    float g_run[NG][2], p_unit[NG][2];  // G of the score columns, 2^5 / G
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       g_run[j][0] = g_run[j][1] = kTsMinUnit;
@@ -463,7 +480,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
     }
 
     // One slice of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
-    auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int64_t pos0) {
+    auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int pos0) {
       constexpr bool EDGE = decltype(edge_tag)::value;
       const uint8_t *kt = st, *vt = st + Cfg::kOffV;
       float s[NG][2][4];  // two accumulators, alternate steps
@@ -570,7 +587,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
           float x = (s[j][0][i] + s[j][1][i]) * q_scale[j][i & 1];
           if constexpr (kQuant) x *= k_unit[i >> 1];
           if constexpr (EDGE) {
-            const int64_t pos = pos0 + g + (i >> 1) * 8, u = pos - past;
+            const int pos = pos0 + g + (i >> 1) * 8, u = pos - past;
             const int t = tok[j][i & 1];
             bool ok = t >= 0 && pos < vis;
             if (ok && u >= 0)
@@ -581,7 +598,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
             sees[j][i] = true;
           }
           sc[j][i] = x;
-          above |= x > m_run[j][i & 1] + kTsSlack;
+          above |= x > m_run[j][i & 1] + kTsSlack<FMT>;
         }
       // ---- the reference moves (for every column) when a score passes it by the slack
       if (__any_sync(kFull, above)) {
@@ -675,7 +692,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
       auto clean = [&](uint32_t (&a)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int64_t pos = pos0 + 2 * tq + (i >> 1) * 8;
+          const int pos = pos0 + 2 * tq + (i >> 1) * 8;
           if (pos >= vis) a[i] = 0u;
           else if (pos + 1 >= vis) a[i] &= 0x0000ffffu;
           uint32_t two = 0;
@@ -796,14 +813,14 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
       }
     };
 
-    for (int t = w.t0; t < w.t1; ++t, ++it) {
+    for (int t = w.t0; t < w.t1; ++t) {
       const bool mine = pw_n < 4 || turn == (pw >> 2);
       if (mine) {
         if (!dead && !mbar_wait_bounded(&full[stage], phase, &g_tree_errors)) dead = true;
         const uint8_t* st = smem + stage * Cfg::kStage;
         for (int i = 0; i < slices; ++i) {
           const int r0 = (slice0 + i) * 16;
-          const int64_t pos0 = static_cast<int64_t>(t) * kTsTile + r0;
+          const int pos0 = t * kTsTile + r0;
           if (dead || pos0 >= vis) break;
           if (pos0 + 16 <= past) slice(std::false_type{}, st, r0, pos0);
           else slice(std::true_type{}, st, r0, pos0);

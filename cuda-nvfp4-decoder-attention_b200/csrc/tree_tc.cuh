@@ -15,7 +15,7 @@
 //   129 to 256 rows  each stream holds half of the rows and takes every tile.
 //
 // Roles: warps 0-3 and 4-7 softmax of streams 0 and 1 (one query row per
-// thread); warps 8-15 prepare operands; warps 16 and 18 issue the MMAs of a
+// thread); warps 8-15 prepare operands (K and V); warps 16 and 18 issue the MMAs of a
 // stream each (one warp for both could not issue them fast enough beside the
 // others on its scheduler); warp 17 the loads.  Per tile of 64 keys:
 //   load     codes and scales (TMA, bulk copies) into a ring; BF16 K and V
@@ -28,13 +28,13 @@
 //   softmax  scores times the row scale of K (FP32), mask, P = 2^(s - m) times
 //            the row scale of V over G, to FP16 (BF16 caches: two BF16 terms),
 //            written over the scores in tensor memory; the reference m and the
-//            scale G move only when passed by a slack of 2^4 and 2^3, and only
-//            then the accumulator is rescaled;
+//            scale G move only when passed by a slack (2^10 and 2^3, for BF16
+//            2^20), and only then the accumulator is rescaled;
 //   O += P V  M 128, N = D, P read from tensor memory, accumulated there.
 // Shared memory feeds the MMAs, so P stays out of it: with P as a
 // shared-memory operand its reads and writes took a third of the bandwidth and
 // the kernel 1.6 times as long.
-// The numerics are those of tree_stream.cuh (P is 2^7 p_j gamma_j / G here).
+// The numerics are those of tree_stream.cuh (P is 2^2 p_j gamma_j / G here).
 //
 // Waits are bounded (one second, shared give-up flag, recorded in
 // g_tree_errors); tensor memory is freed on every path.
@@ -54,7 +54,7 @@ constexpr int kTtThreads = (kTtSoftmaxWarps + kTtPrepWarps + 4) * 32;  // whole 
 // the others give: 256 * 144 + 384 * 64 = 640 * 96.
 constexpr int kTtSoftmaxRegs = 144, kTtOtherRegs = 64;
 constexpr int kTtUnitSlots = 8;  // tiles whose row scales are kept
-constexpr float kTtPScale = 128.0f;
+constexpr float kTtPScale = 4.0f;
 constexpr float kTtUnitSlack = 8.0f;
 
 template <int D, int FMT, bool SPLIT>  // SPLIT: 129 to 256 rows, half of them per stream
@@ -77,7 +77,7 @@ struct TtCfg {
   static constexpr uint32_t kOffPrefix = kOffUnits + kUnits;
   // Stream 1's o of up to 64 rows overlays Q when the streams are joined.
   static_assert(kPanels * kQPanel >= 64u * D * 4, "room to join the streams");
-  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 8u * (batch + 1) + 1024; }
+  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 4u * (batch + 1) + 1024; }
 };
 
 // ---------------------------------------------------------------- tcgen05
@@ -224,6 +224,12 @@ __device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t parity, volatile
 // (row, 16-byte chunk) of a tile of 128-byte swizzled rows.
 __device__ __forceinline__ uint32_t tt_chunk(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 
+// The exponent of a normal x > 0, and a power of two in [2^-126, 2^127] (0 below).
+__device__ __forceinline__ int tt_log2(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
+__device__ __forceinline__ float tt_pow2(int e) {
+  return e < -126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
 // A counter modulo N with the phase of its mbarriers.
 template <int N>
 struct TtRing {
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   __shared__ volatile unsigned s_bad;    // a wait gave up
   __shared__ volatile unsigned s_wild;   // an infinity or NaN was taken out of V
   __shared__ float4 join[kTtRows];       // stream 1's m, l and the unit of its o
-  long long* prefix = reinterpret_cast<long long*>(smem + C::kOffPrefix);
+  int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   float* units_kv = reinterpret_cast<float*>(smem + C::kOffUnits);  // [slot][kUnitFloats]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -282,10 +288,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(&ring_full[i], 1);
       mbar_init(&ring_free[i], kTtPrepWarps);
-      mbar_init(&k_full[i], kQuant ? kTtPrepWarps : 1);
+      mbar_init(&k_full[i], kQuant ? kTtPrepWarps / 2 : 1);
       mbar_init(&k_free[i], SPLIT ? 2 : 1);  // each stream that reads the tile
       mbar_init(&v_raw[i], 1);
-      mbar_init(&v_full[i], kTtPrepWarps);
+      mbar_init(&v_full[i], kTtPrepWarps / 2);
       mbar_init(&v_free[i], SPLIT ? 2 : 1);
     }
     mbar_init(&q_full, kTtSoftmaxWarps);
@@ -304,39 +310,33 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     s_bad = 0u;
     s_wild = 0u;
   }
-  for (int b = tid; b < p.batch; b += kTtThreads) prefix[b + 1] = (ts_visible(p, b) + kTtKeys - 1) / kTtKeys * units;
-  tt_fence_before();
-  __syncthreads();
-  tt_fence_after();
-  if (warp == 0) {
-    long long carry = 0;
-    for (int base = 0; base < p.batch; base += 32) {
-      const int b = base + lane;
-      long long v = b < p.batch ? prefix[b + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(kFull, v, o);
-        if (lane >= o) v += u;
-      }
-      if (b < p.batch) prefix[b + 1] = carry + v;
-      carry += __shfl_sync(kFull, v, 31);
-    }
-    if (lane == 0) prefix[0] = 0;
-  }
   if (tid < 2) p.part_slots[2 * cta + tid] = make_int4(-1, 0, 0, 0);
-  __syncthreads();
+  tt_fence_before();
+  ts_prefix(p, units, prefix);
+  tt_fence_after();
   const uint32_t tmem = tmem_slot;
-  const long long n_tiles = prefix[p.batch];
-  const int G = n_tiles < p.grid ? static_cast<int>(n_tiles) : p.grid;
-  const long long x0 = cta < G ? n_tiles * cta / G : 0, x1 = cta < G ? n_tiles * (cta + 1) / G : 0;
-  TsWalk w;
-  bool more = w.begin(prefix, p.batch, units, x0, x1);
   // Tensor memory columns: scores [stream][buffer][64], then o [stream][D].
   auto s_col = [&](int s, int buf) { return tmem + static_cast<uint32_t>((2 * s + buf) * kTtKeys); };
   auto o_col = [&](int s) { return tmem + 256u + static_cast<uint32_t>(s * D); };
 
+  // Each role walks the CTA's range itself (kept apart, so that no role holds
+  // another's registers).
+  auto range = [&](int& n_tiles, int& G, int& x0) {
+    n_tiles = prefix[p.batch];
+    G = min(n_tiles, p.grid);
+    x0 = cta < G ? ts_first_tile(n_tiles, cta, G) : 0;
+    return cta < G ? ts_first_tile(n_tiles, cta + 1, G) : 0;
+  };
+  auto begin = [&](TsWalk& w) {
+    int n_tiles, G, x0;
+    const int x1 = range(n_tiles, G, x0);
+    return w.begin(prefix, p.batch, units, x0, x1);
+  };
+
   if (warp >= kTtSoftmaxWarps) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtOtherRegs));
+  TsWalk w;
+  bool more = begin(w);
   if (warp == kTtLoadWarp) {
     // ---------------------------------------------------------------- loads
     if (lane == 0) {
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       for (; more && ok; more = w.next()) {
         const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
         for (int t = w.t0; t < w.t1 && ok; ++t) {
-          const int64_t row = row0 + static_cast<int64_t>(t) * kTtKeys;
+          const int64_t row = row0 + t * kTtKeys;
           if constexpr (kQuant) {
             ok = tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad);
             if (!ok) break;
@@ -466,66 +466,66 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       __syncwarp();
     }
   } else if (warp >= kTtSoftmaxWarps && warp < kTtMmaWarp) {
-    // ---------------------------------------------------------------- operands
-    const int pt = tid - kTtSoftmaxWarps * 32;  // 0 .. 255
-    constexpr int kN = kTtPrepWarps * 32;
+    // ---------------------------------------------------------------- operands: warps 8-11 K, 12-15 V
+    const bool is_v = warp >= kTtSoftmaxWarps + kTtPrepWarps / 2;
+    constexpr int kN = kTtPrepWarps / 2 * 32;
+    const int pt = (tid - kTtSoftmaxWarps * 32) % kN;
     TtRing<C::kStages ? C::kStages : 1> rr;
     TtRing<C::kK> rk;
     TtRing<C::kV> rv;
     int slot = 0;
     bool ok = true;
     for (; more && ok; more = w.next()) {
-      const int64_t past = tree_past(p.past_lengths, p.past_length, w.b, p.capacity);
-      const int64_t vis = min(past + p.tokens, p.capacity);
+      const int past = ts_past(p, w.b), vis = ts_visible(p, w.b);
       for (int t = w.t0; t < w.t1; ++t) {
-        const int64_t key0 = static_cast<int64_t>(t) * kTtKeys;
+        const int key0 = t * kTtKeys;
         const bool edge = key0 + kTtKeys > past;
-        const int live = static_cast<int>(min(static_cast<int64_t>(kTtKeys), vis - key0));  // keys before the end
+        const int live = min(kTtKeys, vis - key0);  // keys before the end
         if constexpr (kQuant) {
-          // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16), eight keys side by side;
-          // K's and V's are read together, before either is converted.
+          // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16), eight keys side by side.
           constexpr int kItems = Codes::kRowBytes / 16;
           constexpr int kRounds = (kTtKeys * kItems + kN - 1) / kN;
           ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad);
           if (!(ok = __all_sync(kFull, ok))) break;
           const uint8_t* st = smem + C::kOffRing + rr.i * Codes::kStage;
-          uint4 raw[2][kRounds];
-          [[maybe_unused]] uint32_t scales[2][kRounds];
+          const uint8_t* codes = st + (is_v ? Codes::kOffV : 0);
+          uint4 raw[kRounds];
+          [[maybe_unused]] uint32_t scales[kRounds];
 #pragma unroll
           for (int x = 0; x < kRounds; ++x) {
             const int i = pt + x * kN, c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
-            if (i < kTtKeys * kItems) {
-              const uint32_t at = ts_swz(r * Codes::kRowBytes + 16 * c);
-              raw[0][x] = *reinterpret_cast<const uint4*>(st + at);
-              raw[1][x] = *reinterpret_cast<const uint4*>(st + Codes::kOffV + at);
-              if constexpr (FMT == kKvFmtNvfp4) {
-                scales[0][x] = *reinterpret_cast<const uint16_t*>(st + Codes::kOffKb + r * (D / 16) + 2 * c);
-                scales[1][x] = *reinterpret_cast<const uint16_t*>(st + Codes::kOffVb + r * (D / 16) + 2 * c);
-              }
-            }
+            raw[x] = *reinterpret_cast<const uint4*>(codes + ts_swz(r * Codes::kRowBytes + 16 * c));
+            if constexpr (FMT == kKvFmtNvfp4)
+              scales[x] = *reinterpret_cast<const uint16_t*>(st + (is_v ? Codes::kOffVb : Codes::kOffKb) + r * (D / 16) + 2 * c);
           }
+          [[maybe_unused]] float2 kr, vr;
+          if (warp == kTtSoftmaxWarps) {
+            kr = reinterpret_cast<const float2*>(st + Codes::kOffKr)[lane];
+            vr = reinterpret_cast<const float2*>(st + Codes::kOffVr)[lane];
+          }
+          __syncwarp();
+          if (lane == 0) ts_arrive(&ring_free[rr.i]);
+          rr.next();
+          ok = is_v ? tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad) : tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+          if (!(ok = __all_sync(kFull, ok))) break;
           if (warp == kTtSoftmaxWarps) {  // the first of these warps: the row scales
             float* un = units_kv + slot * C::kUnitFloats;
-            const float2 kr = reinterpret_cast<const float2*>(st + Codes::kOffKr)[lane];
-            const float2 vr = reinterpret_cast<const float2*>(st + Codes::kOffVr)[lane];
             reinterpret_cast<float2*>(un)[lane] = make_float2(kr.x * p.scale_log2, kr.y * p.scale_log2);
             reinterpret_cast<float2*>(un + kTtKeys)[lane] = vr;
             const float top = warp_max_f32(fmaxf(vr.x < INFINITY ? vr.x : 0.0f, vr.y < INFINITY ? vr.y : 0.0f));
             if (lane == 0) un[2 * kTtKeys] = top;
           }
           slot = slot + 1 == kTtUnitSlots ? 0 : slot + 1;
-          __syncwarp();
-          if (lane == 0) ts_arrive(&ring_free[rr.i]);
-          rr.next();
-          auto prepare = [&](int which, uint8_t* out, bool clean) {
+          uint8_t* out = smem + (is_v ? C::kOffV + rv.i * C::kOperand : C::kOffK + rk.i * C::kOperand);
+          auto prepare = [&](auto clean_tag) {
+            constexpr bool CLEAN = decltype(clean_tag)::value;
 #pragma unroll
             for (int x = 0; x < kRounds; ++x) {
               const int i = pt + x * kN, c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
-              if (i >= kTtKeys * kItems) break;
-              const uint32_t word[4] = {raw[which][x].x, raw[which][x].y, raw[which][x].z, raw[which][x].w};
-              uint32_t b0 = 0, b1 = 0;
+              const uint32_t word[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+              [[maybe_unused]] uint32_t b0 = 0, b1 = 0;
               if constexpr (FMT == kKvFmtNvfp4) {
-                const uint32_t both = e4m3x2_to_f16x2(scales[which][x]);
+                const uint32_t both = e4m3x2_to_f16x2(scales[x]);
                 b0 = __byte_perm(both, both, 0x1010);
                 b1 = __byte_perm(both, both, 0x3232);
               }
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                   ts_e4m3x4(word[2 * y], h[0], h[1]);
                   ts_e4m3x4(word[2 * y + 1], h[2], h[3]);
                 }
-                if (clean) {
+                if constexpr (CLEAN) {
                   uint32_t bad = 0;
 #pragma unroll
                   for (int z = 0; z < 4; ++z) h[z] = r < live ? ts_finite<FMT>(h[z], bad) : 0u;
@@ -554,22 +554,14 @@ __global__ void __launch_bounds__(kTtThreads, 1)
               }
             }
           };
-          ok = tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
-          if (!(ok = __all_sync(kFull, ok))) break;
-          prepare(0, smem + C::kOffK + rk.i * C::kOperand, false);
+          if (is_v && edge) prepare(std::true_type{});
+          else prepare(std::false_type{});
           tt_fence_async();
           __syncwarp();
-          if (lane == 0) ts_arrive(&k_full[rk.i]);
+          if (lane == 0) ts_arrive(is_v ? &v_full[rv.i] : &k_full[rk.i]);
           rk.next();
-          ok = tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad);
-          if (!(ok = __all_sync(kFull, ok))) break;
-          if (edge) prepare(1, smem + C::kOffV + rv.i * C::kOperand, true);
-          else prepare(1, smem + C::kOffV + rv.i * C::kOperand, false);
-          tt_fence_async();
-          __syncwarp();
-          if (lane == 0) ts_arrive(&v_full[rv.i]);
           rv.next();
-        } else {
+        } else if (is_v) {
           ok = tt_wait(&v_raw[rv.i], rv.phase, &s_bad);
           if (!(ok = __all_sync(kFull, ok))) break;
           if (edge) {
@@ -602,6 +594,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   } else {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTtSoftmaxRegs));
+    TsWalk w;
+    bool more = begin(w);
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;  // stream, row of its tile
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t s_count = 0, o_count = 0, end_phase = 0, o_end_phase = 0;  // scores seen, P tiles given, segments ended
@@ -610,8 +604,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     bool ok = true;
     for (; more && ok; more = w.next()) {
       const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes, tiles = w.t1 - w.t0;
-      const int64_t past = tree_past(p.past_lengths, p.past_length, b, p.capacity);
-      const int64_t vis = min(past + p.tokens, p.capacity);
+      const int past = ts_past(p, b), vis = ts_visible(p, b);
       const int n_first = pass * p.rows_per_pass, rows = min(p.rows_per_pass, nq - n_first);
       const bool shifted = !SPLIT && rows <= 64;
       const int half = (rows + 1) / 2;
@@ -620,8 +613,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const bool has = n >= 0 && n < rows;
       const bool warp_has = __any_sync(kFull, has);
       const int tok = has ? (n_first + n) / p.group : 0;
-      const int64_t q_row = (static_cast<int64_t>(b) * p.tokens + tok) * p.q_heads +
-                            static_cast<int64_t>(kvh) * p.group + (has ? (n_first + n) % p.group : 0);
+      const int64_t q_row = (b * p.tokens + tok) * p.q_heads + kvh * p.group + (has ? (n_first + n) % p.group : 0);
       if (!SPLIT && s == 1 && !first_segment) {  // stream 0 has read what the join left in the place of Q
         ok = tt_wait(&join_read, end_phase ^ 1u, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
@@ -665,12 +657,13 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       __syncwarp();
       if (lane == 0) ts_arrive(&q_full);
 
-      float m = -INFINITY, l = 0.0f, g_run = kTsMinUnit, p_unit = kTtPScale / kTsMinUnit;
+      // l and the weights are 2^shift of what they stand for, 2^shift = 2^2 / G (BF16: 1).
+      float m = -INFINITY, l = 0.0f, g_run = kTsMinUnit, shift = kQuant ? 102.0f : 0.0f;
       const uint8_t* mask_row = p.mask ? p.mask + b * p.mask_stride + static_cast<int64_t>(tok) * p.tokens : nullptr;
       int done = 0;  // jobs of this stream in the segment
       for (int i = SPLIT ? 0 : s; i < tiles && ok; i += SPLIT ? 1 : 2, ++done) {
         const int buf = s_count & 1;
-        const int64_t key0 = static_cast<int64_t>(w.t0 + i) * kTtKeys;
+        const int key0 = (w.t0 + i) * kTtKeys;
         ok = tt_wait(&s_full[s][buf], (s_count >> 1) & 1, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
         tt_fence_after();
@@ -682,11 +675,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           // Keys of the tile this row sees, one bit each.
           [[maybe_unused]] unsigned long long seen = ~0ull;
           if constexpr (EDGE) {
-            const int64_t old = past - key0;  // committed keys of the tile
+            const int old = past - key0;  // committed keys of the tile
             seen = old <= 0 ? 0ull : (1ull << old) - 1;  // fewer than 64 in such a tile
-            const int64_t first = max(past, key0), last = min(vis, key0 + kTtKeys);
+            const int first = max(past, key0), last = min(vis, key0 + kTtKeys);
             if (has)
-              for (int64_t pos = first; pos < last; ++pos)
+              for (int pos = first; pos < last; ++pos)
                 if (tree_sees(mask_row, tok, pos - past)) seen |= 1ull << (pos - key0);
           }
           // 32 scores in units of own; unseen keys -inf.
@@ -711,90 +704,129 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                 if (!((bits >> e) & 1)) x[e] = -INFINITY;
             }
           };
+          // 32 keys' P against m_ref into out (BF16: second terms into out2), their sum into l_tile.
+          float l_tile = 0.0f;
+          auto weights = [&](int h, const float (&x)[32], float m_ref, uint32_t (&out)[16],
+                             [[maybe_unused]] uint32_t (&out2)[16]) {
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              [[maybe_unused]] float4 u;
+              if constexpr (kQuant) u = *reinterpret_cast<const float4*>(unit + kTtKeys + 32 * h + e);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float2 y = tt_fma2(make_float2(x[e + 2 * i], x[e + 2 * i + 1]), make_float2(own, own),
+                                   make_float2(-m_ref, -m_ref));
+                y.x = ts_exp2(y.x);
+                y.y = ts_exp2(y.y);
+                sum[i] = tt_add2(sum[i], y);
+                const int at = e / 2 + i;
+                if constexpr (kQuant) {
+                  y = tt_mul2(y, i ? make_float2(u.z, u.w) : make_float2(u.x, u.y));
+                  if constexpr (EDGE) {  // a row that is not seen may have any scale
+                    if (!((seen >> (32 * h + e + 2 * i)) & 1)) y.x = 0.0f;
+                    if (!((seen >> (32 * h + e + 2 * i)) & 2)) y.y = 0.0f;
+                  }
+                  out[at] = ts_pack_f16(y.x, y.y);
+                } else {
+                  out[at] = ts_pack_bf16(y.x, y.y);
+                  out2[at] = ts_pack_bf16(y.x - __uint_as_float(out[at] << 16),
+                                          y.y - __uint_as_float(out[at] & 0xffff0000u));
+                }
+              }
+            }
+            l_tile += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          };
+          auto maxima = [&](const float (&x)[32], float (&mx)[4]) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+          };
+          // The row scale of V that decides on G.
+          [[maybe_unused]] float vx = 0.0f;
+          if constexpr (kQuant) {
+            vx = unit[2 * kTtKeys];
+            if constexpr (EDGE) {
+              vx = 0.0f;
+#pragma unroll 1
+              for (int e = 0; e < kTtKeys; ++e) {
+                const float u = unit[kTtKeys + e];
+                if (((seen >> e) & 1) && u < INFINITY) vx = fmaxf(vx, u);
+              }
+            }
+          }
+          // First against the reference and G as they are; again, after both have moved, if that was too low.
           float f = 1.0f;  // what the accumulator is to be scaled by
+          bool again = false;
           if (warp_has) {
+            uint32_t out[2][16];
+            [[maybe_unused]] uint32_t out2[2][16];
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            const float m_ref = m == -INFINITY ? -shift : m - shift;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float x[32];
               scores(h, x);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+              maxima(x, mx);
+              weights(h, x, m_ref, out[h], out2[h]);
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * own;
-            if (has && top > m + kTsSlack) {
-              f = m == -INFINITY ? 0.0f : ts_exp2(m - top);
-              l *= f;
-              m = top;
-            }
-            if constexpr (kQuant) {
-              float vx = unit[2 * kTtKeys];
-              if constexpr (EDGE) {
-                vx = 0.0f;
-#pragma unroll 1
-                for (int e = 0; e < kTtKeys; ++e) {
-                  const float u = unit[kTtKeys + e];
-                  if (((seen >> e) & 1) && u < INFINITY) vx = fmaxf(vx, u);
+            again = has && (top > m + kTsSlack<FMT> || (kQuant && vx > g_run * kTtUnitSlack));
+            again = __any_sync(kFull, again);
+            if (again) {
+              if (has && top > m + kTsSlack<FMT>) {
+                f = m == -INFINITY ? 0.0f : ts_exp2(m - top);
+                l *= f;
+                m = top;
+              }
+              if constexpr (kQuant) {
+                if (has && vx > g_run * kTtUnitSlack) {  // G up to the next power of two
+                  const int old = tt_log2(g_run), next = tt_log2(vx) + 1;
+                  const float down = tt_pow2(old - next);
+                  g_run = tt_pow2(next);
+                  f *= down;
+                  l *= down;  // l is in units of 2^shift, as the weights are
+                  shift -= static_cast<float>(next - old);
                 }
               }
-              if (has && vx > g_run * kTtUnitSlack) {
-                f *= __fdiv_rn(g_run, vx);
-                g_run = vx;
-                p_unit = __fdiv_rn(kTtPScale, vx);
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                tt_st16(s_at + tt_p_col<FMT>(2 * h), out[h]);
+                if constexpr (!kQuant) tt_st16(s_at + tt_p_col<FMT>(2 * h) + 16, out2[h]);
               }
             }
           }
-          // ---- the accumulator, once P V of the tile before is done
-          if (done > 0 && __any_sync(kFull, f != 1.0f)) {
-            // The scores of this job were issued after the P V of the job before last: one phase is in question.
-            ok = tt_wait(&o_done[s], (o_count - 1) & 1, &s_bad);
-            if (!(ok = __all_sync(kFull, ok))) return;
-            tt_fence_after();
+          if (again) {  // uniform in the warp
+            // ---- the accumulator, once P V of the tile before is done
+            if (done > 0 && __any_sync(kFull, f != 1.0f)) {
+              // The scores of this job were issued after the P V of the job before last: one phase is in question.
+              ok = tt_wait(&o_done[s], (o_count - 1) & 1, &s_bad);
+              if (!(ok = __all_sync(kFull, ok))) return;
+              tt_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              float o[16];
-              tt_ld16(o_col(s) + lanes + c, o);
-              uint32_t y[16];
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                tt_ld16(o_col(s) + lanes + c, o);
+                uint32_t y[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(o[e] * f);
-              tt_st16(o_col(s) + lanes + c, y);
+                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(o[e] * f);
+                tt_st16(o_col(s) + lanes + c, y);
+              }
             }
-          }
-          // ---- P over the scores; scores of -inf (unseen among them) weigh 0 against the finite m_ref
-          if (warp_has) {
-            const float m_ref = m == -INFINITY ? 0.0f : m;
-            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
+            const float m_ref = m == -INFINITY ? -shift : m - shift;
+            l_tile = 0.0f;
+#pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               float x[32];
               scores(h, x);
               uint32_t out[16];
               [[maybe_unused]] uint32_t out2[16];
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                float2 y = tt_fma2(make_float2(x[e], x[e + 1]), make_float2(own, own), make_float2(-m_ref, -m_ref));
-                y.x = ts_exp2(y.x);
-                y.y = ts_exp2(y.y);
-                sum[(e >> 1) & 1] = tt_add2(sum[(e >> 1) & 1], y);
-                if constexpr (kQuant) {
-                  const float2 u = *reinterpret_cast<const float2*>(unit + kTtKeys + 32 * h + e);
-                  y = tt_mul2(y, tt_mul2(u, make_float2(p_unit, p_unit)));
-                  if constexpr (EDGE) {  // a row that is not seen may have any scale
-                    if (!((seen >> (32 * h + e)) & 1)) y.x = 0.0f;
-                    if (!((seen >> (32 * h + e)) & 2)) y.y = 0.0f;
-                  }
-                  out[e / 2] = ts_pack_f16(y.x, y.y);
-                } else {
-                  out[e / 2] = ts_pack_bf16(y.x, y.y);
-                  out2[e / 2] = ts_pack_bf16(y.x - __uint_as_float(out[e / 2] << 16),
-                                             y.y - __uint_as_float(out[e / 2] & 0xffff0000u));
-                }
-              }
+              weights(h, x, m_ref, out, out2);
               tt_st16(s_at + tt_p_col<FMT>(2 * h), out);
               if constexpr (!kQuant) tt_st16(s_at + tt_p_col<FMT>(2 * h) + 16, out2);
             }
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           }
+          l += l_tile;
           tt_wait_st();
           tt_fence_before();
           __syncwarp();
@@ -811,7 +843,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       o_end_phase ^= 1u;
       tt_fence_after();
       // ---- the segment's (m, l, o)
-      const float unit_o = kQuant ? g_run * (1.0f / kTtPScale) : 1.0f;
+      const float unit_o = kQuant ? g_run * (1.0f / kTtPScale) : 1.0f;  // 2^-shift
+      l *= unit_o;
       float4* area = reinterpret_cast<float4*>(smem + C::kOffQ);  // [D / 4][64 rows]
       if (!SPLIT) {
         // Every MMA of the segment has read its Q.  Stream 0 reads stream 1's accumulator in tensor memory,
@@ -854,10 +887,12 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           f1 = other.z * a1;
         }
         const bool whole = w.t0 == 0 && w.t1 == w.nt;
+        int n_tiles, G, x0;
+        range(n_tiles, G, x0);
         const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
         if (!whole && tid == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
         const float inv = lj == 0.0f ? 0.0f : __fdiv_rn(1.0f, lj);
-        const int64_t v_row = (static_cast<int64_t>(b) * p.kv_heads + kvh) * p.capacity;
+        const int64_t v_row = (b * p.kv_heads + kvh) * p.capacity;
 #pragma unroll 1
         for (int c = 0; c < D; c += 16) {
           float o[16], o1[16];
@@ -882,9 +917,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           for (int e = 0; e < 16; ++e)
             o[e] = (f0 == 0.0f ? 0.0f : o[e] * f0) + (f1 == 0.0f ? 0.0f : o1[e] * f1);
           if (s_wild) {  // infinities and NaN of V that were taken out, for the rows that see them
-            const int64_t first = max(past, static_cast<int64_t>(w.t0) * kTtKeys);
-            const int64_t last = min(vis, static_cast<int64_t>(w.t1) * kTtKeys);
-            for (int64_t pos = first; pos < last; ++pos) {
+            const int first = max(past, w.t0 * kTtKeys), last = min(vis, w.t1 * kTtKeys);
+            for (int pos = first; pos < last; ++pos) {
               if (!tree_sees(mask_row, tok, pos - past)) continue;
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
