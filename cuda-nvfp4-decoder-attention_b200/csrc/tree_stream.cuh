@@ -59,7 +59,10 @@ namespace nvfp4da {
 
 __device__ unsigned g_tree_errors;
 
-constexpr int kTsTile = 64;        // positions per stage
+// Positions per stage: with 64, the 4 KB pieces of NVFP4 codes reached two
+// thirds of the HBM rate even with nothing else to do.
+template <int FMT>
+constexpr int kTsTile = FMT == kKvFmtBf16 ? 64 : 128;
 constexpr int kTsMaxBatch = 1024;  // sequences whose prefix shared memory holds
 // A score may pass the reference m by 2^kTsSlack: P in FP16 then stays below
 // kTsPScale 2^10 = 2^15; BF16 terms have the range of FP32.
@@ -68,31 +71,35 @@ constexpr float kTsSlack = FMT == kKvFmtBf16 ? 20.0f : 10.0f;
 constexpr float kTsPScale = 32.0f;
 constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 
-template <int D, int FMT, int NG, int NW>
+template <int D, int FMT, int NG, int NW, int SL, int TILE = kTsTile<FMT>>
 struct TsCfg {
   static_assert(D == 64 || D == 128 || D == 256, "head_dim 64, 128 or 256");
-  static constexpr int kThreads = (NW + 1) * 32;
+  static constexpr int kThreads = (NW + 4) * 32;  // consumers, two loading and two joining warps
   static constexpr int kRowBytes = FMT == kKvFmtBf16 ? 2 * D : (FMT == kKvFmtE4m3 ? D : D / 2);
-  static constexpr uint32_t kCodes = kTsTile * kRowBytes;  // one of K, V
-  static constexpr uint32_t kBlockScales = FMT == kKvFmtNvfp4 ? kTsTile * (D / 16) : 0;
-  static constexpr uint32_t kRowScales = FMT == kKvFmtBf16 ? 0 : kTsTile * 4;
+  static constexpr uint32_t kCodes = TILE * kRowBytes;  // one of K, V
+  static constexpr uint32_t kBlockScales = FMT == kKvFmtNvfp4 ? TILE * (D / 16) : 0;
+  static constexpr uint32_t kRowScales = FMT == kKvFmtBf16 ? 0 : TILE * 4;
   static constexpr uint32_t kOffV = kCodes, kOffKb = 2 * kCodes, kOffVb = kOffKb + kBlockScales,
                             kOffKr = kOffVb + kBlockScales, kOffVr = kOffKr + kRowScales;
   static constexpr uint32_t kTx = kOffVr + kRowScales;  // bytes a stage receives
   static constexpr uint32_t kStage = (kTx + 1023) / 1024 * 1024;
   static constexpr int kRows = 8 * NG;                               // query rows per warp
-  static constexpr uint32_t kComb = NW * kRows * D * 4;              // per-warp O for the join
-  static constexpr uint32_t kMl = 3 * NW * kRows * 4 + NW * kRows * 8;  // m, l, factor; joined (m, l)
-  static constexpr int kGroups = NW / 4;                             // most tile groups
-  static constexpr int kFit = static_cast<int>((217u * 1024 - kComb - kMl) / kStage);
+  // What the consumer warps leave of a segment for the joining warps: o, m, l;
+  // twice, so that they go on to the next segment, where it fits.
+  static constexpr int kJoins = NG == 1 && D <= 128 ? 2 : 1;
+  static constexpr int kJoinStride = D + (FMT == kKvFmtBf16 ? 8 : 2);  // floats between rows (bank conflicts)
+  static constexpr uint32_t kJoinO = NW * kRows * kJoinStride * 4;
+  static constexpr uint32_t kComb = kJoins * (kJoinO + 2 * NW * kRows * 4);
+  static constexpr int kTurns = TILE / 16 / SL;                              // warps' turns per tile
+  static constexpr int kGroups = NW / kTurns;                        // most tile groups
+  static constexpr int kFit = static_cast<int>((217u * 1024 - kComb) / kStage);
   // A whole number of groups: the CTA's n-th tile goes to stage n % kStages and
   // group n % groups, so every stage serves one group only.
-  static constexpr int kStages = (kFit > 12 ? 12 : kFit) / kGroups * kGroups;
+  static constexpr int kStages = (kFit > 14 ? 14 : kFit) / kGroups * kGroups;
   static_assert(kStages >= 2, "two stages at least");
   static constexpr uint32_t kOffComb = kStages * kStage;
-  static constexpr uint32_t kOffMl = kOffComb + kComb;
-  static constexpr uint32_t kOffBar = kOffMl + kMl;
-  static constexpr uint32_t kOffPrefix = kOffBar + 2 * kStages * 8;
+  static constexpr uint32_t kOffBar = kOffComb + kComb;
+  static constexpr uint32_t kOffPrefix = kOffBar + (2 * kStages + 2 * kJoins) * 8;
   static constexpr uint32_t bytes(int batch) { return kOffPrefix + 4u * (batch + 1) + 1024; }
 };
 
@@ -123,13 +130,19 @@ __device__ __forceinline__ void ts_tma_2d(void* dst, const CUtensorMap* map, int
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
       : "memory");
 }
+// 16 bytes by this thread, and its arrival on `bar` once all it copied so is there.
+__device__ __forceinline__ void ts_copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ts_copy_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void ts_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void ts_bar_sync(int threads) { asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory"); }
 __device__ __forceinline__ uint32_t ts_transpose(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ float ts_exp2(float x) {
@@ -141,12 +154,12 @@ template <int FMT>
 __device__ __forceinline__ void ts_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
   if constexpr (FMT == kKvFmtBf16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -255,9 +268,9 @@ __device__ __forceinline__ int ts_first_tile(int n, int c, int g) {
 }
 
 // The tiles before every sequence, into prefix[0 .. B]; all threads of the block.
-__device__ __forceinline__ void ts_prefix(const TreeStreamParams& p, int units, int* prefix) {
+__device__ __forceinline__ void ts_prefix(const TreeStreamParams& p, int units, int tile, int* prefix) {
   for (int b = threadIdx.x; b < p.batch; b += blockDim.x)
-    prefix[b + 1] = (ts_visible(p, b) + kTsTile - 1) / kTsTile * units;
+    prefix[b + 1] = (ts_visible(p, b) + tile - 1) / tile * units;
   __syncthreads();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
@@ -298,7 +311,7 @@ __device__ __forceinline__ void ts_write_slot(const TreeStreamParams& p, int n_t
 template <int D, int FMT>
 __device__ __forceinline__ float ts_v_element(const uint8_t* vt, const uint8_t* vb, int r, int d) {
   if (FMT == kKvFmtBf16) {
-    const uint32_t o = (d >> 6) * (kTsTile * 128) + ts_swz(r * 128 + (d & 63) * 2);
+    const uint32_t o = (d >> 6) * (kTsTile<FMT> * 128) + ts_swz(r * 128 + (d & 63) * 2);
     return bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(vt + o));
   }
   if (FMT == kKvFmtE4m3) return f16x2_to_f32x2(e4m3x2_to_f16x2(vt[ts_swz(r * D + d)])).x;
@@ -307,45 +320,85 @@ __device__ __forceinline__ float ts_v_element(const uint8_t* vt, const uint8_t* 
   return ((d & 1) ? pair.y : pair.x) * f16x2_to_f32x2(e4m3x2_to_f16x2(vb[r * (D / 16) + d / 16])).x;
 }
 
+// The scales of the TILE rows from `row` on, by one warp; rows past the cache's
+// last are left out (they belong to no position that is seen).
+template <int D, int FMT, typename Cfg, int TILE>
+__device__ __forceinline__ void ts_load_scales(uint8_t* st, const TreeStreamParams& p, int64_t row, int64_t rows,
+                                               int lane) {
+  const int left = static_cast<int>(min(rows - row, static_cast<int64_t>(TILE)));
+  if constexpr (FMT == kKvFmtNvfp4) {
+#pragma unroll
+    for (uint32_t i = 0; i < Cfg::kBlockScales; i += 512) {
+      const uint32_t o = i + lane * 16;
+      if (o < static_cast<uint32_t>(left) * (D / 16)) {
+        ts_copy16(st + Cfg::kOffKb + o, p.k.block_scales + row * (D / 16) + o);
+        ts_copy16(st + Cfg::kOffVb + o, p.v.block_scales + row * (D / 16) + o);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TILE; i += 128) {
+    const int r = i + lane * 4;
+    if (r < left) {
+      ts_copy16(st + Cfg::kOffKr + r * 4, p.k.row_scales + row + r);
+      ts_copy16(st + Cfg::kOffVr + r * 4, p.v.row_scales + row + r);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- the streaming kernel
-template <int D, int FMT, int NG, int NW>
-__global__ void __launch_bounds__((NW + 1) * 32, 1)
+template <int D, int FMT, int NG, int NW, int SL>
+__global__ void __launch_bounds__((NW + 4) * 32, 1)
     tree_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const TreeStreamParams p) {
-  using Cfg = TsCfg<D, FMT, NG, NW>;
+  using Cfg = TsCfg<D, FMT, NG, NW, SL>;
   constexpr int KS = D / 16;  // MMA steps of K Q^T, 16-element row blocks of O^T
   constexpr bool kQuant = FMT != kKvFmtBf16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // Pointer arithmetic, not an integer round trip: the compiler then knows that
   // what it points to is shared memory.
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* so = reinterpret_cast<float*>(smem + Cfg::kOffComb);  // [warp][row][D]
-  float* sm_m = reinterpret_cast<float*>(smem + Cfg::kOffMl);  // [warp][row]
-  float* sm_l = sm_m + NW * Cfg::kRows;
-  float* sm_f = sm_l + NW * Cfg::kRows;
-  float2* sm_ml = reinterpret_cast<float2*>(sm_f + NW * Cfg::kRows);  // [row of the pass]
+  // Joining buffers: o [warp][row][kJoinStride], then m [warp][row] and l [warp][row].
+  auto join_o = [&](int i) { return reinterpret_cast<float*>(smem + Cfg::kOffComb + i * (Cfg::kComb / Cfg::kJoins)); };
+  auto join_m = [&](int i) { return join_o(i) + Cfg::kJoinO / 4; };
+  // Element e of row r (of 8 NG): rows in the order that keeps stores of a
+  // fragment in different banks, elements of quantised formats rotated in their
+  // lane's D / 8 for the same reason.
+  auto join_at = [&](int r, int e) {
+    constexpr int W = D / 8;
+    const int row = (r & ~7) + (r & 1) * 4 + ((r & 7) >> 1);
+    const int at = kQuant ? e / W * W + (e % W + 4 * (e / W * W / 32)) % W : e;
+    return row * Cfg::kJoinStride + at;
+  };
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t* empty = full + Cfg::kStages;
+  uint64_t* join_full = empty + Cfg::kStages;
+  uint64_t* join_free = join_full + Cfg::kJoins;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::kOffPrefix);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   const int rc_n = p.row_chunks, pw_n = NW / rc_n;       // row chunks, position warps per chunk
-  const int groups = pw_n >= 4 ? pw_n / 4 : 1;           // tiles alternate between groups
+  constexpr int kTurns = Cfg::kTurns;
+  const int groups = pw_n >= kTurns ? pw_n / kTurns : 1; // tiles alternate between groups
   const int units = p.kv_heads * p.passes;
   const int nq = p.group * p.tokens;                     // query rows per KV head
 
   pdl_launch_dependents();  // the join waits for this kernel's memory itself
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], pw_n >= 4 ? 4 * rc_n : NW);
+      mbar_init(&full[s], kQuant ? 34 : 2);  // K's and V's bytes, and the lanes that copy scales
+      mbar_init(&empty[s], pw_n >= kTurns ? kTurns * rc_n : NW);
+    }
+    for (int i = 0; i < Cfg::kJoins; ++i) {
+      mbar_init(&join_full[i], NW);
+      mbar_init(&join_free[i], 2);
     }
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
   }
-  ts_prefix(p, units, prefix);
+  ts_prefix(p, units, kTsTile<FMT>, prefix);
   const int n_tiles = prefix[p.batch];
   // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
   // every CTA between a unit's first and last holds one of its tiles.
@@ -355,37 +408,91 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
   const int x0 = ts_first_tile(n_tiles, cta, G), x1 = ts_first_tile(n_tiles, cta + 1, G);
   __syncthreads();
 
-  if (warp == NW) {
-    // ---------------------------------------------------------------- producer
-    if (lane != 0) return;
+  if (warp >= NW + 2) {
+    // ---------------------------------------------------------------- joins: every other row of a segment
+    TsWalk w;
+    bool more = w.begin(prefix, p.batch, units, x0, x1);
+    int buf = 0;
+    uint32_t phase = 0;
+    for (; more; more = w.next()) {
+      const int pass = w.u % p.passes, kvh = w.u / p.passes, n_first = pass * p.rows_per_pass;
+      const int rows = min(p.rows_per_pass, nq - n_first);
+      const bool whole = w.t0 == 0 && w.t1 == w.nt;
+      const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
+      if (!whole && warp == NW + 2 && lane == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
+      if (!mbar_wait_bounded(&join_full[buf], phase, &g_tree_errors)) return;
+      const float *so = join_o(buf), *sm_m = join_m(buf), *sm_l = sm_m + NW * Cfg::kRows;
+      for (int r = warp - NW - 2; r < rows; r += 2) {
+        // Position warp `lane` of the row's chunk: its factor.
+        const int chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
+        const int at = (lane * rc_n + chunk) * Cfg::kRows + rr;
+        const float mu = lane < pw_n ? sm_m[at] : -INFINITY, lu = lane < pw_n ? sm_l[at] : 0.0f;
+        const float mx = warp_max_f32(mu);
+        const float fu = mu == -INFINITY ? (lu == 0.0f ? 0.0f : 1.0f) : ts_exp2(mu - mx);
+        const float l = warp_sum_f32(lu * fu), inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        const int n = n_first + r;
+        const int64_t out = static_cast<int64_t>((w.b * p.tokens + n / p.group) * p.q_heads + kvh * p.group + n % p.group) * D;
+#pragma unroll
+        for (int e = 2 * lane; e < D; e += 64) {
+          float2 o = make_float2(0.0f, 0.0f);
+          for (int u = 0; u < pw_n; ++u) {
+            const float f = __shfl_sync(kFull, fu, u);
+            const float2 v = *reinterpret_cast<const float2*>(so + (u * rc_n + chunk) * Cfg::kRows * Cfg::kJoinStride + join_at(rr, e));
+            o.x = f == 0.0f ? o.x : fmaf(v.x, f, o.x);
+            o.y = f == 0.0f ? o.y : fmaf(v.y, f, o.y);
+          }
+          if (whole)
+            *reinterpret_cast<uint32_t*>(p.ctx + out + e) = l == 0.0f ? 0u : ts_pack_bf16(o.x * inv, o.y * inv);
+          else
+            *reinterpret_cast<float2*>(p.part_o + (slot * p.rows_per_pass + r) * D + e) = o;
+        }
+        if (!whole && lane == 0) p.part_ml[slot * p.rows_per_pass + r] = make_float2(mx, l);
+      }
+      __syncwarp();
+      if (lane == 0) ts_arrive(&join_free[buf]);
+      if (++buf == Cfg::kJoins) {
+        buf = 0;
+        phase ^= 1u;
+      }
+    }
+    return;
+  }
+
+  if (warp >= NW) {
+    // ---------------------------------------------------------------- loads: warp NW K, the next one V and scales
+    // Scales go by 16-byte copies of a whole warp: a bulk copy takes one thread over a hundred cycles to
+    // issue, and four of them per tile held E4M3 and NVFP4 caches at 0.8 and 0.4 of the HBM rate.
+    const bool is_v = warp > NW;
+    if (lane != 0 && !(is_v && kQuant)) return;
     TsWalk w;
     bool more = w.begin(prefix, p.batch, units, x0, x1);
     int stage = 0;
     uint32_t phase = 0;
+    [[maybe_unused]] const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
     bool lapped = false;  // every stage has been filled once
     while (more) {
       const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
       for (int t = w.t0; t < w.t1; ++t) {
         if (lapped && !mbar_wait_bounded(&empty[stage], phase ^ 1u, &g_tree_errors)) return;
         uint8_t* st = smem + stage * Cfg::kStage;
-        mbar_arrive_expect_tx(&full[stage], Cfg::kTx);
-        const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile;
-        if constexpr (!kQuant) {
+        const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile<FMT>;
+        if (lane == 0) {
+          uint8_t* dst = st + (is_v ? Cfg::kOffV : 0);
+          const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+          mbar_arrive_expect_tx(&full[stage], Cfg::kCodes);
+          if constexpr (!kQuant) {
 #pragma unroll
-          for (int bx = 0; bx < D / 64; ++bx) {
-            ts_tma_2d(st + bx * (kTsTile * 128), &tm_k, bx * 64, static_cast<int>(row), &full[stage]);
-            ts_tma_2d(st + Cfg::kOffV + bx * (kTsTile * 128), &tm_v, bx * 64, static_cast<int>(row), &full[stage]);
+            for (int bx = 0; bx < D / 64; ++bx)
+              ts_tma_2d(dst + bx * (kTsTile<FMT> * 128), map, bx * 64, static_cast<int>(row), &full[stage]);
+          } else {  // the codes as a matrix of 128-byte lines
+            ts_tma_2d(dst, map, 0, static_cast<int>(row * Cfg::kRowBytes / 128), &full[stage]);
           }
-        } else {  // the codes as a matrix of 128-byte lines
-          const int line = static_cast<int>(row * Cfg::kRowBytes / 128);
-          ts_tma_2d(st, &tm_k, 0, line, &full[stage]);
-          ts_tma_2d(st + Cfg::kOffV, &tm_v, 0, line, &full[stage]);
-          if constexpr (FMT == kKvFmtNvfp4) {
-            bulk_g2s(st + Cfg::kOffKb, p.k.block_scales + row * (D / 16), Cfg::kBlockScales, &full[stage]);
-            bulk_g2s(st + Cfg::kOffVb, p.v.block_scales + row * (D / 16), Cfg::kBlockScales, &full[stage]);
+        }
+        if constexpr (kQuant) {
+          if (is_v) {
+            ts_load_scales<D, FMT, Cfg, kTsTile<FMT>>(st, p, row, all_rows, lane);
+            ts_copy_arrive(&full[stage]);
           }
-          bulk_g2s(st + Cfg::kOffKr, p.k.row_scales + row, Cfg::kRowScales, &full[stage]);
-          bulk_g2s(st + Cfg::kOffVr, p.v.row_scales + row, Cfg::kRowScales, &full[stage]);
         }
         if (++stage == Cfg::kStages) {
           stage = 0;
@@ -401,11 +508,14 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
   // ------------------------------------------------------------------ consumers
   const int g = lane >> 2, tq = lane & 3;  // fragment row / column pair
   const int rc = warp % rc_n, pw = warp / rc_n;
-  const int slices = pw_n >= 4 ? 1 : 4 / pw_n;  // per tile and warp
-  const int slice0 = pw_n >= 4 ? pw % 4 : pw * slices;
+  const int turns = pw_n >= kTurns ? 1 : kTurns / pw_n;  // per tile and warp
+  const int turn0 = pw_n >= kTurns ? pw % kTurns : pw * turns;
   TsWalk w;
   bool more = w.begin(prefix, p.batch, units, x0, x1);
   bool dead = false;
+  const int warp_slot = pw * rc_n + rc;
+  int join = 0;
+  uint32_t join_phase = 0;
   int stage = 0, turn = 0;  // the CTA's tile counter modulo kStages, modulo groups
   uint32_t phase = 0;
   while (more) {
@@ -479,16 +589,16 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
       p_unit[j][0] = p_unit[j][1] = kTsPScale / kTsMinUnit;
     }
 
-    // One slice of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
+    // SL slices of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
     auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int pos0) {
       constexpr bool EDGE = decltype(edge_tag)::value;
       const uint8_t *kt = st, *vt = st + Cfg::kOffV;
-      float s[NG][2][4];  // two accumulators, alternate steps
+      // ---- S^T = K Q^T of one slice; score rows: its positions g and 8 + g
+      auto scores = [&](int r0, float (&s)[NG][2][4]) {  // two accumulators, alternate steps
 #pragma unroll
       for (int j = 0; j < NG; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) s[j][h][0] = s[j][h][1] = s[j][h][2] = s[j][h][3] = 0.0f;
-      // ---- S^T = K Q^T; score rows: positions pos0 + g and pos0 + 8 + g
       if constexpr (FMT == kKvFmtBf16) {
         const int mat = lane >> 3, r = r0 + (mat & 1) * 8 + (lane & 7);
         const uint32_t base = smem_u32(kt) + r * 128;
@@ -496,7 +606,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
         for (int ks = 0; ks < KS; ++ks) {
           const int c = (ks & 3) * 2 + (mat >> 1);
           uint32_t a[4];
-          ts_ldsm4(base + (ks >> 2) * (kTsTile * 128) + ((c ^ (lane & 7)) << 4), a);
+          ts_ldsm4(base + (ks >> 2) * (kTsTile<FMT> * 128) + ((c ^ (lane & 7)) << 4), a);
 #pragma unroll
           for (int j = 0; j < NG; ++j) ts_mma<FMT>(s[j][ks & 1], a[0], a[1], a[2], a[3], qb[j][ks][0], qb[j][ks][1]);
         }
@@ -567,39 +677,48 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
         }
       }
 
-      // ---- scores in log2 units; sc[j][i]: position pos0 + g (+ 8 for i >= 2), column 2 tq + (i & 1)
-      [[maybe_unused]] float k_unit[2] = {1.0f, 1.0f}, v_unit[2] = {1.0f, 1.0f};
+      };
+      float s[SL][NG][2][4];
+#pragma unroll
+      for (int z = 0; z < SL; ++z) scores(r0 + 16 * z, s[z]);
+
+      // ---- scores in log2 units; sc[z][j][i]: position pos0 + 16 z + g (+ 8 for i >= 2), column 2 tq + (i & 1)
+      [[maybe_unused]] float k_unit[SL][2], v_unit[SL][2];
       if constexpr (kQuant) {
-        const float* kr = reinterpret_cast<const float*>(st + Cfg::kOffKr) + r0 + g;
-        const float* vr = reinterpret_cast<const float*>(st + Cfg::kOffVr) + r0 + g;
-        k_unit[0] = kr[0];
-        k_unit[1] = kr[8];
-        v_unit[0] = vr[0];
-        v_unit[1] = vr[8];
+#pragma unroll
+        for (int z = 0; z < SL; ++z)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = r0 + 16 * z + 8 * h + g;
+            k_unit[z][h] = reinterpret_cast<const float*>(st + Cfg::kOffKr)[r];
+            v_unit[z][h] = reinterpret_cast<const float*>(st + Cfg::kOffVr)[r];
+          }
       }
-      float sc[NG][4];
-      bool sees[NG][4];
+      float sc[SL][NG][4];
+      bool sees[SL][NG][4];
       bool above = false;
 #pragma unroll
-      for (int j = 0; j < NG; ++j)
+      for (int z = 0; z < SL; ++z)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = (s[j][0][i] + s[j][1][i]) * q_scale[j][i & 1];
-          if constexpr (kQuant) x *= k_unit[i >> 1];
-          if constexpr (EDGE) {
-            const int pos = pos0 + g + (i >> 1) * 8, u = pos - past;
-            const int t = tok[j][i & 1];
-            bool ok = t >= 0 && pos < vis;
-            if (ok && u >= 0)
-              ok = p.mask ? p.mask[b * p.mask_stride + static_cast<int64_t>(t) * p.tokens + u] != 0 : u <= t;
-            sees[j][i] = ok;
-            if (!ok) x = -INFINITY;
-          } else {
-            sees[j][i] = true;
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = (s[z][j][0][i] + s[z][j][1][i]) * q_scale[j][i & 1];
+            if constexpr (kQuant) x *= k_unit[z][i >> 1];
+            if constexpr (EDGE) {
+              const int pos = pos0 + 16 * z + g + (i >> 1) * 8, u = pos - past;
+              const int t = tok[j][i & 1];
+              bool ok = t >= 0 && pos < vis;
+              if (ok && u >= 0)
+                ok = p.mask ? p.mask[b * p.mask_stride + static_cast<int64_t>(t) * p.tokens + u] != 0 : u <= t;
+              sees[z][j][i] = ok;
+              if (!ok) x = -INFINITY;
+            } else {
+              sees[z][j][i] = true;
+            }
+            sc[z][j][i] = x;
+            above |= x > m_run[j][i & 1] + kTsSlack<FMT>;
           }
-          sc[j][i] = x;
-          above |= x > m_run[j][i & 1] + kTsSlack<FMT>;
-        }
       // ---- the reference moves (for every column) when a score passes it by the slack
       if (__any_sync(kFull, above)) {
 #pragma unroll
@@ -607,7 +726,9 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
           float alpha[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(sc[j][c], sc[j][c + 2]);
+            float mx = fmaxf(sc[0][j][c], sc[0][j][c + 2]);
+#pragma unroll
+            for (int z = 1; z < SL; ++z) mx = fmaxf(mx, fmaxf(sc[z][j][c], sc[z][j][c + 2]));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
@@ -628,10 +749,12 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
       if constexpr (kQuant) {  // the largest finite row scale of V that each column has seen
         bool up = false;
 #pragma unroll
-        for (int j = 0; j < NG; ++j)
+        for (int z = 0; z < SL; ++z)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            up |= sees[j][i] && v_unit[i >> 1] > g_run[j][i & 1] && v_unit[i >> 1] < INFINITY;
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              up |= sees[z][j][i] && v_unit[z][i >> 1] > g_run[j][i & 1] && v_unit[z][i >> 1] < INFINITY;
         if (__any_sync(kFull, up)) {
 #pragma unroll
           for (int j = 0; j < NG; ++j) {
@@ -639,8 +762,11 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               float mx = g_run[j][c];
-              if (sees[j][c] && v_unit[0] < INFINITY) mx = fmaxf(mx, v_unit[0]);
-              if (sees[j][c + 2] && v_unit[1] < INFINITY) mx = fmaxf(mx, v_unit[1]);
+#pragma unroll
+              for (int z = 0; z < SL; ++z) {
+                if (sees[z][j][c] && v_unit[z][0] < INFINITY) mx = fmaxf(mx, v_unit[z][0]);
+                if (sees[z][j][c + 2] && v_unit[z][1] < INFINITY) mx = fmaxf(mx, v_unit[z][1]);
+              }
               mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
@@ -659,34 +785,40 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
         }
       }
       // ---- P^T as B fragments
-      uint32_t ph[NG][2];
-      [[maybe_unused]] uint32_t pl[NG][2];  // second term, BF16 only
-      float pr[NG][4];
+      uint32_t ph[SL][NG][2];
+      [[maybe_unused]] uint32_t pl[SL][NG][2];  // second term, BF16 only
+      float pr[SL][NG][4];
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        float wt[4];
+      for (int z = 0; z < SL; ++z)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // -inf only stands for a key that is not seen, or one that weighs nothing
-          pr[j][i] = sc[j][i] == -INFINITY ? 0.0f : ts_exp2(sc[j][i] - m_run[j][i & 1]);
-          wt[i] = pr[j][i];
-          if constexpr (kQuant) wt[i] *= v_unit[i >> 1] * p_unit[j][i & 1];
-          if constexpr (EDGE) wt[i] = sees[j][i] ? wt[i] : 0.0f;
+        for (int j = 0; j < NG; ++j) {
+          float wt[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // -inf only stands for a key that is not seen, or one that weighs nothing
+            pr[z][j][i] = sc[z][j][i] == -INFINITY ? 0.0f : ts_exp2(sc[z][j][i] - m_run[j][i & 1]);
+            wt[i] = pr[z][j][i];
+            if constexpr (kQuant) wt[i] *= v_unit[z][i >> 1] * p_unit[j][i & 1];
+            if constexpr (EDGE) wt[i] = sees[z][j][i] ? wt[i] : 0.0f;
+          }
+          l_run[j][0] += pr[z][j][0] + pr[z][j][2];
+          l_run[j][1] += pr[z][j][1] + pr[z][j][3];
+          if constexpr (kQuant) {
+            ph[z][j][0] = ts_transpose(ts_pack_f16(wt[0], wt[1]));
+            ph[z][j][1] = ts_transpose(ts_pack_f16(wt[2], wt[3]));
+          } else {
+            const uint32_t h0 = ts_pack_bf16(wt[0], wt[1]), h1 = ts_pack_bf16(wt[2], wt[3]);
+            ph[z][j][0] = ts_transpose(h0);
+            ph[z][j][1] = ts_transpose(h1);
+            pl[z][j][0] =
+                ts_transpose(ts_pack_bf16(wt[0] - __uint_as_float(h0 << 16), wt[1] - __uint_as_float(h0 & 0xffff0000u)));
+            pl[z][j][1] =
+                ts_transpose(ts_pack_bf16(wt[2] - __uint_as_float(h1 << 16), wt[3] - __uint_as_float(h1 & 0xffff0000u)));
+          }
         }
-        l_run[j][0] += pr[j][0] + pr[j][2];
-        l_run[j][1] += pr[j][1] + pr[j][3];
-        if constexpr (kQuant) {
-          ph[j][0] = ts_transpose(ts_pack_f16(wt[0], wt[1]));
-          ph[j][1] = ts_transpose(ts_pack_f16(wt[2], wt[3]));
-        } else {
-          const uint32_t h0 = ts_pack_bf16(wt[0], wt[1]), h1 = ts_pack_bf16(wt[2], wt[3]);
-          ph[j][0] = ts_transpose(h0);
-          ph[j][1] = ts_transpose(h1);
-          pl[j][0] = ts_transpose(ts_pack_bf16(wt[0] - __uint_as_float(h0 << 16), wt[1] - __uint_as_float(h0 & 0xffff0000u)));
-          pl[j][1] = ts_transpose(ts_pack_bf16(wt[2] - __uint_as_float(h1 << 16), wt[3] - __uint_as_float(h1 & 0xffff0000u)));
-        }
-      }
-      // ---- O^T += V^T P^T
+      // ---- O^T += V^T P^T of one slice
+      auto output = [&](int r0, int pos0, const uint32_t (&ph)[NG][2], [[maybe_unused]] const uint32_t (&pl)[NG][2],
+                        [[maybe_unused]] const float (&pr)[NG][4], [[maybe_unused]] const bool (&sees)[NG][4]) {
       uint32_t bad = 0;  // positions (bits) whose V holds an infinity or NaN somewhere in this lane's part
       // Positions of the fragments' halves: 2 tq, 2 tq + 1 (registers 0, 1) and + 8 (registers 2, 3).
       auto clean = [&](uint32_t (&a)[4]) {
@@ -715,7 +847,7 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
         for (int mt = 0; mt < KS; ++mt) {
           const int c = (mt & 3) * 2 + (mat & 1);
           uint32_t a[4];
-          ts_ldsm4_trans(base + (mt >> 2) * (kTsTile * 128) + ((c ^ (lane & 7)) << 4), a);
+          ts_ldsm4_trans(base + (mt >> 2) * (kTsTile<FMT> * 128) + ((c ^ (lane & 7)) << 4), a);
           pv(mt, a);
         }
       } else {
@@ -811,18 +943,21 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
             }
         }
       }
+      };
+#pragma unroll
+      for (int z = 0; z < SL; ++z) output(r0 + 16 * z, pos0 + 16 * z, ph[z], pl[z], pr[z], sees[z]);
     };
 
     for (int t = w.t0; t < w.t1; ++t) {
-      const bool mine = pw_n < 4 || turn == (pw >> 2);
+      const bool mine = pw_n < kTurns || turn == pw / kTurns;
       if (mine) {
         if (!dead && !mbar_wait_bounded(&full[stage], phase, &g_tree_errors)) dead = true;
         const uint8_t* st = smem + stage * Cfg::kStage;
-        for (int i = 0; i < slices; ++i) {
-          const int r0 = (slice0 + i) * 16;
-          const int pos0 = t * kTsTile + r0;
+        for (int i = 0; i < turns; ++i) {
+          const int r0 = (turn0 + i) * 16 * SL;
+          const int pos0 = t * kTsTile<FMT> + r0;
           if (dead || pos0 >= vis) break;
-          if (pos0 + 16 <= past) slice(std::false_type{}, st, r0, pos0);
+          if (pos0 + 16 * SL <= past) slice(std::false_type{}, st, r0, pos0);
           else slice(std::true_type{}, st, r0, pos0);
         }
         __syncwarp();
@@ -835,7 +970,9 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
       }
     }
 
-    // ---- this segment's (m, l, o): join the position warps of each row chunk
+    // ---- this segment's (m, l, o) to the joining warps
+    if (!dead && !mbar_wait_bounded(&join_free[join], join_phase ^ 1u, &g_tree_errors)) dead = true;
+    float *so = join_o(join), *sm_m = join_m(join), *sm_l = sm_m + NW * Cfg::kRows;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
 #pragma unroll
@@ -845,68 +982,30 @@ __global__ void __launch_bounds__((NW + 1) * 32, 1)
         l += __shfl_xor_sync(kFull, l, 4);
         l += __shfl_xor_sync(kFull, l, 8);
         l += __shfl_xor_sync(kFull, l, 16);
-        const int row = warp * Cfg::kRows + 8 * j + 2 * tq + c;
+        const int r = 8 * j + 2 * tq + c;
         if (g == 0) {
-          sm_m[row] = m_run[j][c];
-          sm_l[row] = l;
+          sm_m[warp_slot * Cfg::kRows + r] = m_run[j][c];
+          sm_l[warp_slot * Cfg::kRows + r] = l;
         }
-        float* o = so + row * D;
+        float* o = so + warp_slot * Cfg::kRows * Cfg::kJoinStride;
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt) {
           if constexpr (kQuant) {
-            *reinterpret_cast<float2*>(o + D / 8 * g + 2 * mt) =
+            *reinterpret_cast<float2*>(o + join_at(r, D / 8 * g + 2 * mt)) =
                 make_float2(acc[j][mt][c] * unit, acc[j][mt][2 + c] * unit);
           } else {
-            o[16 * mt + g] = acc[j][mt][c];
-            o[16 * mt + 8 + g] = acc[j][mt][2 + c];
+            o[join_at(r, 16 * mt + g)] = acc[j][mt][c];
+            o[join_at(r, 16 * mt + 8 + g)] = acc[j][mt][2 + c];
           }
         }
       }
     }
-    ts_bar_sync(NW * 32);
-    const int n_first = pass * p.rows_per_pass;
-    const int rows = min(p.rows_per_pass, nq - n_first);
-    for (int r = threadIdx.x; r < rows; r += NW * 32) {
-      const int chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
-      float mx = -INFINITY, l = 0.0f;
-      for (int u = 0; u < pw_n; ++u) mx = fmaxf(mx, sm_m[(u * rc_n + chunk) * Cfg::kRows + rr]);
-      for (int u = 0; u < pw_n; ++u) {
-        const int i = (u * rc_n + chunk) * Cfg::kRows + rr;
-        const float f = sm_m[i] == -INFINITY ? (sm_l[i] == 0.0f ? 0.0f : 1.0f) : ts_exp2(sm_m[i] - mx);
-        sm_f[i] = f;
-        l = fmaf(sm_l[i], f, l);
-      }
-      sm_ml[r] = make_float2(mx, l);
+    __syncwarp();
+    if (lane == 0) ts_arrive(&join_full[join]);
+    if (++join == Cfg::kJoins) {
+      join = 0;
+      join_phase ^= 1u;
     }
-    ts_bar_sync(NW * 32);
-    const bool whole = w.t0 == 0 && w.t1 == w.nt;
-    const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
-    if (!whole && threadIdx.x == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
-    for (int i = threadIdx.x; i < rows * (D / 4); i += NW * 32) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4, chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int u = 0; u < pw_n; ++u) {
-        const int k = (u * rc_n + chunk) * Cfg::kRows + rr;
-        const float f = sm_f[k];
-        if (f == 0.0f) continue;
-        const float4 v = *reinterpret_cast<const float4*>(so + k * D + d);
-        o.x = fmaf(v.x, f, o.x);
-        o.y = fmaf(v.y, f, o.y);
-        o.z = fmaf(v.z, f, o.z);
-        o.w = fmaf(v.w, f, o.w);
-      }
-      if (whole) {
-        const float l = sm_ml[r].y;
-        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-        if (l == 0.0f) o = make_float4(0.f, 0.f, 0.f, 0.f);
-        *reinterpret_cast<uint2*>(p.ctx + q_row(n_first + r) * D + d) =
-            make_uint2(ts_pack_bf16(o.x * inv, o.y * inv), ts_pack_bf16(o.z * inv, o.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (slot * p.rows_per_pass + r) * D + d) = o;
-        if (d == 0) p.part_ml[slot * p.rows_per_pass + r] = sm_ml[r];
-      }
-    }
-    ts_bar_sync(NW * 32);  // the join's shared memory is reused by the next segment
     more = w.next();
   }
 }

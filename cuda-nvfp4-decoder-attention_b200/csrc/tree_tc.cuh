@@ -60,7 +60,7 @@ constexpr float kTtUnitSlack = 8.0f;
 template <int D, int FMT, bool SPLIT>  // SPLIT: 129 to 256 rows, half of them per stream
 struct TtCfg {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
-  using Codes = TsCfg<D, FMT, 1, 8>;  // the layout of a ring stage of codes
+  using Codes = TsCfg<D, FMT, 1, 8, 1, 64>;  // the layout of a ring stage of codes
   static constexpr bool kQuant = FMT != kKvFmtBf16;
   static constexpr int kPanels = D / 64;                      // 64-element panels of a row
   static constexpr uint32_t kOperand = kPanels * kTtKeys * 128;  // a K or V tile, 16-bit
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   if (tid < 2) p.part_slots[2 * cta + tid] = make_int4(-1, 0, 0, 0);
   tt_fence_before();
-  ts_prefix(p, units, prefix);
+  ts_prefix(p, units, kTtKeys, prefix);
   tt_fence_after();
   const uint32_t tmem = tmem_slot;
   // Tensor memory columns: scores [stream][buffer][64], then o [stream][D].
