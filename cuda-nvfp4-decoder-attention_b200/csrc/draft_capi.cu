@@ -20,9 +20,10 @@ constexpr int64_t kI32Max = std::numeric_limits<int32_t>::max();
 // a * b <= limit for nonnegative a, b without overflow.
 bool product_within(int64_t a, int64_t b, int64_t limit) { return a == 0 || b <= limit / a; }
 
-int lanes_per_row(int64_t head_dim) {
-  int lanes = 2;
-  while (lanes * 8 < head_dim) lanes *= 2;
+// Lanes (a power of two) that hold a row `elements` a lane.
+int lanes_per_row(int64_t head_dim, int elements) {
+  int lanes = 1;
+  while (lanes * elements < head_dim) lanes *= 2;
   return lanes;
 }
 
@@ -299,9 +300,8 @@ int nvfp4da_kv_quant_append(const nvfp4da_kv_cache* c, const uint16_t* new_k, co
       return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "past_length + current token count exceeds cache capacity");
   }
   KvAppendParams p{};
-  p.lanes = lanes_per_row(c->head_dim);
-  if (!product_within(c->batch * c->kv_heads, tokens, kI32Max / p.lanes))
-    return fail(NVFP4DA_ERR_UNSUPPORTED, "kv_quant_append: too many rows for a one-dimensional grid");
+  p.lanes = lanes_per_row(c->head_dim, 16);
+  if (tokens > kI32Max - kKvThreads) return fail(NVFP4DA_ERR_UNSUPPORTED, "kv_quant_append: too many tokens");
   p.k = k_store(*c);
   p.v = v_store(*c);
   p.new_k = new_k;
@@ -320,8 +320,8 @@ int nvfp4da_kv_quant_append(const nvfp4da_kv_cache* c, const uint16_t* new_k, co
   p.past_length = past_length;
   p.past_lengths = past_lengths;
   p.counts = counts;
-  const int64_t threads = c->batch * c->kv_heads * tokens * p.lanes;
-  const unsigned grid = static_cast<unsigned>(ceil_div(threads, kKvThreads));
+  const dim3 grid(static_cast<unsigned>(ceil_div(tokens, kKvThreads / p.lanes)),
+                  static_cast<unsigned>(c->batch * c->kv_heads));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c->format == NVFP4DA_KV_E4M3) kv_quant_append_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p);
   else kv_quant_append_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p);
@@ -343,9 +343,9 @@ int nvfp4da_kv_quant_read(const nvfp4da_kv_cache* c, int64_t start, const int64_
                 static_cast<long long>(start), static_cast<long long>(start), static_cast<long long>(length),
                 static_cast<long long>(c->capacity));
   KvReadParams p{};
-  p.lanes = lanes_per_row(c->head_dim);
-  if (!product_within(c->batch * c->kv_heads, length, (int64_t(1) << 32) / p.lanes - kKvThreads))
-    return fail(NVFP4DA_ERR_UNSUPPORTED, "kv_quant_read: too many rows for a one-dimensional grid");
+  p.lanes = lanes_per_row(c->head_dim, 8);
+  if (ceil_div(length, kKvReadRows * (kKvThreads / p.lanes)) > kI32Max)
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "kv_quant_read: too many rows for the grid");
   p.k = k_store(*c);
   p.v = v_store(*c);
   p.out_k = k_out;
@@ -357,8 +357,8 @@ int nvfp4da_kv_quant_read(const nvfp4da_kv_cache* c, int64_t start, const int64_
   p.length = length;
   p.start = start;
   p.starts = starts;
-  const int64_t threads = c->batch * c->kv_heads * length * p.lanes;
-  const unsigned grid = static_cast<unsigned>(ceil_div(threads, kKvThreads));
+  const dim3 grid(static_cast<unsigned>(ceil_div(length, kKvReadRows * (kKvThreads / p.lanes))),
+                  static_cast<unsigned>(c->batch * c->kv_heads));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (c->format == NVFP4DA_KV_E4M3) kv_quant_read_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p);
   else kv_quant_read_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p);
@@ -452,7 +452,7 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
   p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c->head_dim)));
   p.splits = pl.splits;
   p.split_len = pl.split_len;
-  p.lanes = lanes_per_row(c->head_dim);
+  p.lanes = std::max(2, lanes_per_row(c->head_dim, 8));
   const int64_t group = q_heads / c->kv_heads;
   const dim3 grid(static_cast<unsigned>(pl.splits), static_cast<unsigned>(ceil_div(group * tokens, kTreeWarps)),
                   static_cast<unsigned>(c->batch * c->kv_heads));

@@ -21,9 +21,13 @@
 // A row that holds an infinity or NaN is stored with gamma = NaN and zero
 // codes: it reads back as NaN throughout, and no code ever is NaN itself.
 //
-// 8 elements (16 BF16 bytes) per lane, D / 8 lanes of a power-of-two group per
-// row, K and V in the same thread: the row maximum is a shuffle reduction and
-// nothing is staged.  Both kernels are bound by HBM.
+// Append: a lane takes one 16-element block of a row's K and of its V, D / 16
+// lanes (a power of two) a row: the row maximum is a shuffle reduction over
+// few lanes, and the divisions of the scales are shared by 16 elements (with 8
+// per lane they were half of the instructions, which bound the kernel).  Read:
+// 8 elements per lane, so that 16-byte stores of a warp are contiguous, and
+// several rows of K and V in flight per thread.  Both are bound by HBM at the
+// sizes that fill the GPU.
 #pragma once
 
 #include <float.h>
@@ -52,7 +56,7 @@ struct KvAppendParams {
   int64_t past_length;          // used when past_lengths == nullptr
   const int64_t* past_lengths;  // device [B]
   const int64_t* counts;        // device [B] or nullptr: tokens t >= counts[b] are not written
-  int lanes;                    // lanes per row (power of two >= D / 8)
+  int lanes;                    // lanes per row (power of two >= D / 16)
   int vec_k, vec_v;             // 16-byte loads are aligned
 };
 
@@ -65,7 +69,7 @@ struct KvReadParams {
   int64_t length;
   int64_t start;          // used when starts == nullptr
   const int64_t* starts;  // device [B]
-  int lanes;
+  int lanes;              // lanes per row (power of two >= D / 8)
 };
 
 // Two FP32 values -> two E4M3 bytes (lo in the low byte), nearest even, saturating.
@@ -93,31 +97,35 @@ __device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// The lane's 8 elements (d0 = 8 * lane in the row) of a row, BF16 pairs.
-__device__ __forceinline__ uint4 kv_load8(const uint16_t* row, int d0, bool vec) {
-  if (vec) return __ldg(reinterpret_cast<const uint4*>(row + d0));
-  uint32_t w[4];
+// A lane's 16 elements of a row, BF16 pairs.
+__device__ __forceinline__ void kv_load16(const uint16_t* src, bool vec, uint32_t (&w)[8]) {
+  if (vec) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(src)), b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = static_cast<uint32_t>(row[d0 + 2 * i]) | (static_cast<uint32_t>(row[d0 + 2 * i + 1]) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 8; ++i)
+      w[i] = static_cast<uint32_t>(src[2 * i]) | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
+  }
 }
 
-// Quantise one row held 8 elements per lane by a group of `lanes` lanes and
+// Quantise one row held 16 elements per lane by a group of `lanes` lanes and
 // write it.  Every lane of the warp takes part in the shuffles; `live` lanes
-// store (d0 < D and the slot exists).
+// store (16 sub < D and the slot exists).
 template <int FMT>
-__device__ __forceinline__ void kv_quantize_row(const uint4& raw, int lanes, int sub, bool live, const KvStore& st,
-                                                int64_t row, int head_dim) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+__device__ __forceinline__ void kv_quantize_row(const uint32_t (&w)[8], int lanes, int sub, bool live,
+                                                const KvStore& st, int64_t row, int head_dim) {
   // max |x| on the bit patterns: for finite values the integer order is the
   // float order, and any infinity or NaN is >= 0x7f80.
-  uint32_t top = 0;
+  uint32_t lo = 0, hi = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-  uint32_t pair_top = max(top, __shfl_xor_sync(kFull, top, 1));  // the 16-element block
-  top = pair_top;
-  for (int o = 2; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+  for (int i = 0; i < 8; ++i) {
+    lo = max(lo, w[i] & 0x7fffu);
+    hi = max(hi, w[i] & 0x7fff0000u);
+  }
+  const uint32_t block_top = max(lo, hi >> 16);
+  uint32_t top = block_top;
+  for (int o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
   const bool finite = top < 0x7f80u;
   const float amax = __uint_as_float(top << 16);
   const float range = FMT == kKvFmtE4m3 ? 448.0f : 2688.0f;
@@ -125,88 +133,102 @@ __device__ __forceinline__ void kv_quantize_row(const uint4& raw, int lanes, int
   const float gamma =
       finite ? __fmul_rn(amax, static_cast<float>(FMT == kKvFmtE4m3 ? 1.0 / 448.0 : 1.0 / 2688.0))
              : __uint_as_float(0x7fc00000u);
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  auto lower = [&](int i) { return __uint_as_float(w[i] << 16); };
+  auto upper = [&](int i) { return __uint_as_float(w[i] & 0xffff0000u); };
   if (FMT == kKvFmtE4m3) {
     uint32_t c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = f32x2_to_e4m3x2(__fmul_rn(x[2 * i], enc), __fmul_rn(x[2 * i + 1], enc));
-    if (live)
-      *reinterpret_cast<uint2*>(st.codes + row * head_dim + sub * 8) =
-          finite ? make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16)) : make_uint2(0u, 0u);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = f32x2_to_e4m3x2(__fmul_rn(lower(2 * i), enc), __fmul_rn(upper(2 * i), enc));
+      const uint32_t b = f32x2_to_e4m3x2(__fmul_rn(lower(2 * i + 1), enc), __fmul_rn(upper(2 * i + 1), enc));
+      c[i] = finite ? a | (b << 16) : 0u;
+    }
+    if (live) *reinterpret_cast<uint4*>(st.codes + row * head_dim + sub * 16) = make_uint4(c[0], c[1], c[2], c[3]);
   } else {
-    const float bmax = __uint_as_float(pair_top << 16);
+    const float bmax = __uint_as_float(block_top << 16);
     const float mult = __fmul_rn(enc, static_cast<float>(1.0 / 6.0));
     const uint32_t sc = finite ? f32x2_to_e4m3x2(__fmul_rn(bmax, mult), 0.0f) & 0xffu : 0u;
     const float beta = decode_ue4m3(sc);
-    uint32_t codes = 0;
+    uint32_t c[2] = {0u, 0u};
     if (beta > 0.0f) {
-      const float factor = fminf(__fdiv_rn(1.0f, __fmul_rn(beta, __fdiv_rn(1.0f, enc))), FLT_MAX);
+      const float factor = fminf(__frcp_rn(__fmul_rn(beta, __frcp_rn(enc))), FLT_MAX);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        codes |= f32x2_to_e2m1x2(__fmul_rn(x[2 * i], factor), __fmul_rn(x[2 * i + 1], factor)) << (8 * i);
+      for (int i = 0; i < 8; ++i)
+        c[i / 4] |= f32x2_to_e2m1x2(__fmul_rn(lower(i), factor), __fmul_rn(upper(i), factor)) << (8 * (i % 4));
     }
     if (live) {
-      *reinterpret_cast<uint32_t*>(st.codes + row * (head_dim / 2) + sub * 4) = codes;
-      if ((sub & 1) == 0) st.block_scales[row * (head_dim / 16) + (sub >> 1)] = static_cast<uint8_t>(sc);
+      *reinterpret_cast<uint2*>(st.codes + row * (head_dim / 2) + sub * 8) = make_uint2(c[0], c[1]);
+      st.block_scales[row * (head_dim / 16) + sub] = static_cast<uint8_t>(sc);
     }
   }
   if (live && sub == 0) st.row_scales[row] = gamma;
 }
 
+// Grid (rows of T, B * Hkv).
 template <int FMT>
 __global__ void __launch_bounds__(kKvThreads) kv_quant_append_kernel(const KvAppendParams p) {
-  const int lane = threadIdx.x & 31;
-  const int sub = lane & (p.lanes - 1);
-  const uint32_t group = (blockIdx.x * kKvThreads + threadIdx.x) / p.lanes;
-  const uint32_t total = static_cast<uint32_t>(p.batch) * p.kv_heads * p.tokens;
-  // Row order (b, h, t): consecutive groups write consecutive cache rows.
-  const uint32_t i = group < total ? group : 0;
-  const uint32_t t = i % p.tokens, bh = i / p.tokens, h = bh % p.kv_heads, b = bh / p.kv_heads;
+  const int sub = threadIdx.x & (p.lanes - 1);
+  const int t = blockIdx.x * (kKvThreads / p.lanes) + threadIdx.x / p.lanes;
+  const int h = blockIdx.y % p.kv_heads, b = blockIdx.y / p.kv_heads;
   const int64_t past = p.past_lengths ? p.past_lengths[b] : p.past_length;
   const int64_t slot = past + t;
-  bool live = group < total && sub * 8 < p.head_dim && past >= 0 && past < p.capacity && slot < p.capacity;
+  bool live = t < p.tokens && sub * 16 < p.head_dim && past >= 0 && past < p.capacity && slot < p.capacity;
   if (live && p.counts) live = t < p.counts[b];
-  uint4 rk = make_uint4(0, 0, 0, 0), rv = rk;
+  uint32_t wk[8] = {}, wv[8] = {};
   if (live) {
-    rk = kv_load8(p.new_k + b * p.k_stride[0] + t * p.k_stride[1] + h * p.k_stride[2], sub * 8, p.vec_k);
-    rv = kv_load8(p.new_v + b * p.v_stride[0] + t * p.v_stride[1] + h * p.v_stride[2], sub * 8, p.vec_v);
+    kv_load16(p.new_k + b * p.k_stride[0] + t * p.k_stride[1] + h * p.k_stride[2] + sub * 16, p.vec_k, wk);
+    kv_load16(p.new_v + b * p.v_stride[0] + t * p.v_stride[1] + h * p.v_stride[2] + sub * 16, p.vec_v, wv);
   }
-  const int64_t row = static_cast<int64_t>(bh) * p.capacity + slot;
-  kv_quantize_row<FMT>(rk, p.lanes, sub, live, p.k, row, p.head_dim);
-  kv_quantize_row<FMT>(rv, p.lanes, sub, live, p.v, row, p.head_dim);
+  const int64_t row = static_cast<int64_t>(blockIdx.y) * p.capacity + slot;
+  kv_quantize_row<FMT>(wk, p.lanes, sub, live, p.k, row, p.head_dim);
+  kv_quantize_row<FMT>(wv, p.lanes, sub, live, p.v, row, p.head_dim);
 }
 
-// 8 elements of a stored row, FP32: (code * beta) * gamma, or code * gamma.
+// 8 elements of a stored row as they are in memory (zeros: a row of zeros).
+template <int FMT>
+struct KvRaw {
+  uint32_t c[FMT == kKvFmtE4m3 ? 2 : 1] = {};
+  uint32_t beta = 0;
+  float gamma = 0.0f;
+};
+
+template <int FMT>
+__device__ __forceinline__ KvRaw<FMT> kv_fetch8(const KvStore& st, int64_t row, int d0, int head_dim) {
+  KvRaw<FMT> r;
+  r.gamma = __ldg(st.row_scales + row);
+  if constexpr (FMT == kKvFmtE4m3) {
+    const uint2 c = __ldg(reinterpret_cast<const uint2*>(st.codes + row * head_dim + d0));
+    r.c[0] = c.x;
+    r.c[1] = c.y;
+  } else {
+    r.c[0] = __ldg(reinterpret_cast<const uint32_t*>(st.codes + row * (head_dim / 2) + d0 / 2));
+    r.beta = __ldg(st.block_scales + row * (head_dim / 16) + d0 / 16);
+  }
+  return r;
+}
+
+// Their FP32 values: (code * beta) * gamma, or code * gamma.
+template <int FMT>
+__device__ __forceinline__ void kv_decode8(const KvRaw<FMT>& r, float (&x)[8]) {
+  uint32_t h[4];
+  if constexpr (FMT == kKvFmtE4m3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = e4m3x2_to_f16x2(r.c[i / 2] >> (16 * (i % 2)) & 0xffffu);
+  } else {
+    e2m1x8_to_f16x2x4(r.c[0], h);
+  }
+  const float beta = FMT == kKvFmtNvfp4 ? decode_ue4m3(r.beta) : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = f16x2_to_f32x2(h[i]);
+    x[2 * i] = __fmul_rn(FMT == kKvFmtNvfp4 ? __fmul_rn(f.x, beta) : f.x, r.gamma);
+    x[2 * i + 1] = __fmul_rn(FMT == kKvFmtNvfp4 ? __fmul_rn(f.y, beta) : f.y, r.gamma);
+  }
+}
+
 template <int FMT>
 __device__ __forceinline__ void kv_decode8(const KvStore& st, int64_t row, int d0, int head_dim, float (&x)[8]) {
-  const float gamma = __ldg(st.row_scales + row);
-  if (FMT == kKvFmtE4m3) {
-    const uint2 c = __ldg(reinterpret_cast<const uint2*>(st.codes + row * head_dim + d0));
-    const uint32_t h[4] = {e4m3x2_to_f16x2(c.x & 0xffffu), e4m3x2_to_f16x2(c.x >> 16), e4m3x2_to_f16x2(c.y & 0xffffu),
-                           e4m3x2_to_f16x2(c.y >> 16)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = f16x2_to_f32x2(h[i]);
-      x[2 * i] = __fmul_rn(f.x, gamma);
-      x[2 * i + 1] = __fmul_rn(f.y, gamma);
-    }
-  } else {
-    const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(st.codes + row * (head_dim / 2) + d0 / 2));
-    const float beta = decode_ue4m3(__ldg(st.block_scales + row * (head_dim / 16) + d0 / 16));
-    uint32_t h[4];
-    e2m1x8_to_f16x2x4(c, h);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = f16x2_to_f32x2(h[i]);
-      x[2 * i] = __fmul_rn(__fmul_rn(f.x, beta), gamma);
-      x[2 * i + 1] = __fmul_rn(__fmul_rn(f.y, beta), gamma);
-    }
-  }
+  kv_decode8<FMT>(kv_fetch8<FMT>(st, row, d0, head_dim), x);
 }
 
 __device__ __forceinline__ uint4 kv_pack8(const float (&x)[8]) {
@@ -218,26 +240,39 @@ __device__ __forceinline__ uint4 kv_pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Grid (rows of the window, B * Hkv); a thread takes kKvReadRows rows.
+constexpr int kKvReadRows = 4;
+
 template <int FMT>
 __global__ void __launch_bounds__(kKvThreads) kv_quant_read_kernel(const KvReadParams p) {
-  const int sub = threadIdx.x & (p.lanes - 1);
-  const uint32_t group = (blockIdx.x * kKvThreads + threadIdx.x) / p.lanes;
-  const uint32_t len = static_cast<uint32_t>(p.length);
-  const uint32_t total = static_cast<uint32_t>(p.batch) * p.kv_heads * len;
-  if (group >= total || sub * 8 >= p.head_dim) return;
-  const uint32_t j = group % len, bh = group / len, b = bh / p.kv_heads;
-  const int64_t start = p.starts ? p.starts[b] : p.start;
+  const int sub = threadIdx.x & (p.lanes - 1), d0 = sub * 8;
+  if (d0 >= p.head_dim) return;
+  const int step = kKvThreads / p.lanes;
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x) * step * kKvReadRows + threadIdx.x / p.lanes;
+  const int64_t start = p.starts ? p.starts[blockIdx.y / p.kv_heads] : p.start;
   // Rows outside the cache read as zeros.
-  const bool inside = start > -static_cast<int64_t>(len) && start < p.capacity && start + j >= 0 && start + j < p.capacity;
-  float k[8] = {}, v[8] = {};
-  if (inside) {
-    const int64_t row = static_cast<int64_t>(bh) * p.capacity + start + j;
-    kv_decode8<FMT>(p.k, row, sub * 8, p.head_dim, k);
-    kv_decode8<FMT>(p.v, row, sub * 8, p.head_dim, v);
+  const int64_t first = start > -p.length && start < p.capacity ? start : p.capacity;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * p.capacity + first;
+  KvRaw<FMT> k[kKvReadRows], v[kKvReadRows];
+#pragma unroll
+  for (int i = 0; i < kKvReadRows; ++i) {
+    const int64_t j = j0 + i * step;
+    if (j < p.length && first + j >= 0 && first + j < p.capacity) {
+      k[i] = kv_fetch8<FMT>(p.k, row0 + j, d0, p.head_dim);
+      v[i] = kv_fetch8<FMT>(p.v, row0 + j, d0, p.head_dim);
+    }
   }
-  const int64_t dst = static_cast<int64_t>(group) * p.head_dim + sub * 8;
-  *reinterpret_cast<uint4*>(p.out_k + dst) = kv_pack8(k);
-  *reinterpret_cast<uint4*>(p.out_v + dst) = kv_pack8(v);
+#pragma unroll
+  for (int i = 0; i < kKvReadRows; ++i) {
+    const int64_t j = j0 + i * step;
+    if (j >= p.length) return;
+    const int64_t dst = (static_cast<int64_t>(blockIdx.y) * p.length + j) * p.head_dim + d0;
+    float x[8];
+    kv_decode8<FMT>(k[i], x);
+    *reinterpret_cast<uint4*>(p.out_k + dst) = kv_pack8(x);
+    kv_decode8<FMT>(v[i], x);
+    *reinterpret_cast<uint4*>(p.out_v + dst) = kv_pack8(x);
+  }
 }
 
 }  // namespace nvfp4da

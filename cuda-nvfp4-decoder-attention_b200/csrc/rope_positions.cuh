@@ -21,7 +21,7 @@
 
 namespace nvfp4da {
 
-constexpr int kRopeThreads = 128;
+constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxPairs = 1024;  // (cos, sin) pairs a block keeps
 
 struct RopeQkParams {
@@ -73,6 +73,63 @@ __global__ void __launch_bounds__(kRopeThreads) rope_qk_kernel(const RopeQkParam
   const int pairs = p.rotary_dim / 2;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block;
   const int n_rows = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.rows - row0));
+  // Items of V elements (half layout, and adjacent pairs that no 4-byte access
+  // covers: V pairs); those past the rotated part are copies.
+  constexpr bool kTwo = !ADJACENT || V == 1;  // an item is two pieces
+  const int rot = kTwo ? pairs / V : p.rotary_dim / V;
+  const int items = rot + (p.head_dim - p.rotary_dim) / V;
+  const int heads = p.q_heads + p.kv_heads, total = n_rows * heads * items;
+  struct Item {
+    alignas(16) uint16_t x[V], z[V];
+    uint16_t* dst;  // of x
+    int apart;      // elements from x to z; 0: one piece
+    int at;         // its first pair in the table; -1: a copy
+  };
+  auto load = [&](int i, Item& it) {
+    const int c = i % items, rh = i / items, hh = rh % heads, r = rh / heads;
+    const int64_t row = row0 + r, b = row / p.tokens, t = row % p.tokens;
+    const bool is_q = hh < p.q_heads;
+    const int h = is_q ? hh : hh - p.q_heads;
+    const uint16_t* src = is_q ? p.q + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2]
+                               : p.k + b * p.k_stride[0] + t * p.k_stride[1] + h * p.k_stride[2];
+    it.dst = is_q ? p.q_out + (row * p.q_heads + h) * p.head_dim : p.k_out + (row * p.kv_heads + h) * p.head_dim;
+    int d = 0;
+    it.apart = 0;
+    it.at = -1;
+    if (c >= rot) {
+      d = p.rotary_dim + (c - rot) * V;
+    } else if constexpr (ADJACENT) {
+      d = V == 1 ? 2 * c : c * V;
+      it.at = r * pairs + d / 2;
+      it.apart = V == 1 ? 1 : 0;
+    } else {
+      d = c * V;
+      it.at = r * pairs + d;
+      it.apart = pairs;
+    }
+    it.dst += d;
+    rope_load<V>(src + d, it.x);
+    if (kTwo && it.apart) rope_load<V>(src + d + it.apart, it.z);
+  };
+  auto finish = [&](Item& it) {
+    if (it.at >= 0) {
+      if constexpr (kTwo) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          rope_turn(bf16_bits_to_f32(it.x[e]), bf16_bits_to_f32(it.z[e]), table[it.at + e], it.x[e], it.z[e]);
+        rope_store<V>(it.dst + it.apart, it.z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e)
+          rope_turn(bf16_bits_to_f32(it.x[2 * e]), bf16_bits_to_f32(it.x[2 * e + 1]), table[it.at + e], it.x[2 * e],
+                    it.x[2 * e + 1]);
+      }
+    }
+    rope_store<V>(it.dst, it.x);
+  };
+  // The first item of every thread is on its way while the table is made.
+  Item first;
+  if (threadIdx.x < total) load(threadIdx.x, first);
   for (int i = threadIdx.x; i < n_rows * pairs; i += kRopeThreads) {
     const int64_t row = row0 + i / pairs;
     const int64_t pos = p.positions[(row / p.tokens) * p.pos_stride + row % p.tokens];
@@ -83,45 +140,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_qk_kernel(const RopeQkParam
     table[i] = make_float2(__fmul_rn(c, p.factor), __fmul_rn(s, p.factor));
   }
   __syncthreads();
-  // Items of V elements (half layout, and adjacent pairs that no 4-byte access
-  // covers: V pairs); those past the rotated part are copies.
-  const int rot = ADJACENT && V > 1 ? p.rotary_dim / V : pairs / V;
-  const int items = rot + (p.head_dim - p.rotary_dim) / V;
-  const int heads = p.q_heads + p.kv_heads;
-  for (int i = threadIdx.x; i < n_rows * heads * items; i += kRopeThreads) {
-    const int c = i % items, rh = i / items, hh = rh % heads, r = rh / heads;
-    const int64_t row = row0 + r, b = row / p.tokens, t = row % p.tokens;
-    const bool is_q = hh < p.q_heads;
-    const int h = is_q ? hh : hh - p.q_heads;
-    const uint16_t* src = is_q ? p.q + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2]
-                               : p.k + b * p.k_stride[0] + t * p.k_stride[1] + h * p.k_stride[2];
-    uint16_t* dst = (is_q ? p.q_out + (row * p.q_heads + h) * p.head_dim : p.k_out + (row * p.kv_heads + h) * p.head_dim);
-    alignas(16) uint16_t x[V];
-    if (c >= rot) {
-      const int d = p.rotary_dim + (c - rot) * V;
-      rope_load<V>(src + d, x);
-      rope_store<V>(dst + d, x);
-    } else if constexpr (ADJACENT && V == 1) {
-      rope_turn(bf16_bits_to_f32(src[2 * c]), bf16_bits_to_f32(src[2 * c + 1]), table[r * pairs + c], dst[2 * c],
-                dst[2 * c + 1]);
-    } else if constexpr (ADJACENT) {
-      alignas(16) uint16_t y[V];
-      rope_load<V>(src + c * V, x);
-#pragma unroll
-      for (int e = 0; e < V / 2; ++e)
-        rope_turn(bf16_bits_to_f32(x[2 * e]), bf16_bits_to_f32(x[2 * e + 1]), table[r * pairs + c * (V / 2) + e],
-                  y[2 * e], y[2 * e + 1]);
-      rope_store<V>(dst + c * V, y);
-    } else {
-      alignas(16) uint16_t z[V], ye[V], yo[V];
-      rope_load<V>(src + c * V, x);
-      rope_load<V>(src + pairs + c * V, z);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        rope_turn(bf16_bits_to_f32(x[e]), bf16_bits_to_f32(z[e]), table[r * pairs + c * V + e], ye[e], yo[e]);
-      rope_store<V>(dst + c * V, ye);
-      rope_store<V>(dst + pairs + c * V, yo);
-    }
+  if (threadIdx.x < total) finish(first);
+  for (int i = threadIdx.x + kRopeThreads; i < total; i += kRopeThreads) {
+    Item it;
+    load(i, it);
+    finish(it);
   }
 }
 
