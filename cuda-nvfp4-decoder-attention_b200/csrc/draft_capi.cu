@@ -80,7 +80,7 @@ cudaError_t launch_rope(RopeQkParams p, cudaStream_t s) {
   int64_t tpb = std::max<int64_t>(1, kRopeThreads / per_token);
   if (pairs > 0) tpb = std::min<int64_t>(tpb, kRopeMaxPairs / pairs);
   p.tokens_per_block = static_cast<int>(tpb);
-  rope_qk_kernel<V, ADJACENT><<<static_cast<unsigned>(ceil_div(p.rows, tpb)), kRopeThreads, 0, s>>>(p);
+  rope_qk_kernel<V, ADJACENT><<<static_cast<unsigned>(ceil_div(static_cast<int64_t>(p.rows), tpb)), kRopeThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -269,8 +269,8 @@ int nvfp4da_apply_rope_qk(const uint16_t* q, const int64_t* q_strides, uint16_t*
   p.pos_stride = position_stride;
   p.inv_freq = inv_freq;
   p.factor = attention_factor;
-  p.rows = batch * tokens;
-  p.tokens = static_cast<int>(tokens);
+  p.rows = static_cast<uint32_t>(batch * tokens);
+  p.tokens = static_cast<uint32_t>(tokens);
   p.q_heads = static_cast<int>(q_heads);
   p.kv_heads = static_cast<int>(kv_heads);
   p.head_dim = static_cast<int>(head_dim);

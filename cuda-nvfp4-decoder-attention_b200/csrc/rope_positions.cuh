@@ -12,9 +12,10 @@
 // position 1e6 as at 1; sine and cosine are FP32, and each output is rounded
 // to BF16 once.  At position 0 elements are only scaled by A.
 //
-// A block takes the tokens of one (token, all heads) group: the (cos, sin)
-// pairs of a token are computed once, in shared memory, and used by every
-// head.  Bound by HBM: each element is read once and written once.
+// A block takes one token (several where heads are few): the sines and cosines
+// are computed once per token, in shared memory, laid out so that one 16-byte
+// load serves two FP32x2 operations.  Bound by HBM: each element is read once
+// and written once, with its first loads on their way while the table is made.
 #pragma once
 
 #include "common.cuh"
@@ -34,8 +35,9 @@ struct RopeQkParams {
   int64_t pos_stride;
   const float* inv_freq;  // [R / 2]
   float factor;
-  int64_t rows;  // B * T
-  int tokens, q_heads, kv_heads, head_dim, rotary_dim;
+  uint32_t rows;  // B * T, below 2^31 (32-bit divisions: 64-bit ones took longer than the memory)
+  uint32_t tokens;
+  int q_heads, kv_heads, head_dim, rotary_dim;
   int tokens_per_block;
 };
 
@@ -55,97 +57,144 @@ __device__ __forceinline__ void rope_store(uint16_t* dst, const uint16_t (&x)[V]
   else *dst = x[0];
 }
 
-// The pair (xe, xo) turned by (c, s).  s == 0 only scales (an infinity in the
-// other element must not reach this one).
-__device__ __forceinline__ void rope_turn(float xe, float xo, float2 cs, uint16_t& ye, uint16_t& yo) {
-  if (cs.y == 0.0f) {
-    ye = f32_to_bf16_bits(__fmul_rn(xe, cs.x));
-    yo = f32_to_bf16_bits(__fmul_rn(xo, cs.x));
-  } else {
-    ye = f32_to_bf16_bits(fmaf(xe, cs.x, -__fmul_rn(xo, cs.y)));
-    yo = f32_to_bf16_bits(fmaf(xe, cs.y, __fmul_rn(xo, cs.x)));
-  }
+__device__ __forceinline__ float2 rope_mul2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}" : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 rope_fma2(float2 a, float2 b, float2 d) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 w, {%6, %7};\n"
+      " fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(d.x), "f"(d.y));
+  return c;
+}
+__device__ __forceinline__ uint32_t rope_pack(float2 v) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
+__device__ __forceinline__ float2 rope_unpack(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// Items of V elements, or where an item is two pieces (half layout; adjacent
+// pairs that no 4-byte access covers) V pairs; those past the rotated part are
+// copies.
 template <int V, bool ADJACENT>
 __global__ void __launch_bounds__(kRopeThreads) rope_qk_kernel(const RopeQkParams p) {
-  __shared__ float2 table[kRopeMaxPairs];
+  constexpr bool kTwo = !ADJACENT || V == 1;
+  constexpr bool kPairs = kTwo && V > 1;  // a table entry serves two pairs: {c0, c1, s0, s1}, else {c, s, -s, c}
+  constexpr int W = kTwo ? V : V / 2;     // pairs per item
+  __shared__ float4 table[kRopeMaxPairs];
+  __shared__ unsigned char at_zero[kRopeMaxPairs];  // tokens at position 0: only scaled
   const int pairs = p.rotary_dim / 2;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block;
-  const int n_rows = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.rows - row0));
-  // Items of V elements (half layout, and adjacent pairs that no 4-byte access
-  // covers: V pairs); those past the rotated part are copies.
-  constexpr bool kTwo = !ADJACENT || V == 1;  // an item is two pieces
+  const uint32_t row0 = blockIdx.x * static_cast<uint32_t>(p.tokens_per_block);
+  const int n_rows = static_cast<int>(min(static_cast<uint32_t>(p.tokens_per_block), p.rows - row0));
   const int rot = kTwo ? pairs / V : p.rotary_dim / V;
   const int items = rot + (p.head_dim - p.rotary_dim) / V;
-  const int heads = p.q_heads + p.kv_heads, total = n_rows * heads * items;
+  const int heads = p.q_heads + p.kv_heads;
+  // Threads as tx items by ty heads.
+  const int tx = min(items, kRopeThreads), ty = kRopeThreads / tx;
+  const int y0 = threadIdx.x / tx, c0 = threadIdx.x - y0 * tx;
+  const uint32_t b0 = row0 / p.tokens, t0 = row0 - b0 * p.tokens;
   struct Item {
-    alignas(16) uint16_t x[V], z[V];
-    uint16_t* dst;  // of x
-    int apart;      // elements from x to z; 0: one piece
-    int at;         // its first pair in the table; -1: a copy
+    alignas(16) uint16_t x[V];
+    alignas(16) uint16_t z[V];
+    uint16_t* dst;
+    int r;
   };
-  auto load = [&](int i, Item& it) {
-    const int c = i % items, rh = i / items, hh = rh % heads, r = rh / heads;
-    const int64_t row = row0 + r, b = row / p.tokens, t = row % p.tokens;
+  auto load = [&](int y, int c, Item& it) {
+    int r = 0, hh = y;
+    uint32_t row = row0, b = b0, t = t0;
+    if (n_rows > 1) {
+      r = y / heads;
+      hh = y - r * heads;
+      row += r;
+      b = row / p.tokens;
+      t = row - b * p.tokens;
+    }
     const bool is_q = hh < p.q_heads;
     const int h = is_q ? hh : hh - p.q_heads;
-    const uint16_t* src = is_q ? p.q + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2]
-                               : p.k + b * p.k_stride[0] + t * p.k_stride[1] + h * p.k_stride[2];
-    it.dst = is_q ? p.q_out + (row * p.q_heads + h) * p.head_dim : p.k_out + (row * p.kv_heads + h) * p.head_dim;
-    int d = 0;
-    it.apart = 0;
-    it.at = -1;
-    if (c >= rot) {
-      d = p.rotary_dim + (c - rot) * V;
-    } else if constexpr (ADJACENT) {
-      d = V == 1 ? 2 * c : c * V;
-      it.at = r * pairs + d / 2;
-      it.apart = V == 1 ? 1 : 0;
-    } else {
-      d = c * V;
-      it.at = r * pairs + d;
-      it.apart = pairs;
-    }
-    it.dst += d;
-    rope_load<V>(src + d, it.x);
-    if (kTwo && it.apart) rope_load<V>(src + d + it.apart, it.z);
+    const int d = c >= rot ? p.rotary_dim + (c - rot) * V : (ADJACENT && V == 1 ? 2 * c : c * V);
+    const uint16_t* src = (is_q ? p.q + b * p.q_stride[0] + t * p.q_stride[1] + h * p.q_stride[2]
+                                : p.k + b * p.k_stride[0] + t * p.k_stride[1] + h * p.k_stride[2]) + d;
+    it.dst = (is_q ? p.q_out + (static_cast<int64_t>(row) * p.q_heads + h) * p.head_dim
+                   : p.k_out + (static_cast<int64_t>(row) * p.kv_heads + h) * p.head_dim) + d;
+    it.r = r;
+    rope_load<V>(src, it.x);
+    if (kTwo && c < rot) rope_load<V>(src + (ADJACENT ? 1 : pairs), it.z);
   };
-  auto finish = [&](Item& it) {
-    if (it.at >= 0) {
-      if constexpr (kTwo) {
+  auto finish = [&](int c, Item& it) {
+    if (c < rot) {
+      const float4* entry = table + it.r * pairs + c;
+      const bool turn = !at_zero[it.r];
+      if constexpr (kPairs) {
+        uint32_t *x = reinterpret_cast<uint32_t*>(it.x), *z = reinterpret_cast<uint32_t*>(it.z);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          rope_turn(bf16_bits_to_f32(it.x[e]), bf16_bits_to_f32(it.z[e]), table[it.at + e], it.x[e], it.z[e]);
-        rope_store<V>(it.dst + it.apart, it.z);
+        for (int e = 0; e < V / 2; ++e) {
+          const float4 u = entry[e * rot];
+          const float2 a = rope_unpack(x[e]), o = rope_unpack(z[e]), cs = make_float2(u.x, u.y);
+          float2 ya = rope_mul2(a, cs), yo = rope_mul2(o, cs);
+          if (turn) {
+            ya = rope_fma2(o, make_float2(-u.z, -u.w), ya);
+            yo = rope_fma2(a, make_float2(u.z, u.w), yo);
+          }
+          x[e] = rope_pack(ya);
+          z[e] = rope_pack(yo);
+        }
+      } else if constexpr (kTwo) {
+        const float4 u = entry[0];
+        const float a = bf16_bits_to_f32(it.x[0]), o = bf16_bits_to_f32(it.z[0]);
+        it.x[0] = f32_to_bf16_bits(turn ? fmaf(o, u.z, __fmul_rn(a, u.x)) : __fmul_rn(a, u.x));
+        it.z[0] = f32_to_bf16_bits(turn ? fmaf(a, u.y, __fmul_rn(o, u.x)) : __fmul_rn(o, u.x));
       } else {
+        uint32_t* x = reinterpret_cast<uint32_t*>(it.x);
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e)
-          rope_turn(bf16_bits_to_f32(it.x[2 * e]), bf16_bits_to_f32(it.x[2 * e + 1]), table[it.at + e], it.x[2 * e],
-                    it.x[2 * e + 1]);
+        for (int e = 0; e < W; ++e) {
+          const float4 u = entry[e * rot];
+          const float2 v = rope_unpack(x[e]);
+          x[e] = rope_pack(turn ? rope_fma2(make_float2(v.y, v.y), make_float2(u.z, u.w),
+                                            rope_mul2(make_float2(v.x, v.x), make_float2(u.x, u.y)))
+                                : rope_mul2(v, make_float2(u.x, u.x)));
+        }
       }
+      if constexpr (kTwo) rope_store<V>(it.dst + (ADJACENT ? 1 : pairs), it.z);
     }
     rope_store<V>(it.dst, it.x);
   };
-  // The first item of every thread is on its way while the table is made.
+  const int last = n_rows * heads;
+  const bool busy = y0 < ty;
   Item first;
-  if (threadIdx.x < total) load(threadIdx.x, first);
+  if (busy && y0 < last && c0 < items) load(y0, c0, first);
   for (int i = threadIdx.x; i < n_rows * pairs; i += kRopeThreads) {
-    const int64_t row = row0 + i / pairs;
-    const int64_t pos = p.positions[(row / p.tokens) * p.pos_stride + row % p.tokens];
+    const int r = n_rows == 1 ? 0 : i / pairs, m = i - r * pairs;
+    const uint32_t row = row0 + r, b = row / p.tokens;
+    const int64_t pos = p.positions[b * p.pos_stride + (row - b * p.tokens)];
     // a / pi, reduced to [-1, 1]
-    const double turns = static_cast<double>(pos) * static_cast<double>(p.inv_freq[i % pairs]) * 0.31830988618379067154;
+    const double turns = static_cast<double>(pos) * static_cast<double>(p.inv_freq[m]) * 0.31830988618379067154;
     float s, c;
     sincospif(static_cast<float>(turns - 2.0 * rint(0.5 * turns)), &s, &c);
-    table[i] = make_float2(__fmul_rn(c, p.factor), __fmul_rn(s, p.factor));
+    c = __fmul_rn(c, p.factor);
+    s = __fmul_rn(s, p.factor);
+    const int e = m % W, item = m / W;
+    if constexpr (kPairs) {
+      float* u = reinterpret_cast<float*>(table + r * pairs + e / 2 * rot + item) + e % 2;
+      u[0] = c;
+      u[2] = s;
+    } else {
+      table[r * pairs + e * rot + item] = make_float4(c, s, -s, c);
+    }
+    if (m == 0) at_zero[r] = pos == 0;
   }
   __syncthreads();
-  if (threadIdx.x < total) finish(first);
-  for (int i = threadIdx.x + kRopeThreads; i < total; i += kRopeThreads) {
-    Item it;
-    load(i, it);
-    finish(it);
-  }
+  if (!busy) return;
+  for (int y = y0; y < last; y += ty)
+    for (int c = c0; c < items; c += tx) {
+      if (y != y0 || c != c0) load(y, c, first);
+      finish(c, first);
+    }
 }
 
 }  // namespace nvfp4da
