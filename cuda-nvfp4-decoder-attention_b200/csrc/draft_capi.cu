@@ -124,8 +124,7 @@ cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const T
     return cudaErrorLaunchOutOfResources;
   cudaError_t e = ensure_smem(kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<p.grid, kTtThreads, smem, s>>>(tk, tv, p);
-  e = cudaGetLastError();
+  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(kTtThreads), smem, s, true, tk, tv, p);
   return e != cudaSuccess ? e : launch_tree_combine<D>(p, s);
 }
 
@@ -137,8 +136,7 @@ cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, con
   const uint32_t smem = TsCfg<D, FMT, NG, NW, SL>::bytes(p.batch);
   cudaError_t e = ensure_smem(kern, smem);
   if (e != cudaSuccess) return e;
-  kern<<<p.grid, TsCfg<D, FMT, NG, NW, SL>::kThreads, smem, s>>>(tk, tv, p);
-  e = cudaGetLastError();
+  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(TsCfg<D, FMT, NG, NW, SL>::kThreads), smem, s, true, tk, tv, p);
   return e != cudaSuccess ? e : launch_tree_combine<D>(p, s);
 }
 

@@ -398,6 +398,8 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
   }
+  // Nothing of global memory before this: the launch may overlap the kernel ahead.
+  pdl_wait();
   ts_prefix(p, units, kTsTile<FMT>, prefix);
   const int n_tiles = prefix[p.batch];
   // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
@@ -1017,6 +1019,7 @@ constexpr int kTsJoinWarps = 8;
 
 template <int D>
 __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(const TreeStreamParams p) {
+  pdl_launch_dependents();
   pdl_wait();
   const int4 unit = __ldcg(&p.part_slots[blockIdx.x]);
   if (unit.x < 0) return;
@@ -1028,29 +1031,41 @@ __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(
   auto at = [&](int c) {
     return (c == c0 ? static_cast<int64_t>(blockIdx.x) : 2 * static_cast<int64_t>(c)) * p.rows_per_pass + r;
   };
+  constexpr int V = D / 32;  // elements per lane
+  constexpr int kAtOnce = 8;  // parts whose loads are in flight together
+  float x[kAtOnce][V];
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (c + i > c1) break;
+      const float* src = p.part_o + at(c + i) * D + lane * V;
+      if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(x[i]) = __ldcg(reinterpret_cast<const float2*>(src));
+      } else {
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k) reinterpret_cast<float4*>(x[i])[k] = __ldcg(reinterpret_cast<const float4*>(src) + k);
+      }
+    }
+  };
+  fetch(c0);  // beside the (m, l) loads
   float mx = -INFINITY;
   for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(&p.part_ml[at(c)]).x);
   mx = warp_max_f32(mx);
-  constexpr int V = D / 32;  // elements per lane
   float o[V] = {}, l = 0.0f;
   for (int base = c0; base <= c1; base += 32) {
     const float2 ml = base + lane <= c1 ? __ldcg(&p.part_ml[at(base + lane)]) : make_float2(-INFINITY, 0.0f);
     const float f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(ml.x - mx);
     l = fmaf(ml.y, f, l);
-    const int count = min(32, c1 - base + 1);
-#pragma unroll 4
-    for (int c = 0; c < count; ++c) {
-      const float fc = __shfl_sync(kFull, f, c);
-      const float* src = p.part_o + at(base + c) * D + lane * V;
-      float x[V];
-      if constexpr (V == 2) {
-        *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(src));
-      } else {
+    const int end = min(base + 31, c1);
+    for (int c = base; c <= end; c += kAtOnce) {
+      if (c != c0) fetch(c);
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i) reinterpret_cast<float4*>(x)[i] = __ldcg(reinterpret_cast<const float4*>(src) + i);
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float fc = __shfl_sync(kFull, f, (c - base + i) & 31);
+        if (c + i > c1 || fc == 0.0f) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = fmaf(x[i][k], fc, o[k]);
       }
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = fc == 0.0f ? o[i] : fmaf(x[i], fc, o[i]);
     }
   }
   l = warp_sum_f32(l);

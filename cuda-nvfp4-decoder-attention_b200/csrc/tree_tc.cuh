@@ -310,6 +310,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     s_bad = 0u;
     s_wild = 0u;
   }
+  // Nothing of global memory before this: the launch may overlap the kernel ahead.
+  pdl_wait();
   if (tid < 2) p.part_slots[2 * cta + tid] = make_int4(-1, 0, 0, 0);
   tt_fence_before();
   ts_prefix(p, units, kTtKeys, prefix);
