@@ -17,7 +17,8 @@
 // Roles: warps 0-3 and 4-7 softmax of streams 0 and 1 (one query row per
 // thread); warps 8-15 prepare operands (K and V); warps 16 and 18 issue the MMAs of a
 // stream each (one warp for both could not issue them fast enough beside the
-// others on its scheduler); warp 17 the loads.  Per tile of 64 keys:
+// others on its scheduler); warp 17 loads, warp
+// 19 the scales.  Per tile of 64 keys:
 //   load     codes and scales (TMA, bulk copies) into a ring; BF16 K and V
 //            straight into operand tiles;
 //   prepare  codes (times the NVFP4 block scale) to FP16, exact, as [key][d]
@@ -49,7 +50,7 @@ constexpr int kTtKeys = 64;
 constexpr int kTtSoftmaxWarps = 8;
 constexpr int kTtPrepWarps = 8;
 constexpr int kTtMmaWarp = kTtSoftmaxWarps + kTtPrepWarps, kTtLoadWarp = kTtMmaWarp + 1;
-constexpr int kTtThreads = (kTtSoftmaxWarps + kTtPrepWarps + 4) * 32;  // whole warpgroups; warp 19 idles
+constexpr int kTtThreads = (kTtSoftmaxWarps + kTtPrepWarps + 4) * 32;  // whole warpgroups
 // Registers: 96 a thread at launch (640 threads); the softmax warps take what
 // the others give: 256 * 144 + 384 * 64 = 640 * 96.
 constexpr int kTtSoftmaxRegs = 144, kTtOtherRegs = 64;
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&ring_full[i], 1);
+      mbar_init(&ring_full[i], 33);  // the codes' bytes, and the lanes that copy scales
       mbar_init(&ring_free[i], kTtPrepWarps);
       mbar_init(&k_full[i], kQuant ? kTtPrepWarps / 2 : 1);
       mbar_init(&k_free[i], SPLIT ? 2 : 1);  // each stream that reads the tile
@@ -294,18 +295,19 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       mbar_init(&v_full[i], kTtPrepWarps / 2);
       mbar_init(&v_free[i], SPLIT ? 2 : 1);
     }
-    mbar_init(&q_full, kTtSoftmaxWarps);
+    const uint32_t active = ((SPLIT ? (p.rows_per_pass + 1) / 2 : p.rows_per_pass) + 31) / 32;  // softmax warps
+    mbar_init(&q_full, 2 * active);
     for (int s = 0; s < 2; ++s) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&s_full[s][i], 1);
-        mbar_init(&p_full[s][i], 4);  // per buffer: a warp may be one job ahead of another
+        mbar_init(&p_full[s][i], active);  // per buffer: a warp may be one job ahead of another
       }
       mbar_init(&o_done[s], 1);
       mbar_init(&o_end[s], 1);
     }
-    mbar_init(&seg_done, kTtSoftmaxWarps);
-    mbar_init(&join_ready, kTtSoftmaxWarps);
-    mbar_init(&join_read, 4);
+    mbar_init(&seg_done, 2 * active);
+    mbar_init(&join_ready, 2 * active);
+    mbar_init(&join_read, active);
     fence_mbar_init();
     s_bad = 0u;
     s_wild = 0u;
@@ -329,6 +331,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     x0 = cta < G ? ts_first_tile(n_tiles, cta, G) : 0;
     return cta < G ? ts_first_tile(n_tiles, cta + 1, G) : 0;
   };
+  // Softmax warps of a stream that hold rows (the others leave at once): those
+  // of the first `active` quarters of a tile, or, where stream 1 sees up to 64
+  // rows in the upper half, from its third on.
+  const bool upper = !SPLIT && p.rows_per_pass <= 64;
+  const int active = ((SPLIT ? (p.rows_per_pass + 1) / 2 : p.rows_per_pass) + 31) / 32;
   auto begin = [&](TsWalk& w) {
     int n_tiles, G, x0;
     const int x1 = range(n_tiles, G, x0);
@@ -339,7 +346,23 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtOtherRegs));
   TsWalk w;
   bool more = begin(w);
-  if (warp == kTtLoadWarp) {
+  if (kQuant && warp == kTtLoadWarp + 2) {
+    // ---------------------------------------------------------------- scales (see ts_load_scales)
+    const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
+    TtRing<C::kStages ? C::kStages : 1> rk;
+    bool ok = true;
+    for (; more && ok; more = w.next()) {
+      const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
+      for (int t = w.t0; t < w.t1; ++t) {
+        ok = __all_sync(kFull, tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad));
+        if (!ok) break;
+        uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
+        ts_load_scales<D, FMT, Codes, kTtKeys>(st, p, row0 + t * kTtKeys, all_rows, lane);
+        ts_copy_arrive(&ring_full[rk.i]);
+        rk.next();
+      }
+    }
+  } else if (warp == kTtLoadWarp) {
     // ---------------------------------------------------------------- loads
     if (lane == 0) {
       TtRing<kQuant ? (C::kStages ? C::kStages : 1) : C::kK> rk;
@@ -354,16 +377,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             if (!ok) break;
             uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
             uint64_t* bar = &ring_full[rk.i];
-            mbar_arrive_expect_tx(bar, Codes::kTx);
+            mbar_arrive_expect_tx(bar, 2 * Codes::kCodes);
             const int line = static_cast<int>(row * Codes::kRowBytes / 128);
             ts_tma_2d(st, &tm_k, 0, line, bar);
             ts_tma_2d(st + Codes::kOffV, &tm_v, 0, line, bar);
-            if constexpr (FMT == kKvFmtNvfp4) {
-              bulk_g2s(st + Codes::kOffKb, p.k.block_scales + row * (D / 16), Codes::kBlockScales, bar);
-              bulk_g2s(st + Codes::kOffVb, p.v.block_scales + row * (D / 16), Codes::kBlockScales, bar);
-            }
-            bulk_g2s(st + Codes::kOffKr, p.k.row_scales + row, Codes::kRowScales, bar);
-            bulk_g2s(st + Codes::kOffVr, p.v.row_scales + row, Codes::kRowScales, bar);
             rk.next();
           } else {
             ok = tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
@@ -401,7 +418,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     for (; more && ok; more = w.next()) {
       const int tiles = w.t1 - w.t0;
       const int rows = min(p.rows_per_pass, nq - (w.u % p.passes) * p.rows_per_pass);
-      const bool shifted = !SPLIT && rows <= 64;
+      const bool shifted = upper;
       // query rows of this stream in the Q tile
       const uint32_t q0 = SPLIT ? s * kTtRows : (shifted && s == 0 ? 64 : 0);
       const uint32_t qa = tt_desc_low(base + C::kOffQ + q0 * 128, 16);
@@ -472,6 +489,22 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     const bool is_v = warp >= kTtSoftmaxWarps + kTtPrepWarps / 2;
     constexpr int kN = kTtPrepWarps / 2 * 32;
     const int pt = (tid - kTtSoftmaxWarps * 32) % kN;
+    // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16),
+    // eight keys side by side; a thread's items of a tile are kStep keys apart
+    // (a multiple of 8: the same swizzle), or, D = 64, all in one row.
+    constexpr int kItems = kQuant ? Codes::kRowBytes / 16 : 1;
+    constexpr int kRounds = (kTtKeys * kItems + kN - 1) / kN, kStep = kN / kItems;
+    constexpr int kChunks = FMT == kKvFmtNvfp4 ? 4 : 2;  // 16-byte chunks of 8 elements an item becomes
+    const int c0 = (pt >> 3) % kItems, r0 = (pt / (8 * kItems)) * 8 + (pt & 7);
+    const bool busy = r0 < kTtKeys;
+    const uint32_t src0 = (is_v ? Codes::kOffV : 0u) + ts_swz(r0 * Codes::kRowBytes + 16 * c0);
+    const uint32_t scale0 = (is_v ? Codes::kOffVb : Codes::kOffKb) + r0 * (D / 16) + 2 * c0;
+    uint32_t dst0[kChunks];
+#pragma unroll
+    for (int y = 0; y < kChunks; ++y) {
+      const int ch = c0 * kChunks + y;  // chunk of the whole row
+      dst0[y] = (ch >> 3) * (kTtKeys * 128) + tt_chunk(r0, ch & 7);
+    }
     TtRing<C::kStages ? C::kStages : 1> rr;
     TtRing<C::kK> rk;
     TtRing<C::kV> rv;
@@ -484,21 +517,18 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         const bool edge = key0 + kTtKeys > past;
         const int live = min(kTtKeys, vis - key0);  // keys before the end
         if constexpr (kQuant) {
-          // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16), eight keys side by side.
-          constexpr int kItems = Codes::kRowBytes / 16;
-          constexpr int kRounds = (kTtKeys * kItems + kN - 1) / kN;
           ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad);
           if (!(ok = __all_sync(kFull, ok))) break;
           const uint8_t* st = smem + C::kOffRing + rr.i * Codes::kStage;
-          const uint8_t* codes = st + (is_v ? Codes::kOffV : 0);
           uint4 raw[kRounds];
           [[maybe_unused]] uint32_t scales[kRounds];
+          if (busy) {
 #pragma unroll
-          for (int x = 0; x < kRounds; ++x) {
-            const int i = pt + x * kN, c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
-            raw[x] = *reinterpret_cast<const uint4*>(codes + ts_swz(r * Codes::kRowBytes + 16 * c));
-            if constexpr (FMT == kKvFmtNvfp4)
-              scales[x] = *reinterpret_cast<const uint16_t*>(st + (is_v ? Codes::kOffVb : Codes::kOffKb) + r * (D / 16) + 2 * c);
+            for (int x = 0; x < kRounds; ++x) {
+              raw[x] = *reinterpret_cast<const uint4*>(st + src0 + x * kStep * Codes::kRowBytes);
+              if constexpr (FMT == kKvFmtNvfp4)
+                scales[x] = *reinterpret_cast<const uint16_t*>(st + scale0 + x * kStep * (D / 16));
+            }
           }
           [[maybe_unused]] float2 kr, vr;
           if (warp == kTtSoftmaxWarps) {
@@ -523,7 +553,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             constexpr bool CLEAN = decltype(clean_tag)::value;
 #pragma unroll
             for (int x = 0; x < kRounds; ++x) {
-              const int i = pt + x * kN, c = (i >> 3) % kItems, r = (i / (8 * kItems)) * 8 + (i & 7);
+              const int r = r0 + x * kStep;
               const uint32_t word[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
               [[maybe_unused]] uint32_t b0 = 0, b1 = 0;
               if constexpr (FMT == kKvFmtNvfp4) {
@@ -531,8 +561,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                 b0 = __byte_perm(both, both, 0x1010);
                 b1 = __byte_perm(both, both, 0x3232);
               }
-              // 16-byte chunks of 8 elements
-              constexpr int kChunks = FMT == kKvFmtNvfp4 ? 4 : 2;
 #pragma unroll
               for (int y = 0; y < kChunks; ++y) {
                 uint32_t h[4];
@@ -550,14 +578,12 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                   for (int z = 0; z < 4; ++z) h[z] = r < live ? ts_finite<FMT>(h[z], bad) : 0u;
                   if (bad) s_wild = 1u;
                 }
-                const int ch = c * kChunks + y;  // chunk of the whole row
-                *reinterpret_cast<uint4*>(out + (ch >> 3) * (kTtKeys * 128) + tt_chunk(r, ch & 7)) =
-                    make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4*>(out + dst0[y] + x * kStep * 128) = make_uint4(h[0], h[1], h[2], h[3]);
               }
             }
           };
-          if (is_v && edge) prepare(std::true_type{});
-          else prepare(std::false_type{});
+          if (busy && is_v && edge) prepare(std::true_type{});
+          else if (busy) prepare(std::false_type{});
           tt_fence_async();
           __syncwarp();
           if (lane == 0) ts_arrive(is_v ? &v_full[rv.i] : &k_full[rk.i]);
@@ -596,8 +622,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   } else {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTtSoftmaxRegs));
+    const int quarter = (warp & 3) - (upper && warp >= 4 ? 2 : 0);
     TsWalk w;
-    bool more = begin(w);
+    bool more = begin(w) && quarter >= 0 && quarter < active;
     const int s = warp >> 2, r = (warp & 3) * 32 + lane;  // stream, row of its tile
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t s_count = 0, o_count = 0, end_phase = 0, o_end_phase = 0;  // scores seen, P tiles given, segments ended
@@ -608,7 +635,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes, tiles = w.t1 - w.t0;
       const int past = ts_past(p, b), vis = ts_visible(p, b);
       const int n_first = pass * p.rows_per_pass, rows = min(p.rows_per_pass, nq - n_first);
-      const bool shifted = !SPLIT && rows <= 64;
+      const bool shifted = upper;
       const int half = (rows + 1) / 2;
       // This thread's query row of the pass (out of [0, rows): none).
       const int n = SPLIT ? (r < half ? s * half + r : rows) : (shifted && s == 1 ? r - 64 : r);
