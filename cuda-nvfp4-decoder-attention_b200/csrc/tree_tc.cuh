@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const bool warp_has = __any_sync(kFull, has);
       const int tok = has ? (n_first + n) / p.group : 0;
       const int64_t q_row = (b * p.tokens + tok) * p.q_heads + kvh * p.group + (has ? (n_first + n) % p.group : 0);
-      if (!SPLIT && s == 1 && !first_segment) {  // stream 0 has read what the join left in the place of Q
+      if (!SPLIT && !first_segment) {  // all of stream 0 has read what the join left in the place of Q
         ok = tt_wait(&join_read, end_phase ^ 1u, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
       }
