@@ -102,7 +102,17 @@ constexpr int kTsWarps = 8;
 template <int D, int FMT, int NG>
 constexpr int ts_slices() { return FMT != kKvFmtBf16 && NG == 1 && D <= 128 ? 2 : 1; }
 
-constexpr int64_t kTcMinRows = 17;  // query rows per KV head from which tree_tc_kernel runs
+// Query rows per KV head from which tree_tc_kernel runs.  The streaming kernel
+// decodes a tile once per 16 rows, this one once per 256.  Both, 8 sequences x 6
+// KV heads x 4 query heads each, us streaming / tcgen05 after 300, 2,000 and
+// 12,000 positions:
+//             20 rows (5 tokens)                 64 rows (16 tokens)
+//   BF16      29 / 28   37 / 31    78 / 72       66 / 27   78 / 33   151 / 75
+//   E4M3      26 / 27   46 / 35   146 / 77       47 / 30   88 / 38   211 / 84
+//   NVFP4     26 / 28   45 / 36   131 / 77       47 / 30   87 / 38   192 / 82
+// Up to 16 rows the streaming kernel reads the cache at up to 0.9 of its floor's
+// rate, and a 128-row tile would be mostly empty.
+constexpr int64_t kTcMinRows = 17;
 
 template <int D>
 cudaError_t launch_tree_combine(const TreeStreamParams& p, cudaStream_t s) {

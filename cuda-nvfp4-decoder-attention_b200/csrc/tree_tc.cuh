@@ -343,282 +343,282 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   };
 
   if (warp >= kTtSoftmaxWarps) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtOtherRegs));
-  TsWalk w;
-  bool more = begin(w);
-  if (kQuant && warp == kTtLoadWarp + 2) {
-    // ---------------------------------------------------------------- scales (see ts_load_scales)
-    const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
-    TtRing<C::kStages ? C::kStages : 1> rk;
-    bool ok = true;
-    for (; more && ok; more = w.next()) {
-      const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
-      for (int t = w.t0; t < w.t1; ++t) {
-        ok = __all_sync(kFull, tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad));
-        if (!ok) break;
-        uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
-        ts_load_scales<D, FMT, Codes, kTtKeys>(st, p, row0 + t * kTtKeys, all_rows, lane);
-        ts_copy_arrive(&ring_full[rk.i]);
-        rk.next();
-      }
-    }
-  } else if (warp == kTtLoadWarp) {
-    // ---------------------------------------------------------------- loads
-    if (lane == 0) {
-      TtRing<kQuant ? (C::kStages ? C::kStages : 1) : C::kK> rk;
-      TtRing<C::kV> rv;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtOtherRegs));
+    TsWalk w;
+    bool more = begin(w);
+    if (kQuant && warp == kTtLoadWarp + 2) {
+      // ---------------------------------------------------------------- scales (see ts_load_scales)
+      const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
+      TtRing<C::kStages ? C::kStages : 1> rk;
       bool ok = true;
       for (; more && ok; more = w.next()) {
         const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
-        for (int t = w.t0; t < w.t1 && ok; ++t) {
-          const int64_t row = row0 + t * kTtKeys;
+        for (int t = w.t0; t < w.t1; ++t) {
+          ok = __all_sync(kFull, tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad));
+          if (!ok) break;
+          uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
+          ts_load_scales<D, FMT, Codes, kTtKeys>(st, p, row0 + t * kTtKeys, all_rows, lane);
+          ts_copy_arrive(&ring_full[rk.i]);
+          rk.next();
+        }
+      }
+    } else if (warp == kTtLoadWarp) {
+      // ---------------------------------------------------------------- loads
+      if (lane == 0) {
+        TtRing<kQuant ? (C::kStages ? C::kStages : 1) : C::kK> rk;
+        TtRing<C::kV> rv;
+        bool ok = true;
+        for (; more && ok; more = w.next()) {
+          const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
+          for (int t = w.t0; t < w.t1 && ok; ++t) {
+            const int64_t row = row0 + t * kTtKeys;
+            if constexpr (kQuant) {
+              ok = tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad);
+              if (!ok) break;
+              uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
+              uint64_t* bar = &ring_full[rk.i];
+              mbar_arrive_expect_tx(bar, 2 * Codes::kCodes);
+              const int line = static_cast<int>(row * Codes::kRowBytes / 128);
+              ts_tma_2d(st, &tm_k, 0, line, bar);
+              ts_tma_2d(st + Codes::kOffV, &tm_v, 0, line, bar);
+              rk.next();
+            } else {
+              ok = tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&k_full[rk.i], C::kOperand);
+              for (int pn = 0; pn < C::kPanels; ++pn)
+                ts_tma_2d(smem + C::kOffK + rk.i * C::kOperand + pn * (kTtKeys * 128), &tm_k, pn * 64,
+                          static_cast<int>(row), &k_full[rk.i]);
+              rk.next();
+              ok = tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&v_raw[rv.i], C::kOperand);
+              for (int pn = 0; pn < C::kPanels; ++pn)
+                ts_tma_2d(smem + C::kOffV + rv.i * C::kOperand + pn * (kTtKeys * 128), &tm_v, pn * 64,
+                          static_cast<int>(row), &v_raw[rv.i]);
+              rv.next();
+            }
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == kTtMmaWarp || warp == kTtMmaWarp + 2) {
+      // ---------------------------------------------------------------- MMAs, a warp per stream
+      // The whole warp walks the line, one lane issues.  The stream's P takes the
+      // place of its scores: the scores of job n + 2 go into the buffer that held
+      // P of job n, after that job's P V in issue order.
+      constexpr uint32_t kIdescS = tt_idesc<FMT>(kTtKeys, false), kIdescO = tt_idesc<FMT>(D, true);
+      const int s = (warp - kTtMmaWarp) / 2;
+      const bool issuer = tt_elect();
+      const uint32_t base = smem_u32(smem), o_at = o_col(s);
+      TtRing<C::kK> rk;
+      TtRing<C::kV> rv;
+      uint32_t q_phase = 0, nth = 0, nth_s = 0;  // P V and scores issued, over all segments
+      bool ok = true;
+      for (; more && ok; more = w.next()) {
+        const int tiles = w.t1 - w.t0;
+        const int rows = min(p.rows_per_pass, nq - (w.u % p.passes) * p.rows_per_pass);
+        const bool shifted = upper;
+        // query rows of this stream in the Q tile
+        const uint32_t q0 = SPLIT ? s * kTtRows : (shifted && s == 0 ? 64 : 0);
+        const uint32_t qa = tt_desc_low(base + C::kOffQ + q0 * 128, 16);
+        ok = __all_sync(kFull, tt_wait(&q_full, q_phase, &s_bad));
+        q_phase ^= 1u;
+        auto scores = [&] {
+          ok = __all_sync(kFull, tt_wait(&k_full[rk.i], rk.phase, &s_bad));
+          if (!ok) return;
+          tt_fence_after();
+          const uint32_t ka = tt_desc_low(base + C::kOffK + rk.i * C::kOperand, 16);
+          const uint32_t d = s_col(s, nth_s & 1);
+          if (issuer) {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+              tt_mma(d, qa + ((ks >> 2) * C::kQPanel + (ks & 3) * 32) / 16,
+                     ka + ((ks >> 2) * (kTtKeys * 128) + (ks & 3) * 32) / 16, kIdescS, ks ? 1u : 0u);
+            tt_commit(&s_full[s][nth_s & 1]);
+            tt_commit(&k_free[rk.i]);
+          }
+          __syncwarp();
+          ++nth_s;
+        };
+        // Tiles in order; without SPLIT every other one is this stream's.
+        int next_s = 0;  // tile whose scores come next
+        auto advance_scores = [&] {
+          while (next_s < tiles) {
+            const bool mine = SPLIT || (next_s & 1) == s;
+            if (mine) scores();
+            rk.next();
+            ++next_s;
+            if (mine) break;
+          }
+        };
+        advance_scores();
+        if (ok) advance_scores();
+        for (int t = 0; t < tiles && ok; ++t) {
+          if (SPLIT || (t & 1) == s) {
+            ok = tt_wait(&p_full[s][nth & 1], (nth >> 1) & 1, &s_bad) && tt_wait(&v_full[rv.i], rv.phase, &s_bad);
+            if (!(ok = __all_sync(kFull, ok))) break;
+            tt_fence_after();
+            const uint32_t va = tt_desc_low(base + C::kOffV + rv.i * C::kOperand, kTtKeys * 128);
+            const uint32_t pa = s_col(s, nth & 1);
+            const uint32_t begun = t >= (SPLIT ? 1 : 2) ? 1u : 0u;  // not the stream's first tile of the segment
+            if (issuer) {
+#pragma unroll
+              for (int ks = 0; ks < kTtKeys / 16; ++ks) {
+                tt_mma_ts(o_at, pa + tt_p_col<FMT>(ks), va + ks * 2048 / 16, kIdescO, ks ? 1u : begun);
+                if constexpr (!kQuant) tt_mma_ts(o_at, pa + tt_p_col<FMT>(ks) + 16, va + ks * 2048 / 16, kIdescO, 1u);
+              }
+              tt_commit(&o_done[s]);
+              tt_commit(&v_free[rv.i]);
+            }
+            __syncwarp();
+            ++nth;
+            advance_scores();
+          }
+          rv.next();
+        }
+        while (next_s < tiles) {  // the other stream's last tile
+          rk.next();
+          ++next_s;
+        }
+        if (ok && issuer) tt_commit(&o_end[s]);
+        __syncwarp();
+      }
+    } else if (warp >= kTtSoftmaxWarps && warp < kTtMmaWarp) {
+      // ---------------------------------------------------------------- operands: warps 8-11 K, 12-15 V
+      const bool is_v = warp >= kTtSoftmaxWarps + kTtPrepWarps / 2;
+      constexpr int kN = kTtPrepWarps / 2 * 32;
+      const int pt = (tid - kTtSoftmaxWarps * 32) % kN;
+      // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16),
+      // eight keys side by side; a thread's items of a tile are kStep keys apart
+      // (a multiple of 8: the same swizzle), or, D = 64, all in one row.
+      constexpr int kItems = kQuant ? Codes::kRowBytes / 16 : 1;
+      constexpr int kRounds = (kTtKeys * kItems + kN - 1) / kN, kStep = kN / kItems;
+      constexpr int kChunks = FMT == kKvFmtNvfp4 ? 4 : 2;  // 16-byte chunks of 8 elements an item becomes
+      const int c0 = (pt >> 3) % kItems, r0 = (pt / (8 * kItems)) * 8 + (pt & 7);
+      const bool busy = r0 < kTtKeys;
+      const uint32_t src0 = (is_v ? Codes::kOffV : 0u) + ts_swz(r0 * Codes::kRowBytes + 16 * c0);
+      const uint32_t scale0 = (is_v ? Codes::kOffVb : Codes::kOffKb) + r0 * (D / 16) + 2 * c0;
+      uint32_t dst0[kChunks];
+#pragma unroll
+      for (int y = 0; y < kChunks; ++y) {
+        const int ch = c0 * kChunks + y;  // chunk of the whole row
+        dst0[y] = (ch >> 3) * (kTtKeys * 128) + tt_chunk(r0, ch & 7);
+      }
+      TtRing<C::kStages ? C::kStages : 1> rr;
+      TtRing<C::kK> rk;
+      TtRing<C::kV> rv;
+      int slot = 0;
+      bool ok = true;
+      for (; more && ok; more = w.next()) {
+        const int past = ts_past(p, w.b), vis = ts_visible(p, w.b);
+        for (int t = w.t0; t < w.t1; ++t) {
+          const int key0 = t * kTtKeys;
+          const bool edge = key0 + kTtKeys > past;
+          const int live = min(kTtKeys, vis - key0);  // keys before the end
           if constexpr (kQuant) {
-            ok = tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad);
-            if (!ok) break;
-            uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
-            uint64_t* bar = &ring_full[rk.i];
-            mbar_arrive_expect_tx(bar, 2 * Codes::kCodes);
-            const int line = static_cast<int>(row * Codes::kRowBytes / 128);
-            ts_tma_2d(st, &tm_k, 0, line, bar);
-            ts_tma_2d(st + Codes::kOffV, &tm_v, 0, line, bar);
+            ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad);
+            if (!(ok = __all_sync(kFull, ok))) break;
+            const uint8_t* st = smem + C::kOffRing + rr.i * Codes::kStage;
+            uint4 raw[kRounds];
+            [[maybe_unused]] uint32_t scales[kRounds];
+            if (busy) {
+#pragma unroll
+              for (int x = 0; x < kRounds; ++x) {
+                raw[x] = *reinterpret_cast<const uint4*>(st + src0 + x * kStep * Codes::kRowBytes);
+                if constexpr (FMT == kKvFmtNvfp4)
+                  scales[x] = *reinterpret_cast<const uint16_t*>(st + scale0 + x * kStep * (D / 16));
+              }
+            }
+            [[maybe_unused]] float2 kr, vr;
+            if (warp == kTtSoftmaxWarps) {
+              kr = reinterpret_cast<const float2*>(st + Codes::kOffKr)[lane];
+              vr = reinterpret_cast<const float2*>(st + Codes::kOffVr)[lane];
+            }
+            __syncwarp();
+            if (lane == 0) ts_arrive(&ring_free[rr.i]);
+            rr.next();
+            ok = is_v ? tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad) : tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+            if (!(ok = __all_sync(kFull, ok))) break;
+            if (warp == kTtSoftmaxWarps) {  // the first of these warps: the row scales
+              float* un = units_kv + slot * C::kUnitFloats;
+              reinterpret_cast<float2*>(un)[lane] = make_float2(kr.x * p.scale_log2, kr.y * p.scale_log2);
+              reinterpret_cast<float2*>(un + kTtKeys)[lane] = vr;
+              const float top = warp_max_f32(fmaxf(vr.x < INFINITY ? vr.x : 0.0f, vr.y < INFINITY ? vr.y : 0.0f));
+              if (lane == 0) un[2 * kTtKeys] = top;
+            }
+            slot = slot + 1 == kTtUnitSlots ? 0 : slot + 1;
+            uint8_t* out = smem + (is_v ? C::kOffV + rv.i * C::kOperand : C::kOffK + rk.i * C::kOperand);
+            auto prepare = [&](auto clean_tag) {
+              constexpr bool CLEAN = decltype(clean_tag)::value;
+#pragma unroll
+              for (int x = 0; x < kRounds; ++x) {
+                const int r = r0 + x * kStep;
+                const uint32_t word[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+                [[maybe_unused]] uint32_t b0 = 0, b1 = 0;
+                if constexpr (FMT == kKvFmtNvfp4) {
+                  const uint32_t both = e4m3x2_to_f16x2(scales[x]);
+                  b0 = __byte_perm(both, both, 0x1010);
+                  b1 = __byte_perm(both, both, 0x3232);
+                }
+#pragma unroll
+                for (int y = 0; y < kChunks; ++y) {
+                  uint32_t h[4];
+                  if constexpr (FMT == kKvFmtNvfp4) {
+                    e2m1x8_to_f16x2x4(word[y], h);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) h[z] = ts_hmul2(h[z], y < 2 ? b0 : b1);
+                  } else {
+                    ts_e4m3x4(word[2 * y], h[0], h[1]);
+                    ts_e4m3x4(word[2 * y + 1], h[2], h[3]);
+                  }
+                  if constexpr (CLEAN) {
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) h[z] = r < live ? ts_finite<FMT>(h[z], bad) : 0u;
+                    if (bad) s_wild = 1u;
+                  }
+                  *reinterpret_cast<uint4*>(out + dst0[y] + x * kStep * 128) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+              }
+            };
+            if (busy && is_v && edge) prepare(std::true_type{});
+            else if (busy) prepare(std::false_type{});
+            tt_fence_async();
+            __syncwarp();
+            if (lane == 0) ts_arrive(is_v ? &v_full[rv.i] : &k_full[rk.i]);
             rk.next();
-          } else {
-            ok = tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&k_full[rk.i], C::kOperand);
-            for (int pn = 0; pn < C::kPanels; ++pn)
-              ts_tma_2d(smem + C::kOffK + rk.i * C::kOperand + pn * (kTtKeys * 128), &tm_k, pn * 64,
-                        static_cast<int>(row), &k_full[rk.i]);
-            rk.next();
-            ok = tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&v_raw[rv.i], C::kOperand);
-            for (int pn = 0; pn < C::kPanels; ++pn)
-              ts_tma_2d(smem + C::kOffV + rv.i * C::kOperand + pn * (kTtKeys * 128), &tm_v, pn * 64,
-                        static_cast<int>(row), &v_raw[rv.i]);
+            rv.next();
+          } else if (is_v) {
+            ok = tt_wait(&v_raw[rv.i], rv.phase, &s_bad);
+            if (!(ok = __all_sync(kFull, ok))) break;
+            if (edge) {
+              uint8_t* v = smem + C::kOffV + rv.i * C::kOperand;
+              for (int i = pt; i < kTtKeys * (D / 8); i += kN) {
+                const int r = i / (D / 8), ch = i % (D / 8);
+                uint4* at = reinterpret_cast<uint4*>(v + (ch >> 3) * (kTtKeys * 128) + tt_chunk(r, ch & 7));
+                if (r >= live) {
+                  *at = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                  uint32_t bad = 0;
+                  const uint4 x = *at;
+                  const uint4 y = make_uint4(ts_finite<FMT>(x.x, bad), ts_finite<FMT>(x.y, bad), ts_finite<FMT>(x.z, bad),
+                                             ts_finite<FMT>(x.w, bad));
+                  if (bad) {
+                    *at = y;
+                    s_wild = 1u;
+                  }
+                }
+              }
+              tt_fence_async();
+            }
+            __syncwarp();
+            if (lane == 0) ts_arrive(&v_full[rv.i]);
             rv.next();
           }
         }
       }
     }
-    __syncwarp();
-  } else if (warp == kTtMmaWarp || warp == kTtMmaWarp + 2) {
-    // ---------------------------------------------------------------- MMAs, a warp per stream
-    // The whole warp walks the line, one lane issues.  The stream's P takes the
-    // place of its scores: the scores of job n + 2 go into the buffer that held
-    // P of job n, after that job's P V in issue order.
-    constexpr uint32_t kIdescS = tt_idesc<FMT>(kTtKeys, false), kIdescO = tt_idesc<FMT>(D, true);
-    const int s = (warp - kTtMmaWarp) / 2;
-    const bool issuer = tt_elect();
-    const uint32_t base = smem_u32(smem), o_at = o_col(s);
-    TtRing<C::kK> rk;
-    TtRing<C::kV> rv;
-    uint32_t q_phase = 0, nth = 0, nth_s = 0;  // P V and scores issued, over all segments
-    bool ok = true;
-    for (; more && ok; more = w.next()) {
-      const int tiles = w.t1 - w.t0;
-      const int rows = min(p.rows_per_pass, nq - (w.u % p.passes) * p.rows_per_pass);
-      const bool shifted = upper;
-      // query rows of this stream in the Q tile
-      const uint32_t q0 = SPLIT ? s * kTtRows : (shifted && s == 0 ? 64 : 0);
-      const uint32_t qa = tt_desc_low(base + C::kOffQ + q0 * 128, 16);
-      ok = __all_sync(kFull, tt_wait(&q_full, q_phase, &s_bad));
-      q_phase ^= 1u;
-      auto scores = [&] {
-        ok = __all_sync(kFull, tt_wait(&k_full[rk.i], rk.phase, &s_bad));
-        if (!ok) return;
-        tt_fence_after();
-        const uint32_t ka = tt_desc_low(base + C::kOffK + rk.i * C::kOperand, 16);
-        const uint32_t d = s_col(s, nth_s & 1);
-        if (issuer) {
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            tt_mma(d, qa + ((ks >> 2) * C::kQPanel + (ks & 3) * 32) / 16,
-                   ka + ((ks >> 2) * (kTtKeys * 128) + (ks & 3) * 32) / 16, kIdescS, ks ? 1u : 0u);
-          tt_commit(&s_full[s][nth_s & 1]);
-          tt_commit(&k_free[rk.i]);
-        }
-        __syncwarp();
-        ++nth_s;
-      };
-      // Tiles in order; without SPLIT every other one is this stream's.
-      int next_s = 0;  // tile whose scores come next
-      auto advance_scores = [&] {
-        while (next_s < tiles) {
-          const bool mine = SPLIT || (next_s & 1) == s;
-          if (mine) scores();
-          rk.next();
-          ++next_s;
-          if (mine) break;
-        }
-      };
-      advance_scores();
-      if (ok) advance_scores();
-      for (int t = 0; t < tiles && ok; ++t) {
-        if (SPLIT || (t & 1) == s) {
-          ok = tt_wait(&p_full[s][nth & 1], (nth >> 1) & 1, &s_bad) && tt_wait(&v_full[rv.i], rv.phase, &s_bad);
-          if (!(ok = __all_sync(kFull, ok))) break;
-          tt_fence_after();
-          const uint32_t va = tt_desc_low(base + C::kOffV + rv.i * C::kOperand, kTtKeys * 128);
-          const uint32_t pa = s_col(s, nth & 1);
-          const uint32_t begun = t >= (SPLIT ? 1 : 2) ? 1u : 0u;  // not the stream's first tile of the segment
-          if (issuer) {
-#pragma unroll
-            for (int ks = 0; ks < kTtKeys / 16; ++ks) {
-              tt_mma_ts(o_at, pa + tt_p_col<FMT>(ks), va + ks * 2048 / 16, kIdescO, ks ? 1u : begun);
-              if constexpr (!kQuant) tt_mma_ts(o_at, pa + tt_p_col<FMT>(ks) + 16, va + ks * 2048 / 16, kIdescO, 1u);
-            }
-            tt_commit(&o_done[s]);
-            tt_commit(&v_free[rv.i]);
-          }
-          __syncwarp();
-          ++nth;
-          advance_scores();
-        }
-        rv.next();
-      }
-      while (next_s < tiles) {  // the other stream's last tile
-        rk.next();
-        ++next_s;
-      }
-      if (ok && issuer) tt_commit(&o_end[s]);
-      __syncwarp();
-    }
-  } else if (warp >= kTtSoftmaxWarps && warp < kTtMmaWarp) {
-    // ---------------------------------------------------------------- operands: warps 8-11 K, 12-15 V
-    const bool is_v = warp >= kTtSoftmaxWarps + kTtPrepWarps / 2;
-    constexpr int kN = kTtPrepWarps / 2 * 32;
-    const int pt = (tid - kTtSoftmaxWarps * 32) % kN;
-    // Items of 16 bytes of codes of one key (NVFP4: 32 elements, E4M3: 16),
-    // eight keys side by side; a thread's items of a tile are kStep keys apart
-    // (a multiple of 8: the same swizzle), or, D = 64, all in one row.
-    constexpr int kItems = kQuant ? Codes::kRowBytes / 16 : 1;
-    constexpr int kRounds = (kTtKeys * kItems + kN - 1) / kN, kStep = kN / kItems;
-    constexpr int kChunks = FMT == kKvFmtNvfp4 ? 4 : 2;  // 16-byte chunks of 8 elements an item becomes
-    const int c0 = (pt >> 3) % kItems, r0 = (pt / (8 * kItems)) * 8 + (pt & 7);
-    const bool busy = r0 < kTtKeys;
-    const uint32_t src0 = (is_v ? Codes::kOffV : 0u) + ts_swz(r0 * Codes::kRowBytes + 16 * c0);
-    const uint32_t scale0 = (is_v ? Codes::kOffVb : Codes::kOffKb) + r0 * (D / 16) + 2 * c0;
-    uint32_t dst0[kChunks];
-#pragma unroll
-    for (int y = 0; y < kChunks; ++y) {
-      const int ch = c0 * kChunks + y;  // chunk of the whole row
-      dst0[y] = (ch >> 3) * (kTtKeys * 128) + tt_chunk(r0, ch & 7);
-    }
-    TtRing<C::kStages ? C::kStages : 1> rr;
-    TtRing<C::kK> rk;
-    TtRing<C::kV> rv;
-    int slot = 0;
-    bool ok = true;
-    for (; more && ok; more = w.next()) {
-      const int past = ts_past(p, w.b), vis = ts_visible(p, w.b);
-      for (int t = w.t0; t < w.t1; ++t) {
-        const int key0 = t * kTtKeys;
-        const bool edge = key0 + kTtKeys > past;
-        const int live = min(kTtKeys, vis - key0);  // keys before the end
-        if constexpr (kQuant) {
-          ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad);
-          if (!(ok = __all_sync(kFull, ok))) break;
-          const uint8_t* st = smem + C::kOffRing + rr.i * Codes::kStage;
-          uint4 raw[kRounds];
-          [[maybe_unused]] uint32_t scales[kRounds];
-          if (busy) {
-#pragma unroll
-            for (int x = 0; x < kRounds; ++x) {
-              raw[x] = *reinterpret_cast<const uint4*>(st + src0 + x * kStep * Codes::kRowBytes);
-              if constexpr (FMT == kKvFmtNvfp4)
-                scales[x] = *reinterpret_cast<const uint16_t*>(st + scale0 + x * kStep * (D / 16));
-            }
-          }
-          [[maybe_unused]] float2 kr, vr;
-          if (warp == kTtSoftmaxWarps) {
-            kr = reinterpret_cast<const float2*>(st + Codes::kOffKr)[lane];
-            vr = reinterpret_cast<const float2*>(st + Codes::kOffVr)[lane];
-          }
-          __syncwarp();
-          if (lane == 0) ts_arrive(&ring_free[rr.i]);
-          rr.next();
-          ok = is_v ? tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad) : tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
-          if (!(ok = __all_sync(kFull, ok))) break;
-          if (warp == kTtSoftmaxWarps) {  // the first of these warps: the row scales
-            float* un = units_kv + slot * C::kUnitFloats;
-            reinterpret_cast<float2*>(un)[lane] = make_float2(kr.x * p.scale_log2, kr.y * p.scale_log2);
-            reinterpret_cast<float2*>(un + kTtKeys)[lane] = vr;
-            const float top = warp_max_f32(fmaxf(vr.x < INFINITY ? vr.x : 0.0f, vr.y < INFINITY ? vr.y : 0.0f));
-            if (lane == 0) un[2 * kTtKeys] = top;
-          }
-          slot = slot + 1 == kTtUnitSlots ? 0 : slot + 1;
-          uint8_t* out = smem + (is_v ? C::kOffV + rv.i * C::kOperand : C::kOffK + rk.i * C::kOperand);
-          auto prepare = [&](auto clean_tag) {
-            constexpr bool CLEAN = decltype(clean_tag)::value;
-#pragma unroll
-            for (int x = 0; x < kRounds; ++x) {
-              const int r = r0 + x * kStep;
-              const uint32_t word[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-              [[maybe_unused]] uint32_t b0 = 0, b1 = 0;
-              if constexpr (FMT == kKvFmtNvfp4) {
-                const uint32_t both = e4m3x2_to_f16x2(scales[x]);
-                b0 = __byte_perm(both, both, 0x1010);
-                b1 = __byte_perm(both, both, 0x3232);
-              }
-#pragma unroll
-              for (int y = 0; y < kChunks; ++y) {
-                uint32_t h[4];
-                if constexpr (FMT == kKvFmtNvfp4) {
-                  e2m1x8_to_f16x2x4(word[y], h);
-#pragma unroll
-                  for (int z = 0; z < 4; ++z) h[z] = ts_hmul2(h[z], y < 2 ? b0 : b1);
-                } else {
-                  ts_e4m3x4(word[2 * y], h[0], h[1]);
-                  ts_e4m3x4(word[2 * y + 1], h[2], h[3]);
-                }
-                if constexpr (CLEAN) {
-                  uint32_t bad = 0;
-#pragma unroll
-                  for (int z = 0; z < 4; ++z) h[z] = r < live ? ts_finite<FMT>(h[z], bad) : 0u;
-                  if (bad) s_wild = 1u;
-                }
-                *reinterpret_cast<uint4*>(out + dst0[y] + x * kStep * 128) = make_uint4(h[0], h[1], h[2], h[3]);
-              }
-            }
-          };
-          if (busy && is_v && edge) prepare(std::true_type{});
-          else if (busy) prepare(std::false_type{});
-          tt_fence_async();
-          __syncwarp();
-          if (lane == 0) ts_arrive(is_v ? &v_full[rv.i] : &k_full[rk.i]);
-          rk.next();
-          rv.next();
-        } else if (is_v) {
-          ok = tt_wait(&v_raw[rv.i], rv.phase, &s_bad);
-          if (!(ok = __all_sync(kFull, ok))) break;
-          if (edge) {
-            uint8_t* v = smem + C::kOffV + rv.i * C::kOperand;
-            for (int i = pt; i < kTtKeys * (D / 8); i += kN) {
-              const int r = i / (D / 8), ch = i % (D / 8);
-              uint4* at = reinterpret_cast<uint4*>(v + (ch >> 3) * (kTtKeys * 128) + tt_chunk(r, ch & 7));
-              if (r >= live) {
-                *at = make_uint4(0u, 0u, 0u, 0u);
-              } else {
-                uint32_t bad = 0;
-                const uint4 x = *at;
-                const uint4 y = make_uint4(ts_finite<FMT>(x.x, bad), ts_finite<FMT>(x.y, bad), ts_finite<FMT>(x.z, bad),
-                                           ts_finite<FMT>(x.w, bad));
-                if (bad) {
-                  *at = y;
-                  s_wild = 1u;
-                }
-              }
-            }
-            tt_fence_async();
-          }
-          __syncwarp();
-          if (lane == 0) ts_arrive(&v_full[rv.i]);
-          rv.next();
-        }
-      }
-    }
-  }
   } else {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTtSoftmaxRegs));
@@ -631,6 +631,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     bool first_segment = true;
     int slot0 = 0;  // unit slot of the segment's first tile
     bool ok = true;
+    // Row of Q and of the context of row n of a pass of unit u.
+    auto q_row = [&](int64_t b, int u, int n) {
+      const int at = u % p.passes * p.rows_per_pass + n;
+      return (b * p.tokens + at / p.group) * p.q_heads + static_cast<int64_t>(u / p.passes) * p.group + at % p.group;
+    };
     for (; more && ok; more = w.next()) {
       const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes, tiles = w.t1 - w.t0;
       const int past = ts_past(p, b), vis = ts_visible(p, b);
@@ -642,7 +647,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const bool has = n >= 0 && n < rows;
       const bool warp_has = __any_sync(kFull, has);
       const int tok = has ? (n_first + n) / p.group : 0;
-      const int64_t q_row = (b * p.tokens + tok) * p.q_heads + kvh * p.group + (has ? (n_first + n) % p.group : 0);
+      const int64_t q_row_own = q_row(b, w.u, n);
       if (!SPLIT && !first_segment) {  // all of stream 0 has read what the join left in the place of Q
         ok = tt_wait(&join_read, end_phase ^ 1u, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
@@ -650,36 +655,62 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       first_segment = false;
       // ---- Q: this thread's row (SPLIT: all of it; else the panel of its stream)
       float own = kQuant ? 1.0f : p.scale_log2;
-      if (has) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row * D);
-        float up = 1.0f;
-        if constexpr (kQuant) {
-          uint32_t top = 0;
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 v = __ldg(src + c);
-            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+      // Eight lanes a row and panel, all loads in flight: a segment waits for these rows, and with a row per lane every
+      // load touched 32 lines (48 tokens after 32 positions, BF16: 42.4 us so, 40.8 us as here).
+      if (warp_has) {
+        constexpr bool kHalves = !SPLIT && C::kPanels == 2;
+        constexpr int kMine = SPLIT ? C::kPanels : 1;  // panels this stream stores
+        const int64_t own_row = has ? q_row(b, w.u, n) : 0;
+        const int held = __popc(__ballot_sync(kFull, has));
+        const int first = kHalves ? s : 0;
+        uint4 v[kMine][8], other[8];  // rows 4 i + lane / 8
 #pragma unroll
-            for (int x = 0; x < 4; ++x) top = max(top, max(e[x] & 0x7fffu, (e[x] >> 16) & 0x7fffu));
-          }
-          const int ex = static_cast<int>(top >> 7);
-          const int e = (ex == 0 || ex == 255) ? 0 : min(14 - (ex - 127), 100);
-          up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          own = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        for (int i = 0; i < 8; ++i) {
+          const bool there = 4 * i + (lane >> 3) < held;
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + __shfl_sync(kFull, own_row, 4 * i + (lane >> 3)) * D);
+#pragma unroll
+          for (int pn = 0; pn < kMine; ++pn)
+            v[pn][i] = there ? __ldg(src + 8 * (first + pn) + (lane & 7)) : make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (kQuant && kHalves)
+            other[i] = there ? __ldg(src + 8 * (1 - first) + (lane & 7)) : make_uint4(0u, 0u, 0u, 0u);
         }
-        const int at = SPLIT ? s * kTtRows + r : (shifted ? 64 + n : n);
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          if (!SPLIT && C::kPanels == 2 && (c >> 3) != s) continue;
-          if (!SPLIT && C::kPanels == 1 && s == 1) continue;
-          uint4 v = __ldg(src + c);
-          if constexpr (kQuant) {
-            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+        const int at0 = SPLIT ? s * kTtRows + (warp & 3) * 32 : (shifted ? 64 : 0) + __shfl_sync(kFull, n, 0);
+        uint8_t* dst = smem + C::kOffQ + first * C::kQPanel;
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              e[x] = ts_pack_f16(__uint_as_float(e[x] << 16) * up, __uint_as_float(e[x] & 0xffff0000u) * up);
+        for (int i = 0; i < 8; ++i) {
+          const int row = 4 * i + (lane >> 3);
+          [[maybe_unused]] float up = 1.0f;
+          if constexpr (kQuant) {  // by a power of two, the row's largest element below 2^15
+            uint32_t top = 0;
+            auto largest = [&](const uint4& x) {
+              top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                           __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+            };
+#pragma unroll
+            for (int pn = 0; pn < kMine; ++pn) largest(v[pn][i]);
+            if constexpr (kHalves) largest(other[i]);
+            top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(kFull, top, o));
+            const int ex = static_cast<int>(top >> 7);
+            const int e = (ex == 0 || ex == 255) ? 0 : min(14 - (ex - 127), 100);
+            up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            const int mine = __shfl_sync(kFull, e, (lane & 3) * 8);  // row 4 i + lane % 4
+            if ((lane >> 2) == i) own = __uint_as_float(static_cast<uint32_t>(127 - mine) << 23);
           }
-          *reinterpret_cast<uint4*>(smem + C::kOffQ + (c >> 3) * C::kQPanel + tt_chunk(at, c & 7)) = v;
+          if (row < held && (SPLIT || kHalves || s == 0)) {
+#pragma unroll
+            for (int pn = 0; pn < kMine; ++pn) {
+              uint4 x = v[pn][i];
+              if constexpr (kQuant) {
+                uint32_t* e = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  e[y] = ts_pack_f16(__uint_as_float(e[y] << 16) * up, __uint_as_float(e[y] & 0xffff0000u) * up);
+              }
+              *reinterpret_cast<uint4*>(dst + pn * C::kQPanel + tt_chunk(at0 + row, lane & 7)) = x;
+            }
+          }
         }
       }
       tt_fence_async();
@@ -693,6 +724,33 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       for (int i = SPLIT ? 0 : s; i < tiles && ok; i += SPLIT ? 1 : 2, ++done) {
         const int buf = s_count & 1;
         const int key0 = (w.t0 + i) * kTtKeys;
+        // Keys of the tile this row sees, one bit each.  With a mask, a lane per key and a vote per token: a byte at a
+        // time per row, it took a fifth of a one-tile segment's time.
+        const bool edge = key0 + kTtKeys > past;
+        unsigned long long seen = ~0ull;
+        if (edge) {
+          if (!p.mask) {
+            const int see = min(past + tok + 1, vis) - key0;
+            seen = see <= 0 ? 0ull : see >= 64 ? ~0ull : (1ull << see) - 1;
+          } else {
+            // Opaque: what follows is worked out here, not kept in registers over the other tiles.
+            int mine = tok;
+            asm volatile("" : "+r"(mine));
+            const uint8_t* mask_b = p.mask + b * p.mask_stride;
+            auto sees = [&](int t, int pos) {
+              if (pos < past) return true;
+              return pos < vis && mask_b[static_cast<int64_t>(t) * p.tokens + (pos - past)] != 0;
+            };
+            // Tokens of the warp's rows (those that hold one come first).
+            const int tok_lo = __shfl_sync(kFull, mine, 0), tok_hi = __reduce_max_sync(kFull, mine);
+#pragma unroll 4
+            for (int t = tok_lo; t <= tok_hi; ++t) {
+              const uint32_t lo = __ballot_sync(kFull, sees(t, key0 + lane));
+              const uint32_t hi = __ballot_sync(kFull, sees(t, key0 + 32 + lane));
+              if (t == tok) seen = lo | static_cast<unsigned long long>(hi) << 32;
+            }
+          }
+        }
         ok = tt_wait(&s_full[s][buf], (s_count >> 1) & 1, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
         tt_fence_after();
@@ -701,16 +759,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         const float* unit = units_kv + ((slot0 + i) & (kTtUnitSlots - 1)) * C::kUnitFloats;
         auto tile = [&](auto edge_tag) {
           constexpr bool EDGE = decltype(edge_tag)::value;
-          // Keys of the tile this row sees, one bit each.
-          [[maybe_unused]] unsigned long long seen = ~0ull;
-          if constexpr (EDGE) {
-            const int old = past - key0;  // committed keys of the tile
-            seen = old <= 0 ? 0ull : (1ull << old) - 1;  // fewer than 64 in such a tile
-            const int first = max(past, key0), last = min(vis, key0 + kTtKeys);
-            if (has)
-              for (int pos = first; pos < last; ++pos)
-                if (tree_sees(mask_row, tok, pos - past)) seen |= 1ull << (pos - key0);
-          }
           // 32 scores in units of own; unseen keys -inf.
           auto scores = [&](int h, float (&x)[32]) {
             tt_ld32(s_at + 32 * h, x);
@@ -776,10 +824,14 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             vx = unit[2 * kTtKeys];
             if constexpr (EDGE) {
               vx = 0.0f;
-#pragma unroll 1
-              for (int e = 0; e < kTtKeys; ++e) {
-                const float u = unit[kTtKeys + e];
-                if (((seen >> e) & 1) && u < INFINITY) vx = fmaxf(vx, u);
+#pragma unroll 4
+              for (int e = 0; e < kTtKeys; e += 4) {
+                const float4 u = *reinterpret_cast<const float4*>(unit + kTtKeys + e);
+                const float of[4] = {u.x, u.y, u.z, u.w};
+                const uint32_t bits = static_cast<uint32_t>(seen >> e);
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  if (((bits >> y) & 1) && of[y] < INFINITY) vx = fmaxf(vx, of[y]);
               }
             }
           }
@@ -862,7 +914,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           if (lane == 0) ts_arrive(&p_full[s][buf]);
           ++o_count;
         };
-        if (key0 + kTtKeys > past) tile(std::true_type{});
+        if (edge) tile(std::true_type{});
         else tile(std::false_type{});
       }
       slot0 = (slot0 + tiles) & (kTtUnitSlots - 1);
@@ -922,54 +974,107 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         if (!whole && tid == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
         const float inv = lj == 0.0f ? 0.0f : __fdiv_rn(1.0f, lj);
         const int64_t v_row = (b * p.kv_heads + kvh) * p.capacity;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          float o[16], o1[16];
-          tt_ld16(o_col(s) + lanes + c, o);
-          if (!SPLIT && !shifted && tiles > 1) {
-            tt_ld16(o_col(1) + lanes + c, o1);
-          } else if (!SPLIT && tiles > 1 && has) {
+        // Infinities and NaN of V that were taken out, for the rows that see them: 16 columns.
+        auto add_wild = [&](int c, float (&o)[16]) {
+          const int first = max(past, w.t0 * kTtKeys), last = min(vis, w.t1 * kTtKeys);
+          for (int pos = first; pos < last; ++pos) {
+            if (!tree_sees(mask_row, tok, pos - past)) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 x = area[(c / 4 + e) * 64 + n];
-              o1[4 * e] = x.x;
-              o1[4 * e + 1] = x.y;
-              o1[4 * e + 2] = x.z;
-              o1[4 * e + 3] = x.w;
+            for (int e = 0; e < 16; ++e) {
+              const float x = tt_v_global<D, FMT>(p.v, v_row + pos, c + e);
+              if (!isfinite(x)) o[e] += x;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o1[e] = 0.0f;
           }
-          if (!has) continue;  // the next tt_ld16 brings the lanes together again
+        };
+        if constexpr (SPLIT) {
+          // 32 columns at a time, turned in the place of this warp's own Q rows so that a store's lanes write whole
+          // lines; with a row per lane a store touches 32 (48 tokens after 32 positions, BF16: 37.8 -> 36.2 us).
+          // Without SPLIT the joins leave half of the warps at it, and the turn costs more than it saves
+          // (16 tokens after 1,000 positions, NVFP4: 35.9 -> 41.2 us).
+          uint8_t* turn = smem + C::kOffQ + warp * 4096;
+          const int n0 = __shfl_sync(kFull, n, 0), held = __popc(__ballot_sync(kFull, has));
+          const float f = whole ? f0 * inv : f0;
+          float* part = p.part_o + (slot * p.rows_per_pass + n0 + (lane >> 3)) * D + 4 * (lane & 7);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+#pragma unroll 1
+            for (int h = c; h < c + 32; h += 16) {
+              float o[16];
+              tt_ld16(o_col(s) + lanes + h, o);
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            o[e] = (f0 == 0.0f ? 0.0f : o[e] * f0) + (f1 == 0.0f ? 0.0f : o1[e] * f1);
-          if (s_wild) {  // infinities and NaN of V that were taken out, for the rows that see them
-            const int first = max(past, w.t0 * kTtKeys), last = min(vis, w.t1 * kTtKeys);
-            for (int pos = first; pos < last; ++pos) {
-              if (!tree_sees(mask_row, tok, pos - past)) continue;
+              for (int e = 0; e < 16; ++e) o[e] = f == 0.0f ? 0.0f : o[e] * f;
+              if (has && s_wild && f != 0.0f) add_wild(h, o);
+              if (has)
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float x = tt_v_global<D, FMT>(p.v, v_row + pos, c + e);
-                if (!isfinite(x)) o[e] += x;
+                for (int e = 0; e < 4; ++e)
+                  *reinterpret_cast<float4*>(turn + tt_chunk(lane, (h - c) / 4 + e)) =
+                      make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+            __syncwarp();
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row = i * 8 + (lane >> 2), ch = (lane & 3) * 2;
+                const int64_t to = __shfl_sync(kFull, q_row_own, row);
+                if (row < held) {
+                  const float4 x = *reinterpret_cast<const float4*>(turn + tt_chunk(row, ch));
+                  const float4 y = *reinterpret_cast<const float4*>(turn + tt_chunk(row, ch + 1));
+                  *reinterpret_cast<uint4*>(p.ctx + to * D + c + 4 * ch) =
+                      make_uint4(ts_pack_bf16(x.x, x.y), ts_pack_bf16(x.z, x.w), ts_pack_bf16(y.x, y.y),
+                                 ts_pack_bf16(y.z, y.w));
+                }
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int row = i * 4 + (lane >> 3);
+                if (row < held)
+                  *reinterpret_cast<float4*>(part + c + i * 4 * D) =
+                      *reinterpret_cast<const float4*>(turn + tt_chunk(row, lane & 7));
               }
             }
+            __syncwarp();
           }
-          if (whole) {
-            uint4* dst = reinterpret_cast<uint4*>(p.ctx + q_row * D + c);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float o[16], o1[16];
+            tt_ld16(o_col(s) + lanes + c, o);
+            if (!shifted && tiles > 1) {
+              tt_ld16(o_col(1) + lanes + c, o1);
+            } else if (tiles > 1 && has) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint32_t x[4];
+              for (int e = 0; e < 4; ++e) {
+                const float4 x = area[(c / 4 + e) * 64 + n];
+                o1[4 * e] = x.x;
+                o1[4 * e + 1] = x.y;
+                o1[4 * e + 2] = x.z;
+                o1[4 * e + 3] = x.w;
+              }
+            } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                x[y] = lj == 0.0f ? 0u : ts_pack_bf16(o[8 * e + 2 * y] * inv, o[8 * e + 2 * y + 1] * inv);
-              dst[e] = make_uint4(x[0], x[1], x[2], x[3]);
+              for (int e = 0; e < 16; ++e) o1[e] = 0.0f;
             }
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * p.rows_per_pass + n) * D + c);
+            if (!has) continue;  // the next tt_ld16 brings the lanes together again
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 16; ++e)
+              o[e] = (f0 == 0.0f ? 0.0f : o[e] * f0) + (f1 == 0.0f ? 0.0f : o1[e] * f1);
+            if (s_wild) add_wild(c, o);
+            if (whole) {
+              uint4* dst = reinterpret_cast<uint4*>(p.ctx + q_row_own * D + c);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t x[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  x[y] = lj == 0.0f ? 0u : ts_pack_bf16(o[8 * e + 2 * y] * inv, o[8 * e + 2 * y + 1] * inv);
+                dst[e] = make_uint4(x[0], x[1], x[2], x[3]);
+              }
+            } else {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + (slot * p.rows_per_pass + n) * D + c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
           }
         }
         if (has && !whole) p.part_ml[slot * p.rows_per_pass + n] = make_float2(mj, lj);
@@ -981,7 +1086,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   tt_fence_before();
   __syncthreads();
-  if (warp == kTtMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == kTtMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 }  // namespace nvfp4da
