@@ -478,4 +478,15 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
   return NVFP4DA_OK;
 }
 
+int nvfp4da_tree_attention_sync_status(void* stream, unsigned* flags, int clear) {
+  if (!flags) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "flags is NULL");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  void* word = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&word, g_tree_errors);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(flags, word, sizeof(unsigned), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess && clear) e = cudaMemsetAsync(word, 0, sizeof(unsigned), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "tree attention status read");
+}
+
 }  // extern "C"

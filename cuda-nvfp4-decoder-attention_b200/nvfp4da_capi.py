@@ -30,7 +30,7 @@ EXPORTED = (
     "nvfp4da_gqa_attention_partials_workspace_size", "nvfp4da_gqa_attention_partials",
     "nvfp4da_attention_combine", "nvfp4da_w4a16_gemm", "nvfp4da_decoder_attention_forward_hostio",
     "nvfp4da_apply_rope_qk", "nvfp4da_kv_quant_append", "nvfp4da_kv_quant_read",
-    "nvfp4da_tree_attention_workspace_size", "nvfp4da_tree_attention",
+    "nvfp4da_tree_attention_workspace_size", "nvfp4da_tree_attention", "nvfp4da_tree_attention_sync_status",
 )
 
 PATH_AUTO, PATH_CHAIN, PATH_STEP = 0, 1, 2
@@ -104,6 +104,7 @@ def load() -> C.CDLL:
         "nvfp4da_decoder_attention_forward_path": (C.c_int, [C.POINTER(ForwardArgs), vp, sz, vp, C.c_int]),
         "nvfp4da_forward_step_supported": (C.c_int, [C.POINTER(ForwardArgs)]),
         "nvfp4da_forward_sync_status": (C.c_int, [vp, C.POINTER(C.c_uint), C.c_int]),
+        "nvfp4da_tree_attention_sync_status": (C.c_int, [vp, C.POINTER(C.c_uint), C.c_int]),
         "nvfp4da_debug_wait_timeout": (C.c_int, [vp, C.c_ulonglong, C.POINTER(C.c_uint)]),
         "nvfp4da_qkv_rope_append_shard": (C.c_int, [C.POINTER(ForwardArgs), i64, i64, vp, vp, sz, vp]),
         "nvfp4da_qkv_rope_append_shard_workspace_size": (sz, [C.POINTER(ForwardArgs)]),
@@ -268,6 +269,14 @@ def sync_status(stream=None, clear: bool = True) -> int:
     timed out); synchronises the stream."""
     flags = C.c_uint(0)
     _check(load().nvfp4da_forward_sync_status(_stream(stream), C.byref(flags), 1 if clear else 0))
+    return flags.value
+
+
+def tree_sync_status(stream=None, clear: bool = True) -> int:
+    """Error flags of tree attention on the current device (bit 0: a bounded
+    wait timed out); synchronises the stream."""
+    flags = C.c_uint(0)
+    _check(load().nvfp4da_tree_attention_sync_status(_stream(stream), C.byref(flags), 1 if clear else 0))
     return flags.value
 
 

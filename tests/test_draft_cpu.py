@@ -196,3 +196,9 @@ def test_oracle_planted_mistake_is_seen():
     good, _ = ref.tree_attention(q, k, v, [6], mask)
     mask[0, 2, 0] = ~mask[0, 2, 0]
     assert (ref.tree_attention(q, k, v, [6], mask)[0] - good).abs().max() > 1e-3
+
+
+def test_tree_status_needs_a_place_for_the_flags():
+    import nvfp4da_capi as capi
+
+    assert capi.load().nvfp4da_tree_attention_sync_status(None, None, 1) == capi.ERR_INVALID_ARGUMENT

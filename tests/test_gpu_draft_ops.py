@@ -516,3 +516,27 @@ def test_tree_step_and_acceptance(cp, fmt):
         s = slice(int(past[i]), int(past[i]) + n)
         a, c = (cp.cuda_quantized_kv_read(z)[0][i, :, s].float() for z in (tree, chain))
         assert (a - c).abs().mean() <= 2.0 ** -6 * float(c.abs().mean())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("t", [2, 6, 16, 40])  # 8, 24, 64 and 160 query rows a KV head
+def test_repeated_calls_agree_and_no_wait_gives_up(cp, fmt, t):
+    """Nothing depends on which warp or CTA comes first, across uneven units that many CTAs share."""
+    from tree_decoding import check_tree_wait_status
+
+    b, hkv, group, cap, d = 3, 3, 4, 6144, 128
+    cache = filled(cp, fmt, b, hkv, cap, d, 41)
+    q = randn((b, t, hkv * group, d), 42).cuda()
+    mask, _ = ref.random_tree(b, t, 43)
+    past = torch.tensor([cap - t, 1717, 70]).cuda() if fmt != "bf16" else None
+
+    def call():
+        return cp.cuda_tree_attention_cached(q, cache, 0 if past is not None else cap - t, tree_mask=mask.cuda(),
+                                             past_lengths=past, max_past_length=cap - t)
+
+    check_tree_wait_status()
+    first = call()
+    for _ in range(200):
+        again = call()
+    assert torch.equal(first, again) and torch.isfinite(first.float()).all()
+    check_tree_wait_status()
