@@ -15,10 +15,10 @@
 //   129 to 256 rows  each stream holds half of the rows and takes every tile.
 //
 // Roles: warps 0-3 and 4-7 softmax of streams 0 and 1 (one query row per
-// thread); warps 8-15 prepare operands (K and V); warps 16 and 18 issue the MMAs of a
-// stream each (one warp for both could not issue them fast enough beside the
-// others on its scheduler); warp 17 loads, warp
-// 19 the scales.  Per tile of 64 keys:
+// thread); warps 8-11 prepare K and 12-15 V; warps 16 and 18 issue the MMAs of
+// a stream each (one warp for both could not issue them fast enough beside the
+// others on its scheduler); warp 17 loads codes, warp 19 scales.  Per tile of 64
+// keys:
 //   load     codes and scales (TMA, bulk copies) into a ring; BF16 K and V
 //            straight into operand tiles;
 //   prepare  codes (times the NVFP4 block scale) to FP16, exact, as [key][d]
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile unsigned s_bad;    // a wait gave up
   __shared__ volatile unsigned s_wild;   // an infinity or NaN was taken out of V
-  __shared__ float4 join[kTtRows];       // stream 1's m, l and the unit of its o
+  __shared__ float4 join[2][kTtRows];    // a stream's m, l and the unit of its o, where the two are joined
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   float* units_kv = reinterpret_cast<float*>(smem + C::kOffUnits);  // [slot][kUnitFloats]
 
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     }
     mbar_init(&seg_done, 2 * active);
     mbar_init(&join_ready, 2 * active);
-    mbar_init(&join_read, active);
+    mbar_init(&join_read, 2 * active);
     fence_mbar_init();
     s_bad = 0u;
     s_wild = 0u;
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const bool warp_has = __any_sync(kFull, has);
       const int tok = has ? (n_first + n) / p.group : 0;
       const int64_t q_row_own = q_row(b, w.u, n);
-      if (!SPLIT && !first_segment) {  // all of stream 0 has read what the join left in the place of Q
+      if (!SPLIT && !first_segment) {  // both streams have read what the join left in the place of Q
         ok = tt_wait(&join_read, end_phase ^ 1u, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
       }
@@ -928,25 +928,27 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       l *= unit_o;
       float4* area = reinterpret_cast<float4*>(smem + C::kOffQ);  // [D / 4][64 rows]
       if (!SPLIT) {
-        // Every MMA of the segment has read its Q.  Stream 0 reads stream 1's accumulator in tensor memory,
-        // or, where its rows lie in other lanes, in the place of Q.
+        // Every MMA of the segment has read its Q.  Where the streams' rows lie in different lanes, stream 0
+        // joins the first half of the columns and stream 1 the second, each reading the other's accumulator in the
+        // place of Q (16 tokens over 32,000 positions, NVFP4: 165 us with stream 0 alone, 160 us so).  Else stream 0
+        // joins all, reading both in tensor memory (32 tokens, E4M3: halves took 66 us, this 64).
         __syncwarp();
         if (lane == 0) ts_arrive(&seg_done);
         ok = ok && tt_wait(&seg_done, end_phase, &s_bad);
         ok = __all_sync(kFull, ok);
-        if (ok && s == 1 && warp_has) {
+        if (ok && warp_has) {
           if (done > 0 && shifted) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = (1 - s) * (D / 2), i = 0; i < D / 2; c += 16, i += 16) {
               float o[16];
-              tt_ld16(o_col(1) + lanes + c, o);
+              tt_ld16(o_col(s) + lanes + c, o);
               if (has)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   area[(c / 4 + e) * 64 + n] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
           }
-          if (has) join[n] = make_float4(m, l, unit_o, 0.0f);
+          if (has) join[s][n] = make_float4(m, l, unit_o, 0.0f);
         }
         tt_fence_before();
         __syncwarp();
@@ -956,16 +958,18 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         tt_fence_after();
         end_phase ^= 1u;
       }
-      if (ok && warp_has && (SPLIT || s == 0)) {
-        float f0 = unit_o, f1 = 0.0f, mj = m, lj = l;
-        if (!SPLIT && tiles > 1) {
-          const float4 other = has ? join[n] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-          mj = fmaxf(m, other.x);
-          const float a0 = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ts_exp2(m - mj);
-          const float a1 = other.x == -INFINITY ? (other.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(other.x - mj);
-          lj = l * a0 + other.y * a1;
-          f0 *= a0;
-          f1 = other.z * a1;
+      if (ok && warp_has) {
+        float f_own = unit_o, f_other = 0.0f, mj = m, lj = l;
+        const bool two = !SPLIT && tiles > 1;  // stream 1 had a tile
+        if constexpr (!SPLIT) {
+          const float4 none = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+          const float4 j0 = has ? join[0][n] : none, j1 = has && two ? join[1][n] : none;
+          mj = fmaxf(j0.x, j1.x);
+          const float a0 = j0.x == -INFINITY ? (j0.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(j0.x - mj);
+          const float a1 = j1.x == -INFINITY ? (j1.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(j1.x - mj);
+          lj = j0.y * a0 + j1.y * a1;
+          f_own = s == 0 ? j0.z * a0 : j1.z * a1;
+          f_other = s == 0 ? j1.z * a1 : j0.z * a0;
         }
         const bool whole = w.t0 == 0 && w.t1 == w.nt;
         int n_tiles, G, x0;
@@ -993,7 +997,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           // (16 tokens after 1,000 positions, NVFP4: 35.9 -> 41.2 us).
           uint8_t* turn = smem + C::kOffQ + warp * 4096;
           const int n0 = __shfl_sync(kFull, n, 0), held = __popc(__ballot_sync(kFull, has));
-          const float f = whole ? f0 * inv : f0;
+          const float f = whole ? f_own * inv : f_own;
           float* part = p.part_o + (slot * p.rows_per_pass + n0 + (lane >> 3)) * D + 4 * (lane & 7);
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
@@ -1037,12 +1041,20 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           }
         } else {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = shifted ? s * (D / 2) : s * D, i = 0; i < (shifted ? D / 2 : D) && c < D; c += 16, i += 16) {
             float o[16], o1[16];
-            tt_ld16(o_col(s) + lanes + c, o);
-            if (!shifted && tiles > 1) {
-              tt_ld16(o_col(1) + lanes + c, o1);
-            } else if (tiles > 1 && has) {
+            if (s == 0 || two) {
+              tt_ld16(o_col(s) + lanes + c, o);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+            }
+            if (s == 0 && !two) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o1[e] = 0.0f;
+            } else if (!shifted) {
+              tt_ld16(o_col(1 - s) + lanes + c, o1);
+            } else if (has) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float4 x = area[(c / 4 + e) * 64 + n];
@@ -1051,14 +1063,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                 o1[4 * e + 2] = x.z;
                 o1[4 * e + 3] = x.w;
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o1[e] = 0.0f;
             }
             if (!has) continue;  // the next tt_ld16 brings the lanes together again
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[e] = (f0 == 0.0f ? 0.0f : o[e] * f0) + (f1 == 0.0f ? 0.0f : o1[e] * f1);
+              o[e] = (f_own == 0.0f ? 0.0f : o[e] * f_own) + (f_other == 0.0f ? 0.0f : o1[e] * f_other);
             if (s_wild) add_wild(c, o);
             if (whole) {
               uint4* dst = reinterpret_cast<uint4*>(p.ctx + q_row_own * D + c);
@@ -1077,11 +1086,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             }
           }
         }
-        if (has && !whole) p.part_ml[slot * p.rows_per_pass + n] = make_float2(mj, lj);
+        if (has && !whole && (SPLIT || s == 0)) p.part_ml[slot * p.rows_per_pass + n] = make_float2(mj, lj);
       }
       tt_fence_before();
       __syncwarp();
-      if (!SPLIT && s == 0 && lane == 0) ts_arrive(&join_read);
+      if (!SPLIT && lane == 0) ts_arrive(&join_read);
     }
   }
   tt_fence_before();
