@@ -99,26 +99,34 @@ constexpr int kTsWarps = 8;
 // 16-position slices a warp takes at once: two hide the latency of decoding
 // codes (E4M3 87 -> 77 us, NVFP4 93 -> 81 us on 8 x 32K positions); BF16 has
 // none to hide.
-template <int D, int FMT, int NG>
-constexpr int ts_slices() { return FMT != kKvFmtBf16 && NG == 1 && D <= 128 ? 2 : 1; }
+template <int D, int FMT>
+constexpr int ts_slices() { return FMT != kKvFmtBf16 && D <= 128 ? 2 : 1; }
 
 // Query rows per KV head from which tree_tc_kernel runs.  The streaming kernel
-// decodes a tile once per 16 rows, this one once per 256.  Both, 8 sequences x 6
-// KV heads x 4 query heads each, us streaming / tcgen05 after 300, 2,000 and
-// 12,000 positions:
-//             20 rows (5 tokens)                 64 rows (16 tokens)
-//   BF16      29 / 28   37 / 31    78 / 72       66 / 27   78 / 33   151 / 75
-//   E4M3      26 / 27   46 / 35   146 / 77       47 / 30   88 / 38   211 / 84
-//   NVFP4     26 / 28   45 / 36   131 / 77       47 / 30   87 / 38   192 / 82
-// Up to 16 rows the streaming kernel reads the cache at up to 0.9 of its floor's
-// rate, and a 128-row tile would be mostly empty.
-constexpr int64_t kTcMinRows = 17;
+// decodes codes in registers for the rows of one warp, this one once for all
+// rows.  Both, 8 sequences x 6 KV heads x 4 query heads each, us streaming /
+// tcgen05 after 300, 2,000 and 12,000 positions:
+//          8 rows (2 tokens)        12 rows                  20 rows                  64 rows
+//   BF16   20/27  23/28  58/69      25/26  30/29   65/69     29/28  37/31   78/72     66/27  78/33  151/75
+//   E4M3   20/26  23/33  41/74      22/26  39/32  131/74     26/27  46/35  146/77     47/30  88/38  211/84
+//   NVFP4  20/27  24/33  40/72      22/26  38/33  118/72     26/28  45/36  131/77     47/30  87/38  192/82
+constexpr int64_t tc_min_rows(bool bf16) { return bf16 ? 13 : 9; }
+
+// Rows from which, and parts a unit has at most (CTAs per unit), where a warp
+// joins four rows instead of one: 192 rows over BF16 (16 sequences, 8,000
+// positions) 146 -> 141 us in all, 64 rows over NVFP4 (8, 32,000) 159 -> 155;
+// with 12 parts a unit the few warps take longer (41 -> 42 us).
+constexpr int64_t kJoin4MinRows = 17, kJoin4MaxParts = 8;
 
 template <int D>
 cudaError_t launch_tree_combine(const TreeStreamParams& p, cudaStream_t s) {
+  const int64_t rows = std::min(p.rows_per_pass, p.group * p.tokens);
+  const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * p.passes;
+  const bool four = rows >= kJoin4MinRows && units * kJoin4MaxParts >= p.grid;
   const dim3 grid(static_cast<unsigned>(2 * p.grid),
-                  static_cast<unsigned>(ceil_div(std::min(p.rows_per_pass, p.group * p.tokens), kTsJoinWarps)));
-  return launch(tree_stream_combine_kernel<D>, grid, dim3(kTsJoinWarps * 32), 0, s, true, p);
+                  static_cast<unsigned>(ceil_div(rows, four ? kTsJoinWarps * kTsJoinRows : kTsJoinWarps)));
+  return launch(four ? tree_stream_combine4_kernel<D> : tree_stream_combine_kernel<D>, grid, dim3(kTsJoinWarps * 32), 0,
+                s, true, p);
 }
 
 template <int D, int FMT, bool SPLIT>
@@ -141,7 +149,7 @@ cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const T
 template <int D, int FMT, int NG>
 cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p,
                                cudaStream_t s) {
-  constexpr int SL = ts_slices<D, FMT, NG>(), NW = kTsWarps;
+  constexpr int SL = ts_slices<D, FMT>(), NW = kTsWarps;
   auto* kern = tree_stream_kernel<D, FMT, NG, NW, SL>;
   const uint32_t smem = TsCfg<D, FMT, NG, NW, SL>::bytes(p.batch);
   cudaError_t e = ensure_smem(kern, smem);
@@ -161,9 +169,12 @@ cudaError_t launch_tree_tc_d(int64_t head_dim, bool split, const CUtensorMap& tk
 template <int FMT>
 cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const TreeStreamParams& p, cudaStream_t s) {
+  if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
+    if (wide == 2)
+      return head_dim == 64 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<128, FMT, 2>(tk, tv, p, s);
   switch (head_dim) {
-    case 64: return wide == 2 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
-    case 128: return wide == 2 ? launch_tree_stream<128, FMT, 2>(tk, tv, p, s) : launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
+    case 64: return launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
+    case 128: return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
     default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
   }
 }
@@ -199,7 +210,7 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
   // tile line of 128-byte lines and the prefix of the batch have to fit.
   pl.stream = (d == 64 || d == 128 || d == 256) && c->batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
               product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
-  pl.tc = pl.stream && d <= 128 && nq >= kTcMinRows;
+  pl.tc = pl.stream && d <= 128 && nq >= tc_min_rows(c->format == NVFP4DA_KV_BF16);
   // Tiles and their order are 32-bit in the kernels.
   const int64_t most_passes = ceil_div(nq, 8);
   if (!product_within(c->batch * c->kv_heads * ceil_div(c->capacity, kTtKeys), most_passes, kI32Max))

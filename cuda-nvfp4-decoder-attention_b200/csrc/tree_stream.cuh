@@ -1078,4 +1078,95 @@ __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(
     dst[i] = l == 0.0f ? 0u : ts_pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
 }
 
+// The same where there are many rows of few parts: a warp joins four rows, eight
+// lanes working out one row's weights (eight parts at a time).  With a row per
+// warp the divisions, shuffles and address arithmetic of a row were most of the
+// instructions, which bound the kernel.
+constexpr int kTsJoinRows = 4;
+
+template <int D>
+__global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine4_kernel(const TreeStreamParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int4 unit = __ldcg(&p.part_slots[blockIdx.x]);
+  if (unit.x < 0) return;
+  const int b = unit.x, u = unit.y, c0 = unit.z, c1 = unit.w;
+  const int pass = p.passes == 1 ? 0 : u % p.passes, kvh = p.passes == 1 ? u : u / p.passes;
+  const int lane = threadIdx.x & 31, sub = lane & 7, mine = lane >> 3;  // part and row this lane weighs
+  const int r0 = (blockIdx.y * kTsJoinWarps + (threadIdx.x >> 5)) * kTsJoinRows;
+  const int rows = min(kTsJoinRows, min(p.rows_per_pass, p.group * p.tokens - pass * p.rows_per_pass) - r0);
+  if (rows <= 0) return;
+  // Row of a part's slot (fewer than 2^31 / D of them): the unit's part in its first CTA is in this slot, in the
+  // others in their first.
+  auto at = [&](int c) { return (c == c0 ? static_cast<int>(blockIdx.x) : 2 * c) * p.rows_per_pass + r0; };
+  constexpr int V = D / 32;  // elements per lane
+  float x[2][kTsJoinRows][V];
+  auto fetch = [&](int c, float (&y)[kTsJoinRows][V]) {
+    const float* src = p.part_o + static_cast<int64_t>(at(c)) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < kTsJoinRows; ++i) {
+      if (i >= rows) break;
+      if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(y[i]) = __ldcg(reinterpret_cast<const float2*>(src + i * D));
+      } else {
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k)
+          reinterpret_cast<float4*>(y[i])[k] = __ldcg(reinterpret_cast<const float4*>(src + i * D) + k);
+      }
+    }
+  };
+  auto stats = [&](int c) {
+    return c <= c1 && mine < rows ? __ldcg(&p.part_ml[at(c) + mine]) : make_float2(-INFINITY, 0.0f);
+  };
+  fetch(c0, x[0]);  // beside the (m, l) loads
+  if (c0 < c1) fetch(c0 + 1, x[1]);
+  float2 ml = stats(c0 + sub);
+  float mx = ml.x;
+  for (int c = c0 + 8; c <= c1; c += 8) mx = fmaxf(mx, stats(c + sub).x);
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, o));
+  float o[kTsJoinRows][V] = {}, l = 0.0f, f = 0.0f;
+  auto add = [&](int c, const float (&y)[kTsJoinRows][V]) {
+#pragma unroll
+    for (int i = 0; i < kTsJoinRows; ++i) {
+      const float fc = __shfl_sync(kFull, f, 8 * i + ((c - c0) & 7));
+      if (fc == 0.0f) continue;  // uniform; also rows past the last
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[i][k] = fmaf(y[i][k], fc, o[i][k]);
+    }
+  };
+  for (int c = c0; c <= c1; c += 2) {
+    if (((c - c0) & 7) == 0) {
+      if (c > c0) ml = stats(c + sub);
+      f = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ts_exp2(ml.x - mx);
+      l = fmaf(ml.y, f, l);
+    }
+    add(c, x[0]);
+    if (c + 2 <= c1) fetch(c + 2, x[0]);
+    if (c + 1 <= c1) add(c + 1, x[1]);
+    if (c + 3 <= c1) fetch(c + 3, x[1]);
+  }
+#pragma unroll
+  for (int k = 1; k < 8; k <<= 1) l += __shfl_xor_sync(kFull, l, k);
+  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+  const int n = pass * p.rows_per_pass + r0 + mine, tok = n / p.group;
+  const int row = (b * p.tokens + tok) * p.q_heads + kvh * p.group + (n - tok * p.group);  // below 2^31
+#pragma unroll
+  for (int i = 0; i < kTsJoinRows; ++i) {
+    if (i >= rows) break;
+    const float by = __shfl_sync(kFull, inv, 8 * i);
+    const int64_t to = __shfl_sync(kFull, row, 8 * i);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.ctx + to * D + lane * V);
+    uint32_t y[V / 2];
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) y[k] = by == 0.0f ? 0u : ts_pack_bf16(o[i][2 * k] * by, o[i][2 * k + 1] * by);
+    if constexpr (V == 2) {
+      dst[0] = y[0];
+    } else {
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) reinterpret_cast<uint2*>(dst)[k] = make_uint2(y[2 * k], y[2 * k + 1]);
+    }
+  }
+}
+
 }  // namespace nvfp4da
