@@ -41,6 +41,15 @@
 // infinities and NaN in V before the MMA (0 * NaN would reach queries that do
 // not see the row); queries that do see such an element get it added after.
 //
+// What bounds it: a single token over ragged E4M3 caches (64 sequences x 6 heads,
+// 1,024 to 8,191 positions, 460 MB) takes 94 us, 4.9 TB/s, 0.75 of a copy; of
+// that the launches, the first tiles' latency and the join of partials are some
+// 12 us, the rest streams at 0.85.  Over NVFP4 (8 sequences, 32,768 positions)
+// 70 us, 3.4 TB/s: decoding codes to FP16 in registers, 43 % of the issue slots
+// and the latency between them with two warps a scheduler, no longer the bytes.
+// 12 or 16 consumer warps, for which registers suffice with one slice at a time,
+// were no faster.
+//
 // Waits are bounded: a barrier that does not complete within 2^22 tries records
 // kErrBarrierTimeout in g_tree_errors and the CTA stops waiting (its results
 // are then garbage; the GPU stays usable).

@@ -37,6 +37,22 @@
 // the kernel 1.6 times as long.
 // The numerics are those of tree_stream.cuh (P is 2^2 p_j gamma_j / G here).
 //
+// What bounds it, at 1.9 GHz.  Over codes with up to 128 rows: the roles' own
+// latency.  A tile's MMAs take 650 cycles (49 for a step of K Q^T, read from
+// shared memory, 65 for one of P V), but a softmax warp, alone on its scheduler
+// but for two preparing warps, takes 1,450 a tile of its stream, and preparing
+// one 1,400; the pipeline moves a tile every 1,400.  16 tokens over NVFP4 (8
+// sequences x 6 heads, 30,001 to 32,752 positions): 154 us, 320 TFLOP/s, tensor
+// pipe 31 % busy.  Over BF16 with more than 128 rows: the MMAs, since P is two
+// terms: 1,824 of some 2,400 cycles a tile of 256 rows, 75 % of them rows.  48
+// tokens (16 sequences, 8,000 positions): 127 us, 447 TFLOP/s, pipe 56 % busy.
+// A segment costs 15,000 to 20,000 cycles beside its tiles: the walk, Q, the
+// first tile's second pass, the join and the partial results.
+// Tried, and not kept: the two preparing groups taking K and V of alternate tiles
+// (every ring then needs an even number of buffers; 165 -> 170 us), scores and
+// P V issued in whatever order they are ready (-> 176 us), more buffers for K
+// and V, three shares of registers.
+//
 // Waits are bounded (one second, shared give-up flag, recorded in
 // g_tree_errors); tensor memory is freed on every path.
 #pragma once
@@ -65,7 +81,7 @@ struct TtCfg {
   static constexpr bool kQuant = FMT != kKvFmtBf16;
   static constexpr int kPanels = D / 64;                      // 64-element panels of a row
   static constexpr uint32_t kOperand = kPanels * kTtKeys * 128;  // a K or V tile, 16-bit
-  static constexpr int kK = kQuant ? (SPLIT ? 2 : 3) : 4;   // K and V tiles in flight
+  static constexpr int kK = kQuant ? (SPLIT ? 2 : 3) : 4;  // K and V tiles in flight
   static constexpr int kV = kQuant ? 3 : 4;
   static constexpr int kStages = kQuant ? (FMT == kKvFmtNvfp4 ? 4 : 3) : 0;  // ring of codes
   static constexpr int kQRows = SPLIT ? 256 : 192;
