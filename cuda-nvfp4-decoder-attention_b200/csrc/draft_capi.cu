@@ -99,18 +99,24 @@ constexpr int kTsWarps = 8;
 // 16-position slices a warp takes at once: two hide the latency of decoding
 // codes (E4M3 87 -> 77 us, NVFP4 93 -> 81 us on 8 x 32K positions); BF16 has
 // none to hide.
-template <int D, int FMT>
-constexpr int ts_slices() { return FMT != kKvFmtBf16 && D <= 128 ? 2 : 1; }
+template <int D, int FMT, int NG>
+constexpr int ts_slices() { return FMT != kKvFmtBf16 && NG == 1 && D <= 128 ? 2 : 1; }
 
 // Query rows per KV head from which tree_tc_kernel runs.  The streaming kernel
 // decodes codes in registers for the rows of one warp, this one once for all
 // rows.  Both, 8 sequences x 6 KV heads x 4 query heads each, us streaming /
-// tcgen05 after 300, 2,000 and 12,000 positions:
+// tcgen05 after 300, 2,000 and 12,000 positions, head_dim 128:
 //          8 rows (2 tokens)        12 rows                  20 rows                  64 rows
 //   BF16   20/27  23/28  58/69      25/26  30/29   65/69     29/28  37/31   78/72     66/27  78/33  151/75
 //   E4M3   20/26  23/33  41/74      22/26  39/32  131/74     26/27  46/35  146/77     47/30  88/38  211/84
 //   NVFP4  20/27  24/33  40/72      22/26  38/33  118/72     26/28  45/36  131/77     47/30  87/38  192/82
-constexpr int64_t tc_min_rows(bool bf16) { return bf16 ? 13 : 9; }
+// and head_dim 64, where a tile is half the bytes and the decoding, but the
+// tcgen05 kernel's warps take as long for it:
+//          12 rows                  24 rows                  32 rows                  64 rows
+//   BF16   27/27  26/28  38/57      22/26  27/26  56/58      27/27  31/26  60/59      41/21  48/27   96/62
+//   E4M3   20/23  23/29  45/65      21/24  30/30  62/66      21/24  33/30  66/67      29/25  52/32  106/73
+//   NVFP4  20/24  23/30  43/68      20/24  30/31  61/70      21/25  34/31  64/71      29/26  52/32  107/76
+constexpr int64_t tc_min_rows(int64_t head_dim, bool bf16) { return head_dim == 64 ? 33 : bf16 ? 13 : 9; }
 
 // Rows from which, and parts a unit has at most (CTAs per unit), where a warp
 // joins four rows instead of one: 192 rows over BF16 (16 sequences, 8,000
@@ -149,7 +155,7 @@ cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const T
 template <int D, int FMT, int NG>
 cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p,
                                cudaStream_t s) {
-  constexpr int SL = ts_slices<D, FMT>(), NW = kTsWarps;
+  constexpr int SL = ts_slices<D, FMT, NG>(), NW = kTsWarps;
   auto* kern = tree_stream_kernel<D, FMT, NG, NW, SL>;
   const uint32_t smem = TsCfg<D, FMT, NG, NW, SL>::bytes(p.batch);
   cudaError_t e = ensure_smem(kern, smem);
@@ -169,12 +175,12 @@ cudaError_t launch_tree_tc_d(int64_t head_dim, bool split, const CUtensorMap& tk
 template <int FMT>
 cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const TreeStreamParams& p, cudaStream_t s) {
-  if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
-    if (wide == 2)
-      return head_dim == 64 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<128, FMT, 2>(tk, tv, p, s);
   switch (head_dim) {
-    case 64: return launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
-    case 128: return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
+    case 64: return wide == 2 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
+    case 128:
+      if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
+        if (wide == 2) return launch_tree_stream<128, FMT, 2>(tk, tv, p, s);
+      return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
     default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
   }
 }
@@ -210,7 +216,7 @@ int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_
   // tile line of 128-byte lines and the prefix of the batch have to fit.
   pl.stream = (d == 64 || d == 128 || d == 256) && c->batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
               product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
-  pl.tc = pl.stream && d <= 128 && nq >= tc_min_rows(c->format == NVFP4DA_KV_BF16);
+  pl.tc = pl.stream && d <= 128 && nq >= tc_min_rows(d, c->format == NVFP4DA_KV_BF16);
   // Tiles and their order are 32-bit in the kernels.
   const int64_t most_passes = ceil_div(nq, 8);
   if (!product_within(c->batch * c->kv_heads * ceil_div(c->capacity, kTtKeys), most_passes, kI32Max))

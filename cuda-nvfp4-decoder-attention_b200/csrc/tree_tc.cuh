@@ -45,7 +45,8 @@
 // sequences x 6 heads, 30,001 to 32,752 positions): 154 us, 320 TFLOP/s, tensor
 // pipe 31 % busy.  Over BF16 with more than 128 rows: the MMAs, since P is two
 // terms: 1,824 of some 2,400 cycles a tile of 256 rows, 75 % of them rows.  48
-// tokens (16 sequences, 8,000 positions): 127 us, 447 TFLOP/s, pipe 56 % busy.
+// tokens (16 sequences, 8,000 positions): 127 to 139 us on several machines, 410
+// to 447 TFLOP/s, pipe 56 % busy.
 // A segment costs 15,000 to 20,000 cycles beside its tiles: the walk, Q, the
 // first tile's second pass, the join and the partial results.
 // Tried, and not kept: the two preparing groups taking K and V of alternate tiles
