@@ -26,11 +26,11 @@
 // few lanes, and the divisions of the scales are shared by 16 elements (with 8
 // per lane they were half of the instructions, which bound the kernel).  Read:
 // 8 elements per lane, so that 16-byte stores of a warp are contiguous, and
-// several rows of K and V in flight per thread.  Measured: 32,768
-// positions x 24 heads of E4M3 read back, with an append of 8, in 99 to
-// 104 us (5.9 to 6.2 TB/s, 0.90 to 0.94 of a copy).  Where the cache stays in L2 the instructions bound
-// both: 8,192 tokens x 6 heads to NVFP4 rows in 12 us (issue slots 67 % busy,
-// DRAM 26 %), and back in 10 us (62 %).
+// several rows of K and V in flight per thread.  Measured: 32,768 positions x
+// 24 heads of E4M3 read back, with an append of 8, in 99 to 104 us (5.9 to 6.2
+// TB/s, 0.90 to 0.94 of a copy).  Where the cache stays in L2 the instructions
+// bound both: 8,192 tokens x 6 heads to NVFP4 rows in 12 us (issue slots 67 %
+// busy, DRAM 26 %), and back in 10 us (62 %).
 #pragma once
 
 #include <float.h>

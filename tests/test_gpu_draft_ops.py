@@ -540,3 +540,11 @@ def test_repeated_calls_agree_and_no_wait_gives_up(cp, fmt, t):
         again = call()
     assert torch.equal(first, again) and torch.isfinite(first.float()).all()
     check_tree_wait_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [8, 9, 12, 13, 16, 17, 32, 33, 64, 65, 128, 129, 257])
+def test_rows_on_both_sides_of_every_kernel_rule(cp, fmt, d, rows):
+    """Twenty units of uneven length whose parts several CTAs share, joined one or four rows a warp."""
+    check_tree(cp, fmt, 5, rows, 4, 4, d, [700, 130, 0, 701, 333], 1024, 51 + rows)
