@@ -995,9 +995,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         if (!whole && tid == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
         const float inv = lj == 0.0f ? 0.0f : __fdiv_rn(1.0f, lj);
         const int64_t v_row = (b * p.kv_heads + kvh) * p.capacity;
-        // Infinities and NaN of V that were taken out, for the rows that see them: 16 columns.
+        // Infinities and NaN of V that were taken out, for the rows that see them: 16 columns.  They were taken out of
+        // whole tiles, so the first such tile's committed rows, before P_b, count too.
         auto add_wild = [&](int c, float (&o)[16]) {
-          const int first = max(past, w.t0 * kTtKeys), last = min(vis, w.t1 * kTtKeys);
+          const int first = max(past / kTtKeys * kTtKeys, w.t0 * kTtKeys), last = min(vis, w.t1 * kTtKeys);
           for (int pos = first; pos < last; ++pos) {
             if (!tree_sees(mask_row, tok, pos - past)) continue;
 #pragma unroll
