@@ -29,12 +29,17 @@
 // Numerics.  Codes (times the NVFP4 block scale) are exact in FP16; the query
 // row is scaled by a power of two to FP16 (exact down to 2^-39 of its largest
 // element); the row scale of K multiplies the FP32 score.  P goes to FP16 as
-// p_j gamma_j / G 2^5, G the largest row scale of V that the query has seen so
-// far (>= 2^-100): 11 significant bits down to 2^-19 of the reference, and
-// absolute steps of 2^-29 of it below.  Over BF16 caches Q and V stay
-// BF16 and P is split into two BF16 terms.  The softmax runs in base 2; its
-// reference m moves only when a score passes it by the slack, so most slices
-// need neither a reduction nor a rescale.  m, l, o and all sums are FP32.
+// p_j gamma_j / G 2^5, where G follows the largest contribution p_j gamma_j that
+// the query has met (>= 2^-100): 11 significant bits down to 2^-19 of that
+// contribution, absolute steps of 2^-29 of it below.  (With the largest gamma_j
+// in the place of G, a key that carries nearly all of the weight lost its bits
+// when its row of V was small beside one that weighs nothing.)  Over BF16 caches
+// Q and V stay BF16 and P is split into two BF16 terms.  The softmax runs in base
+// 2; its reference m moves only when a score passes it, to 2^10 above that score
+// (BF16: when one passes it by 2^20, to the score), and G only when a contribution
+// passes it by 2^10, so most slices need neither a reduction nor a rescale.  m, l,
+// o and all sums are FP32; o is held in units of G, which shrinks with p_j when m
+// moves, so that a move of m leaves o as it is.
 //
 // Slices that reach P_b (drafted tokens, the sequence's end) take a second
 // instantiation that applies the mask, drops positions past the end and zeroes
@@ -73,11 +78,16 @@ __device__ unsigned g_tree_errors;
 template <int FMT>
 constexpr int kTsTile = FMT == kKvFmtBf16 ? 64 : 128;
 constexpr int kTsMaxBatch = 1024;  // sequences whose prefix shared memory holds
-// A score may pass the reference m by 2^kTsSlack: P in FP16 then stays below
-// kTsPScale 2^10 = 2^15; BF16 terms have the range of FP32.
+// A score may pass the reference m by kTsSlack (log2), and m moves to kTsLift
+// above the score that passed it.  Over codes p_j <= 1 then, so that p_j gamma_j
+// cannot overflow; it may pass G until P in FP16, kTsPScale p_j gamma_j / G,
+// reaches kTsPLimit.  BF16 terms have the range of FP32.
 template <int FMT>
-constexpr float kTsSlack = FMT == kKvFmtBf16 ? 20.0f : 10.0f;
+constexpr float kTsSlack = FMT == kKvFmtBf16 ? 20.0f : 0.0f;
+template <int FMT>
+constexpr float kTsLift = FMT == kKvFmtBf16 ? 0.0f : 10.0f;
 constexpr float kTsPScale = 32.0f;
+constexpr uint32_t kTsPLimit = 0x7800u;  // 2^15 in FP16
 constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 
 template <int D, int FMT, int NG, int NW, int SL, int TILE = kTsTile<FMT>>
@@ -194,6 +204,12 @@ __device__ __forceinline__ uint32_t ts_pack_bf16(float lo, float hi) {
 __device__ __forceinline__ uint32_t ts_hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Of each FP16 half, the one of larger magnitude (with some sign); NaN only where both are.
+__device__ __forceinline__ uint32_t ts_largest(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 // Two packed pairs of E4M3 -> two f16x2.
@@ -730,11 +746,23 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             sc[z][j][i] = x;
             above |= x > m_run[j][i & 1] + kTsSlack<FMT>;
           }
+      auto rescale = [&](const float (&f)[NG][2]) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            acc[j][i][0] *= f[j][0];
+            acc[j][i][1] *= f[j][1];
+            acc[j][i][2] *= f[j][0];
+            acc[j][i][3] *= f[j][1];
+          }
+      };
       // ---- the reference moves (for every column) when a score passes it by the slack
       if (__any_sync(kFull, above)) {
+        float alpha[NG][2];
+        [[maybe_unused]] bool low = false;
 #pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          float alpha[2];
+        for (int j = 0; j < NG; ++j)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float mx = fmaxf(sc[0][j][c], sc[0][j][c + 2]);
@@ -743,90 +771,109 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-            const float m_new = fmaxf(m_run[j][c], mx);
-            alpha[c] = m_run[j][c] == -INFINITY ? 0.0f : ts_exp2(m_run[j][c] - m_new);
+            const float m_new = fmaxf(m_run[j][c], mx + kTsLift<FMT>);
+            const bool fresh = m_run[j][c] == -INFINITY;
+            alpha[j][c] = fresh ? 0.0f : ts_exp2(m_run[j][c] - m_new);
             m_run[j][c] = m_new;
-            l_run[j][c] *= alpha[c];
-          }
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            acc[j][i][0] *= alpha[0];
-            acc[j][i][1] *= alpha[1];
-            acc[j][i][2] *= alpha[0];
-            acc[j][i][3] *= alpha[1];
-          }
-        }
-      }
-      if constexpr (kQuant) {  // the largest finite row scale of V that each column has seen
-        bool up = false;
-#pragma unroll
-        for (int z = 0; z < SL; ++z)
-#pragma unroll
-          for (int j = 0; j < NG; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              up |= sees[z][j][i] && v_unit[z][i >> 1] > g_run[j][i & 1] && v_unit[z][i >> 1] < INFINITY;
-        if (__any_sync(kFull, up)) {
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            float f[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float mx = g_run[j][c];
-#pragma unroll
-              for (int z = 0; z < SL; ++z) {
-                if (sees[z][j][c] && v_unit[z][0] < INFINITY) mx = fmaxf(mx, v_unit[z][0]);
-                if (sees[z][j][c + 2] && v_unit[z][1] < INFINITY) mx = fmaxf(mx, v_unit[z][1]);
-              }
-              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-              f[c] = __fdiv_rn(g_run[j][c], mx);
-              g_run[j][c] = mx;
-              p_unit[j][c] = __fdiv_rn(kTsPScale, mx);
-            }
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              acc[j][i][0] *= f[0];
-              acc[j][i][1] *= f[1];
-              acc[j][i][2] *= f[0];
-              acc[j][i][3] *= f[1];
+            l_run[j][c] *= alpha[j][c];
+            if constexpr (kQuant) {  // G shrinks as what the accumulators stand for does, down to its least
+              const float g = fresh ? kTsMinUnit : g_run[j][c] * alpha[j][c];
+              alpha[j][c] = g < kTsMinUnit ? __fdiv_rn(g, kTsMinUnit) : 1.0f;
+              low |= g < kTsMinUnit;
+              g_run[j][c] = fmaxf(g, kTsMinUnit);
+              p_unit[j][c] = __fdiv_rn(kTsPScale, g_run[j][c]);
             }
           }
-        }
+        if (!kQuant || __any_sync(kFull, low)) rescale(alpha);
       }
-      // ---- P^T as B fragments
-      uint32_t ph[SL][NG][2];
-      [[maybe_unused]] uint32_t pl[SL][NG][2];  // second term, BF16 only
       float pr[SL][NG][4];
 #pragma unroll
       for (int z = 0; z < SL; ++z)
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          float wt[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            // -inf only stands for a key that is not seen, or one that weighs nothing
+          for (int i = 0; i < 4; ++i)  // -inf only stands for a key that is not seen, or one that weighs nothing
             pr[z][j][i] = sc[z][j][i] == -INFINITY ? 0.0f : ts_exp2(sc[z][j][i] - m_run[j][i & 1]);
-            wt[i] = pr[z][j][i];
-            if constexpr (kQuant) wt[i] *= v_unit[z][i >> 1] * p_unit[j][i & 1];
-            if constexpr (EDGE) wt[i] = sees[z][j][i] ? wt[i] : 0.0f;
-          }
           l_run[j][0] += pr[z][j][0] + pr[z][j][2];
           l_run[j][1] += pr[z][j][1] + pr[z][j][3];
-          if constexpr (kQuant) {
-            ph[z][j][0] = ts_transpose(ts_pack_f16(wt[0], wt[1]));
-            ph[z][j][1] = ts_transpose(ts_pack_f16(wt[2], wt[3]));
-          } else {
-            const uint32_t h0 = ts_pack_bf16(wt[0], wt[1]), h1 = ts_pack_bf16(wt[2], wt[3]);
-            ph[z][j][0] = ts_transpose(h0);
-            ph[z][j][1] = ts_transpose(h1);
-            pl[z][j][0] =
-                ts_transpose(ts_pack_bf16(wt[0] - __uint_as_float(h0 << 16), wt[1] - __uint_as_float(h0 & 0xffff0000u)));
-            pl[z][j][1] =
-                ts_transpose(ts_pack_bf16(wt[2] - __uint_as_float(h1 << 16), wt[3] - __uint_as_float(h1 & 0xffff0000u)));
-          }
         }
+      // ---- P^T as B fragments
+      uint32_t ph[SL][NG][2];
+      [[maybe_unused]] uint32_t pl[SL][NG][2];  // second term, BF16 only
+      if constexpr (kQuant) {
+        float con[SL][NG][4];  // contributions p_j gamma_j
+#pragma unroll
+        for (int z = 0; z < SL; ++z)
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              con[z][j][i] = pr[z][j][i] * v_unit[z][i >> 1];
+              if constexpr (EDGE)  // a row that is not seen may have any scale
+                if (!sees[z][j][i]) con[z][j][i] = 0.0f;
+            }
+        uint32_t top = 0u;
+        auto pack = [&] {
+#pragma unroll
+          for (int z = 0; z < SL; ++z)
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                ph[z][j][i] = ts_pack_f16(con[z][j][2 * i] * p_unit[j][0], con[z][j][2 * i + 1] * p_unit[j][1]);
+                top = ts_largest(top, ph[z][j][i]);
+              }
+        };
+        pack();
+        // G up to the largest finite contribution where one has passed it by the slack
+        if (__any_sync(kFull, max(top & 0x7fffu, top >> 16 & 0x7fffu) >= kTsPLimit)) {
+          float f[NG][2];
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = 0.0f;
+#pragma unroll
+              for (int z = 0; z < SL; ++z)
+#pragma unroll
+                for (int i = c; i < 4; i += 2) {
+                  const float size = fabsf(con[z][j][i]);
+                  if (size < INFINITY) mx = fmaxf(mx, size);
+                }
+              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
+              mx = fmaxf(mx, g_run[j][c]);
+              f[j][c] = __fdiv_rn(g_run[j][c], mx);
+              g_run[j][c] = mx;
+              p_unit[j][c] = __fdiv_rn(kTsPScale, mx);
+            }
+          rescale(f);
+          pack();
+        }
+#pragma unroll
+        for (int z = 0; z < SL; ++z)
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) ph[z][j][i] = ts_transpose(ph[z][j][i]);
+      } else {
+#pragma unroll
+        for (int z = 0; z < SL; ++z)
+#pragma unroll
+          for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float wt[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+                wt[c] = EDGE && !sees[z][j][2 * i + c] ? 0.0f : pr[z][j][2 * i + c];
+              const uint32_t h = ts_pack_bf16(wt[0], wt[1]);
+              ph[z][j][i] = ts_transpose(h);
+              pl[z][j][i] =
+                  ts_transpose(ts_pack_bf16(wt[0] - __uint_as_float(h << 16), wt[1] - __uint_as_float(h & 0xffff0000u)));
+            }
+      }
       // ---- O^T += V^T P^T of one slice
       auto output = [&](int r0, int pos0, const uint32_t (&ph)[NG][2], [[maybe_unused]] const uint32_t (&pl)[NG][2],
                         [[maybe_unused]] const float (&pr)[NG][4], [[maybe_unused]] const bool (&sees)[NG][4]) {

@@ -27,15 +27,17 @@
 //            V rows past the end and infinities or NaN in V become 0;
 //   S = Q K^T   M 128, N 64, into one of the stream's two score buffers;
 //   softmax  scores times the row scale of K (FP32), mask, P = 2^(s - m) times
-//            the row scale of V over G, to FP16 (BF16 caches: two BF16 terms),
-//            written over the scores in tensor memory; the reference m and the
-//            scale G move only when passed by a slack (2^10 and 2^3, for BF16
-//            2^20), and only then the accumulator is rescaled;
+//            the row scale of V, to FP16 (BF16 caches: two BF16 terms), written
+//            over the scores in tensor memory; the reference m moves only when
+//            P would pass 2^15 (BF16: when a score passes m by 2^20), and only
+//            then the accumulator is rescaled;
 //   O += P V  M 128, N = D, P read from tensor memory, accumulated there.
 // Shared memory feeds the MMAs, so P stays out of it: with P as a
 // shared-memory operand its reads and writes took a third of the bandwidth and
 // the kernel 1.6 times as long.
-// The numerics are those of tree_stream.cuh (P is 2^2 p_j gamma_j / G here).
+// The numerics are those of tree_stream.cuh, but that over codes m serves the
+// weights and the contributions 2^(s - m) gamma_j alike: it is set by the largest
+// contribution, which comes to 2^4 to 2^6.
 //
 // What bounds it, at 1.9 GHz.  Over codes with up to 128 rows: the roles' own
 // latency.  A tile's MMAs take 650 cycles (49 for a step of K Q^T, read from
@@ -72,8 +74,11 @@ constexpr int kTtThreads = (kTtSoftmaxWarps + kTtPrepWarps + 4) * 32;  // whole 
 // the others give: 256 * 144 + 384 * 64 = 640 * 96.
 constexpr int kTtSoftmaxRegs = 144, kTtOtherRegs = 64;
 constexpr int kTtUnitSlots = 8;  // tiles whose row scales are kept
-constexpr float kTtPScale = 4.0f;
-constexpr float kTtUnitSlack = 8.0f;
+// Over codes P = 2^(s - m) gamma_j, in FP16, has one reference m for both the softmax and the contributions: the
+// largest contribution that m is set by comes to 2^4 to 2^6, a later one may be up to 2^15.  A weight 2^(s - m)
+// itself is at most 2^kTtHead when m is set, so that rows of V that are all tiny leave l in range.
+constexpr float kTtTop = 5.0f, kTtHead = 100.0f;
+constexpr float kTtSumLimit = 1.32922800e+36f, kTtSumStep = 32.0f;  // 2^120: m moves up by 32 where l would pass it
 
 template <int D, int FMT, bool SPLIT>  // SPLIT: 129 to 256 rows, half of them per stream
 struct TtCfg {
@@ -89,8 +94,8 @@ struct TtCfg {
   static constexpr uint32_t kQPanel = kQRows * 128;
   static constexpr uint32_t kOffK = 0, kOffV = kOffK + kK * kOperand, kOffRing = kOffV + kV * kOperand,
                             kOffQ = kOffRing + kStages * Codes::kStage, kOffUnits = kOffQ + kPanels * kQPanel;
-  // Row scales of a tile's keys: K (times log2(e) / sqrt(D)), V, and V's largest finite one.
-  static constexpr uint32_t kUnitFloats = 2 * kTtKeys + 4;
+  // Row scales of a tile's keys: K (times log2(e) / sqrt(D)), V.
+  static constexpr uint32_t kUnitFloats = 2 * kTtKeys;
   static constexpr uint32_t kUnits = kQuant ? kTtUnitSlots * kUnitFloats * 4 : 0;
   static constexpr uint32_t kOffPrefix = kOffUnits + kUnits;
   // Stream 1's o of up to 64 rows overlays Q when the streams are joined.
@@ -242,10 +247,10 @@ __device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t parity, volatile
 // (row, 16-byte chunk) of a tile of 128-byte swizzled rows.
 __device__ __forceinline__ uint32_t tt_chunk(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-// The exponent of a normal x > 0, and a power of two in [2^-126, 2^127] (0 below).
-__device__ __forceinline__ int tt_log2(float x) { return static_cast<int>(__float_as_uint(x) >> 23) - 127; }
-__device__ __forceinline__ float tt_pow2(int e) {
-  return e < -126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+// The whole part of log2 |x| (-127 below 2^-126), -inf where x is not finite.
+__device__ __forceinline__ float tt_log2(float x) {
+  const uint32_t e = __float_as_uint(x) >> 23 & 0xffu;
+  return e == 255u ? -INFINITY : __uint_as_float(0x4b000000u | e) - 8388735.0f;  // 2^23 + e, less 2^23 + 127
 }
 
 // A counter modulo N with the phase of its mbarriers.
@@ -561,8 +566,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
               float* un = units_kv + slot * C::kUnitFloats;
               reinterpret_cast<float2*>(un)[lane] = make_float2(kr.x * p.scale_log2, kr.y * p.scale_log2);
               reinterpret_cast<float2*>(un + kTtKeys)[lane] = vr;
-              const float top = warp_max_f32(fmaxf(vr.x < INFINITY ? vr.x : 0.0f, vr.y < INFINITY ? vr.y : 0.0f));
-              if (lane == 0) un[2 * kTtKeys] = top;
             }
             slot = slot + 1 == kTtUnitSlots ? 0 : slot + 1;
             uint8_t* out = smem + (is_v ? C::kOffV + rv.i * C::kOperand : C::kOffK + rk.i * C::kOperand);
@@ -734,8 +737,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       __syncwarp();
       if (lane == 0) ts_arrive(&q_full);
 
-      // l and the weights are 2^shift of what they stand for, 2^shift = 2^2 / G (BF16: 1).
-      float m = -INFINITY, l = 0.0f, g_run = kTsMinUnit, shift = kQuant ? 102.0f : 0.0f;
+      float m = -INFINITY, l = 0.0f;  // the reference of the weights 2^(s - m), and their sum
       const uint8_t* mask_row = p.mask ? p.mask + b * p.mask_stride + static_cast<int64_t>(tok) * p.tokens : nullptr;
       int done = 0;  // jobs of this stream in the segment
       for (int i = SPLIT ? 0 : s; i < tiles && ok; i += SPLIT ? 1 : 2, ++done) {
@@ -798,8 +800,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                 if (!((bits >> e) & 1)) x[e] = -INFINITY;
             }
           };
-          // 32 keys' P against m_ref into out (BF16: second terms into out2), their sum into l_tile.
+          // 32 keys' P against m_ref into out (BF16: second terms into out2), the weights' sum into l_tile, over codes
+          // the largest P into p_top.
           float l_tile = 0.0f;
+          [[maybe_unused]] uint32_t p_top[2] = {0u, 0u};
           auto weights = [&](int h, const float (&x)[32], float m_ref, uint32_t (&out)[16],
                              [[maybe_unused]] uint32_t (&out2)[16]) {
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -822,6 +826,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                     if (!((seen >> (32 * h + e + 2 * i)) & 2)) y.y = 0.0f;
                   }
                   out[at] = ts_pack_f16(y.x, y.y);
+                  p_top[i] = ts_largest(p_top[i], out[at]);
                 } else {
                   out[at] = ts_pack_bf16(y.x, y.y);
                   out2[at] = ts_pack_bf16(y.x - __uint_as_float(out[at] << 16),
@@ -835,56 +840,62 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
           };
-          // The row scale of V that decides on G.
-          [[maybe_unused]] float vx = 0.0f;
-          if constexpr (kQuant) {
-            vx = unit[2 * kTtKeys];
-            if constexpr (EDGE) {
-              vx = 0.0f;
-#pragma unroll 4
-              for (int e = 0; e < kTtKeys; e += 4) {
-                const float4 u = *reinterpret_cast<const float4*>(unit + kTtKeys + e);
-                const float of[4] = {u.x, u.y, u.z, u.w};
-                const uint32_t bits = static_cast<uint32_t>(seen >> e);
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  if (((bits >> y) & 1) && of[y] < INFINITY) vx = fmaxf(vx, of[y]);
-              }
-            }
-          }
-          // First against the reference and G as they are; again, after both have moved, if that was too low.
+          // First against the reference as it is; again, after it has moved, if that was too low.  (Leaving the first
+          // pass out in a segment's first tile, where it is always too low, cost 160 to 270 bytes of spilled registers
+          // and 16 tokens over NVFP4 154 -> 160 us.)
           float f = 1.0f;  // what the accumulator is to be scaled by
-          bool again = false;
+          bool over = false, again = false;  // over: this row's reference has to move
           if (warp_has) {
             uint32_t out[2][16];
             [[maybe_unused]] uint32_t out2[2][16];
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            const float m_ref = m == -INFINITY ? -shift : m - shift;
+            const float m_ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float x[32];
               scores(h, x);
-              maxima(x, mx);
+              if constexpr (!kQuant) maxima(x, mx);
               weights(h, x, m_ref, out[h], out2[h]);
             }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * own;
-            again = has && (top > m + kTsSlack<FMT> || (kQuant && vx > g_run * kTtUnitSlack));
-            again = __any_sync(kFull, again);
+            if constexpr (kQuant) {
+              const uint32_t p_max = ts_largest(p_top[0], p_top[1]) & 0x7fff7fffu;
+              over = max(p_max & 0xffffu, p_max >> 16) >= kTsPLimit || l + l_tile > kTtSumLimit ||
+                     (m == -INFINITY && (!EDGE || seen != 0ull));
+            }
+            [[maybe_unused]] float top = 0.0f;
+            if constexpr (!kQuant) {
+              top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * own;
+              over = top > m + kTsSlack<FMT>;
+            }
+            over = over && has;
+            again = __any_sync(kFull, over);
             if (again) {
-              if (has && top > m + kTsSlack<FMT>) {
-                f = m == -INFINITY ? 0.0f : ts_exp2(m - top);
-                l *= f;
-                m = top;
-              }
-              if constexpr (kQuant) {
-                if (has && vx > g_run * kTtUnitSlack) {  // G up to the next power of two
-                  const int old = tt_log2(g_run), next = tt_log2(vx) + 1;
-                  const float down = tt_pow2(old - next);
-                  g_run = tt_pow2(next);
-                  f *= down;
-                  l *= down;  // l is in units of 2^shift, as the weights are
-                  shift -= static_cast<float>(next - old);
+              float next = top;
+              if constexpr (kQuant) {  // by the largest score and the largest contribution of the tile
+                float con = -INFINITY;
+                top = -INFINITY;
+#pragma unroll 1
+                for (int h = 0; h < 4; ++h) {
+                  float x[16];
+                  tt_ld16(s_at + 16 * h, x);
+                  const float* u = unit + 16 * h;
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) {
+                    x[e] *= u[e];
+                    if (EDGE && !((seen >> (16 * h + e)) & 1)) x[e] = -INFINITY;
+                    x[e] *= own;
+                    top = fmaxf(top, x[e]);
+                    con = fmaxf(con, x[e] + tt_log2(u[kTtKeys + e]));
+                  }
                 }
+                // whole numbers: what was summed is rescaled without a rounding
+                next = fmaxf(m, ceilf(fmaxf(con - kTtTop, top - kTtHead)));
+                if (l + l_tile > kTtSumLimit) next = fmaxf(next, m + kTtSumStep);
+              }
+              if ((kQuant ? has : over) && top > -INFINITY) {  // over codes all rows: their next moves come later then
+                f = m == -INFINITY ? 0.0f : ts_exp2(m - next);
+                l *= f;
+                m = next;
               }
             } else {
 #pragma unroll
@@ -911,7 +922,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
                 tt_st16(o_col(s) + lanes + c, y);
               }
             }
-            const float m_ref = m == -INFINITY ? -shift : m - shift;
+            const float m_ref = m == -INFINITY ? 0.0f : m;
             l_tile = 0.0f;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
@@ -941,8 +952,16 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       o_end_phase ^= 1u;
       tt_fence_after();
       // ---- the segment's (m, l, o)
-      const float unit_o = kQuant ? g_run * (1.0f / kTtPScale) : 1.0f;  // 2^-shift
-      l *= unit_o;
+      // Over codes, with l brought into [1, 2): the weights' own range may be far from 1.
+      float unit_o = 1.0f;
+      if constexpr (kQuant) {
+        const int e = static_cast<int>(__float_as_uint(l) >> 23);
+        if (e > 0 && e < 254) {
+          unit_o = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);  // 2^(127 - e)
+          l *= unit_o;
+          m += static_cast<float>(e - 127);
+        }
+      }
       float4* area = reinterpret_cast<float4*>(smem + C::kOffQ);  // [D / 4][64 rows]
       if (!SPLIT) {
         // Every MMA of the segment has read its Q.  Where the streams' rows lie in different lanes, stream 0

@@ -335,6 +335,9 @@ int nvfp4da_kv_quant_read(const nvfp4da_kv_cache* cache, int64_t start, const in
  * holds them in slots P_b .. P_b + T - 1: token t sees slots below P_b and
  * slot P_b + u where tree_mask[b * mask_batch_stride + t * T + u] is not 0
  * (NULL: u <= t).  A query that sees nothing gets zeros.  T = 1 is decode.
+ * Over quantised caches the weights p_j times V's row scales have 11 bits down
+ * to 2^-18 of the largest product that the query meets, and steps of 2^-28 of
+ * that product below (head_dim 64, 128, 256; FP32 for the others).
  * max_past_length >= every P_b (== past_length without past_lengths). */
 size_t nvfp4da_tree_attention_workspace_size(const nvfp4da_kv_cache* cache, int64_t tokens, int64_t q_heads,
                                              int64_t max_past_length);
