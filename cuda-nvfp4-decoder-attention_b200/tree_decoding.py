@@ -71,10 +71,12 @@ def accept_drafted_(cache, new_k: torch.Tensor, new_v: torch.Tensor, path: torch
     """Commit the drafted tokens ``path`` (int64 ``[B, n]``, node indices from the root on) in slots ``P_b ..``.
 
     ``counts`` (CUDA int64 ``[B]``): only the first ``counts[b]`` nodes of a
-    sequence's path.  The rows are quantised again from BF16, so they get the
-    same bytes as before, now in consecutive slots.
+    sequence's path; what stands after them may be any number (-1, say).  The
+    rows are quantised again from BF16, so they get the same bytes as before,
+    now in consecutive slots.
     """
-    index = path[:, :, None, None].expand(-1, -1, *new_k.shape[2:])
+    # A gather outside would stop the device: a number that is no node is taken as the nearest one.
+    index = path.clamp(0, new_k.shape[1] - 1)[:, :, None, None].expand(-1, -1, *new_k.shape[2:])
     cuda_quantized_kv_append_(cache, torch.gather(new_k, 1, index), torch.gather(new_v, 1, index), past_length,
                               past_lengths=past_lengths, counts=counts)
 

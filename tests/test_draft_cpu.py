@@ -202,3 +202,19 @@ def test_tree_status_needs_a_place_for_the_flags():
     import nvfp4da_capi as capi
 
     assert capi.load().nvfp4da_tree_attention_sync_status(None, None, 1) == capi.ERR_INVALID_ARGUMENT
+
+
+def test_accepted_paths_may_be_padded_with_any_number(monkeypatch):
+    """Numbers past a sequence's count are no nodes: they are not looked up (on a device that lookup would stop it)."""
+    import tree_decoding
+
+    got = {}
+    monkeypatch.setattr(tree_decoding, "cuda_quantized_kv_append_",
+                        lambda cache, k, v, past, **kw: got.update(k=k, v=v, past=past, **kw))
+    new_k = torch.arange(2 * 3 * 1 * 4, dtype=torch.float32).view(2, 3, 1, 4)
+    path = torch.tensor([[0, 2, -1, -1], [1, 7, 1 << 40, -(1 << 62)]])
+    counts = torch.tensor([2, 1])
+    tree_decoding.accept_drafted_(object(), new_k, -new_k, path, 5, counts=counts)
+    assert got["past"] == 5 and got["counts"] is counts and got["k"].shape == (2, 4, 1, 4)
+    assert torch.equal(got["k"][0, :2], new_k[0, [0, 2]]) and torch.equal(got["k"][1, :1], new_k[1, [1]])
+    assert torch.equal(got["v"], -got["k"])
