@@ -217,6 +217,19 @@ def test_kv_append_per_sequence_slots(capi):
         assert int(torch.count_nonzero(host[i].float())) == int(torch.count_nonzero(nk[i].float()))
 
 
+def test_kv_append_writes_no_slot_outside_the_cache(capi):
+    """Lengths on the device that no host check sees: before the cache, past it, and where the sum with t wraps."""
+    b, t, hkv, c, d = 6, 3, 2, 16, 8
+    nk = torch.randn((b, t, hkv, d), generator=torch.Generator().manual_seed(5)).to(torch.bfloat16)
+    pl = torch.tensor([-1, 15, 16, 2 ** 63 - 1, 2 ** 63 - 2, -2 ** 63], dtype=torch.int64)
+    kc = torch.zeros((b, hkv, c, d), dtype=torch.bfloat16).cuda()
+    vc = torch.zeros_like(kc)
+    capi.kv_cache_append(kc, vc, nk.cuda(), nk.cuda(), 0, past_lengths=pl.cuda())
+    want = torch.zeros((b, hkv, c, d), dtype=torch.bfloat16)
+    want[1, :, 15] = nk[1, 0]
+    assert torch.equal(kc.cpu(), want) and torch.equal(vc.cpu(), want)
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("i", range(5))
 def test_attention_matches_reference_golden(capi, golden_stages, i):
