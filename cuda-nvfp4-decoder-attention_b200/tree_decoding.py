@@ -70,15 +70,26 @@ def accept_drafted_(cache, new_k: torch.Tensor, new_v: torch.Tensor, path: torch
                     past_lengths: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
     """Commit the drafted tokens ``path`` (int64 ``[B, n]``, node indices from the root on) in slots ``P_b ..``.
 
-    ``counts`` (CUDA int64 ``[B]``): only the first ``counts[b]`` nodes of a
-    sequence's path; what stands after them may be any number (-1, say).  The
-    rows are quantised again from BF16, so they get the same bytes as before,
-    now in consecutive slots.
+    ``cache`` as in ``cuda_decoder_attention_tree_forward_``.  ``counts`` (CUDA
+    int64 ``[B]``): only the first ``counts[b]`` nodes of a sequence's path; what
+    stands after them may be any number (-1, say).  Rows go in as they did
+    before, from BF16: a quantised cache gets the same bytes, now in consecutive
+    slots.
     """
     # A gather outside would stop the device: a number that is no node is taken as the nearest one.
     index = path.clamp(0, new_k.shape[1] - 1)[:, :, None, None].expand(-1, -1, *new_k.shape[2:])
-    cuda_quantized_kv_append_(cache, torch.gather(new_k, 1, index), torch.gather(new_v, 1, index), past_length,
-                              past_lengths=past_lengths, counts=counts)
+    rows = [torch.gather(x, 1, index) for x in (new_k, new_v)]
+    if not isinstance(cache, (tuple, list)):
+        cuda_quantized_kv_append_(cache, *rows, past_length, past_lengths=past_lengths, counts=counts)
+        return
+    if past_lengths is not None:
+        raise ValueError("BF16 caches take a common past_length; per-sequence past_lengths need a QuantizedKVCache")
+    n = path.shape[1]
+    if counts is not None and past_length + n <= cache[0].shape[2]:  # past a count the slots keep what they hold
+        kept = torch.arange(n, device=path.device) < counts[:, None]
+        rows = [torch.where(kept[:, :, None, None], x, c[:, :, past_length:past_length + n].transpose(1, 2))
+                for x, c in zip(rows, cache)]
+    cuda_kv_cache_append_(cache[0], cache[1], *(x.contiguous() for x in rows), past_length)
 
 
 def check_tree_wait_status(stream: torch.cuda.Stream | None = None) -> None:
