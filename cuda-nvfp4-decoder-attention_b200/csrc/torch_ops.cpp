@@ -245,7 +245,9 @@ Tensor gqa_attention_cached(const Tensor& q, const Tensor& k, const Tensor& v, i
   return gqa_common(q, k, v, past_length, false, "k_cache", "v_cache");
 }
 
-void kv_cache_append_(Tensor& kc, Tensor& vc, const Tensor& nk, const Tensor& nv, int64_t past_length) {
+// The shapes of an append, and the call: at a common past_length, or at past_lengths[b] (device int64 [B]).
+void kv_append_common(Tensor& kc, Tensor& vc, const Tensor& nk, const Tensor& nv, int64_t past_length,
+                      const int64_t* past_lengths, const char* what) {
   expect_rank4(kc, "k_cache");
   expect_rank4(vc, "v_cache");
   expect_rank4(nk, "new_k");
@@ -269,8 +271,12 @@ void kv_cache_append_(Tensor& kc, Tensor& vc, const Tensor& nk, const Tensor& nv
               " > ", c, ")");
   const c10::cuda::CUDAGuard g(kc.device());
   check_status(nvfp4da_kv_cache_append(mbits(kc), mbits(vc), bits(nk), bits(nv), b, hkv, c, d, t, past_length,
-                                       nullptr, cur_stream(kc)),
-               "cuda_kv_cache_append_");
+                                       past_lengths, cur_stream(kc)),
+               what);
+}
+
+void kv_cache_append_(Tensor& kc, Tensor& vc, const Tensor& nk, const Tensor& nv, int64_t past_length) {
+  kv_append_common(kc, vc, nk, nv, past_length, nullptr, "cuda_kv_cache_append_");
 }
 
 // ---------------------------------------------------------------- fused forward
@@ -516,6 +522,12 @@ void quantized_kv_append_(Tensor& kc, Tensor& vc, Tensor& kr, Tensor& vr, const 
                "cuda_quantized_kv_append_");
 }
 
+void kv_cache_append_varlen_(Tensor& kc, Tensor& vc, const Tensor& nk, const Tensor& nv, const Tensor& past_lengths) {
+  expect_rank4(kc, "k_cache");
+  kv_append_common(kc, vc, nk, nv, 0, lengths(past_lengths, "past_lengths", kc.size(0), kc, "k_cache"),
+                   "cuda_kv_cache_append_varlen_");
+}
+
 std::tuple<Tensor, Tensor> quantized_kv_read(const Tensor& kc, const Tensor& vc, const Tensor& kr, const Tensor& vr,
                                              const OptTensor& kb, const OptTensor& vb, int64_t start, int64_t length,
                                              const OptTensor& starts) {
@@ -625,6 +637,10 @@ TORCH_LIBRARY(cuda_nvfp4_decoder_attention, m) {
       "v_row_scales, Tensor(e!)? k_block_scales, Tensor(f!)? v_block_scales, Tensor new_k, Tensor new_v, int "
       "past_length=0, Tensor? past_lengths=None, Tensor? counts=None) -> ()",
       TORCH_FN(quantized_kv_append_));
+  m.def(
+      "cuda_kv_cache_append_varlen_(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor new_k, Tensor new_v, Tensor "
+      "past_lengths) -> ()",
+      TORCH_FN(kv_cache_append_varlen_));
   m.def(
       "cuda_quantized_kv_read(Tensor k_codes, Tensor v_codes, Tensor k_row_scales, Tensor v_row_scales, Tensor? "
       "k_block_scales, Tensor? v_block_scales, int start, int length, Tensor? starts=None) -> (Tensor, Tensor)",

@@ -96,10 +96,18 @@ def cuda_gqa_attention_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
 
 
 def cuda_kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, new_k: torch.Tensor,
-                          new_v: torch.Tensor, past_length: int) -> None:
-    """Write token-major K/V into slots ``past_length ..`` in place (reference cuda_primitives.py:186-207)."""
+                          new_v: torch.Tensor, past_length: int = 0, *,
+                          past_lengths: torch.Tensor | None = None) -> None:
+    """Write token-major K/V into slots ``past_length ..`` in place (reference cuda_primitives.py:186-207).
+
+    ``past_lengths`` (CUDA int64 ``[B]``; no reference counterpart) replaces the
+    common past length; a slot outside the cache is not written.
+    """
     _require_int("past_length", past_length)
-    _ops.cuda_kv_cache_append_(k_cache, v_cache, new_k, new_v, past_length)
+    if past_lengths is None:
+        _ops.cuda_kv_cache_append_(k_cache, v_cache, new_k, new_v, past_length)
+    else:
+        _ops.cuda_kv_cache_append_varlen_(k_cache, v_cache, new_k, new_v, past_lengths)
 
 
 # ------------------------------------------------------------------ drafted-token verification

@@ -36,16 +36,13 @@ def cuda_decoder_attention_tree_forward_(x, input_norm_weight, q_weight, k_weigh
     Token t of sequence b sits at position ``P_b + depths[.., t]`` (int64 ``[T]``
     or ``[B, T]``) and sees the committed positions and the drafted tokens its
     row of ``tree_mask`` names (ancestors and itself; without a mask the causal
-    chain).  ``cache`` is a ``QuantizedKVCache`` or, with a common
-    ``past_length``, a pair of BF16 caches; slots ``P_b .. P_b + T - 1`` are
-    written.  ``new_k`` and ``new_v`` ``[B, T, Hkv, D]`` are the rows as they
+    chain).  ``cache`` is a ``QuantizedKVCache`` or a pair of BF16 caches; slots
+    ``P_b .. P_b + T - 1`` are written.  ``new_k`` and ``new_v`` ``[B, T, Hkv, D]`` are the rows as they
     went in, for ``accept_drafted_``.
     """
     if not isinstance(x, torch.Tensor) or x.ndim != 3:
         raise TypeError("x must be a rank-3 torch.Tensor")
     bf16 = isinstance(cache, (tuple, list))
-    if bf16 and past_lengths is not None:
-        raise ValueError("BF16 caches take a common past_length; per-sequence past_lengths need a QuantizedKVCache")
     b, t, hidden = x.shape
     hkv = cache[0].shape[1] if bf16 else cache.k_codes.shape[1]
     d = cache[0].shape[3] if bf16 else cache.head_dim
@@ -58,7 +55,7 @@ def cuda_decoder_attention_tree_forward_(x, input_norm_weight, q_weight, k_weigh
     positions = depths + past_length if past_lengths is None else depths + past_lengths[:, None]
     q, k = cuda_apply_rope_qk(q, k, positions, inv_freq, interleaved=interleaved, attention_factor=attention_factor)
     if bf16:
-        cuda_kv_cache_append_(cache[0], cache[1], k, v, past_length)
+        cuda_kv_cache_append_(cache[0], cache[1], k, v, past_length, past_lengths=past_lengths)
     else:
         cuda_quantized_kv_append_(cache, k, v, past_length, past_lengths=past_lengths)
     ctx = cuda_tree_attention_cached(q, cache, past_length, tree_mask=tree_mask, past_lengths=past_lengths,
@@ -82,14 +79,13 @@ def accept_drafted_(cache, new_k: torch.Tensor, new_v: torch.Tensor, path: torch
     if not isinstance(cache, (tuple, list)):
         cuda_quantized_kv_append_(cache, *rows, past_length, past_lengths=past_lengths, counts=counts)
         return
-    if past_lengths is not None:
-        raise ValueError("BF16 caches take a common past_length; per-sequence past_lengths need a QuantizedKVCache")
-    n = path.shape[1]
-    if counts is not None and past_length + n <= cache[0].shape[2]:  # past a count the slots keep what they hold
-        kept = torch.arange(n, device=path.device) < counts[:, None]
-        rows = [torch.where(kept[:, :, None, None], x, c[:, :, past_length:past_length + n].transpose(1, 2))
-                for x, c in zip(rows, cache)]
-    cuda_kv_cache_append_(cache[0], cache[1], *(x.contiguous() for x in rows), past_length)
+    if counts is not None:  # past a sequence's count the slots keep what they hold
+        t = torch.arange(path.shape[1], device=path.device)
+        slot = (t + (past_length if past_lengths is None else past_lengths[:, None])).clamp(0, cache[0].shape[2] - 1)
+        slot = slot.expand(path.shape)[:, None, :, None].expand(-1, new_k.shape[2], -1, new_k.shape[3])
+        kept = (t < counts[:, None])[:, :, None, None]
+        rows = [torch.where(kept, x, torch.gather(c, 2, slot).transpose(1, 2)) for x, c in zip(rows, cache)]
+    cuda_kv_cache_append_(cache[0], cache[1], *(x.contiguous() for x in rows), past_length, past_lengths=past_lengths)
 
 
 def check_tree_wait_status(stream: torch.cuda.Stream | None = None) -> None:
