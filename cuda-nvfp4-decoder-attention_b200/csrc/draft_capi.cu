@@ -196,6 +196,10 @@ bool tree_map(CUtensorMap* map, const nvfp4da_kv_cache& c, const void* base, int
                      static_cast<uint32_t>(tile * bytes / 128), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+__global__ void tree_status_kernel(unsigned* flags, int clear) {
+  *flags = clear ? atomicExch(&g_tree_errors, 0u) : atomicOr(&g_tree_errors, 0u);
+}
+
 int plan_tree(const nvfp4da_kv_cache* c, int64_t tokens, int64_t q_heads, int64_t max_past, TreePlan& pl) {
   int r = check_cache(c);
   if (r) return r;
@@ -498,10 +502,15 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const u
 int nvfp4da_tree_attention_sync_status(void* stream, unsigned* flags, int clear) {
   if (!flags) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "flags is NULL");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  void* word = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&word, g_tree_errors);
+  // Read and cleared in one operation: a flag that a kernel on another stream sets meanwhile is kept for the next call.
+  unsigned* word = nullptr;
+  cudaError_t e = cudaMallocAsync(reinterpret_cast<void**>(&word), sizeof(unsigned), s);
+  if (e != cudaSuccess) return cuda_fail(e, "tree attention status read");
+  tree_status_kernel<<<1, 1, 0, s>>>(word, clear);
+  e = cudaGetLastError();
   if (e == cudaSuccess) e = cudaMemcpyAsync(flags, word, sizeof(unsigned), cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess && clear) e = cudaMemsetAsync(word, 0, sizeof(unsigned), s);
+  const cudaError_t freed = cudaFreeAsync(word, s);
+  if (e == cudaSuccess) e = freed;
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "tree attention status read");
 }

@@ -89,17 +89,20 @@ def accept_drafted_(cache, new_k: torch.Tensor, new_v: torch.Tensor, path: torch
 
 
 def check_tree_wait_status(stream: torch.cuda.Stream | None = None) -> None:
-    """Raise ``RuntimeError`` if a wait inside tree attention gave up on the current device since the last check.
+    """Raise ``RuntimeError`` if a wait inside tree attention gave up on the stream's device since the last check.
 
     The kernels' warps hand tiles to one another over barriers in shared memory;
     every such wait is bounded, and one that runs out records a flag and lets the
     kernel end with garbage instead of hanging.  The call itself does not read
     the flag back; this function does, synchronises ``stream`` (default: the
-    current one) and clears it.
+    current one) and clears it.  The flag is the device's: calls on other streams
+    are covered as far as they come before ``stream``'s work or have ended.
     """
     import nvfp4da_capi
 
-    flags = nvfp4da_capi.tree_sync_status(stream if stream is not None else torch.cuda.current_stream())
+    stream = stream if stream is not None else torch.cuda.current_stream()
+    with torch.cuda.device(stream.device):
+        flags = nvfp4da_capi.tree_sync_status(stream)
     if flags:
         raise RuntimeError(f"a bounded wait of tree attention timed out (flags 0x{flags:x}); the contexts since the "
                            "last check are not valid")

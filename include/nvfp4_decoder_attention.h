@@ -345,9 +345,12 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* cache, con
                            int64_t mask_batch_stride, uint16_t* context, int64_t tokens, int64_t q_heads,
                            int64_t past_length, const int64_t* past_lengths, int64_t max_past_length,
                            void* workspace, size_t workspace_bytes, void* stream);
-/* Error flags recorded by nvfp4da_tree_attention on the current device, on any
- * stream (bit 0: a bounded wait timed out and the contexts since are not
- * valid); synchronises `stream`; clears them if `clear`. */
+/* Error flags recorded by nvfp4da_tree_attention on the current device, which
+ * `stream` belongs to (bit 0: a bounded wait timed out and the contexts since
+ * are not valid); synchronises `stream`; clears them if `clear`, in the same
+ * operation that reads them.  The flags are the device's: calls ordered before
+ * `stream`'s work are covered whatever stream they ran on; of others, only
+ * those that have ended. */
 int nvfp4da_tree_attention_sync_status(void* stream, unsigned* flags, int clear);
 
 #ifdef __cplusplus

@@ -218,3 +218,32 @@ def test_accepted_paths_may_be_padded_with_any_number(monkeypatch):
     assert got["past"] == 5 and got["counts"] is counts and got["k"].shape == (2, 4, 1, 4)
     assert torch.equal(got["k"][0, :2], new_k[0, [0, 2]]) and torch.equal(got["k"][1, :1], new_k[1, [1]])
     assert torch.equal(got["v"], -got["k"])
+
+
+@pytest.mark.parametrize("flags", [0, 1])
+def test_wait_status_is_read_on_the_device_of_the_stream(monkeypatch, flags):
+    """The flag is one word per device: the current device's says nothing about another's stream."""
+    import contextlib
+    import types
+
+    import nvfp4da_capi
+    import tree_decoding
+
+    at = []
+
+    @contextlib.contextmanager
+    def device(d):
+        at.append(d)
+        yield
+        at.pop()
+
+    def status(stream):
+        assert at == [stream.device]
+        return flags
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(nvfp4da_capi, "tree_sync_status", status)
+    stream = types.SimpleNamespace(device=torch.device("cuda", 3))
+    with pytest.raises(RuntimeError, match="timed out") if flags else contextlib.nullcontext():
+        tree_decoding.check_tree_wait_status(stream)
+    assert at == []
