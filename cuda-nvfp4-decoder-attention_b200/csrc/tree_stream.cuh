@@ -55,9 +55,10 @@
 // 12 or 16 consumer warps, for which registers suffice with one slice at a time,
 // were no faster.
 //
-// Waits are bounded: a barrier that does not complete within 2^22 tries records
-// kErrBarrierTimeout in g_tree_errors and the CTA stops waiting (its results
-// are then garbage; the GPU stays usable).
+// Waits are bounded: one that lasts a second records kErrBarrierTimeout in
+// g_tree_errors, and every role of the CTA leaves (its results are then garbage;
+// the GPU stays usable).  The loading warps leave only when what they copy into
+// shared memory has landed, or after a further limit.
 #pragma once
 
 #include <cuda.h>
@@ -217,6 +218,50 @@ __device__ __forceinline__ void ts_e4m3x4(uint32_t w, uint32_t& lo, uint32_t& hi
   asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
       : "=r"(lo), "=r"(hi) : "r"(w));
 }
+
+// ---------------------------------------------------------------- bounded waits
+// Nanoseconds, modulo 2^32: for differences of a few seconds at most.
+__device__ __forceinline__ uint32_t ts_now() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+  return t;
+}
+// Gives up when another role has (`bad`) or after one second.
+__device__ __forceinline__ bool ts_wait(uint64_t* bar, uint32_t parity, volatile unsigned* bad) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t t0 = ts_now();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0) {
+      if (*bad) return false;
+      if (ts_now() - t0 > 1000000000u) {
+        atomicOr(&g_tree_errors, static_cast<unsigned>(kErrBarrierTimeout));
+        *bad = 1u;
+        return false;
+      }
+    }
+  }
+}
+// The last of n fills, in turn, of N buffers that went to buffer i, and the parity of its phase.
+__host__ __device__ constexpr int ts_last_fill(int n, int N, int i) { return n - 1 - (n - 1 - i) % N; }
+__host__ __device__ constexpr uint32_t ts_fill_parity(int fill, int N) { return static_cast<uint32_t>(fill / N) & 1u; }
+static_assert(ts_last_fill(3, 4, 0) == 0 && ts_last_fill(3, 4, 2) == 2 && ts_last_fill(4, 4, 3) == 3 &&
+                  ts_last_fill(6, 4, 1) == 5 && ts_last_fill(6, 4, 2) == 2 && ts_last_fill(9, 4, 0) == 8 &&
+                  ts_fill_parity(3, 4) == 0 && ts_fill_parity(4, 4) == 1 && ts_fill_parity(8, 4) == 0,
+              "fills of a ring");
+// Waits for the phase, whoever has given up, but 20 ms at most.
+__device__ __forceinline__ void ts_landed(uint64_t* bar, uint32_t parity) {
+  const uint32_t t0 = ts_now();
+  while (!mbar_try_wait(bar, parity) && ts_now() - t0 < 20000000u) {
+  }
+}
+// Of n fills of a ring of N buffers, the last of each.
+template <int N>
+__device__ __forceinline__ void ts_all_landed(uint64_t* bars, int n) {
+  for (int i = 0; i < N && i < n; ++i) ts_landed(&bars[i], ts_fill_parity(ts_last_fill(n, N, i), N));
+}
+// This thread's copies by ts_copy16.
+__device__ __forceinline__ void ts_copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Byte offset o of a tile of 128-byte lines, 16-byte chunks swizzled by line.
 __device__ __forceinline__ uint32_t ts_swz(uint32_t o) { return o ^ ((o >> 3) & 0x70u); }
@@ -400,6 +445,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   uint64_t* join_full = empty + Cfg::kStages;
   uint64_t* join_free = join_full + Cfg::kJoins;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::kOffPrefix);
+  __shared__ volatile unsigned s_bad;  // a wait gave up
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
@@ -420,6 +466,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       mbar_init(&join_free[i], 2);
     }
     fence_mbar_init();
+    s_bad = 0u;
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
   }
@@ -447,7 +494,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
       if (!whole && warp == NW + 2 && lane == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
-      if (!mbar_wait_bounded(&join_full[buf], phase, &g_tree_errors)) return;
+      if (!__all_sync(kFull, ts_wait(&join_full[buf], phase, &s_bad))) return;
       const float *so = join_o(buf), *sm_m = join_m(buf), *sm_l = sm_m + NW * Cfg::kRows;
       for (int r = warp - NW - 2; r < rows; r += 2) {
         // Position warp `lane` of the row's chunk: its factor.
@@ -496,11 +543,13 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     int stage = 0;
     uint32_t phase = 0;
     [[maybe_unused]] const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
-    bool lapped = false;  // every stage has been filled once
-    while (more) {
+    int filled = 0;  // stages, from the first tile on
+    bool ok = true;
+    while (more && ok) {
       const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
       for (int t = w.t0; t < w.t1; ++t) {
-        if (lapped && !mbar_wait_bounded(&empty[stage], phase ^ 1u, &g_tree_errors)) return;
+        ok = filled < Cfg::kStages || ts_wait(&empty[stage], phase ^ 1u, &s_bad);
+        if (!ok) break;
         uint8_t* st = smem + stage * Cfg::kStage;
         const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile<FMT>;
         if (lane == 0) {
@@ -521,14 +570,16 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             ts_copy_arrive(&full[stage]);
           }
         }
+        ++filled;
         if (++stage == Cfg::kStages) {
           stage = 0;
           phase ^= 1u;
-          lapped = true;
         }
       }
       more = w.next();
     }
+    if constexpr (kQuant) ts_copies_landed();
+    if (lane == 0) ts_all_landed<Cfg::kStages>(full, filled);
     return;
   }
 
@@ -539,7 +590,6 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   const int turn0 = pw_n >= kTurns ? pw % kTurns : pw * turns;
   TsWalk w;
   bool more = w.begin(prefix, p.batch, units, x0, x1);
-  bool dead = false;
   const int warp_slot = pw * rc_n + rc;
   int join = 0;
   uint32_t join_phase = 0;
@@ -1009,12 +1059,12 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     for (int t = w.t0; t < w.t1; ++t) {
       const bool mine = pw_n < kTurns || turn == pw / kTurns;
       if (mine) {
-        if (!dead && !mbar_wait_bounded(&full[stage], phase, &g_tree_errors)) dead = true;
+        if (!__all_sync(kFull, ts_wait(&full[stage], phase, &s_bad))) return;
         const uint8_t* st = smem + stage * Cfg::kStage;
         for (int i = 0; i < turns; ++i) {
           const int r0 = (turn0 + i) * 16 * SL;
           const int pos0 = t * kTsTile<FMT> + r0;
-          if (dead || pos0 >= vis) break;
+          if (pos0 >= vis) break;
           if (pos0 + 16 * SL <= past) slice(std::false_type{}, st, r0, pos0);
           else slice(std::true_type{}, st, r0, pos0);
         }
@@ -1029,7 +1079,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     }
 
     // ---- this segment's (m, l, o) to the joining warps
-    if (!dead && !mbar_wait_bounded(&join_free[join], join_phase ^ 1u, &g_tree_errors)) dead = true;
+    if (!__all_sync(kFull, ts_wait(&join_free[join], join_phase ^ 1u, &s_bad))) return;
     float *so = join_o(join), *sm_m = join_m(join), *sm_l = sm_m + NW * Cfg::kRows;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {

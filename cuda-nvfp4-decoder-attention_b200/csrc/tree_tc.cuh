@@ -56,8 +56,8 @@
 // P V issued in whatever order they are ready (-> 176 us), more buffers for K
 // and V, three shares of registers.
 //
-// Waits are bounded (one second, shared give-up flag, recorded in
-// g_tree_errors); tensor memory is freed on every path.
+// Waits are bounded as in tree_stream.cuh; a CTA that gives up lets its copies
+// and MMAs in flight end (or a further limit pass), and frees its tensor memory.
 #pragma once
 
 #include "tree_stream.cuh"
@@ -224,26 +224,6 @@ __device__ __forceinline__ float2 tt_fma2(float2 a, float2 b, float2 d) {
   return c;
 }
 
-// Bounded wait; gives up when another role has (`bad`) or after one second.
-__device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t parity, volatile unsigned* bad) {
-  if (mbar_try_wait(bar, parity)) return true;
-  uint64_t t0;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 0) {
-      if (*bad) return false;
-      uint64_t t;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t - t0 > 1000000000ull) {
-        atomicOr(&g_tree_errors, static_cast<unsigned>(kErrBarrierTimeout));
-        *bad = 1u;
-        return false;
-      }
-    }
-  }
-}
-
 // (row, 16-byte chunk) of a tile of 128-byte swizzled rows.
 __device__ __forceinline__ uint32_t tt_chunk(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -287,7 +267,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   // what it points to is shared memory.
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ uint64_t ring_full[4], ring_free[4], k_full[4], k_free[4], v_raw[4], v_full[4], v_free[4], q_full,
-      s_full[2][2], p_full[2][2], o_done[2], o_end[2], seg_done, join_ready, join_read;
+      s_full[2][2], p_full[2][2], o_done[2], o_end[2], seg_done, join_ready, join_read, drained[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile unsigned s_bad;    // a wait gave up
   __shared__ volatile unsigned s_wild;   // an infinity or NaN was taken out of V
@@ -326,6 +306,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
       mbar_init(&o_done[s], 1);
       mbar_init(&o_end[s], 1);
+      mbar_init(&drained[s], 1);
     }
     mbar_init(&seg_done, 2 * active);
     mbar_init(&join_ready, 2 * active);
@@ -376,7 +357,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       for (; more && ok; more = w.next()) {
         const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
         for (int t = w.t0; t < w.t1; ++t) {
-          ok = __all_sync(kFull, tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad));
+          ok = __all_sync(kFull, ts_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad));
           if (!ok) break;
           uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
           ts_load_scales<D, FMT, Codes, kTtKeys>(st, p, row0 + t * kTtKeys, all_rows, lane);
@@ -384,18 +365,20 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           rk.next();
         }
       }
+      ts_copies_landed();
     } else if (warp == kTtLoadWarp) {
       // ---------------------------------------------------------------- loads
       if (lane == 0) {
         TtRing<kQuant ? (C::kStages ? C::kStages : 1) : C::kK> rk;
         TtRing<C::kV> rv;
+        int filled = 0, filled_v = 0;  // codes or K, V
         bool ok = true;
         for (; more && ok; more = w.next()) {
           const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
           for (int t = w.t0; t < w.t1 && ok; ++t) {
             const int64_t row = row0 + t * kTtKeys;
             if constexpr (kQuant) {
-              ok = tt_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad);
+              ok = ts_wait(&ring_free[rk.i], rk.phase ^ 1u, &s_bad);
               if (!ok) break;
               uint8_t* st = smem + C::kOffRing + rk.i * Codes::kStage;
               uint64_t* bar = &ring_full[rk.i];
@@ -403,24 +386,33 @@ __global__ void __launch_bounds__(kTtThreads, 1)
               const int line = static_cast<int>(row * Codes::kRowBytes / 128);
               ts_tma_2d(st, &tm_k, 0, line, bar);
               ts_tma_2d(st + Codes::kOffV, &tm_v, 0, line, bar);
+              ++filled;
               rk.next();
             } else {
-              ok = tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+              ok = ts_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
               if (!ok) break;
               mbar_arrive_expect_tx(&k_full[rk.i], C::kOperand);
               for (int pn = 0; pn < C::kPanels; ++pn)
                 ts_tma_2d(smem + C::kOffK + rk.i * C::kOperand + pn * (kTtKeys * 128), &tm_k, pn * 64,
                           static_cast<int>(row), &k_full[rk.i]);
+              ++filled;
               rk.next();
-              ok = tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad);
+              ok = ts_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad);
               if (!ok) break;
               mbar_arrive_expect_tx(&v_raw[rv.i], C::kOperand);
               for (int pn = 0; pn < C::kPanels; ++pn)
                 ts_tma_2d(smem + C::kOffV + rv.i * C::kOperand + pn * (kTtKeys * 128), &tm_v, pn * 64,
                           static_cast<int>(row), &v_raw[rv.i]);
+              ++filled_v;
               rv.next();
             }
           }
+        }
+        if constexpr (kQuant) {
+          ts_all_landed<C::kStages ? C::kStages : 1>(ring_full, filled);
+        } else {
+          ts_all_landed<C::kK>(k_full, filled);
+          ts_all_landed<C::kV>(v_raw, filled_v);
         }
       }
       __syncwarp();
@@ -444,10 +436,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         // query rows of this stream in the Q tile
         const uint32_t q0 = SPLIT ? s * kTtRows : (shifted && s == 0 ? 64 : 0);
         const uint32_t qa = tt_desc_low(base + C::kOffQ + q0 * 128, 16);
-        ok = __all_sync(kFull, tt_wait(&q_full, q_phase, &s_bad));
+        ok = __all_sync(kFull, ts_wait(&q_full, q_phase, &s_bad));
         q_phase ^= 1u;
         auto scores = [&] {
-          ok = __all_sync(kFull, tt_wait(&k_full[rk.i], rk.phase, &s_bad));
+          ok = __all_sync(kFull, ts_wait(&k_full[rk.i], rk.phase, &s_bad));
           if (!ok) return;
           tt_fence_after();
           const uint32_t ka = tt_desc_low(base + C::kOffK + rk.i * C::kOperand, 16);
@@ -478,7 +470,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         if (ok) advance_scores();
         for (int t = 0; t < tiles && ok; ++t) {
           if (SPLIT || (t & 1) == s) {
-            ok = tt_wait(&p_full[s][nth & 1], (nth >> 1) & 1, &s_bad) && tt_wait(&v_full[rv.i], rv.phase, &s_bad);
+            ok = ts_wait(&p_full[s][nth & 1], (nth >> 1) & 1, &s_bad) && ts_wait(&v_full[rv.i], rv.phase, &s_bad);
             if (!(ok = __all_sync(kFull, ok))) break;
             tt_fence_after();
             const uint32_t va = tt_desc_low(base + C::kOffV + rv.i * C::kOperand, kTtKeys * 128);
@@ -539,7 +531,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           const bool edge = key0 + kTtKeys > past;
           const int live = min(kTtKeys, vis - key0);  // keys before the end
           if constexpr (kQuant) {
-            ok = tt_wait(&ring_full[rr.i], rr.phase, &s_bad);
+            ok = ts_wait(&ring_full[rr.i], rr.phase, &s_bad);
             if (!(ok = __all_sync(kFull, ok))) break;
             const uint8_t* st = smem + C::kOffRing + rr.i * Codes::kStage;
             uint4 raw[kRounds];
@@ -560,7 +552,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             __syncwarp();
             if (lane == 0) ts_arrive(&ring_free[rr.i]);
             rr.next();
-            ok = is_v ? tt_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad) : tt_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
+            ok = is_v ? ts_wait(&v_free[rv.i], rv.phase ^ 1u, &s_bad) : ts_wait(&k_free[rk.i], rk.phase ^ 1u, &s_bad);
             if (!(ok = __all_sync(kFull, ok))) break;
             if (warp == kTtSoftmaxWarps) {  // the first of these warps: the row scales
               float* un = units_kv + slot * C::kUnitFloats;
@@ -610,7 +602,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             rk.next();
             rv.next();
           } else if (is_v) {
-            ok = tt_wait(&v_raw[rv.i], rv.phase, &s_bad);
+            ok = ts_wait(&v_raw[rv.i], rv.phase, &s_bad);
             if (!(ok = __all_sync(kFull, ok))) break;
             if (edge) {
               uint8_t* v = smem + C::kOffV + rv.i * C::kOperand;
@@ -669,7 +661,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const int tok = has ? (n_first + n) / p.group : 0;
       const int64_t q_row_own = q_row(b, w.u, n);
       if (!SPLIT && !first_segment) {  // both streams have read what the join left in the place of Q
-        ok = tt_wait(&join_read, end_phase ^ 1u, &s_bad);
+        ok = ts_wait(&join_read, end_phase ^ 1u, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
       }
       first_segment = false;
@@ -770,7 +762,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             }
           }
         }
-        ok = tt_wait(&s_full[s][buf], (s_count >> 1) & 1, &s_bad);
+        ok = ts_wait(&s_full[s][buf], (s_count >> 1) & 1, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
         tt_fence_after();
         ++s_count;
@@ -909,7 +901,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
             // ---- the accumulator, once P V of the tile before is done
             if (done > 0 && __any_sync(kFull, f != 1.0f)) {
               // The scores of this job were issued after the P V of the job before last: one phase is in question.
-              ok = tt_wait(&o_done[s], (o_count - 1) & 1, &s_bad);
+              ok = ts_wait(&o_done[s], (o_count - 1) & 1, &s_bad);
               if (!(ok = __all_sync(kFull, ok))) return;
               tt_fence_after();
 #pragma unroll 1
@@ -947,7 +939,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
       slot0 = (slot0 + tiles) & (kTtUnitSlots - 1);
       // Every P V of the segment.  (Waiting on o_done here could miss it: it may be one or two phases on.)
-      ok = ok && tt_wait(&o_end[s], o_end_phase, &s_bad);
+      ok = ok && ts_wait(&o_end[s], o_end_phase, &s_bad);
       ok = __all_sync(kFull, ok);
       o_end_phase ^= 1u;
       tt_fence_after();
@@ -970,7 +962,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         // joins all, reading both in tensor memory (32 tokens, E4M3: halves took 66 us, this 64).
         __syncwarp();
         if (lane == 0) ts_arrive(&seg_done);
-        ok = ok && tt_wait(&seg_done, end_phase, &s_bad);
+        ok = ok && ts_wait(&seg_done, end_phase, &s_bad);
         ok = __all_sync(kFull, ok);
         if (ok && warp_has) {
           if (done > 0 && shifted) {
@@ -989,7 +981,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         tt_fence_before();
         __syncwarp();
         if (lane == 0) ts_arrive(&join_ready);
-        ok = ok && tt_wait(&join_ready, end_phase, &s_bad);
+        ok = ok && ts_wait(&join_ready, end_phase, &s_bad);
         ok = __all_sync(kFull, ok);
         tt_fence_after();
         end_phase ^= 1u;
@@ -1129,6 +1121,16 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       __syncwarp();
       if (!SPLIT && lane == 0) ts_arrive(&join_read);
     }
+  }
+  // Where a wait gave up, the MMAs in flight end before their tiles and tensor memory go to another.  (Here, not in the
+  // issuing warps' branch: there it took 16 tokens over NVFP4 from 157 to 162 us.)
+  if (__any_sync(kFull, s_bad) && (warp == kTtMmaWarp || warp == kTtMmaWarp + 2)) {
+    if (tt_elect()) {  // the lane that issued them: the election is the same each time
+      uint64_t* bar = &drained[(warp - kTtMmaWarp) / 2];
+      tt_commit(bar);
+      ts_landed(bar, 0);
+    }
+    __syncwarp();
   }
   tt_fence_before();
   __syncthreads();
