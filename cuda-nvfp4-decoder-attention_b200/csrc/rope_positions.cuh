@@ -14,11 +14,12 @@
 //
 // A block takes one token (several where heads are few): the sines and cosines
 // are computed once per token, in shared memory, laid out so that one 16-byte
-// load serves two FP32x2 operations.  Bound by HBM: each element is read once
-// and written once, with its first loads on their way while the table is made.
-// Measured: 8,192 tokens x 30 heads x 128 elements, 126 MB, in 26.8 us (4.7
-// TB/s, 0.72 of a copy); instructions issue in 80 % of the cycles there, so the
-// FP64 angles and the table weigh beside the bytes.  A single token: 7.8 us, the
+// load serves two FP32x2 operations.  Each element is read once and written once,
+// with its first loads on their way while the table is made.
+// Measured: 8,192 tokens x 30 heads x 128 elements, 126 MB, in 27 us (4.7
+// TB/s, 0.72 of a copy); instructions issue in 80 % of the cycles there: 310 a
+// thread for its one item of 16 elements, most of them what a block of one token
+// sets up (divisions of indices, the table).  A single token: 7.8 us, the
 // launch.
 #pragma once
 

@@ -4,20 +4,21 @@
 //
 // Work decomposition.  The group * T query rows of one (sequence, KV head) are
 // cut into passes of RP rows (nearly always one pass).  Every (sequence, KV
-// head, pass) owns the ceil((P_b + T) / 64) tiles of 64 positions its keys
-// fill; all of them are laid end to end and one CTA per SM takes an equal
-// contiguous range of that line, so every SM streams the same bytes whatever
-// the lengths.  A CTA's part of one unit either is the whole unit (the result
-// is written) or leaves a partial (o, m, l): only a CTA's first and last parts
-// can be partial, so it has two slots.  tree_stream_combine_kernel joins a
-// unit's partials in CTA order.
+// head, pass) owns the tiles that its P_b + T keys fill, of 64 positions over
+// BF16 and of 128 over codes; all of them are laid end to end and one CTA per SM
+// takes an equal contiguous range of that line, so every SM streams the same
+// bytes whatever the lengths.  A CTA's part of one unit either is the whole unit
+// (the result is written) or leaves a partial (o, m, l): only a CTA's first and
+// last parts can be partial, so it has two slots.  tree_stream_combine_kernel
+// joins a unit's partials in CTA order.
 //
-// Per CTA: a producer lane moves K and V tiles (TMA, 128-byte swizzle) and
-// their scales (bulk copies) into a ring of stages.  NW consumer warps: RC row
-// chunks of 8 NG query rows, NW / RC position warps per chunk; a warp takes
-// 16-position slices, whole tiles alternating between groups of four position
-// warps.  With x^T for a fragment that holds positions or head elements in its
-// 16 rows and queries in its 8 columns:
+// Per CTA: two warps fill a ring of stages, one with K and one with V tiles (TMA,
+// 128-byte swizzle) and the scales of both (16-byte asynchronous copies by all of
+// its lanes); two more join and write what the consumers leave of a segment.  NW
+// consumer warps: RC row chunks of 8 NG query rows, NW / RC position warps per
+// chunk; a warp takes 16-position slices, whole tiles alternating between groups
+// of four position warps.  With x^T for a fragment that holds positions or head
+// elements in its 16 rows and queries in its 8 columns:
 //   S^T[pos, q] = K[pos, :] . Q^T      mma.m16n8k16, FP32 accumulators
 //   O^T[d, q]  += V^T[d, pos] P^T
 // The element k of an MMA step may be any element of the head as long as K and
@@ -47,11 +48,12 @@
 // not see the row); queries that do see such an element get it added after.
 //
 // What bounds it: a single token over ragged E4M3 caches (64 sequences x 6 heads,
-// 1,024 to 8,191 positions, 460 MB) takes 94 us, 4.9 TB/s, 0.75 of a copy; of
+// 1,024 to 8,191 positions, 460 MB) takes 92 us, 5.0 TB/s, 0.76 of a copy; of
 // that the launches, the first tiles' latency and the join of partials are some
-// 12 us, the rest streams at 0.85.  Over NVFP4 (8 sequences, 32,768 positions)
-// 70 us, 3.4 TB/s: decoding codes to FP16 in registers, 43 % of the issue slots
+// 12 us, the rest streams at 0.87.  Over NVFP4 (8 sequences, 32,768 positions)
+// 71 us, 3.4 TB/s: decoding codes to FP16 in registers, 43 % of the issue slots
 // and the latency between them with two warps a scheduler, no longer the bytes.
+// G by the largest row scale alone, checked before the exponentials, took 70 us there.
 // 12 or 16 consumer warps, for which registers suffice with one slice at a time,
 // were no faster.
 //

@@ -19,8 +19,8 @@
 // a stream each (one warp for both could not issue them fast enough beside the
 // others on its scheduler); warp 17 loads codes, warp 19 scales.  Per tile of 64
 // keys:
-//   load     codes and scales (TMA, bulk copies) into a ring; BF16 K and V
-//            straight into operand tiles;
+//   load     codes (TMA) and scales (16-byte asynchronous copies) into a ring;
+//            BF16 K and V straight into operand tiles;
 //   prepare  codes (times the NVFP4 block scale) to FP16, exact, as [key][d]
 //            tiles of 128-byte swizzled rows: K is a K-major operand, V an
 //            MN-major one, so neither is transposed.  In tiles that reach P_b,
@@ -31,7 +31,9 @@
 //            over the scores in tensor memory; the reference m moves only when
 //            P would pass 2^15 (BF16: when a score passes m by 2^20), and only
 //            then the accumulator is rescaled;
-//   O += P V  M 128, N = D, P read from tensor memory, accumulated there.
+//   O += P V  M 128, N = D, P read from tensor memory, accumulated there over the
+//            segment.  The tensor cores' sums round down: 131,008 equal values in
+//            one segment (D 64) come out low by 2^-13, 1/16 of BF16's half step.
 // Shared memory feeds the MMAs, so P stays out of it: with P as a
 // shared-memory operand its reads and writes took a third of the bandwidth and
 // the kernel 1.6 times as long.
@@ -44,11 +46,12 @@
 // shared memory, 65 for one of P V), but a softmax warp, alone on its scheduler
 // but for two preparing warps, takes 1,450 a tile of its stream, and preparing
 // one 1,400; the pipeline moves a tile every 1,400.  16 tokens over NVFP4 (8
-// sequences x 6 heads, 30,001 to 32,752 positions): 154 us, 320 TFLOP/s, tensor
-// pipe 31 % busy.  Over BF16 with more than 128 rows: the MMAs, since P is two
+// sequences x 6 heads, 30,001 to 32,752 positions): 155 to 157 us, 316 TFLOP/s,
+// tensor pipe 32 % busy; where the compiler puts the rarely run code moves that by
+// up to 14 %.  Over BF16 with more than 128 rows: the MMAs, since P is two
 // terms: 1,824 of some 2,400 cycles a tile of 256 rows, 75 % of them rows.  48
-// tokens (16 sequences, 8,000 positions): 127 to 139 us on several machines, 410
-// to 447 TFLOP/s, pipe 56 % busy.
+// tokens (16 sequences, 8,000 positions): 130 to 137 us on several machines, 416
+// to 438 TFLOP/s, pipe 56 % busy.
 // A segment costs 15,000 to 20,000 cycles beside its tiles: the walk, Q, the
 // first tile's second pass, the join and the partial results.
 // Tried, and not kept: the two preparing groups taking K and V of alternate tiles
