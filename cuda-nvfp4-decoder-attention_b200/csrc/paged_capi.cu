@@ -1,0 +1,301 @@
+// C ABI of serving drafted tokens from a paged KV cache: pages reserved and
+// given back, rows by slots, attention through the block table, and the
+// verification of drafted tokens.
+// Declarations: include/nvfp4_decoder_attention.h.
+#include <algorithm>
+#include <cmath>
+
+#include "host_util.cuh"
+#include "kv_host.cuh"
+#include "page_table.cuh"
+#include "paged_kv.cuh"
+#include "tree_attention.cuh"
+#include "verify_drafted.cuh"
+
+namespace nvfp4da {
+namespace {
+
+int check_table(const nvfp4da_page_table* t, PageTableParams& p) {
+  if (!t) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "the page table is NULL");
+  if (!t->pages || !t->held || !t->free_pages || !t->free_count)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "a field of the page table is NULL");
+  if (t->batch <= 0 || t->max_pages <= 0 || t->pool <= 0 || t->page_size <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "the page table's dimensions must all be positive");
+  if (t->page_size % NVFP4DA_PAGE_SIZE_MULTIPLE != 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "the page size must be a multiple of %d, got %lld",
+                NVFP4DA_PAGE_SIZE_MULTIPLE, static_cast<long long>(t->page_size));
+  if (!product_within(t->batch, t->max_pages, kI32Max) || !product_within(t->max_pages, t->page_size, kI32Max / 2) ||
+      !product_within(t->pool, t->page_size, kI32Max))
+    return fail(NVFP4DA_ERR_UNSUPPORTED,
+                "a page table holds fewer than 2^31 entries, 2^30 positions a sequence and 2^31 slots in its pool");
+  p.table = t->pages;
+  p.held = t->held;
+  p.free_pages = t->free_pages;
+  p.free_count = t->free_count;
+  p.batch = static_cast<int>(t->batch);
+  p.max_pages = static_cast<int>(t->max_pages);
+  p.pages = static_cast<int>(t->pool);
+  p.page_size = static_cast<int>(t->page_size);
+  return NVFP4DA_OK;
+}
+
+// Plan of the paged attention.
+struct PagedPlan {
+  int splits;
+  int64_t split_len;
+  size_t bytes;
+};
+
+int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int64_t tokens, int64_t q_heads,
+               int64_t max_past, PagedPlan& pl) {
+  int r = check_pool(c);
+  if (r) return r;
+  if (batch <= 0 || max_pages <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "the block table's dimensions must all be positive");
+  if (!product_within(batch, c->kv_heads, 65535))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "B*Hkv must be at most 65535");
+  if (!product_within(max_pages, c->capacity, kI32Max / 2) || !product_within(batch, max_pages, kI32Max))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "a block table holds fewer than 2^31 entries and 2^30 positions a sequence");
+  if (tokens <= 0 || q_heads <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "token and query head counts must be positive");
+  if (q_heads % c->kv_heads != 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "number of query heads must be divisible by number of KV heads");
+  if (max_past < 0) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "max_past_length must be nonnegative");
+  const int64_t capacity = max_pages * c->capacity;
+  if (tokens > capacity || max_past > capacity - tokens)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "max_past_length + token count exceeds the block table (%lld + %lld > %lld)",
+                static_cast<long long>(max_past), static_cast<long long>(tokens), static_cast<long long>(capacity));
+  const int64_t group = q_heads / c->kv_heads;
+  if (!product_within(group, tokens, 65535) || !product_within(batch * q_heads, tokens, kI32Max))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "too many query rows: (Hq/Hkv)*T must be at most 65535 and B*T*Hq below 2^31");
+  const int64_t visible = max_past + tokens;
+  const int64_t base = batch * c->kv_heads * ceil_div(group * tokens, kTreeWarps);
+  int64_t splits = std::min(ceil_div(8LL * sm_count(), base), ceil_div(visible, 128));
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, 1024));
+  pl.split_len = ceil_div(ceil_div(visible, splits), 32) * 32;
+  pl.splits = static_cast<int>(ceil_div(visible, pl.split_len));
+  const size_t rows = static_cast<size_t>(batch * tokens * q_heads);
+  pl.bytes = align_up(pl.splits > 1 ? rows * pl.splits * (c->head_dim + 2) * 4 : 16, 256);
+  return NVFP4DA_OK;
+}
+
+}  // namespace
+}  // namespace nvfp4da
+
+using namespace nvfp4da;
+
+extern "C" {
+
+int nvfp4da_reserve_pages(const nvfp4da_page_table* table, const int64_t* past_lengths, const int64_t* counts,
+                          int64_t tokens, int64_t* slots, int64_t* granted, void* stream) {
+  PageTableParams p{};
+  int r = check_table(table, p);
+  if (r) return r;
+  if (!past_lengths || !slots || !granted || tokens <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "reserve_pages: invalid arguments");
+  if (tokens > 1 << 20 || !product_within(table->batch, tokens, kI32Max))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "reserve_pages: at most 2^20 tokens a sequence and fewer than 2^31 in all");
+  p.lengths = past_lengths;
+  p.counts = counts;
+  p.tokens = static_cast<int>(tokens);
+  p.slots = slots;
+  p.granted = granted;
+  cudaError_t e = launch_cluster(reserve_pages_kernel, dim3(1), dim3(kPageThreads), 0,
+                                 static_cast<cudaStream_t>(stream), false, 1u, p);
+  return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "reserve_pages launch");
+}
+
+int nvfp4da_release_pages(const nvfp4da_page_table* table, const int64_t* lengths, void* stream) {
+  PageTableParams p{};
+  int r = check_table(table, p);
+  if (r) return r;
+  if (!lengths) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "release_pages: invalid arguments");
+  p.lengths = lengths;
+  release_pages_kernel<<<1, kPageThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  NVFP4DA_CHECK_LAUNCH("release_pages launch");
+  return NVFP4DA_OK;
+}
+
+int nvfp4da_paged_kv_append(const nvfp4da_kv_cache* c, const uint16_t* new_k, const int64_t* k_strides,
+                            const uint16_t* new_v, const int64_t* v_strides, int64_t batch, int64_t tokens,
+                            const int64_t* slots, int64_t slot_stride, const int64_t* source, int64_t rows,
+                            const int64_t* counts, void* stream) {
+  int r = check_pool(c);
+  if (r) return r;
+  if (!new_k || !new_v || !k_strides || !v_strides || !slots || batch <= 0 || tokens <= 0 || rows <= 0 ||
+      slot_stride < rows || (!source && rows != tokens))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "paged_kv_append: invalid arguments");
+  if (!product_within(batch, c->kv_heads, 65535))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "B*Hkv must be at most 65535");
+  if (tokens > kI32Max - kKvThreads || rows > kI32Max - kKvThreads)
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "paged_kv_append: too many tokens");
+  PagedAppendParams p{};
+  p.k = k_store(*c);
+  p.v = v_store(*c);
+  p.new_k = new_k;
+  p.new_v = new_v;
+  for (int i = 0; i < 3; ++i) {
+    p.k_stride[i] = k_strides[i];
+    p.v_stride[i] = v_strides[i];
+  }
+  p.slots = slots;
+  p.slot_stride = slot_stride;
+  p.source = source;
+  p.counts = counts;
+  p.rows = static_cast<int>(rows);
+  p.tokens = static_cast<int>(tokens);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.head_dim = static_cast<int>(c->head_dim);
+  p.pages = static_cast<int>(c->batch);
+  p.page_size = static_cast<int>(c->capacity);
+  p.lanes = lanes_per_row(c->head_dim, 16);
+  p.vec_k = row_vector(new_k, k_strides) == 8;
+  p.vec_v = row_vector(new_v, v_strides) == 8;
+  const dim3 grid(static_cast<unsigned>(ceil_div(rows, kKvThreads / p.lanes)), static_cast<unsigned>(batch * c->kv_heads));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (c->format) {
+    case NVFP4DA_KV_BF16: paged_append_kernel<kKvFmtBf16><<<grid, kKvThreads, 0, s>>>(p); break;
+    case NVFP4DA_KV_E4M3: paged_append_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p); break;
+    default: paged_append_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p); break;
+  }
+  NVFP4DA_CHECK_LAUNCH("paged_kv_append launch");
+  return NVFP4DA_OK;
+}
+
+int nvfp4da_paged_kv_read(const nvfp4da_kv_cache* c, const int64_t* slots, int64_t batch, int64_t length,
+                          uint16_t* k_out, uint16_t* v_out, void* stream) {
+  int r = check_pool(c);
+  if (r) return r;
+  if (!slots || !k_out || !v_out || batch <= 0 || length <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "paged_kv_read: invalid arguments");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "paged_kv_read outputs must be 16-byte aligned");
+  if (!product_within(batch, c->kv_heads, 65535))
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "B*Hkv must be at most 65535");
+  if (length > kI32Max / 2) return fail(NVFP4DA_ERR_UNSUPPORTED, "paged_kv_read: too many rows");
+  PagedReadParams p{};
+  p.k = k_store(*c);
+  p.v = v_store(*c);
+  p.slots = slots;
+  p.out_k = k_out;
+  p.out_v = v_out;
+  p.rows = static_cast<int>(length);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.head_dim = static_cast<int>(c->head_dim);
+  p.pages = static_cast<int>(c->batch);
+  p.page_size = static_cast<int>(c->capacity);
+  p.lanes = lanes_per_row(c->head_dim, 8);
+  const dim3 grid(static_cast<unsigned>(ceil_div(length, kKvReadRows * (kKvThreads / p.lanes))),
+                  static_cast<unsigned>(batch * c->kv_heads));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (c->format) {
+    case NVFP4DA_KV_BF16: paged_read_kernel<kKvFmtBf16><<<grid, kKvThreads, 0, s>>>(p); break;
+    case NVFP4DA_KV_E4M3: paged_read_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p); break;
+    default: paged_read_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p); break;
+  }
+  NVFP4DA_CHECK_LAUNCH("paged_kv_read launch");
+  return NVFP4DA_OK;
+}
+
+size_t nvfp4da_paged_attention_workspace_size(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages,
+                                              int64_t tokens, int64_t q_heads, int64_t max_past_length) {
+  PagedPlan pl;
+  return plan_paged(c, batch, max_pages, tokens, q_heads, max_past_length, pl) ? 0 : pl.bytes;
+}
+
+int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const int32_t* block_table, int64_t batch,
+                            int64_t max_pages, const uint8_t* tree_mask, int64_t mask_batch_stride, uint16_t* context,
+                            int64_t tokens, int64_t q_heads, const int64_t* past_lengths, int64_t max_past_length,
+                            const int64_t* counts, void* ws, size_t ws_bytes, void* stream) {
+  PagedPlan pl;
+  int r = plan_paged(c, batch, max_pages, tokens, q_heads, max_past_length, pl);
+  if (r) return r;
+  if (!q || !context || !block_table || !past_lengths)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "paged attention: NULL pointer");
+  if (!aligned(q, 16) || !aligned(context, 16))
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
+  const bool needs_ws = pl.splits > 1;
+  if (needs_ws && (!ws || ws_bytes < pl.bytes))
+    return fail(NVFP4DA_ERR_WORKSPACE, "paged attention workspace too small (%zu < %zu bytes)", ws ? ws_bytes : size_t(0),
+                pl.bytes);
+  if (needs_ws && !aligned(ws, 16))
+    return fail(NVFP4DA_ERR_WORKSPACE, "the paged attention workspace must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  TreeAttnParams p{};
+  p.pg = {block_table, static_cast<int>(c->batch), static_cast<int>(max_pages), static_cast<int>(c->capacity), counts};
+  p.q = q;
+  p.k = k_store(*c);
+  p.v = v_store(*c);
+  p.mask = tree_mask;
+  p.mask_stride = mask_batch_stride;
+  p.ctx = context;
+  p.partials = static_cast<float*>(ws);
+  p.batch = static_cast<int>(batch);
+  p.tokens = static_cast<int>(tokens);
+  p.q_heads = static_cast<int>(q_heads);
+  p.kv_heads = static_cast<int>(c->kv_heads);
+  p.head_dim = static_cast<int>(c->head_dim);
+  p.capacity = max_pages * c->capacity;
+  p.past_lengths = past_lengths;
+  p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c->head_dim)));
+  p.splits = pl.splits;
+  p.split_len = pl.split_len;
+  p.lanes = std::max(2, lanes_per_row(c->head_dim, 8));
+  const int64_t group = q_heads / c->kv_heads;
+  const dim3 grid(static_cast<unsigned>(pl.splits), static_cast<unsigned>(ceil_div(group * tokens, kTreeWarps)),
+                  static_cast<unsigned>(batch * c->kv_heads));
+  switch (c->format) {
+    case NVFP4DA_KV_BF16: tree_attn_general_kernel<kKvFmtBf16, true><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
+    case NVFP4DA_KV_E4M3: tree_attn_general_kernel<kKvFmtE4m3, true><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
+    default: tree_attn_general_kernel<kKvFmtNvfp4, true><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
+  }
+  NVFP4DA_CHECK_LAUNCH("paged attention launch");
+  if (pl.splits > 1) {
+    const int64_t rows = batch * tokens * q_heads;
+    tree_combine_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, s>>>(p);
+    NVFP4DA_CHECK_LAUNCH("paged attention combine launch");
+  }
+  return NVFP4DA_OK;
+}
+
+int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, const float* draft,
+                           const int64_t* draft_strides, const int64_t* tokens, const int64_t* parents,
+                           int64_t parent_stride, const float* uniforms, const int64_t* counts, int64_t batch,
+                           int64_t nodes, int64_t vocab, int64_t* path, int64_t* accepted, int64_t* next_tokens,
+                           void* stream) {
+  if (!target || !target_strides || (draft && !draft_strides) || !tokens || !uniforms || !path || !accepted ||
+      !next_tokens || batch <= 0 || nodes <= 0 || vocab <= 0)
+    return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "verify_drafted: invalid arguments");
+  if (nodes > kVerifyMaxNodes)
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "verify_drafted: at most %d nodes a tree, got %lld", kVerifyMaxNodes,
+                static_cast<long long>(nodes));
+  if (vocab > kI32Max - 65536 || batch > kI32Max / kVerifyMaxCluster)
+    return fail(NVFP4DA_ERR_UNSUPPORTED, "verify_drafted: vocabulary or batch too large");
+  VerifyParams p{};
+  p.target = target;
+  p.draft = draft;
+  p.vec = aligned(target, 16) && (!draft || aligned(draft, 16));
+  for (int i = 0; i < 2; ++i) {
+    p.target_stride[i] = target_strides[i];
+    p.draft_stride[i] = draft ? draft_strides[i] : 0;
+    p.vec = p.vec && p.target_stride[i] % 4 == 0 && p.draft_stride[i] % 4 == 0;
+  }
+  p.tokens = tokens;
+  p.parents = parents;
+  p.parent_stride = parent_stride;
+  p.uniforms = uniforms;
+  p.counts = counts;
+  p.nodes = static_cast<int>(nodes);
+  p.vocab = static_cast<int>(vocab);
+  p.path = path;
+  p.accepted = accepted;
+  p.next = next_tokens;
+  const unsigned ctas = 1;
+  cudaError_t e = ensure_smem(verify_drafted_kernel, static_cast<uint32_t>(verify_smem(p.nodes)));
+  if (e == cudaSuccess)
+    e = launch_cluster(verify_drafted_kernel, dim3(static_cast<unsigned>(batch) * ctas), dim3(kVerifyThreads),
+                       verify_smem(p.nodes), static_cast<cudaStream_t>(stream), false, ctas, p);
+  return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "verify_drafted launch");
+}
+
+}  // extern "C"

@@ -41,6 +41,9 @@ const char* dtype_name(at::ScalarType t) {
     case at::kBFloat16: return "torch.bfloat16";
     case at::kByte: return "torch.uint8";
     case at::kFloat: return "torch.float32";
+    case at::kInt: return "torch.int32";
+    case at::kLong: return "torch.int64";
+    case at::kBool: return "torch.bool";
     default: return "?";
   }
 }
@@ -544,6 +547,24 @@ std::tuple<Tensor, Tensor> quantized_kv_read(const Tensor& kc, const Tensor& vc,
   return {k, v};
 }
 
+// A bool [T, T] or [B, T, T] mask of q's drafted tokens, if there is one.
+struct Mask {
+  const uint8_t* data = nullptr;
+  int64_t stride = 0;
+};
+Mask mask_of(const OptTensor& tree_mask, const Tensor& q) {
+  if (!tree_mask.has_value()) return {};
+  const int64_t b = q.size(0), t = q.size(1);
+  expect(*tree_mask, "tree_mask", at::kBool);
+  const bool shared = tree_mask->dim() == 2;
+  const int64_t o = shared ? 0 : 1;
+  TORCH_CHECK((shared || (tree_mask->dim() == 3 && tree_mask->size(0) == b)) && tree_mask->size(o) == t &&
+                  tree_mask->size(o + 1) == t,
+              "tree_mask must have shape [T, T] or [B, T, T]; got ", tree_mask->sizes());
+  expect_same_device(*tree_mask, "tree_mask", q, "q");
+  return {static_cast<const uint8_t*>(tree_mask->data_ptr()), shared ? 0 : t * t};
+}
+
 Tensor tree_attention_cached(const Tensor& q, const Tensor& kc, const Tensor& vc, const OptTensor& kr,
                              const OptTensor& vr, const OptTensor& kb, const OptTensor& vb, const OptTensor& tree_mask,
                              int64_t past_length, const OptTensor& past_lengths, int64_t max_past_length) {
@@ -560,28 +581,199 @@ Tensor tree_attention_cached(const Tensor& q, const Tensor& kc, const Tensor& vc
   TORCH_CHECK(max_past >= 0, pl ? "max_past_length" : "past_length", " must be nonnegative");
   TORCH_CHECK(max_past <= c.capacity - t, pl ? "max_past_length" : "past_length",
               " + drafted token count exceeds cache capacity (", max_past, " + ", t, " > ", c.capacity, ")");
-  const uint8_t* mask = nullptr;
-  int64_t mask_stride = 0;
-  if (tree_mask.has_value()) {
-    expect(*tree_mask, "tree_mask", at::kBool);
-    const bool shared = tree_mask->dim() == 2;
-    const int64_t o = shared ? 0 : 1;
-    TORCH_CHECK((shared || (tree_mask->dim() == 3 && tree_mask->size(0) == b)) && tree_mask->size(o) == t &&
-                    tree_mask->size(o + 1) == t,
-                "tree_mask must have shape [T, T] or [B, T, T]; got ", tree_mask->sizes());
-    expect_same_device(*tree_mask, "tree_mask", q, "q");
-    mask = static_cast<const uint8_t*>(tree_mask->data_ptr());
-    mask_stride = shared ? 0 : t * t;
-  }
+  const Mask m = mask_of(tree_mask, q);
   const c10::cuda::CUDAGuard g(q.device());
   Tensor ctx = at::empty(q.sizes(), q.options());
   const size_t wsb = nvfp4da_tree_attention_workspace_size(&c, t, hq, max_past);
   TORCH_CHECK(wsb > 0, "cuda_tree_attention_cached rejected its arguments: ", nvfp4da_last_error());
   Tensor ws = workspace(q, wsb);
-  check_status(nvfp4da_tree_attention(bits(q), &c, mask, mask_stride, mbits(ctx), t, hq, past_length, pl, max_past,
+  check_status(nvfp4da_tree_attention(bits(q), &c, m.data, m.stride, mbits(ctx), t, hq, past_length, pl, max_past,
                                       ws.data_ptr(), wsb, cur_stream(q)),
                "cuda_tree_attention_cached");
   return ctx;
+}
+
+// ---------------------------------------------------------------- the paged KV cache
+nvfp4da_page_table page_table(const Tensor& pages, const Tensor& held, const Tensor& free_pages,
+                              const Tensor& free_count, int64_t page_size) {
+  expect(pages, "pages", at::kInt);
+  TORCH_CHECK(pages.dim() == 2 && pages.size(0) > 0 && pages.size(1) > 0, "pages must have shape [B, M], got ",
+              pages.sizes());
+  expect(free_pages, "free_pages", at::kInt);
+  TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) > 0, "free_pages must have shape [N], got ",
+              free_pages.sizes());
+  expect_same_device(free_pages, "free_pages", pages, "pages");
+  nvfp4da_page_table t{};
+  t.held = const_cast<int64_t*>(lengths(held, "held", pages.size(0), pages, "pages"));
+  expect(free_count, "free_count", at::kLong);
+  TORCH_CHECK(free_count.dim() == 1 && free_count.size(0) == 1, "free_count must have shape [1], got ",
+              free_count.sizes());
+  expect_same_device(free_count, "free_count", pages, "pages");
+  TORCH_CHECK(page_size > 0 && page_size % NVFP4DA_PAGE_SIZE_MULTIPLE == 0, "page_size must be a positive multiple of ",
+              NVFP4DA_PAGE_SIZE_MULTIPLE, ", got ", page_size);
+  t.pages = pages.data_ptr<int32_t>();
+  t.free_pages = free_pages.data_ptr<int32_t>();
+  t.free_count = free_count.data_ptr<int64_t>();
+  t.batch = pages.size(0);
+  t.max_pages = pages.size(1);
+  t.pool = free_pages.size(0);
+  t.page_size = page_size;
+  return t;
+}
+
+std::tuple<Tensor, Tensor> reserve_pages_(Tensor& pages, Tensor& held, Tensor& free_pages, Tensor& free_count,
+                                          int64_t page_size, const Tensor& past_lengths, int64_t tokens,
+                                          const OptTensor& counts) {
+  const nvfp4da_page_table t = page_table(pages, held, free_pages, free_count, page_size);
+  const int64_t* pl = lengths(past_lengths, "past_lengths", t.batch, pages, "pages");
+  const int64_t* n = lengths(counts, "counts", t.batch, pages, "pages");
+  TORCH_CHECK(tokens > 0, "tokens must be positive, got ", tokens);
+  const c10::cuda::CUDAGuard g(pages.device());
+  Tensor slots = at::empty({t.batch, tokens}, held.options()), granted = at::empty({t.batch}, held.options());
+  check_status(nvfp4da_reserve_pages(&t, pl, n, tokens, slots.data_ptr<int64_t>(), granted.data_ptr<int64_t>(),
+                                     cur_stream(pages)),
+               "cuda_reserve_pages_");
+  return {slots, granted};
+}
+
+void release_pages_(Tensor& pages, Tensor& held, Tensor& free_pages, Tensor& free_count, int64_t page_size,
+                    const Tensor& kept) {
+  const nvfp4da_page_table t = page_table(pages, held, free_pages, free_count, page_size);
+  const int64_t* len = lengths(kept, "lengths", t.batch, pages, "pages");
+  const c10::cuda::CUDAGuard g(pages.device());
+  check_status(nvfp4da_release_pages(&t, len, cur_stream(pages)), "cuda_release_pages_");
+}
+
+// int64 [B, n] on the pool's device.
+const int64_t* indices(const Tensor& t, const char* name, const Tensor& ref) {
+  expect(t, name, at::kLong);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) > 0 && t.size(1) > 0, name, " must have shape [B, n], got ", t.sizes());
+  expect_same_device(t, name, ref, "the cache");
+  return t.data_ptr<int64_t>();
+}
+
+void paged_kv_append_(Tensor& kc, Tensor& vc, const OptTensor& kr, const OptTensor& vr, const OptTensor& kb,
+                      const OptTensor& vb, const Tensor& nk, const Tensor& nv, const Tensor& slots,
+                      const OptTensor& source, const OptTensor& counts) {
+  const nvfp4da_kv_cache c = kv_cache(kc, vc, kr, vr, kb, vb);
+  expect_rows(nk, "new_k");
+  expect_rows(nv, "new_v");
+  TORCH_CHECK(nv.sizes() == nk.sizes(), "new_v must have the same shape as new_k; got ", nv.sizes(), " and ",
+              nk.sizes());
+  expect_same_device(nk, "new_k", kc, "the cache");
+  expect_same_device(nv, "new_v", kc, "the cache");
+  TORCH_CHECK(nk.size(2) == c.kv_heads && nk.size(3) == c.head_dim,
+              "new K/V must have shape [B, T, Hkv, D] matching the cache; got ", nk.sizes());
+  const int64_t b = nk.size(0), t = nk.size(1);
+  const int64_t* to = indices(slots, "slots", kc);
+  const int64_t* from = source.has_value() ? indices(*source, "source", kc) : nullptr;
+  const int64_t rows = from ? source->size(1) : t;
+  TORCH_CHECK(slots.size(0) == b && slots.size(1) >= rows, "slots must have shape [B, n] with n >= ", rows, "; got ",
+              slots.sizes());
+  TORCH_CHECK(!from || source->size(0) == b, "source must have shape [B, n]; got ", source->sizes());
+  const int64_t* n = lengths(counts, "counts", b, kc, "the cache");
+  const c10::cuda::CUDAGuard g(kc.device());
+  const RowStrides ks = row_strides(nk), vs = row_strides(nv);
+  check_status(nvfp4da_paged_kv_append(&c, bits(nk), ks.v, bits(nv), vs.v, b, t, to, slots.size(1), from, rows, n,
+                                       cur_stream(kc)),
+               "cuda_paged_kv_append_");
+}
+
+std::tuple<Tensor, Tensor> paged_kv_read(const Tensor& kc, const Tensor& vc, const OptTensor& kr, const OptTensor& vr,
+                                         const OptTensor& kb, const OptTensor& vb, const Tensor& slots) {
+  const nvfp4da_kv_cache c = kv_cache(kc, vc, kr, vr, kb, vb);
+  const int64_t* from = indices(slots, "slots", kc);
+  const c10::cuda::CUDAGuard g(kc.device());
+  const auto options = kc.options().dtype(at::kBFloat16);
+  Tensor k = at::empty({slots.size(0), c.kv_heads, slots.size(1), c.head_dim}, options), v = at::empty(k.sizes(), options);
+  check_status(nvfp4da_paged_kv_read(&c, from, slots.size(0), slots.size(1), mbits(k), mbits(v), cur_stream(kc)),
+               "cuda_paged_kv_read");
+  return {k, v};
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const OptTensor& kr, const OptTensor& vr,
+                       const OptTensor& kb, const OptTensor& vb, const Tensor& block_table,
+                       const OptTensor& tree_mask, const Tensor& past_lengths, int64_t max_past_length,
+                       const OptTensor& counts) {
+  expect_rank4(q, "q");
+  const nvfp4da_kv_cache c = kv_cache(kc, vc, kr, vr, kb, vb);
+  expect_same_device(kc, "the cache", q, "q");
+  const int64_t b = q.size(0), t = q.size(1), hq = q.size(2);
+  TORCH_CHECK(q.size(3) == c.head_dim, "q and cache head dimensions must match (", q.size(3), " != ", c.head_dim, ")");
+  TORCH_CHECK(c.kv_heads > 0 && hq % c.kv_heads == 0, "number of query heads must be divisible by number of KV heads (",
+              hq, " % ", c.kv_heads, " != 0)");
+  expect(block_table, "block_table", at::kInt);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == b && block_table.size(1) > 0,
+              "block_table must have shape [B, M]; got ", block_table.sizes());
+  expect_same_device(block_table, "block_table", q, "q");
+  const int64_t* pl = lengths(past_lengths, "past_lengths", b, q, "q");
+  const int64_t* n = lengths(counts, "counts", b, q, "q");
+  const Mask m = mask_of(tree_mask, q);
+  const c10::cuda::CUDAGuard g(q.device());
+  Tensor ctx = at::empty(q.sizes(), q.options());
+  const size_t wsb = nvfp4da_paged_attention_workspace_size(&c, b, block_table.size(1), t, hq, max_past_length);
+  TORCH_CHECK(wsb > 0, "cuda_paged_attention rejected its arguments: ", nvfp4da_last_error());
+  Tensor ws = workspace(q, wsb);
+  check_status(nvfp4da_paged_attention(bits(q), &c, block_table.data_ptr<int32_t>(), b, block_table.size(1), m.data,
+                                       m.stride, mbits(ctx), t, hq, pl, max_past_length, n, ws.data_ptr(), wsb,
+                                       cur_stream(q)),
+               "cuda_paged_attention");
+  return ctx;
+}
+
+// float32 [B, T, V] by strides: only the last dimension has to be contiguous.
+void expect_probs(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kFloat, name, " must have dtype torch.float32");
+  TORCH_CHECK(t.dim() == 3, name, " must have rank 3, got rank ", t.dim());
+  TORCH_CHECK(t.size(0) > 0 && t.size(1) > 0 && t.size(2) > 0, name, " dimensions must all be positive");
+  TORCH_CHECK(t.stride(2) == 1 || t.size(2) == 1, name, " must be contiguous in its last dimension");
+}
+
+std::tuple<Tensor, Tensor, Tensor> verify_drafted(const Tensor& target, const Tensor& tokens, const Tensor& uniforms,
+                                                  const OptTensor& draft, const OptTensor& parents,
+                                                  const OptTensor& counts) {
+  expect_probs(target, "target_probs");
+  const int64_t b = target.size(0), t = target.size(1), v = target.size(2);
+  auto like_nodes = [&](const Tensor& x, const char* name, at::ScalarType type) {
+    expect(x, name, type);
+    TORCH_CHECK(x.dim() == 2 && x.size(0) == b && x.size(1) == t, name, " must have shape [B, T] = [", b, ", ", t,
+                "]; got ", x.sizes());
+    expect_same_device(x, name, target, "target_probs");
+  };
+  like_nodes(tokens, "tokens", at::kLong);
+  like_nodes(uniforms, "uniforms", at::kFloat);
+  if (draft.has_value()) {
+    expect_probs(*draft, "draft_probs");
+    TORCH_CHECK(draft->sizes() == target.sizes(), "draft_probs must have the same shape as target_probs; got ",
+                draft->sizes(), " and ", target.sizes());
+    expect_same_device(*draft, "draft_probs", target, "target_probs");
+  }
+  bool shared = false;
+  if (parents.has_value()) {
+    expect(*parents, "parents", at::kLong);
+    shared = parents->dim() == 1;
+    TORCH_CHECK(shared ? parents->size(0) == t : (parents->dim() == 2 && parents->size(0) == b && parents->size(1) == t),
+                "parents must have shape [T] or [B, T]; got ", parents->sizes());
+    expect_same_device(*parents, "parents", target, "target_probs");
+  }
+  const int64_t* n = lengths(counts, "counts", b, target, "target_probs");
+  auto strides = [](const Tensor& x, int64_t (&s)[2]) {
+    for (int i = 0; i < 2; ++i) s[i] = x.size(i) > 1 ? x.stride(i) : 0;
+  };
+  int64_t ts[2], ds[2] = {0, 0};
+  strides(target, ts);
+  if (draft.has_value()) strides(*draft, ds);
+  const c10::cuda::CUDAGuard g(target.device());
+  Tensor path = at::empty({b, t}, tokens.options()), accepted = at::empty({b}, tokens.options()),
+         next = at::empty({b}, tokens.options());
+  check_status(nvfp4da_verify_drafted(target.data_ptr<float>(), ts, draft.has_value() ? draft->data_ptr<float>() : nullptr,
+                                      ds, tokens.data_ptr<int64_t>(),
+                                      parents.has_value() ? parents->data_ptr<int64_t>() : nullptr, shared ? 0 : t,
+                                      uniforms.data_ptr<float>(), n, b, t, v, path.data_ptr<int64_t>(),
+                                      accepted.data_ptr<int64_t>(), next.data_ptr<int64_t>(), cur_stream(target)),
+               "cuda_verify_drafted");
+  return {path, accepted, next};
 }
 
 }  // namespace
@@ -650,4 +842,31 @@ TORCH_LIBRARY(cuda_nvfp4_decoder_attention, m) {
       "k_block_scales, Tensor? v_block_scales, Tensor? tree_mask=None, int past_length=0, Tensor? past_lengths=None, "
       "int max_past_length=0) -> Tensor",
       TORCH_FN(tree_attention_cached));
+  // Serving drafted tokens from a paged KV cache; a pool's formats as above.
+  m.def(
+      "cuda_reserve_pages_(Tensor(a!) pages, Tensor(b!) held, Tensor(c!) free_pages, Tensor(d!) free_count, int "
+      "page_size, Tensor past_lengths, int tokens, Tensor? counts=None) -> (Tensor, Tensor)",
+      TORCH_FN(reserve_pages_));
+  m.def(
+      "cuda_release_pages_(Tensor(a!) pages, Tensor(b!) held, Tensor(c!) free_pages, Tensor(d!) free_count, int "
+      "page_size, Tensor lengths) -> ()",
+      TORCH_FN(release_pages_));
+  m.def(
+      "cuda_paged_kv_append_(Tensor(a!) k, Tensor(b!) v, Tensor(c!)? k_row_scales, Tensor(d!)? v_row_scales, "
+      "Tensor(e!)? k_block_scales, Tensor(f!)? v_block_scales, Tensor new_k, Tensor new_v, Tensor slots, Tensor? "
+      "source=None, Tensor? counts=None) -> ()",
+      TORCH_FN(paged_kv_append_));
+  m.def(
+      "cuda_paged_kv_read(Tensor k, Tensor v, Tensor? k_row_scales, Tensor? v_row_scales, Tensor? k_block_scales, "
+      "Tensor? v_block_scales, Tensor slots) -> (Tensor, Tensor)",
+      TORCH_FN(paged_kv_read));
+  m.def(
+      "cuda_paged_attention(Tensor q, Tensor k, Tensor v, Tensor? k_row_scales, Tensor? v_row_scales, Tensor? "
+      "k_block_scales, Tensor? v_block_scales, Tensor block_table, Tensor? tree_mask, Tensor past_lengths, int "
+      "max_past_length, Tensor? counts=None) -> Tensor",
+      TORCH_FN(paged_attention));
+  m.def(
+      "cuda_verify_drafted(Tensor target_probs, Tensor tokens, Tensor uniforms, Tensor? draft_probs=None, Tensor? "
+      "parents=None, Tensor? counts=None) -> (Tensor, Tensor, Tensor)",
+      TORCH_FN(verify_drafted));
 }

@@ -74,7 +74,7 @@
 
 namespace nvfp4da {
 
-__device__ unsigned g_tree_errors;
+static __device__ unsigned g_tree_errors;  // of the translation unit's kernels
 
 // Positions per stage: with 64, the 4 KB pieces of NVFP4 codes reached two
 // thirds of the HBM rate even with nothing else to do.

@@ -16,6 +16,7 @@ from pathlib import Path
 import torch
 
 from nvfp4_tensor import NVFP4Tensor, is_nvfp4_tensor, quantize_nvfp4  # noqa: F401
+from paged_kv_cache import PagedKVCache, PageTable  # noqa: F401
 from quantized_kv_cache import QuantizedKVCache, rope_frequencies  # noqa: F401
 
 _PACKAGE_DIR = Path(__file__).resolve().parent
@@ -181,6 +182,100 @@ def cuda_tree_attention_cached(q: torch.Tensor, cache, past_length: int = 0, *, 
                                            past_lengths, max_past_length)
 
 
+# ------------------------------------------------------------------ the paged cache
+def _pool(cache) -> tuple:
+    return (cache.k_codes, cache.v_codes, cache.k_row_scales, cache.v_row_scales, cache.k_block_scales,
+            cache.v_block_scales)
+
+
+def cuda_reserve_pages_(table, past_lengths: torch.Tensor, tokens: int, *,
+                        counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Give every sequence of a ``PageTable`` room for its next tokens, in place; returns ``(slots, granted)``.
+
+    Sequence b gets the pages it lacks for positions ``P_b .. P_b + n_b - 1``
+    (``past_lengths`` CUDA int64 ``[B]``; ``n_b`` is ``counts[b]`` or ``tokens``).
+    ``slots`` int64 ``[B, tokens]`` names the slot of each, -1 for
+    ``t >= counts[b]``.  Sequences are served in order from the top of the free
+    stack; ``granted`` int64 ``[B]`` is ``n_b``, or 0 for a sequence that got
+    nothing: the needs up to and including its own pass the stack, or its
+    positions do not fit the table.
+    """
+    _require_int("tokens", tokens)
+    return _ops.cuda_reserve_pages_(table.pages, table.held, table.free_pages, table.free_count, table.page_size,
+                                    past_lengths, tokens, counts)
+
+
+def cuda_release_pages_(table, lengths: torch.Tensor) -> None:
+    """Let sequence b of a ``PageTable`` keep the pages of its first ``lengths[b]`` positions (CUDA int64 ``[B]``).
+
+    The others go back on the free stack, the last sequence's last page first, so
+    that a release undoes the reserve before it; length 0 ends a sequence.
+    """
+    _ops.cuda_release_pages_(table.pages, table.held, table.free_pages, table.free_count, table.page_size, lengths)
+
+
+def cuda_paged_kv_append_(cache, new_k: torch.Tensor, new_v: torch.Tensor, slots: torch.Tensor, *,
+                          source: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
+    """Write ``[B, T, Hkv, D]`` BF16 rows into ``slots`` (CUDA int64 ``[B, n]``) of a ``PagedKVCache`` in place.
+
+    Row i of sequence b is token i, or ``source[b, i]`` (CUDA int64 ``[B, m]``,
+    ``m <= n``); it is quantised as the pool is.  Rows ``i >= counts[b]`` (CUDA
+    int64 ``[B]``), slots outside the pool and tokens outside ``[0, T)`` are not
+    written.  Slots have to differ: what a slot that two rows name holds
+    afterwards is undefined.
+    """
+    _ops.cuda_paged_kv_append_(*_pool(cache), new_k, new_v, slots, source, counts)
+
+
+def cuda_paged_kv_read(cache, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows of ``slots`` (CUDA int64 ``[B, L]``) of a ``PagedKVCache`` as BF16 K and V ``[B, Hkv, L, D]``.
+
+    Slots outside the pool read as zeros.
+    """
+    return _ops.cuda_paged_kv_read(*_pool(cache), slots)
+
+
+def cuda_paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, *, past_lengths: torch.Tensor,
+                         max_past_length: int, tree_mask: torch.Tensor | None = None,
+                         counts: torch.Tensor | None = None) -> torch.Tensor:
+    """``cuda_tree_attention_cached`` over a ``PagedKVCache``, read through ``block_table`` (CUDA int32 ``[B, M]``).
+
+    Position j of sequence b is row ``j % S`` of page ``block_table[b, j // S]``;
+    token t of q ``[B, T, Hq, D]`` sees positions below P_b (``past_lengths`` CUDA
+    int64 ``[B]``, ``max_past_length`` a host bound on them) and ``P_b + u`` where
+    ``tree_mask[b, t, u]`` (without one ``u <= t``).  Positions whose entry names no
+    page are not seen.  Tokens ``t >= counts[b]`` (CUDA int64 ``[B]``) are padding
+    and give zeros.  T = 1 is single-token decode.
+    """
+    _require_int("max_past_length", max_past_length)
+    return _ops.cuda_paged_attention(q, *_pool(cache), block_table, tree_mask, past_lengths, max_past_length, counts)
+
+
+def cuda_verify_drafted(target_probs: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, *,
+                        draft_probs: torch.Tensor | None = None, parents: torch.Tensor | None = None,
+                        counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Verify trees of drafted tokens; returns ``(path, counts, next_tokens)``, int64 ``[B, T]``, ``[B]``, ``[B]``.
+
+    ``tokens`` int64 ``[B, T]``, parents first (``parents`` int64 ``[T]`` or
+    ``[B, T]``; without them the chain); node 0 is the token that the last step
+    ended with.  ``target_probs`` float32 ``[B, T, V]``: row t is the target's
+    distribution of the token after node t; ``draft_probs``: the one node t's
+    children were drawn from, independently.  Without them the children are given
+    (a search, the likeliest tokens) and only the target's row counts.
+    ``uniforms`` float32 ``[B, T]`` in [0, 1): node t's decides on it, node 0's
+    draws the next token, so the tokens follow the target's distribution and the
+    same numbers give the same result.  At a node with r = its target row and
+    s = 1 the children are tried in order: token x with random number u goes on
+    the path where ``u q(x) s < r(x)``, else r becomes ``max(r - s q, 0)`` and s its
+    sum (FP64; without ``draft_probs`` q is 1 at x and r(x) becomes 0).  The next
+    token is drawn from what is left of r at the path's last node.  ``path`` (-1
+    behind its ``counts`` nodes) is what ``accept_drafted_`` and
+    ``accept_drafted_paged_`` take.  A tree has ``counts[b]`` nodes where that is
+    given; one of none gives counts 0 and token -1.
+    """
+    return _ops.cuda_verify_drafted(target_probs, tokens, uniforms, draft_probs, parents, counts)
+
+
 __all__ = [
     "cuda_apply_rope",
     "cuda_apply_rope_qk",
@@ -188,15 +283,23 @@ __all__ = [
     "cuda_gqa_attention",
     "cuda_gqa_attention_cached",
     "cuda_kv_cache_append_",
+    "cuda_paged_attention",
+    "cuda_paged_kv_append_",
+    "cuda_paged_kv_read",
     "cuda_quantized_kv_append_",
     "cuda_quantized_kv_read",
+    "cuda_release_pages_",
+    "cuda_reserve_pages_",
     "cuda_rms_norm",
     "cuda_tree_attention_cached",
     "cuda_unpack_e2m1_codes",
+    "cuda_verify_drafted",
     "cuda_w4a16_linear",
     "cuda_w4a16_linear_grouped_decode",
     "quantize_nvfp4",
     "rope_frequencies",
     "NVFP4Tensor",
+    "PageTable",
+    "PagedKVCache",
     "QuantizedKVCache",
 ]

@@ -31,6 +31,8 @@ EXPORTED = (
     "nvfp4da_attention_combine", "nvfp4da_w4a16_gemm", "nvfp4da_decoder_attention_forward_hostio",
     "nvfp4da_apply_rope_qk", "nvfp4da_kv_quant_append", "nvfp4da_kv_quant_read",
     "nvfp4da_tree_attention_workspace_size", "nvfp4da_tree_attention", "nvfp4da_tree_attention_sync_status",
+    "nvfp4da_reserve_pages", "nvfp4da_release_pages", "nvfp4da_paged_kv_append", "nvfp4da_paged_kv_read",
+    "nvfp4da_paged_attention_workspace_size", "nvfp4da_paged_attention", "nvfp4da_verify_drafted",
 )
 
 PATH_AUTO, PATH_CHAIN, PATH_STEP = 0, 1, 2
@@ -69,6 +71,11 @@ class KvCache(C.Structure):
                 ("k_block_scales", C.c_void_p), ("v_block_scales", C.c_void_p), ("k_row_scales", C.c_void_p),
                 ("v_row_scales", C.c_void_p), ("batch", C.c_int64), ("kv_heads", C.c_int64),
                 ("capacity", C.c_int64), ("head_dim", C.c_int64)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p), ("free_count", C.c_void_p),
+                ("batch", C.c_int64), ("max_pages", C.c_int64), ("pool", C.c_int64), ("page_size", C.c_int64)]
 
 
 _lib: C.CDLL | None = None
@@ -121,6 +128,16 @@ def load() -> C.CDLL:
         "nvfp4da_tree_attention_workspace_size": (sz, [C.POINTER(KvCache), i64, i64, i64]),
         "nvfp4da_tree_attention": (C.c_int, [vp, C.POINTER(KvCache), vp, i64, vp, i64, i64, i64, vp, i64, vp, sz,
                                              vp]),
+        "nvfp4da_reserve_pages": (C.c_int, [C.POINTER(PageTable), vp, vp, i64, vp, vp, vp]),
+        "nvfp4da_release_pages": (C.c_int, [C.POINTER(PageTable), vp, vp]),
+        "nvfp4da_paged_kv_append": (C.c_int, [C.POINTER(KvCache), vp, C.POINTER(i64), vp, C.POINTER(i64), i64, i64, vp,
+                                              i64, vp, i64, vp, vp]),
+        "nvfp4da_paged_kv_read": (C.c_int, [C.POINTER(KvCache), vp, i64, i64, vp, vp, vp]),
+        "nvfp4da_paged_attention_workspace_size": (sz, [C.POINTER(KvCache), i64, i64, i64, i64, i64]),
+        "nvfp4da_paged_attention": (C.c_int, [vp, C.POINTER(KvCache), vp, i64, i64, vp, i64, vp, i64, i64, vp, i64, vp,
+                                              vp, sz, vp]),
+        "nvfp4da_verify_drafted": (C.c_int, [vp, C.POINTER(i64), vp, C.POINTER(i64), vp, vp, i64, vp, vp, i64, i64,
+                                             i64, vp, vp, vp, vp]),
         "nvfp4da_decoder_attention_forward_hostio": (C.c_int, [C.POINTER(ForwardArgs), vp, vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():

@@ -353,6 +353,91 @@ int nvfp4da_tree_attention(const uint16_t* q, const nvfp4da_kv_cache* cache, con
  * those that have ended. */
 int nvfp4da_tree_attention_sync_status(void* stream, unsigned* flags, int clear);
 
+/* ---- Serving drafted tokens from a paged KV cache (no counterpart in the
+ * reference, whose cache reserves C slots a sequence).  One step:
+ * nvfp4da_reserve_pages, projections and nvfp4da_apply_rope_qk,
+ * nvfp4da_paged_kv_append into the slots it gave, nvfp4da_paged_attention, the O
+ * projection; nvfp4da_verify_drafted, nvfp4da_paged_kv_append of the accepted
+ * path's rows, nvfp4da_release_pages of what the rejected tokens held.
+ *
+ * A pool of N pages is an nvfp4da_kv_cache with batch = N and capacity = S, the
+ * page size: codes [N, Hkv, S, D] and so on.  Slot s is row s % S of page s / S in
+ * every head.  A block table int32 [B, M] names the pages of each sequence in
+ * order; an entry outside [0, N) names none. */
+/* Page sizes are multiples of this. */
+#define NVFP4DA_PAGE_SIZE_MULTIPLE 16
+/* The sequences' pages and the free ones; all in device memory. */
+typedef struct nvfp4da_page_table {
+  int32_t* pages;      /* [B, M]: the block table */
+  int64_t* held;       /* [B]: pages of each sequence */
+  int32_t* free_pages; /* [pool]: a stack */
+  int64_t* free_count; /* [1]: pages on it */
+  int64_t batch, max_pages, pool, page_size;
+} nvfp4da_page_table;
+
+/* Room for tokens P_b .. P_b + n_b - 1 of every sequence, n_b = counts[b] (device
+ * int64 [B], or NULL: T) in [0, T].  Pages that are missing come from the top of
+ * the free stack, sequence by sequence.  slots int64 [B, T]: the slot of token t,
+ * -1 for t >= n_b and where no page is named.  granted int64 [B]: n_b, or 0 for a
+ * sequence that gets nothing: P_b < 0, P_b + n_b > M S, or pages needed when the
+ * needs up to and including its own pass the stack. */
+int nvfp4da_reserve_pages(const nvfp4da_page_table* table, const int64_t* past_lengths, const int64_t* counts,
+                          int64_t tokens, int64_t* slots, int64_t* granted, void* stream);
+/* Sequence b keeps ceil(lengths[b] / S) of its pages (none for a length below 1);
+ * the others go back on the stack, the last sequence's last page first, and their
+ * entries become -1: a release undoes the reserve before it. */
+int nvfp4da_release_pages(const nvfp4da_page_table* table, const int64_t* lengths, void* stream);
+
+/* Rows of new_k, new_v [B, T, Hkv, D] (BF16, by element strides of batch, token
+ * and head) into slots: row i of sequence b, i < rows, is token source[b * rows + i]
+ * (NULL: i, rows = T) and goes to slots[b * slot_stride + i], quantised as the pool
+ * is.  Not written: i >= counts[b] (device int64 [B], optional), slots outside the
+ * pool, tokens outside [0, T).  Slots have to differ: what a slot that two rows name
+ * holds after the call is undefined. */
+int nvfp4da_paged_kv_append(const nvfp4da_kv_cache* pool, const uint16_t* new_k, const int64_t* k_strides,
+                            const uint16_t* new_v, const int64_t* v_strides, int64_t batch, int64_t tokens,
+                            const int64_t* slots, int64_t slot_stride, const int64_t* source, int64_t rows,
+                            const int64_t* counts, void* stream);
+/* The rows of slots [B, length] as BF16 [B, Hkv, length, D]; zeros for slots outside the pool. */
+int nvfp4da_paged_kv_read(const nvfp4da_kv_cache* pool, const int64_t* slots, int64_t batch, int64_t length,
+                          uint16_t* k_out, uint16_t* v_out, void* stream);
+
+/* nvfp4da_tree_attention through a block table [B, M]: position j of sequence b is
+ * row j % S of page block_table[b * M + j / S].  Positions whose entry names no page
+ * are not seen.  counts (device int64 [B], optional): tokens t >= counts[b] are
+ * padding; their context is zeros.  T = 1 is decode.  The flags of
+ * nvfp4da_tree_attention_sync_status are these kernels' too. */
+size_t nvfp4da_paged_attention_workspace_size(const nvfp4da_kv_cache* pool, int64_t batch, int64_t max_pages,
+                                              int64_t tokens, int64_t q_heads, int64_t max_past_length);
+int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* pool, const int32_t* block_table,
+                            int64_t batch, int64_t max_pages, const uint8_t* tree_mask, int64_t mask_batch_stride,
+                            uint16_t* context, int64_t tokens, int64_t q_heads, const int64_t* past_lengths,
+                            int64_t max_past_length, const int64_t* counts, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Verification of trees of drafted tokens.  target, draft: float32 [B, T, V] by
+ * element strides of batch and node (rows contiguous): row t holds the target's
+ * probabilities of the token after node t, and the draft's that node t's children
+ * were drawn from (draft NULL: children given without probabilities).  tokens int64
+ * [B, T]; parents int64 [b * parent_stride + t] < t (NULL: t - 1), node 0 the root;
+ * uniforms float32 [B, T]; counts (device int64 [B], optional): nodes of each tree.
+ * The walk starts at the root.  At a node with r = target row, s = 1 its children
+ * are tried in order: child c with token x goes on the path where
+ * uniforms[c] q(x) s < r(x), q the draft's row (1 without one); else
+ * r = max(r - s q, 0), s = sum r (without a draft r(x) = 0 and s = sum r).  Where
+ * s = 0, r is the target's row again and no further child is tried.
+ * path int64 [B, T]: the accepted nodes from the root on, -1 behind them;
+ * accepted int64 [B]: their number; next_tokens int64 [B]: the first y with
+ * sum_{z <= y} r(z) > uniforms[b, 0] sum r, the last y with r(y) > 0 where none has,
+ * -1 where r has none.  Probabilities that are not positive and finite count as 0; a
+ * child with a token outside [0, V) or a parent outside [0, t) is none; a tree of 0
+ * nodes gives path -1, accepted 0, next token -1.  At most 1,024 nodes. */
+int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, const float* draft,
+                           const int64_t* draft_strides, const int64_t* tokens, const int64_t* parents,
+                           int64_t parent_stride, const float* uniforms, const int64_t* counts, int64_t batch,
+                           int64_t nodes, int64_t vocab, int64_t* path, int64_t* accepted, int64_t* next_tokens,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif
