@@ -8,7 +8,7 @@
 #include "kv_host.cuh"
 #include "rope_positions.cuh"
 #include "tree_attention.cuh"
-#include "tree_stream.cuh"
+#include "tree_launch.cuh"
 #include "tree_tc.cuh"
 
 namespace nvfp4da {
@@ -39,13 +39,6 @@ struct TreePlan {
   size_t bytes;
 };
 
-constexpr int kTsWarps = 8;
-// 16-position slices a warp takes at once: two hide the latency of decoding
-// codes (E4M3 87 -> 77 us, NVFP4 93 -> 81 us on 8 x 32K positions); BF16 has
-// none to hide.
-template <int D, int FMT, int NG>
-constexpr int ts_slices() { return FMT != kKvFmtBf16 && NG == 1 && D <= 128 ? 2 : 1; }
-
 // Query rows per KV head from which tree_tc_kernel runs.  The streaming kernel
 // decodes codes in registers for the rows of one warp, this one once for all
 // rows.  Both, 8 sequences x 6 KV heads x 4 query heads each, us streaming /
@@ -61,23 +54,6 @@ constexpr int ts_slices() { return FMT != kKvFmtBf16 && NG == 1 && D <= 128 ? 2 
 //   E4M3   20/23  23/29  45/65      21/24  30/30  62/66      21/24  33/30  66/67      29/25  52/32  106/73
 //   NVFP4  20/24  23/30  43/68      20/24  30/31  61/70      21/25  34/31  64/71      29/26  52/32  107/76
 constexpr int64_t tc_min_rows(int64_t head_dim, bool bf16) { return head_dim == 64 ? 33 : bf16 ? 13 : 9; }
-
-// Rows from which, and parts a unit has at most (CTAs per unit), where a warp
-// joins four rows instead of one: 192 rows over BF16 (16 sequences, 8,000
-// positions) 146 -> 141 us in all, 64 rows over NVFP4 (8, 32,000) 159 -> 155;
-// with 12 parts a unit the few warps take longer (41 -> 42 us).
-constexpr int64_t kJoin4MinRows = 17, kJoin4MaxParts = 8;
-
-template <int D>
-cudaError_t launch_tree_combine(const TreeStreamParams& p, cudaStream_t s) {
-  const int64_t rows = std::min(p.rows_per_pass, p.group * p.tokens);
-  const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * p.passes;
-  const bool four = rows >= kJoin4MinRows && units * kJoin4MaxParts >= p.grid;
-  const dim3 grid(static_cast<unsigned>(2 * p.grid),
-                  static_cast<unsigned>(ceil_div(rows, four ? kTsJoinWarps * kTsJoinRows : kTsJoinWarps)));
-  return launch(four ? tree_stream_combine4_kernel<D> : tree_stream_combine_kernel<D>, grid, dim3(kTsJoinWarps * 32), 0,
-                s, true, p);
-}
 
 template <int D, int FMT, bool SPLIT>
 cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p, cudaStream_t s) {
@@ -96,48 +72,12 @@ cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const T
   return e != cudaSuccess ? e : launch_tree_combine<D>(p, s);
 }
 
-template <int D, int FMT, int NG>
-cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p,
-                               cudaStream_t s) {
-  constexpr int SL = ts_slices<D, FMT, NG>(), NW = kTsWarps;
-  auto* kern = tree_stream_kernel<D, FMT, NG, NW, SL>;
-  const uint32_t smem = TsCfg<D, FMT, NG, NW, SL>::bytes(p.batch);
-  cudaError_t e = ensure_smem(kern, smem);
-  if (e != cudaSuccess) return e;
-  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(TsCfg<D, FMT, NG, NW, SL>::kThreads), smem, s, true, tk, tv, p);
-  return e != cudaSuccess ? e : launch_tree_combine<D>(p, s);
-}
-
 template <int FMT>
 cudaError_t launch_tree_tc_d(int64_t head_dim, bool split, const CUtensorMap& tk, const CUtensorMap& tv,
                              const TreeStreamParams& p, cudaStream_t s) {
   if (head_dim == 64)
     return split ? launch_tree_tc<64, FMT, true>(tk, tv, p, s) : launch_tree_tc<64, FMT, false>(tk, tv, p, s);
   return split ? launch_tree_tc<128, FMT, true>(tk, tv, p, s) : launch_tree_tc<128, FMT, false>(tk, tv, p, s);
-}
-
-template <int FMT>
-cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& tk, const CUtensorMap& tv,
-                                 const TreeStreamParams& p, cudaStream_t s) {
-  switch (head_dim) {
-    case 64: return wide == 2 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
-    case 128:
-      if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
-        if (wide == 2) return launch_tree_stream<128, FMT, 2>(tk, tv, p, s);
-      return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
-    default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
-  }
-}
-
-// The tensor map of K or V: BF16 rows in 64-element boxes, codes as 128-byte lines.
-bool tree_map(CUtensorMap* map, const nvfp4da_kv_cache& c, const void* base, int64_t tile) {
-  const uint64_t rows = static_cast<uint64_t>(c.batch * c.kv_heads * c.capacity), d = c.head_dim;
-  if (c.format == NVFP4DA_KV_BF16)
-    return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, d, rows, d * 2, 64, static_cast<uint32_t>(tile),
-                       CU_TENSOR_MAP_SWIZZLE_128B);
-  const uint64_t bytes = c.format == NVFP4DA_KV_E4M3 ? d : d / 2;
-  return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 128, rows * bytes / 128, 128, 128,
-                     static_cast<uint32_t>(tile * bytes / 128), CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 __global__ void tree_status_kernel(unsigned* flags, int clear) {
@@ -452,6 +392,7 @@ int nvfp4da_tree_attention_sync_status(void* stream, unsigned* flags, int clear)
   if (e != cudaSuccess) return cuda_fail(e, "tree attention status read");
   tree_status_kernel<<<1, 1, 0, s>>>(word, clear);
   e = cudaGetLastError();
+  if (e == cudaSuccess) e = paged_attention_flags(word, clear, s);
   if (e == cudaSuccess) e = cudaMemcpyAsync(flags, word, sizeof(unsigned), cudaMemcpyDeviceToHost, s);
   const cudaError_t freed = cudaFreeAsync(word, s);
   if (e == cudaSuccess) e = freed;

@@ -10,6 +10,7 @@
 #include "page_table.cuh"
 #include "paged_kv.cuh"
 #include "tree_attention.cuh"
+#include "tree_launch.cuh"
 #include "verify_drafted.cuh"
 
 namespace nvfp4da {
@@ -41,7 +42,9 @@ int check_table(const nvfp4da_page_table* t, PageTableParams& p) {
 
 // Plan of the paged attention.
 struct PagedPlan {
-  int splits;
+  bool stream;  // tree_stream_kernel, else the general kernel
+  int wide, row_chunks, rows_per_pass, passes, box;
+  int splits;   // general kernel
   int64_t split_len;
   size_t bytes;
 };
@@ -68,7 +71,26 @@ int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int6
   const int64_t group = q_heads / c->kv_heads;
   if (!product_within(group, tokens, 65535) || !product_within(batch * q_heads, tokens, kI32Max))
     return fail(NVFP4DA_ERR_UNSUPPORTED, "too many query rows: (Hq/Hkv)*T must be at most 65535 and B*T*Hq below 2^31");
-  const int64_t visible = max_past + tokens;
+  const int64_t visible = max_past + tokens, d = c->head_dim, nq = group * tokens;
+  // The streaming kernel: tensor-core tiles for these head dimensions; the tile
+  // line, the pool's 128-byte lines and the prefix of the batch have to fit.
+  const int64_t tile = c->format == NVFP4DA_KV_BF16 ? kTsTile<kKvFmtBf16> : kTsTile<kKvFmtE4m3>;
+  pl.stream = (d == 64 || d == 128 || d == 256) && batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
+              product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
+  if (pl.stream) {
+    pl.wide = nq > 8 && (d == 64 || (d == 128 && c->format == NVFP4DA_KV_BF16)) ? 2 : 1;
+    pl.row_chunks = 1;
+    while (pl.row_chunks < kTsWarps && 8 * pl.wide * pl.row_chunks < nq) pl.row_chunks *= 2;
+    pl.rows_per_pass = 8 * pl.wide * pl.row_chunks;
+    pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
+    pl.box = static_cast<int>(std::min(tile, c->capacity & -c->capacity));
+    // Tiles and their order are 32-bit in the kernel.
+    pl.stream = product_within(batch * c->kv_heads * ceil_div(capacity, tile), pl.passes, kI32Max);
+  }
+  if (pl.stream) {
+    pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * (pl.rows_per_pass * (d * 4 + 8) + 16), 256);
+    return NVFP4DA_OK;
+  }
   const int64_t base = batch * c->kv_heads * ceil_div(group * tokens, kTreeWarps);
   int64_t splits = std::min(ceil_div(8LL * sm_count(), base), ceil_div(visible, 128));
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, 1024));
@@ -79,7 +101,17 @@ int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int6
   return NVFP4DA_OK;
 }
 
+__global__ void paged_status_kernel(unsigned* flags, int clear) {
+  *flags |= clear ? atomicExch(&g_tree_errors, 0u) : atomicOr(&g_tree_errors, 0u);
+}
+
 }  // namespace
+
+cudaError_t paged_attention_flags(unsigned* flags, int clear, cudaStream_t s) {
+  paged_status_kernel<<<1, 1, 0, s>>>(flags, clear);
+  return cudaGetLastError();
+}
+
 }  // namespace nvfp4da
 
 using namespace nvfp4da;
@@ -214,15 +246,52 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "paged attention: NULL pointer");
   if (!aligned(q, 16) || !aligned(context, 16))
     return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "attention tensors must be 16-byte aligned");
-  const bool needs_ws = pl.splits > 1;
+  const bool needs_ws = pl.stream || pl.splits > 1;
   if (needs_ws && (!ws || ws_bytes < pl.bytes))
     return fail(NVFP4DA_ERR_WORKSPACE, "paged attention workspace too small (%zu < %zu bytes)", ws ? ws_bytes : size_t(0),
                 pl.bytes);
   if (needs_ws && !aligned(ws, 16))
     return fail(NVFP4DA_ERR_WORKSPACE, "the paged attention workspace must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const PagedView pg = {block_table, static_cast<int>(c->batch), static_cast<int>(max_pages),
+                        static_cast<int>(c->capacity), counts};
+  if (pl.stream) {
+    CUtensorMap tk, tv;
+    if (!tree_map(&tk, *c, c->k_codes, pl.box) || !tree_map(&tv, *c, c->v_codes, pl.box))
+      return fail(NVFP4DA_ERR_CUDA, "tensor map encoding failed for the paged attention");
+    TreeStreamParams t{};
+    t.q = q;
+    t.k = k_store(*c);
+    t.v = v_store(*c);
+    t.mask = tree_mask;
+    t.mask_stride = mask_batch_stride;
+    t.ctx = context;
+    t.batch = static_cast<int>(batch);
+    t.tokens = static_cast<int>(tokens);
+    t.q_heads = static_cast<int>(q_heads);
+    t.kv_heads = static_cast<int>(c->kv_heads);
+    t.group = static_cast<int>(q_heads / c->kv_heads);
+    t.capacity = max_pages * c->capacity;
+    t.past_lengths = past_lengths;
+    t.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c->head_dim)));
+    t.row_chunks = pl.row_chunks;
+    t.rows_per_pass = pl.rows_per_pass;
+    t.passes = pl.passes;
+    t.grid = sm_count();
+    t.part_slots = static_cast<int4*>(ws);
+    t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
+    t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
+    t.pg = pg;
+    t.box = pl.box;
+    cudaError_t e = c->format == NVFP4DA_KV_BF16
+                        ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, pl.wide, tk, tv, t, s)
+                    : c->format == NVFP4DA_KV_E4M3
+                        ? launch_tree_stream_d<kKvFmtE4m3, true>(c->head_dim, pl.wide, tk, tv, t, s)
+                        : launch_tree_stream_d<kKvFmtNvfp4, true>(c->head_dim, pl.wide, tk, tv, t, s);
+    return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "streaming paged attention launch");
+  }
   TreeAttnParams p{};
-  p.pg = {block_table, static_cast<int>(c->batch), static_cast<int>(max_pages), static_cast<int>(c->capacity), counts};
+  p.pg = pg;
   p.q = q;
   p.k = k_store(*c);
   p.v = v_store(*c);

@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kTreeWarps * 32) tree_attn_general_kernel(cons
   const int64_t past = tree_past(p.past_lengths, p.past_length, b, p.capacity);
   int tokens = p.tokens;
   if constexpr (PAGED) tokens = paged_count(p.pg, b, p.tokens);
-  const int64_t end = min(past + tokens, p.capacity);
+  const int64_t end = PAGED && tokens == 0 ? 0 : min(past + tokens, p.capacity);
   const int64_t j0 = blockIdx.x * p.split_len, j1 = min(j0 + p.split_len, end);
   const uint8_t* mask_row = p.mask ? p.mask + b * p.mask_stride + static_cast<int64_t>(t) * p.tokens : nullptr;
   const int64_t out_row = (static_cast<int64_t>(b) * p.tokens + t) * p.q_heads + h;

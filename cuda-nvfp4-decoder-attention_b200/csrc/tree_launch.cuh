@@ -1,0 +1,78 @@
+// Launches of the streaming tree attention and its joins, over caches of whole
+// sequences and (PAGED) over pools of pages.
+#pragma once
+
+#include "kv_host.cuh"
+#include "tree_stream.cuh"
+
+namespace nvfp4da {
+
+// Adds (or moves, with `clear`) the flags of the paged attention's waits to *flags (paged_capi.cu).
+__attribute__((visibility("hidden"))) cudaError_t paged_attention_flags(unsigned* flags, int clear, cudaStream_t s);
+
+namespace {
+
+constexpr int kTsWarps = 8;
+// 16-position slices a warp takes at once: two hide the latency of decoding
+// codes (E4M3 87 -> 77 us, NVFP4 93 -> 81 us on 8 x 32K positions); BF16 has
+// none to hide.
+template <int D, int FMT, int NG>
+constexpr int ts_slices() { return FMT != kKvFmtBf16 && NG == 1 && D <= 128 ? 2 : 1; }
+
+// Rows from which, and parts a unit has at most (CTAs per unit), where a warp
+// joins four rows instead of one: 192 rows over BF16 (16 sequences, 8,000
+// positions) 146 -> 141 us in all, 64 rows over NVFP4 (8, 32,000) 159 -> 155;
+// with 12 parts a unit the few warps take longer (41 -> 42 us).
+constexpr int64_t kJoin4MinRows = 17, kJoin4MaxParts = 8;
+
+template <int D, bool PAGED = false>
+cudaError_t launch_tree_combine(const TreeStreamParams& p, cudaStream_t s) {
+  const int64_t rows = std::min(p.rows_per_pass, p.group * p.tokens);
+  const int64_t units = static_cast<int64_t>(p.batch) * p.kv_heads * p.passes;
+  const bool four = rows >= kJoin4MinRows && units * kJoin4MaxParts >= p.grid;
+  const dim3 grid(static_cast<unsigned>(2 * p.grid),
+                  static_cast<unsigned>(ceil_div(rows, four ? kTsJoinWarps * kTsJoinRows : kTsJoinWarps)));
+  return launch(four ? tree_stream_combine4_kernel<D, PAGED> : tree_stream_combine_kernel<D, PAGED>, grid,
+                dim3(kTsJoinWarps * 32), 0, s, true, p);
+}
+
+template <int D, int FMT, int NG, bool PAGED = false>
+cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p,
+                               cudaStream_t s) {
+  constexpr int SL = ts_slices<D, FMT, NG>(), NW = kTsWarps;
+  auto* kern = tree_stream_kernel<D, FMT, NG, NW, SL, PAGED>;
+  const uint32_t smem = TsCfg<D, FMT, NG, NW, SL>::bytes(p.batch);
+  cudaError_t e = ensure_smem(kern, smem);
+  if (e != cudaSuccess) return e;
+  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(TsCfg<D, FMT, NG, NW, SL>::kThreads), smem, s, true, tk, tv, p);
+  return e != cudaSuccess ? e : launch_tree_combine<D, PAGED>(p, s);
+}
+
+template <int FMT, bool PAGED = false>
+cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& tk, const CUtensorMap& tv,
+                                 const TreeStreamParams& p, cudaStream_t s) {
+  switch (head_dim) {
+    case 64:
+      return wide == 2 ? launch_tree_stream<64, FMT, 2, PAGED>(tk, tv, p, s)
+                       : launch_tree_stream<64, FMT, 1, PAGED>(tk, tv, p, s);
+    case 128:
+      if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
+        if (wide == 2) return launch_tree_stream<128, FMT, 2, PAGED>(tk, tv, p, s);
+      return launch_tree_stream<128, FMT, 1, PAGED>(tk, tv, p, s);
+    default: return launch_tree_stream<256, FMT, 1, PAGED>(tk, tv, p, s);
+  }
+}
+
+// The tensor map of K or V: BF16 rows in 64-element boxes, codes as 128-byte lines.
+bool tree_map(CUtensorMap* map, const nvfp4da_kv_cache& c, const void* base, int64_t tile) {
+  const uint64_t rows = static_cast<uint64_t>(c.batch * c.kv_heads * c.capacity), d = c.head_dim;
+  if (c.format == NVFP4DA_KV_BF16)
+    return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, d, rows, d * 2, 64, static_cast<uint32_t>(tile),
+                       CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t bytes = c.format == NVFP4DA_KV_E4M3 ? d : d / 2;
+  return make_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 128, rows * bytes / 128, 128, 128,
+                     static_cast<uint32_t>(tile * bytes / 128), CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+}  // namespace
+}  // namespace nvfp4da

@@ -70,6 +70,7 @@
 
 #include "common.cuh"
 #include "kv_quant.cuh"
+#include "paged_kv.cuh"
 #include "tree_attention.cuh"
 
 namespace nvfp4da {
@@ -143,6 +144,8 @@ struct TreeStreamParams {
   float* part_o;       // [2 grid][RP][D]: slots 2 CTA (its first segment) and 2 CTA + 1 (its last)
   float2* part_ml;     // [2 grid][RP]
   int4* part_slots;    // [2 grid]: see ts_write_slot
+  PagedView pg;        // PAGED: the block table; the stores are a pool's, capacity = M * S
+  int box;             // PAGED: positions that one copy brings, a power of two >= 16 that divides the page and the tile
 };
 
 // ---------------------------------------------------------------- PTX
@@ -330,8 +333,17 @@ struct TsWalk {
 __device__ __forceinline__ int ts_past(const TreeStreamParams& p, int b) {
   return static_cast<int>(tree_past(p.past_lengths, p.past_length, b, p.capacity));
 }
+// Tokens of sequence b that are no padding.
+template <bool PAGED>
+__device__ __forceinline__ int ts_tokens(const TreeStreamParams& p, int b) {
+  if constexpr (PAGED) return paged_count(p.pg, b, p.tokens);
+  return p.tokens;
+}
+template <bool PAGED = false>
 __device__ __forceinline__ int ts_visible(const TreeStreamParams& p, int b) {
-  return static_cast<int>(min(static_cast<int64_t>(ts_past(p, b)) + p.tokens, p.capacity));
+  const int tokens = ts_tokens<PAGED>(p, b);
+  if (PAGED && tokens == 0) return 0;
+  return static_cast<int>(min(static_cast<int64_t>(ts_past(p, b)) + tokens, p.capacity));
 }
 
 // First tile of CTA c of g over n tiles.
@@ -340,9 +352,13 @@ __device__ __forceinline__ int ts_first_tile(int n, int c, int g) {
 }
 
 // The tiles before every sequence, into prefix[0 .. B]; all threads of the block.
+template <bool PAGED = false>
 __device__ __forceinline__ void ts_prefix(const TreeStreamParams& p, int units, int tile, int* prefix) {
-  for (int b = threadIdx.x; b < p.batch; b += blockDim.x)
-    prefix[b + 1] = (ts_visible(p, b) + tile - 1) / tile * units;
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+    int tiles = (ts_visible<PAGED>(p, b) + tile - 1) / tile;
+    if constexpr (PAGED) tiles = max(tiles, 1);  // a sequence of nothing but padding: one that nobody sees
+    prefix[b + 1] = tiles * units;
+  }
   __syncthreads();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
@@ -418,8 +434,73 @@ __device__ __forceinline__ void ts_load_scales(uint8_t* st, const TreeStreamPara
   }
 }
 
+// ---------------------------------------------------------------- tiles of a paged cache
+// Where a tile's boxes (p.box positions each) stand.  A lane looks up one box:
+// 32 / boxes tiles at a time, the next ones while these are fetched, so that the
+// table's latency is not in the way of the copies.
+template <int TILE>
+struct TsBoxes {
+  int boxes, tiles;    // per tile; tiles that 32 lanes hold
+  int cur, next, t0;   // this lane's box of tiles t0 .. and of those behind them: its first row of the pool, -1: none
+  int b, kvh, vis, t_end;
+  __device__ int look(const TreeStreamParams& p, int t, int lane) const {
+    const int pos = (t + lane / boxes) * TILE + lane % boxes * p.box;
+    if (pos >= vis || t + lane / boxes >= t_end) return -1;
+    const int page = paged_page(p.pg, b, pos);
+    return page < 0 ? -1 : (page * p.kv_heads + kvh) * p.pg.page_size + pos % p.pg.page_size;
+  }
+  __device__ void begin(const TreeStreamParams& p, int b_, int kvh_, int t, int t1, int lane) {
+    boxes = TILE / p.box;
+    tiles = 32 / boxes;
+    b = b_;
+    kvh = kvh_;
+    vis = ts_visible<true>(p, b);
+    t0 = t;
+    t_end = t1;
+    cur = look(p, t, lane);
+    next = look(p, t + tiles, lane);
+  }
+  // For tile t (in order): the row of box `i`; all lanes.
+  __device__ void advance(const TreeStreamParams& p, int t, int lane) {
+    if (t < t0 + tiles) return;
+    t0 += tiles;
+    cur = next;
+    next = look(p, t0 + tiles, lane);
+  }
+  __device__ int row(int t, int i) const { return __shfl_sync(kFull, cur, (t - t0) * boxes + (i & (boxes - 1))); }
+};
+
+// ts_load_scales for a tile whose boxes stand apart.
+template <int D, int FMT, typename Cfg, int TILE>
+__device__ __forceinline__ void ts_load_scales_paged(uint8_t* st, const TreeStreamParams& p, const TsBoxes<TILE>& at,
+                                                     int t, int lane) {
+  if constexpr (FMT == kKvFmtNvfp4) {
+#pragma unroll
+    for (uint32_t i = 0; i < Cfg::kBlockScales; i += 512) {
+      const uint32_t o = i + lane * 16;
+      const int r = o / (D / 16), row = at.row(t, r / p.box);
+      if (o < Cfg::kBlockScales && row >= 0) {
+        const int64_t from = static_cast<int64_t>(row + r % p.box) * (D / 16);
+        ts_copy16(st + Cfg::kOffKb + o, p.k.block_scales + from);
+        ts_copy16(st + Cfg::kOffVb + o, p.v.block_scales + from);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TILE; i += 128) {
+    const int r = i + lane * 4, row = at.row(t, r / p.box);
+    if (r < TILE && row >= 0) {
+      ts_copy16(st + Cfg::kOffKr + r * 4, p.k.row_scales + row + r % p.box);
+      ts_copy16(st + Cfg::kOffVr + r * 4, p.v.row_scales + row + r % p.box);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- the streaming kernel
-template <int D, int FMT, int NG, int NW, int SL>
+// PAGED: a tile comes in boxes, each from its own page, to the places that a whole
+// tile's copy would bring it; 16-position slices of pages that are not there (their
+// boxes come in as zeros) are left out.
+template <int D, int FMT, int NG, int NW, int SL, bool PAGED = false>
 __global__ void __launch_bounds__((NW + 4) * 32, 1)
     tree_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const TreeStreamParams p) {
@@ -448,6 +529,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   uint64_t* join_free = join_full + Cfg::kJoins;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::kOffPrefix);
   __shared__ volatile unsigned s_bad;  // a wait gave up
+  [[maybe_unused]] __shared__ unsigned s_absent[PAGED ? Cfg::kStages : 1];  // slices of a stage that are not there
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
@@ -474,7 +556,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   }
   // Nothing of global memory before this: the launch may overlap the kernel ahead.
   pdl_wait();
-  ts_prefix(p, units, kTsTile<FMT>, prefix);
+  ts_prefix<PAGED>(p, units, kTsTile<FMT>, prefix);
   const int n_tiles = prefix[p.batch];
   // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
   // every CTA between a unit's first and last holds one of its tiles.
@@ -493,6 +575,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     for (; more; more = w.next()) {
       const int pass = w.u % p.passes, kvh = w.u / p.passes, n_first = pass * p.rows_per_pass;
       const int rows = min(p.rows_per_pass, nq - n_first);
+      [[maybe_unused]] const int tokens = ts_tokens<PAGED>(p, w.b);
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
       if (!whole && warp == NW + 2 && lane == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
@@ -507,6 +590,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
         const float fu = mu == -INFINITY ? (lu == 0.0f ? 0.0f : 1.0f) : ts_exp2(mu - mx);
         const float l = warp_sum_f32(lu * fu), inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
         const int n = n_first + r;
+        [[maybe_unused]] const bool padding = PAGED && n / p.group >= tokens;
         const int64_t out = static_cast<int64_t>((w.b * p.tokens + n / p.group) * p.q_heads + kvh * p.group + n % p.group) * D;
 #pragma unroll
         for (int e = 2 * lane; e < D; e += 64) {
@@ -518,7 +602,8 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             o.y = f == 0.0f ? o.y : fmaf(v.y, f, o.y);
           }
           if (whole)
-            *reinterpret_cast<uint32_t*>(p.ctx + out + e) = l == 0.0f ? 0u : ts_pack_bf16(o.x * inv, o.y * inv);
+            *reinterpret_cast<uint32_t*>(p.ctx + out + e) =
+                l == 0.0f || padding ? 0u : ts_pack_bf16(o.x * inv, o.y * inv);
           else
             *reinterpret_cast<float2*>(p.part_o + (slot * p.rows_per_pass + r) * D + e) = o;
         }
@@ -539,22 +624,51 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     // Scales go by 16-byte copies of a whole warp: a bulk copy takes one thread over a hundred cycles to
     // issue, and four of them per tile held E4M3 and NVFP4 caches at 0.8 and 0.4 of the HBM rate.
     const bool is_v = warp > NW;
-    if (lane != 0 && !(is_v && kQuant)) return;
+    if (!PAGED && lane != 0 && !(is_v && kQuant)) return;
     TsWalk w;
     bool more = w.begin(prefix, p.batch, units, x0, x1);
     int stage = 0;
     uint32_t phase = 0;
     [[maybe_unused]] const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
+    [[maybe_unused]] TsBoxes<kTsTile<FMT>> at;
     int filled = 0;  // stages, from the first tile on
     bool ok = true;
     while (more && ok) {
       const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
+      if constexpr (PAGED) at.begin(p, w.b, w.u / p.passes, w.t0, w.t1, lane);
       for (int t = w.t0; t < w.t1; ++t) {
         ok = filled < Cfg::kStages || ts_wait(&empty[stage], phase ^ 1u, &s_bad);
+        if constexpr (PAGED) ok = __all_sync(kFull, ok);
         if (!ok) break;
         uint8_t* st = smem + stage * Cfg::kStage;
         const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile<FMT>;
-        if (lane == 0) {
+        if constexpr (PAGED) {
+          at.advance(p, t, lane);
+          // Lane i's box, and lane i's 16-position slice.
+          const int mine = at.row(t, lane), of_slice = at.row(t, lane * 16 / p.box);
+          const unsigned absent = __ballot_sync(kFull, lane < kTsTile<FMT> / 16 && of_slice < 0);
+          if (lane == 0) {
+            if (!is_v) s_absent[stage] = absent;
+            mbar_arrive_expect_tx(&full[stage], Cfg::kCodes);
+          }
+          __syncwarp();
+          if (lane < at.boxes) {
+            // Behind the pool's last row: zeros.
+            const int64_t from = mine >= 0 ? mine : static_cast<int64_t>(p.pg.pages) * p.kv_heads * p.pg.page_size;
+            uint8_t* dst = st + (is_v ? Cfg::kOffV : 0);
+            const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+            if constexpr (!kQuant) {
+#pragma unroll
+              for (int bx = 0; bx < D / 64; ++bx)
+                ts_tma_2d(dst + bx * (kTsTile<FMT> * 128) + lane * p.box * 128, map, bx * 64, static_cast<int>(from),
+                          &full[stage]);
+            } else {
+              ts_tma_2d(dst + lane * p.box * Cfg::kRowBytes, map, 0, static_cast<int>(from * Cfg::kRowBytes / 128),
+                        &full[stage]);
+            }
+          }
+          __syncwarp();
+        } else if (lane == 0) {
           uint8_t* dst = st + (is_v ? Cfg::kOffV : 0);
           const CUtensorMap* map = is_v ? &tm_v : &tm_k;
           mbar_arrive_expect_tx(&full[stage], Cfg::kCodes);
@@ -568,7 +682,8 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
         }
         if constexpr (kQuant) {
           if (is_v) {
-            ts_load_scales<D, FMT, Cfg, kTsTile<FMT>>(st, p, row, all_rows, lane);
+            if constexpr (PAGED) ts_load_scales_paged<D, FMT, Cfg, kTsTile<FMT>>(st, p, at, t, lane);
+            else ts_load_scales<D, FMT, Cfg, kTsTile<FMT>>(st, p, row, all_rows, lane);
             ts_copy_arrive(&full[stage]);
           }
         }
@@ -599,7 +714,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   uint32_t phase = 0;
   while (more) {
     const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes;
-    const int past = ts_past(p, b), vis = ts_visible(p, b);
+    const int past = ts_past(p, b), vis = ts_visible<PAGED>(p, b);
     const int n0 = pass * p.rows_per_pass + rc * Cfg::kRows;  // this warp's first query row
     // Query row n = t * group + j; global row of q and ctx:
     auto q_row = [&](int n) -> int64_t {
@@ -668,8 +783,9 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       p_unit[j][0] = p_unit[j][1] = kTsPScale / kTsMinUnit;
     }
 
-    // SL slices of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
-    auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int pos0) {
+    // SL slices of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile); `gone`: those (bits)
+    // whose page is not there.
+    auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int pos0, [[maybe_unused]] unsigned gone) {
       constexpr bool EDGE = decltype(edge_tag)::value;
       const uint8_t *kt = st, *vt = st + Cfg::kOffV;
       // ---- S^T = K Q^T of one slice; score rows: its positions g and 8 + g
@@ -788,6 +904,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
               const int pos = pos0 + 16 * z + g + (i >> 1) * 8, u = pos - past;
               const int t = tok[j][i & 1];
               bool ok = t >= 0 && pos < vis;
+              if constexpr (PAGED) ok &= (gone >> z & 1u) == 0u;
               if (ok && u >= 0)
                 ok = p.mask ? p.mask[b * p.mask_stride + static_cast<int64_t>(t) * p.tokens + u] != 0 : u <= t;
               sees[z][j][i] = ok;
@@ -1063,12 +1180,16 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       if (mine) {
         if (!__all_sync(kFull, ts_wait(&full[stage], phase, &s_bad))) return;
         const uint8_t* st = smem + stage * Cfg::kStage;
+        unsigned absent = 0u;
+        if constexpr (PAGED) absent = s_absent[stage];
         for (int i = 0; i < turns; ++i) {
           const int r0 = (turn0 + i) * 16 * SL;
           const int pos0 = t * kTsTile<FMT> + r0;
           if (pos0 >= vis) break;
-          if (pos0 + 16 * SL <= past) slice(std::false_type{}, st, r0, pos0);
-          else slice(std::true_type{}, st, r0, pos0);
+          const unsigned gone = absent >> (r0 / 16) & ((1u << SL) - 1u);
+          if (PAGED && gone == (1u << SL) - 1u) continue;
+          if (pos0 + 16 * SL <= past && !gone) slice(std::false_type{}, st, r0, pos0, gone);
+          else slice(std::true_type{}, st, r0, pos0, gone);
         }
         __syncwarp();
         if (lane == 0) ts_arrive(&empty[stage]);
@@ -1125,7 +1246,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
 // CTAs share, in CTA order.  Only the slot of the unit's first part has work.
 constexpr int kTsJoinWarps = 8;
 
-template <int D>
+template <int D, bool PAGED = false>
 __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(const TreeStreamParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -1180,10 +1301,11 @@ __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(
   const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
   const int64_t row = (static_cast<int64_t>(b) * p.tokens + n / p.group) * p.q_heads +
                       static_cast<int64_t>(kvh) * p.group + n % p.group;
+  const bool none = l == 0.0f || (PAGED && n / p.group >= ts_tokens<PAGED>(p, b));
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.ctx + row * D + lane * V);
 #pragma unroll
   for (int i = 0; i < V / 2; ++i)
-    dst[i] = l == 0.0f ? 0u : ts_pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
+    dst[i] = none ? 0u : ts_pack_bf16(o[2 * i] * inv, o[2 * i + 1] * inv);
 }
 
 // The same where there are many rows of few parts: a warp joins four rows, eight
@@ -1192,7 +1314,7 @@ __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine_kernel(
 // instructions, which bound the kernel.
 constexpr int kTsJoinRows = 4;
 
-template <int D>
+template <int D, bool PAGED = false>
 __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine4_kernel(const TreeStreamParams p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -1256,8 +1378,8 @@ __global__ void __launch_bounds__(kTsJoinWarps * 32) tree_stream_combine4_kernel
   }
 #pragma unroll
   for (int k = 1; k < 8; k <<= 1) l += __shfl_xor_sync(kFull, l, k);
-  const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
   const int n = pass * p.rows_per_pass + r0 + mine, tok = n / p.group;
+  const float inv = l == 0.0f || (PAGED && tok >= ts_tokens<PAGED>(p, b)) ? 0.0f : __fdiv_rn(1.0f, l);
   const int row = (b * p.tokens + tok) * p.q_heads + kvh * p.group + (n - tok * p.group);  // below 2^31
 #pragma unroll
   for (int i = 0; i < kTsJoinRows; ++i) {
