@@ -282,7 +282,7 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
     t.pg = pg;
-    t.box = pl.box;
+    while (2 << t.box_log2 <= pl.box) ++t.box_log2;
     cudaError_t e = c->format == NVFP4DA_KV_BF16
                         ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, pl.wide, tk, tv, t, s)
                     : c->format == NVFP4DA_KV_E4M3

@@ -145,7 +145,7 @@ struct TreeStreamParams {
   float2* part_ml;     // [2 grid][RP]
   int4* part_slots;    // [2 grid]: see ts_write_slot
   PagedView pg;        // PAGED: the block table; the stores are a pool's, capacity = M * S
-  int box;             // PAGED: positions that one copy brings, a power of two >= 16 that divides the page and the tile
+  int box_log2;        // PAGED: positions that one copy brings, a power of two >= 16 that divides the page and the tile
 };
 
 // ---------------------------------------------------------------- PTX
@@ -435,23 +435,24 @@ __device__ __forceinline__ void ts_load_scales(uint8_t* st, const TreeStreamPara
 }
 
 // ---------------------------------------------------------------- tiles of a paged cache
-// Where a tile's boxes (p.box positions each) stand.  A lane looks up one box:
+// Where a tile's boxes (2^box_log2 positions each) stand.  A lane looks up one box:
 // 32 / boxes tiles at a time, the next ones while these are fetched, so that the
 // table's latency is not in the way of the copies.
 template <int TILE>
 struct TsBoxes {
-  int boxes, tiles;    // per tile; tiles that 32 lanes hold
+  int box_log2, per_log2, tiles;  // of a box's positions, a tile's boxes; tiles that 32 lanes hold
   int cur, next, t0;   // this lane's box of tiles t0 .. and of those behind them: its first row of the pool, -1: none
   int b, kvh, vis, t_end;
   __device__ int look(const TreeStreamParams& p, int t, int lane) const {
-    const int pos = (t + lane / boxes) * TILE + lane % boxes * p.box;
-    if (pos >= vis || t + lane / boxes >= t_end) return -1;
+    const int pos = t * TILE + (lane << box_log2), of = t + (lane >> per_log2);
+    if (pos >= vis || of >= t_end) return -1;
     const int page = paged_page(p.pg, b, pos);
     return page < 0 ? -1 : (page * p.kv_heads + kvh) * p.pg.page_size + pos % p.pg.page_size;
   }
   __device__ void begin(const TreeStreamParams& p, int b_, int kvh_, int t, int t1, int lane) {
-    boxes = TILE / p.box;
-    tiles = 32 / boxes;
+    box_log2 = p.box_log2;
+    per_log2 = (TILE == 64 ? 6 : 7) - box_log2;
+    tiles = 32 >> per_log2;
     b = b_;
     kvh = kvh_;
     vis = ts_visible<true>(p, b);
@@ -460,39 +461,35 @@ struct TsBoxes {
     cur = look(p, t, lane);
     next = look(p, t + tiles, lane);
   }
-  // For tile t (in order): the row of box `i`; all lanes.
+  // For tile t, in order; all lanes.
   __device__ void advance(const TreeStreamParams& p, int t, int lane) {
     if (t < t0 + tiles) return;
     t0 += tiles;
     cur = next;
     next = look(p, t0 + tiles, lane);
   }
-  __device__ int row(int t, int i) const { return __shfl_sync(kFull, cur, (t - t0) * boxes + (i & (boxes - 1))); }
+  // The first row of position r's box (r modulo the tile); all lanes.
+  __device__ int row(int t, int r) const { return __shfl_sync(kFull, cur, ((t - t0) << per_log2) + ((r & (TILE - 1)) >> box_log2)); }
 };
 
-// ts_load_scales for a tile whose boxes stand apart.
+// ts_load_scales of K or of V (`from`, to `blocks` and `rows`) for a tile whose boxes stand apart.
 template <int D, int FMT, typename Cfg, int TILE>
-__device__ __forceinline__ void ts_load_scales_paged(uint8_t* st, const TreeStreamParams& p, const TsBoxes<TILE>& at,
-                                                     int t, int lane) {
+__device__ __forceinline__ void ts_load_scales_paged(uint8_t* blocks, uint8_t* rows, const KvStore& from,
+                                                     const TsBoxes<TILE>& at, int t, int lane) {
+  const int in_box = (1 << at.box_log2) - 1;
   if constexpr (FMT == kKvFmtNvfp4) {
 #pragma unroll
     for (uint32_t i = 0; i < Cfg::kBlockScales; i += 512) {
       const uint32_t o = i + lane * 16;
-      const int r = o / (D / 16), row = at.row(t, r / p.box);
-      if (o < Cfg::kBlockScales && row >= 0) {
-        const int64_t from = static_cast<int64_t>(row + r % p.box) * (D / 16);
-        ts_copy16(st + Cfg::kOffKb + o, p.k.block_scales + from);
-        ts_copy16(st + Cfg::kOffVb + o, p.v.block_scales + from);
-      }
+      const int r = o / (D / 16), row = at.row(t, r);
+      if (o < Cfg::kBlockScales && row >= 0)
+        ts_copy16(blocks + o, from.block_scales + static_cast<int64_t>(row + (r & in_box)) * (D / 16));
     }
   }
 #pragma unroll
   for (int i = 0; i < TILE; i += 128) {
-    const int r = i + lane * 4, row = at.row(t, r / p.box);
-    if (r < TILE && row >= 0) {
-      ts_copy16(st + Cfg::kOffKr + r * 4, p.k.row_scales + row + r % p.box);
-      ts_copy16(st + Cfg::kOffVr + r * 4, p.v.row_scales + row + r % p.box);
-    }
+    const int r = i + lane * 4, row = at.row(t, r);
+    if (r < TILE && row >= 0) ts_copy16(rows + r * 4, from.row_scales + row + (r & in_box));
   }
 }
 
@@ -542,7 +539,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   pdl_launch_dependents();  // the join waits for this kernel's memory itself
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(&full[s], kQuant ? 34 : 2);  // K's and V's bytes, and the lanes that copy scales
+      mbar_init(&full[s], !kQuant ? 2 : PAGED ? 66 : 34);  // K's and V's bytes, and the lanes that copy scales
       mbar_init(&empty[s], pw_n >= kTurns ? kTurns * rc_n : NW);
     }
     for (int i = 0; i < Cfg::kJoins; ++i) {
@@ -645,25 +642,24 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
         if constexpr (PAGED) {
           at.advance(p, t, lane);
           // Lane i's box, and lane i's 16-position slice.
-          const int mine = at.row(t, lane), of_slice = at.row(t, lane * 16 / p.box);
+          const int mine = at.row(t, lane << p.box_log2), of_slice = at.row(t, lane * 16);
           const unsigned absent = __ballot_sync(kFull, lane < kTsTile<FMT> / 16 && of_slice < 0);
           if (lane == 0) {
             if (!is_v) s_absent[stage] = absent;
             mbar_arrive_expect_tx(&full[stage], Cfg::kCodes);
           }
           __syncwarp();
-          if (lane < at.boxes) {
+          if (lane < 1 << at.per_log2) {
             // Behind the pool's last row: zeros.
-            const int64_t from = mine >= 0 ? mine : static_cast<int64_t>(p.pg.pages) * p.kv_heads * p.pg.page_size;
+            const int from = mine >= 0 ? mine : p.pg.pages * p.kv_heads * p.pg.page_size;
             uint8_t* dst = st + (is_v ? Cfg::kOffV : 0);
             const CUtensorMap* map = is_v ? &tm_v : &tm_k;
             if constexpr (!kQuant) {
 #pragma unroll
               for (int bx = 0; bx < D / 64; ++bx)
-                ts_tma_2d(dst + bx * (kTsTile<FMT> * 128) + lane * p.box * 128, map, bx * 64, static_cast<int>(from),
-                          &full[stage]);
-            } else {
-              ts_tma_2d(dst + lane * p.box * Cfg::kRowBytes, map, 0, static_cast<int>(from * Cfg::kRowBytes / 128),
+                ts_tma_2d(dst + bx * (kTsTile<FMT> * 128) + (lane << p.box_log2) * 128, map, bx * 64, from, &full[stage]);
+            } else {  // rows stand in groups of 16
+              ts_tma_2d(dst + (lane << p.box_log2) * Cfg::kRowBytes, map, 0, from / 16 * (16 * Cfg::kRowBytes / 128),
                         &full[stage]);
             }
           }
@@ -680,10 +676,14 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             ts_tma_2d(dst, map, 0, static_cast<int>(row * Cfg::kRowBytes / 128), &full[stage]);
           }
         }
-        if constexpr (kQuant) {
+        if constexpr (kQuant && PAGED) {
+          ts_load_scales_paged<D, FMT, Cfg, kTsTile<FMT>>(st + (is_v ? Cfg::kOffVb : Cfg::kOffKb),
+                                                          st + (is_v ? Cfg::kOffVr : Cfg::kOffKr), is_v ? p.v : p.k, at, t,
+                                                          lane);
+          ts_copy_arrive(&full[stage]);
+        } else if constexpr (kQuant) {
           if (is_v) {
-            if constexpr (PAGED) ts_load_scales_paged<D, FMT, Cfg, kTsTile<FMT>>(st, p, at, t, lane);
-            else ts_load_scales<D, FMT, Cfg, kTsTile<FMT>>(st, p, row, all_rows, lane);
+            ts_load_scales<D, FMT, Cfg, kTsTile<FMT>>(st, p, row, all_rows, lane);
             ts_copy_arrive(&full[stage]);
           }
         }
