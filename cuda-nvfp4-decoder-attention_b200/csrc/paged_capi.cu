@@ -359,11 +359,19 @@ int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, c
   p.path = path;
   p.accepted = accepted;
   p.next = next_tokens;
-  const unsigned ctas = 1;
-  cudaError_t e = ensure_smem(verify_drafted_kernel, static_cast<uint32_t>(verify_smem(p.nodes)));
+  p.pieces = static_cast<int>(ceil_div(ceil_div(vocab, kVerifyPiece), kVerifyMaxSegments));
+  p.segments = static_cast<int>(ceil_div(vocab, static_cast<int64_t>(kVerifyPiece) * p.pieces));
+  // CTAs a sequence, a power of two: as many as have a segment for every warp and as fit the GPU two to an SM with
+  // the rest of the batch.  us for 1, 2, 4, 8 CTAs: one sequence of 128,000 tokens 37, 27, 20, 16; 8 of them 74, 46,
+  // 33, 25; 64 of them 105, 68, 57, 63; 128 of 32,000 24, 25, 31, 47.
+  const int64_t most = std::min<int64_t>(2LL * sm_count() / batch, ceil_div(p.segments, kVerifyWarps));
+  unsigned ctas = 1;
+  while (ctas < kVerifyMaxCluster && 2 * ctas <= most) ctas *= 2;
+  const size_t smem = verify_smem(p.nodes, p.segments);
+  cudaError_t e = ensure_smem(verify_drafted_kernel, static_cast<uint32_t>(smem));
   if (e == cudaSuccess)
-    e = launch_cluster(verify_drafted_kernel, dim3(static_cast<unsigned>(batch) * ctas), dim3(kVerifyThreads),
-                       verify_smem(p.nodes), static_cast<cudaStream_t>(stream), false, ctas, p);
+    e = launch_cluster(verify_drafted_kernel, dim3(static_cast<unsigned>(batch) * ctas), dim3(kVerifyThreads), smem,
+                       static_cast<cudaStream_t>(stream), false, ctas, p);
   return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "verify_drafted launch");
 }
 

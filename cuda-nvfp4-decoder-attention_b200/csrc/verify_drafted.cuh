@@ -17,13 +17,17 @@
 // without positive elements gives token -1.
 //
 // All of r, s and the sums are FP64: token numbers are borders of sums, which
-// FP32 would move by more than a token's probability.
+// FP32 would move by more than a token's probability.  Rejections of drawn
+// children add up: r = max(p - c q, 0) with c the sum of their s.  Given children
+// need one sum a node: that of p without all of them, to which those that are yet
+// to be tried add their own p(x).
 //
 // A cluster of CTAs takes a sequence.  Every CTA gathers the children's p(x) and
-// q(x) first, so that the walk reads shared memory, and walks by itself; a sum
-// over the vocabulary is cut into one contiguous segment a warp, whose sums all
-// CTAs exchange and add in the same order (the same bits everywhere).  The warp
-// whose segment holds the border of u_0 looks for it.
+// q(x) first, so that the walk reads shared memory, and walks by itself.  A row is
+// cut into segments, dealt to the cluster's warps in turn; a warp has all of a
+// segment (16 elements a lane) in flight at once.  All CTAs exchange the segments'
+// sums and add them in the same order (the same bits everywhere), and one warp
+// looks for the border of u_0 in the segment that holds it.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -33,7 +37,9 @@
 namespace nvfp4da {
 
 constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyMaxNodes = 1024, kVerifyMaxCluster = 16;
+constexpr int kVerifyMaxNodes = 1024, kVerifyMaxCluster = 8;
+constexpr int kVerifyPiece = 512;  // elements a warp has in flight
+constexpr int kVerifyMaxSegments = 1024;
 
 struct VerifyParams {
   const float* target;  // [B, T, V] by strides over b and t
@@ -46,13 +52,17 @@ struct VerifyParams {
   const int64_t* counts;  // [B] or nullptr: nodes of the tree
   int nodes, vocab;       // T, V
   int vec;                // rows are 16-byte aligned
+  int pieces, segments;   // of kVerifyPiece elements a segment; segments of a row
   int64_t* path;          // [B, T]
   int64_t* accepted;      // [B]
   int64_t* next;          // [B]
 };
 
-// Shared memory of the nodes: p(x), q(x), u, token, parent, path, rejected children; then s of each rejection.
-constexpr size_t verify_smem(int nodes) { return static_cast<size_t>(nodes) * 28 + 8 + (nodes + 1) * 8; }
+// Shared memory: two sets of the segments' sums, then of the nodes p(x), q(x), u, token, parent, path, and the
+// tokens of a node's given children.
+constexpr size_t verify_smem(int nodes, int segments) {
+  return static_cast<size_t>(segments) * 16 + static_cast<size_t>(nodes) * 28;
+}
 
 __device__ __forceinline__ double verify_clean(float x) {
   return x > 0.0f && x < INFINITY ? static_cast<double>(x) : 0.0;
@@ -63,15 +73,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   extern __shared__ __align__(16) uint8_t verify_raw[];
-  __shared__ double s_part[2][kVerifyMaxCluster * kVerifyWarps];
-  double* s_scale = reinterpret_cast<double*>(verify_raw);  // s after each rejection at the node
-  float* s_p = reinterpret_cast<float*>(s_scale + p.nodes + 1);
+  double* s_part = reinterpret_cast<double*>(verify_raw);  // [2][segments]
+  float* s_p = reinterpret_cast<float*>(s_part + 2 * p.segments);
   float* s_q = s_p + p.nodes;
   float* s_u = s_q + p.nodes;
   int* s_token = reinterpret_cast<int*>(s_u + p.nodes);  // -1: no child
   int* s_parent = s_token + p.nodes;
   int* s_path = s_parent + p.nodes;
-  int* s_gone = s_path + p.nodes;  // tokens rejected at the node
+  int* s_given = s_path + p.nodes;
   const int64_t b = blockIdx.x / ctas;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int nodes = p.nodes;
@@ -98,92 +107,191 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
     s_p[t] = child ? target[from * p.target_stride[1] + x] : 0.0f;
     s_q[t] = child && draft ? draft[from * p.draft_stride[1] + x] : 1.0f;
   }
-  cluster.sync();  // every CTA has begun: its shared memory may be written
-
-  // This warp's segment of a row.
-  const int segments = ctas * kVerifyWarps, mine = rank * kVerifyWarps + warp;
-  const int seg = static_cast<int>(((static_cast<int64_t>(p.vocab) + segments - 1) / segments + 3) / 4 * 4);
-  const int y0 = static_cast<int>(min(static_cast<int64_t>(mine) * seg, static_cast<int64_t>(p.vocab)));
-  const int y1 = min(y0 + min(seg, p.vocab - y0), p.vocab);
-
-  // What `level` rejections have left of p at token y.
-  auto left = [&](float pv, float qv, int y, int level) -> double {
-    double r = verify_clean(pv);
-    if (draft) {
-      const double q = verify_clean(qv);
-      for (int l = 0; l < level; ++l) r = fmax(r - s_scale[l] * q, 0.0);
-    } else {
-      for (int l = 0; l < level; ++l)
-        if (s_gone[l] == y) r = 0.0;
+  __syncthreads();
+  if (!draft) {  // a sibling before has the token: once that is rejected, nothing of p(x) is left
+    for (int t = threadIdx.x; t < nodes; t += kVerifyThreads) {
+      const int from = s_parent[t], x = s_token[t];
+      for (int i = 1; i < t && from >= 0; ++i)
+        if (s_parent[i] == from && s_token[i] == x) s_p[t] = 0.0f;
     }
-    return r;
+  }
+  auto sync = [&] {
+    if (ctas == 1) __syncthreads();
+    else cluster.sync();
   };
-  // Four elements of a row from y on, of those below y1.
-  auto load4 = [&](const float* row, int y, float (&x)[4]) {
-    if (p.vec && y + 4 <= y1) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(row + y));
-      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-    } else {
+  sync();  // every CTA has begun: its shared memory may be written
+
+  // What is left of a row, element by element: p - c q, or p without the first `given` of s_given.
+  struct Left {
+    const float* p;
+    const float* q;  // nullptr: p alone
+    double c;
+    int given;
+  };
+  // Four elements of a row from `at` on, zeros behind its end.
+  auto fetch4 = [&](const float* row, int at) {
+    if (p.vec && at + 4 <= p.vocab) return __ldg(reinterpret_cast<const float4*>(row + at));
+    float x[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = y + i < y1 ? __ldg(row + y + i) : 0.0f;
+    for (int i = 0; i < 4; ++i) x[i] = at + i < p.vocab ? __ldg(row + at + i) : 0.0f;
+    return make_float4(x[0], x[1], x[2], x[3]);
+  };
+  // What is left of them.
+  auto rest4 = [&](const Left& l, int at, float4 x, float4 z, double (&r)[4]) {
+    r[0] = verify_clean(x.x), r[1] = verify_clean(x.y), r[2] = verify_clean(x.z), r[3] = verify_clean(x.w);
+    if (l.q) {
+      r[0] = fmax(fma(-l.c, verify_clean(z.x), r[0]), 0.0);
+      r[1] = fmax(fma(-l.c, verify_clean(z.y), r[1]), 0.0);
+      r[2] = fmax(fma(-l.c, verify_clean(z.z), r[2]), 0.0);
+      r[3] = fmax(fma(-l.c, verify_clean(z.w), r[3]), 0.0);
+    }
+#pragma unroll 1
+    for (int i = 0; i < l.given; ++i) {
+      const int e = s_given[i] - at;
+      r[0] = e == 0 ? 0.0 : r[0];
+      r[1] = e == 1 ? 0.0 : r[1];
+      r[2] = e == 2 ? 0.0 : r[2];
+      r[3] = e == 3 ? 0.0 : r[3];
     }
   };
-  int buf = 0;
-  // Sum of what is left at `node`, the segments' sums in s_part[buf ^ 1].  All threads of the cluster.
-  auto total_left = [&](int node, int level) -> double {
-    const float* pr = target + node * p.target_stride[1];
-    const float* qr = draft ? draft + node * p.draft_stride[1] : nullptr;
-    double sum = 0.0;
-    for (int y = y0 + 4 * lane; y < y1; y += 128) {
-      float x[4], z[4] = {};
-      load4(pr, y, x);
-      if (qr && level) load4(qr, y, z);
+  int buf = 0;  // s_part's other half holds the last row's sums
+  // Sum of what is left.  All threads of the cluster.
+  auto sum_left = [&](const Left& l) -> double {
+    double* part = s_part + buf * p.segments;
+#pragma unroll 1
+    for (int seg = rank * kVerifyWarps + warp; seg < p.segments; seg += ctas * kVerifyWarps) {
+      double sum = 0.0;
+#pragma unroll 1
+      for (int k = 0; k < p.pieces; ++k) {
+        const int y = (seg * p.pieces + k) * kVerifyPiece;
+        if (y >= p.vocab) break;
+        float4 x[4], z[4] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += left(x[i], z[i], y + i, level);
+        for (int i = 0; i < 4; ++i) x[i] = fetch4(l.p, y + 128 * i + 4 * lane);
+        if (l.q) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[i] = fetch4(l.q, y + 128 * i + 4 * lane);
+        }
+        // Elements as they should be, no negative ones, infinities or NaN: below the bits of infinity.
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          top = max(top, max(max(__float_as_uint(x[i].x), __float_as_uint(x[i].y)),
+                             max(__float_as_uint(x[i].z), __float_as_uint(x[i].w))));
+          top = max(top, max(max(__float_as_uint(z[i].x), __float_as_uint(z[i].y)),
+                             max(__float_as_uint(z[i].z), __float_as_uint(z[i].w))));
+        }
+        // Given children's tokens, out of the lanes that hold them.
+#pragma unroll 1
+        for (int j = 0; j < l.given; j += 32) {
+          const int of = j + lane < l.given ? s_given[j + lane] - y : -1;
+          unsigned votes = __ballot_sync(kFull, static_cast<unsigned>(of) < kVerifyPiece);
+          while (votes) {
+            const int e = __shfl_sync(kFull, of, __ffs(votes) - 1);
+            votes &= votes - 1;
+            if ((e >> 2 & 31) == lane) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (e >> 7 == i && (e & 3) == 0) x[i].x = 0.0f;
+                if (e >> 7 == i && (e & 3) == 1) x[i].y = 0.0f;
+                if (e >> 7 == i && (e & 3) == 2) x[i].z = 0.0f;
+                if (e >> 7 == i && (e & 3) == 3) x[i].w = 0.0f;
+              }
+            }
+          }
+        }
+        if (!__any_sync(kFull, top >= 0x7f800000u)) {
+          double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;
+          auto add = [&](double& to, float pv, float qv) {
+            const double r = l.q ? fma(-l.c, static_cast<double>(qv), static_cast<double>(pv)) : static_cast<double>(pv);
+            if (r > 0.0) to += r;
+          };
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            add(s0, x[i].x, z[i].x);
+            add(s1, x[i].y, z[i].y);
+            add(s2, x[i].z, z[i].z);
+            add(s3, x[i].w, z[i].w);
+          }
+          sum += (s0 + s1) + (s2 + s3);
+        } else {
+#pragma unroll 1
+          for (int at = y + 4 * lane; at < y + kVerifyPiece; at += 128) {
+            double r[4];
+            rest4(l, at, fetch4(l.p, at), l.q ? fetch4(l.q, at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f), r);
+            sum += (r[0] + r[1]) + (r[2] + r[3]);
+          }
+        }
+      }
+      sum = warp_sum_f64(sum);
+      if (lane < ctas) cluster.map_shared_rank(part, lane)[seg] = sum;
     }
-    sum = warp_sum_f64(sum);
-    if (lane < ctas) cluster.map_shared_rank(s_part[buf], lane)[mine] = sum;
-    cluster.sync();
-    const double* part = s_part[buf];
+    sync();
     buf ^= 1;
     double all = 0.0;
-    for (int i = lane; i < segments; i += 32) all += part[i];
+    for (int i = lane; i < p.segments; i += 32) all += part[i];
     return warp_sum_f64(all);
   };
 
   // ---- the walk: the same in every thread of the cluster
-  int node = 0, length = 1, level = 0;
-  double scale = 1.0;
-  bool open = true, summed = false;  // summed: s_part[buf ^ 1] holds the present row's sums
-  for (int t = 1; t < nodes; ++t) {
-    if (s_parent[t] != node || !open) continue;
-    const int x = s_token[t];
-    const double q = verify_clean(s_q[t]), r = left(s_p[t], s_q[t], x, level);
-    if (static_cast<double>(s_u[t]) * q * scale < r) {
-      node = t;
-      level = 0;
-      scale = 1.0;
-      summed = false;
+  int node = 0, length = 1;
+  bool open = true, summed = false;  // summed: the last sums are those of `left`
+  double scale = 1.0, total = 0.0;   // s; sum of `left`
+  Left left{target, nullptr, 0.0, 0};
+  // The first child of `node` behind node t, `nodes`: none.
+  auto child_behind = [&](int t) {
+    for (int base = t + 1; base < nodes; base += 32) {
+      const unsigned votes = __ballot_sync(kFull, base + lane < nodes && s_parent[base + lane] == node);
+      if (votes) return base + __ffs(votes) - 1;
+    }
+    return nodes;
+  };
+  for (int t = child_behind(0); t < nodes && open; t = child_behind(t)) {
+    const double u = s_u[t], pv = verify_clean(s_p[t]), q = draft ? verify_clean(s_q[t]) : 1.0;
+    const bool take = u * q * scale < (left.q ? fmax(fma(-left.c, q, pv), 0.0) : pv);
+    if (take) {
       if (threadIdx.x == 0) s_path[length] = t;
       ++length;
+      node = t;
+      scale = 1.0;
+      summed = false;
+      left = {target + node * p.target_stride[1], nullptr, 0.0, 0};
       continue;
     }
-    __syncthreads();  // the lists are read
-    if (threadIdx.x == 0) {
-      s_scale[level] = scale;
-      s_gone[level] = x;
+    if (draft) {
+      left.q = draft + node * p.draft_stride[1];
+      left.c += scale;
+      scale = total = sum_left(left);
+      summed = true;
+    } else {
+      if (!summed) {  // the node's first rejection
+        __syncthreads();  // s_given is read
+        int n = 0;
+        for (int base = t; base < nodes; base += 32) {
+          const bool mine = base + lane < nodes && s_parent[base + lane] == node;
+          const unsigned votes = __ballot_sync(kFull, mine);
+          if (mine && warp == 0) s_given[n + __popc(votes & ((1u << lane) - 1u))] = s_token[base + lane];
+          n += __popc(votes);
+        }
+        left.given = n;
+        __syncthreads();
+        total = sum_left(left);
+        summed = true;
+      }
+      // s: what is left without the children so far, those to come still in it
+      double more = 0.0;
+      for (int i = t + 1 + lane; i < nodes; i += 32)
+        if (s_parent[i] == node) more += verify_clean(s_p[i]);
+      scale = total + warp_sum_f64(more);
     }
-    __syncthreads();
-    scale = total_left(node, ++level);
-    summed = true;
     if (scale == 0.0) {
       open = false;
-      level = 0;
       summed = false;
+      left = {target + node * p.target_stride[1], nullptr, 0.0, 0};
     }
   }
-  const double total = summed ? scale : total_left(node, 0);
-  const double* part = s_part[buf ^ 1];
+  if (!summed) total = sum_left(left);
+  const double* part = s_part + (buf ^ 1) * p.segments;
   __syncthreads();
   if (rank == 0) {
     for (int t = threadIdx.x; t < p.nodes; t += kVerifyThreads)
@@ -197,7 +305,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
 
   // ---- the next token: the first segment whose end passes u_0 sum r, else the last with anything in it
   const double border = static_cast<double>(s_u[0]) * total;
-  const int per_lane = (segments + 31) / 32, i0 = lane * per_lane, i1 = min(i0 + per_lane, segments);
+  const int per_lane = (p.segments + 31) / 32, i0 = lane * per_lane, i1 = min(i0 + per_lane, p.segments);
   double own = 0.0;
   for (int i = i0; i < i1; ++i) own += part[i];
   double upto = own;
@@ -221,23 +329,15 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
   before = __shfl_sync(kFull, before, holders ? __ffs(holders) - 1 : 0);
   last = __shfl_sync(kFull, last, lasts ? 31 - __clz(lasts) : 0);
   const bool found = holder >= 0;
-  if (mine != (found ? holder : last)) return;
-  const float* pr = target + node * p.target_stride[1];
-  const float* qr = draft ? draft + node * p.draft_stride[1] : nullptr;
+  const int seg = found ? holder : last;
+  if (seg % (ctas * kVerifyWarps) != rank * kVerifyWarps + warp) return;
   int best = -1;  // the last element so far that is left
-  for (int base = y0; base < y1; base += 128) {
-    const int y = base + 4 * lane;
-    float x[4], z[4] = {};
-    double r[4] = {}, sum = 0.0;
-    if (y < y1) {
-      load4(pr, y, x);
-      if (qr && level) load4(qr, y, z);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        r[i] = left(x[i], z[i], y + i, level);
-        sum += r[i];
-      }
-    }
+#pragma unroll 1
+  for (int y = seg * p.pieces * kVerifyPiece; y < min((seg + 1) * p.pieces * kVerifyPiece, p.vocab); y += 128) {
+    const int at = y + 4 * lane;
+    double r[4];
+    rest4(left, at, fetch4(left.p, at), left.q ? fetch4(left.q, at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f), r);
+    const double sum = (r[0] + r[1]) + (r[2] + r[3]);
     double scan = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -247,17 +347,17 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
     int hit = -1, any = -1;
     double run = before + (scan - sum);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      run += r[i];
-      if (r[i] > 0.0) any = y + i;
-      if (found && hit < 0 && r[i] > 0.0 && run > border) hit = y + i;
+    for (int e = 0; e < 4; ++e) {
+      run += r[e];
+      if (r[e] > 0.0) any = at + e;
+      if (found && hit < 0 && r[e] > 0.0 && run > border) hit = at + e;
     }
     const unsigned hits = __ballot_sync(kFull, hit >= 0), anys = __ballot_sync(kFull, any >= 0);
-    if (anys) best = __shfl_sync(kFull, any, 31 - __clz(anys));
     if (hits) {
       best = __shfl_sync(kFull, hit, __ffs(hits) - 1);
       break;
     }
+    if (anys) best = __shfl_sync(kFull, any, 31 - __clz(anys));
     before += __shfl_sync(kFull, scan, 31);
   }
   if (lane == 0) p.next[b] = best;
