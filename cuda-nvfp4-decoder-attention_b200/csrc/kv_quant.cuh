@@ -237,9 +237,7 @@ __device__ __forceinline__ void kv_decode8(const KvStore& st, int64_t row, int d
 __device__ __forceinline__ uint4 kv_pack8(const float (&x)[8]) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = static_cast<uint32_t>(f32_to_bf16_bits(x[2 * i])) |
-           (static_cast<uint32_t>(f32_to_bf16_bits(x[2 * i + 1])) << 16);
+  for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 

@@ -15,8 +15,8 @@
 // Release: sequence b keeps ceil(L_b / S) pages; the others go back, the last
 // sequence's last page first: a release undoes the reserve before it.
 //
-// Numbers of pages to scan are one scan over the batch, which every CTA of one
-// cluster does for itself, 1,024 sequences at a time; the CTAs share the writing
+// Numbers of pages to scan are one scan over the batch, which every CTA of a
+// cluster of eight does for itself, 1,024 sequences at a time; the CTAs share the writing
 // of slots.  held and free_count change when the whole cluster has read them.
 #pragma once
 
@@ -27,6 +27,9 @@
 namespace nvfp4da {
 
 constexpr int kPageThreads = 1024;
+constexpr unsigned kPageCtas = 8;
+constexpr int kAtOnce = 4;  // loads of a thread in flight
+constexpr int kFew = 4;  // pages of a sequence that one thread gives back
 
 struct PageTableParams {
   int32_t* table;  // [B, M]
@@ -69,6 +72,8 @@ __device__ __forceinline__ int pages_scan(int x, int* warp_sums, int& total) {
 __global__ void __launch_bounds__(kPageThreads) reserve_pages_kernel(const PageTableParams p) {
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
+  pdl_launch_dependents();
+  pdl_wait();  // nothing of global memory before this: the launch may overlap the kernel ahead
   const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
   __shared__ int s_scan[kPageThreads / 32];
   __shared__ int s_past[kPageThreads], s_count[kPageThreads], s_held[kPageThreads], s_need[kPageThreads],
@@ -108,22 +113,39 @@ __global__ void __launch_bounds__(kPageThreads) reserve_pages_kernel(const PageT
     }
     const int chunk = min(kPageThreads, p.batch - base);
     for (int i = rank * (kPageThreads / 32) + warp; i < chunk; i += ctas * (kPageThreads / 32))
-      for (int k = lane; k < s_need[i]; k += 32)
-        p.table[static_cast<int64_t>(base + i) * p.max_pages + s_held[i] + k] =
-            p.free_pages[free_count - 1 - (s_first[i] + k)];
-    // Slots: a page number is the old table's, or comes from the stack (the table is being written).
-    const uint32_t items = static_cast<uint32_t>(chunk) * p.tokens;
-    for (uint32_t x = rank * kPageThreads + threadIdx.x; x < items; x += ctas * kPageThreads) {
-      const uint32_t i = x / p.tokens, t = x % p.tokens;
-      int64_t slot = -1;
-      if (static_cast<int>(t) < s_count[i]) {
-        const uint32_t j = s_past[i] + t, k = j / size;
-        const int extra = static_cast<int>(k) - s_held[i];
-        const int page = extra < 0 ? p.table[static_cast<int64_t>(base + i) * p.max_pages + k]
-                                   : p.free_pages[free_count - 1 - (s_first[i] + extra)];
-        if (static_cast<unsigned>(page) < static_cast<unsigned>(p.pages)) slot = static_cast<int64_t>(page) * size + j % size;
+      for (int k0 = lane; k0 < s_need[i]; k0 += 32 * kAtOnce) {
+        int page[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+          if (k0 + 32 * u < s_need[i]) page[u] = __ldg(p.free_pages + (free_count - 1 - (s_first[i] + k0 + 32 * u)));
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+          if (k0 + 32 * u < s_need[i])
+            p.table[static_cast<int64_t>(base + i) * p.max_pages + s_held[i] + k0 + 32 * u] = page[u];
       }
-      p.slots[static_cast<int64_t>(base) * p.tokens + x] = slot;
+    // Slots: a page number is the old table's, or comes from the stack (the table is being written).
+    // Neither is written where it is read here, so that several loads are in flight.
+    const uint32_t items = static_cast<uint32_t>(chunk) * p.tokens, step = ctas * kPageThreads;
+    for (uint32_t x0 = rank * kPageThreads + threadIdx.x; x0 < items; x0 += kAtOnce * step) {
+      int page[kAtOnce], at[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const uint32_t x = x0 + u * step, i = x / p.tokens, t = x % p.tokens;
+        page[u] = -1;
+        if (x < items && static_cast<int>(t) < s_count[i]) {
+          const uint32_t j = s_past[i] + t, k = j / size;
+          const int extra = static_cast<int>(k) - s_held[i];
+          at[u] = j % size;
+          page[u] = __ldg(extra < 0 ? p.table + static_cast<int64_t>(base + i) * p.max_pages + k
+                                    : p.free_pages + (free_count - 1 - (s_first[i] + extra)));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (x0 + u * step < items)
+          p.slots[static_cast<int64_t>(base) * p.tokens + x0 + u * step] =
+              static_cast<unsigned>(page[u]) < static_cast<unsigned>(p.pages)
+                  ? static_cast<int64_t>(page[u]) * size + at[u] : -1;
     }
     __syncthreads();
   }
@@ -135,6 +157,8 @@ __global__ void __launch_bounds__(kPageThreads) reserve_pages_kernel(const PageT
 
 // One CTA.
 __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PageTableParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ int s_scan[kPageThreads / 32];
   __shared__ int s_keep[kPageThreads], s_held[kPageThreads], s_back[kPageThreads], s_upto[kPageThreads];
   const int free_count = pages_clamp(*p.free_count, p.pages);
@@ -154,10 +178,23 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PageT
     __syncthreads();
     auto entry = [&](int i, int k) { return p.table + static_cast<int64_t>(base + i) * p.max_pages + k; };
     auto named = [&](int page) { return static_cast<unsigned>(page) < static_cast<unsigned>(p.pages); };
-    for (int i = warp; i < chunk; i += kPageThreads / 32) {  // pages that go back (entries may name none)
+    // A sequence's own thread where few of its pages go back (most steps: none or one), else a warp.
+    const int i_own = threadIdx.x;
+    const int few = i_own < chunk && s_held[i_own] - s_keep[i_own] <= kFew ? s_held[i_own] - s_keep[i_own] : -1;
+    int own[kFew];
+    if (few >= 0) {  // pages that go back (entries may name none)
       int n = 0;
-      for (int k = s_keep[i] + lane; k - lane < s_held[i]; k += 32)
-        n += __popc(__ballot_sync(kFull, k < s_held[i] && named(*entry(i, k))));
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) own[k] = k < few ? *entry(i_own, s_keep[i_own] + k) : -1;
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) n += named(own[k]);
+      s_back[i_own] = n;
+    }
+    for (int i = warp; i < chunk; i += kPageThreads / 32) {
+      if (s_held[i] - s_keep[i] <= kFew) continue;
+      int n = 0;
+      for (int k = s_keep[i] + lane; k < s_held[i]; k += 32) n += named(*entry(i, k));
+      n = __reduce_add_sync(kFull, n);
       if (lane == 0) s_back[i] = n;
     }
     __syncthreads();
@@ -166,8 +203,20 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PageT
     const int upto = pages_scan(mine, s_scan, total);  // from the last sequence on
     if (static_cast<int>(threadIdx.x) < chunk) s_upto[chunk - 1 - threadIdx.x] = upto;
     __syncthreads();
+    if (few > 0) {
+      int to = free_count + pushed + s_upto[i_own] - 1;  // of the first page that goes back
+#pragma unroll
+      for (int k = 0; k < kFew; ++k) {
+        if (k < few) *entry(i_own, s_keep[i_own] + k) = -1;
+        if (named(own[k])) {
+          if (to < p.pages) p.free_pages[to] = own[k];
+          --to;
+        }
+      }
+    }
     for (int i = warp; i < chunk; i += kPageThreads / 32) {
-      int to = free_count + pushed + s_upto[i] - 1;  // of the first page that goes back
+      if (s_held[i] - s_keep[i] <= kFew) continue;
+      int to = free_count + pushed + s_upto[i] - 1;
       for (int k = s_keep[i] + lane; k - lane < s_held[i]; k += 32) {
         const int page = k < s_held[i] ? *entry(i, k) : -1;
         const bool back = named(page);

@@ -132,8 +132,8 @@ int nvfp4da_reserve_pages(const nvfp4da_page_table* table, const int64_t* past_l
   p.tokens = static_cast<int>(tokens);
   p.slots = slots;
   p.granted = granted;
-  cudaError_t e = launch_cluster(reserve_pages_kernel, dim3(1), dim3(kPageThreads), 0,
-                                 static_cast<cudaStream_t>(stream), false, 1u, p);
+  cudaError_t e = launch_cluster(reserve_pages_kernel, dim3(kPageCtas), dim3(kPageThreads), 0,
+                                 static_cast<cudaStream_t>(stream), true, kPageCtas, p);
   return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "reserve_pages launch");
 }
 
@@ -143,9 +143,8 @@ int nvfp4da_release_pages(const nvfp4da_page_table* table, const int64_t* length
   if (r) return r;
   if (!lengths) return fail(NVFP4DA_ERR_INVALID_ARGUMENT, "release_pages: invalid arguments");
   p.lengths = lengths;
-  release_pages_kernel<<<1, kPageThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  NVFP4DA_CHECK_LAUNCH("release_pages launch");
-  return NVFP4DA_OK;
+  cudaError_t e = launch(release_pages_kernel, dim3(1), dim3(kPageThreads), 0, static_cast<cudaStream_t>(stream), true, p);
+  return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "release_pages launch");
 }
 
 int nvfp4da_paged_kv_append(const nvfp4da_kv_cache* c, const uint16_t* new_k, const int64_t* k_strides,
@@ -184,14 +183,11 @@ int nvfp4da_paged_kv_append(const nvfp4da_kv_cache* c, const uint16_t* new_k, co
   p.vec_k = row_vector(new_k, k_strides) == 8;
   p.vec_v = row_vector(new_v, v_strides) == 8;
   const dim3 grid(static_cast<unsigned>(ceil_div(rows, kKvThreads / p.lanes)), static_cast<unsigned>(batch * c->kv_heads));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (c->format) {
-    case NVFP4DA_KV_BF16: paged_append_kernel<kKvFmtBf16><<<grid, kKvThreads, 0, s>>>(p); break;
-    case NVFP4DA_KV_E4M3: paged_append_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p); break;
-    default: paged_append_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p); break;
-  }
-  NVFP4DA_CHECK_LAUNCH("paged_kv_append launch");
-  return NVFP4DA_OK;
+  auto* kernel = c->format == NVFP4DA_KV_BF16   ? paged_append_kernel<kKvFmtBf16>
+                 : c->format == NVFP4DA_KV_E4M3 ? paged_append_kernel<kKvFmtE4m3>
+                                                : paged_append_kernel<kKvFmtNvfp4>;
+  cudaError_t e = launch(kernel, grid, dim3(kKvThreads), 0, static_cast<cudaStream_t>(stream), true, p);
+  return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "paged_kv_append launch");
 }
 
 int nvfp4da_paged_kv_read(const nvfp4da_kv_cache* c, const int64_t* slots, int64_t batch, int64_t length,
@@ -219,14 +215,11 @@ int nvfp4da_paged_kv_read(const nvfp4da_kv_cache* c, const int64_t* slots, int64
   p.lanes = lanes_per_row(c->head_dim, 8);
   const dim3 grid(static_cast<unsigned>(ceil_div(length, kKvReadRows * (kKvThreads / p.lanes))),
                   static_cast<unsigned>(batch * c->kv_heads));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  switch (c->format) {
-    case NVFP4DA_KV_BF16: paged_read_kernel<kKvFmtBf16><<<grid, kKvThreads, 0, s>>>(p); break;
-    case NVFP4DA_KV_E4M3: paged_read_kernel<kKvFmtE4m3><<<grid, kKvThreads, 0, s>>>(p); break;
-    default: paged_read_kernel<kKvFmtNvfp4><<<grid, kKvThreads, 0, s>>>(p); break;
-  }
-  NVFP4DA_CHECK_LAUNCH("paged_kv_read launch");
-  return NVFP4DA_OK;
+  auto* kernel = c->format == NVFP4DA_KV_BF16   ? paged_read_kernel<kKvFmtBf16>
+                 : c->format == NVFP4DA_KV_E4M3 ? paged_read_kernel<kKvFmtE4m3>
+                                                : paged_read_kernel<kKvFmtNvfp4>;
+  cudaError_t e = launch(kernel, grid, dim3(kKvThreads), 0, static_cast<cudaStream_t>(stream), true, p);
+  return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "paged_kv_read launch");
 }
 
 size_t nvfp4da_paged_attention_workspace_size(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages,
@@ -371,7 +364,7 @@ int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, c
   cudaError_t e = ensure_smem(verify_drafted_kernel, static_cast<uint32_t>(smem));
   if (e == cudaSuccess)
     e = launch_cluster(verify_drafted_kernel, dim3(static_cast<unsigned>(batch) * ctas), dim3(kVerifyThreads), smem,
-                       static_cast<cudaStream_t>(stream), false, ctas, p);
+                       static_cast<cudaStream_t>(stream), true, ctas, p);
   return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "verify_drafted launch");
 }
 

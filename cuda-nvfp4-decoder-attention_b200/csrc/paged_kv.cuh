@@ -75,6 +75,8 @@ __device__ __forceinline__ int64_t paged_row(int64_t slot, int page_size, int kv
 // Grid (rows, B * Hkv).
 template <int FMT>
 __global__ void __launch_bounds__(kKvThreads) paged_append_kernel(const PagedAppendParams p) {
+  pdl_launch_dependents();
+  pdl_wait();  // nothing of global memory before this: the launch may overlap the kernel ahead
   const int sub = threadIdx.x & (p.lanes - 1);
   const int i = blockIdx.x * (kKvThreads / p.lanes) + threadIdx.x / p.lanes;
   const int h = blockIdx.y % p.kv_heads, b = blockIdx.y / p.kv_heads;
@@ -110,6 +112,8 @@ __global__ void __launch_bounds__(kKvThreads) paged_append_kernel(const PagedApp
 // Grid (rows, B * Hkv); a thread takes kKvReadRows rows.  Slots outside the pool read as zeros.
 template <int FMT>
 __global__ void __launch_bounds__(kKvThreads) paged_read_kernel(const PagedReadParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int sub = threadIdx.x & (p.lanes - 1), d0 = sub * 8;
   if (d0 >= p.head_dim) return;
   const int step = kKvThreads / p.lanes, h = blockIdx.y % p.kv_heads;

@@ -71,6 +71,8 @@ __device__ __forceinline__ double verify_clean(float x) {
 __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const VerifyParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
+  pdl_launch_dependents();
+  pdl_wait();  // nothing of global memory before this: the launch may overlap the kernel ahead
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   extern __shared__ __align__(16) uint8_t verify_raw[];
   double* s_part = reinterpret_cast<double*>(verify_raw);  // [2][segments]
