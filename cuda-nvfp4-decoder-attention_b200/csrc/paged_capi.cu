@@ -4,6 +4,7 @@
 // Declarations: include/nvfp4_decoder_attention.h.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "host_util.cuh"
 #include "kv_host.cuh"
@@ -275,6 +276,7 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
     t.pg = pg;
+    t.seg = atoi(getenv("SEG"));
     while (2 << t.box_log2 <= pl.box) ++t.box_log2;
     cudaError_t e = c->format == NVFP4DA_KV_BF16
                         ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, pl.wide, tk, tv, t, s)

@@ -41,10 +41,11 @@ cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, con
                                cudaStream_t s) {
   constexpr int SL = ts_slices<D, FMT, NG>(), NW = kTsWarps;
   auto* kern = tree_stream_kernel<D, FMT, NG, NW, SL, PAGED>;
-  const uint32_t smem = TsCfg<D, FMT, NG, NW, SL>::bytes(p.batch);
+  using Cfg = TsCfg<D, FMT, NG, NW, SL, kTsTile<FMT>, PAGED>;
+  const uint32_t smem = Cfg::bytes(p.batch);
   cudaError_t e = ensure_smem(kern, smem);
   if (e != cudaSuccess) return e;
-  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(TsCfg<D, FMT, NG, NW, SL>::kThreads), smem, s, true, tk, tv, p);
+  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(Cfg::kThreads), smem, s, true, tk, tv, p);
   return e != cudaSuccess ? e : launch_tree_combine<D, PAGED>(p, s);
 }
 

@@ -94,7 +94,7 @@ constexpr float kTsPScale = 32.0f;
 constexpr uint32_t kTsPLimit = 0x7800u;  // 2^15 in FP16
 constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 
-template <int D, int FMT, int NG, int NW, int SL, int TILE = kTsTile<FMT>>
+template <int D, int FMT, int NG, int NW, int SL, int TILE = kTsTile<FMT>, bool PAGED = false>
 struct TsCfg {
   static_assert(D == 64 || D == 128 || D == 256, "head_dim 64, 128 or 256");
   static constexpr int kThreads = (NW + 4) * 32;  // consumers, two loading and two joining warps
@@ -115,7 +115,9 @@ struct TsCfg {
   static constexpr uint32_t kComb = kJoins * (kJoinO + 2 * NW * kRows * 4);
   static constexpr int kTurns = TILE / 16 / SL;                              // warps' turns per tile
   static constexpr int kGroups = NW / kTurns;                        // most tile groups
-  static constexpr int kFit = static_cast<int>((217u * 1024 - kComb) / kStage);
+  // PAGED: a sequence's P_b and end beside its prefix.
+  static constexpr uint32_t kPerSequence = PAGED ? 12 : 4;
+  static constexpr int kFit = static_cast<int>(((PAGED ? 209u : 217u) * 1024 - kComb) / kStage);
   // A whole number of groups: the CTA's n-th tile goes to stage n % kStages and
   // group n % groups, so every stage serves one group only.
   static constexpr int kStages = (kFit > 14 ? 14 : kFit) / kGroups * kGroups;
@@ -123,7 +125,7 @@ struct TsCfg {
   static constexpr uint32_t kOffComb = kStages * kStage;
   static constexpr uint32_t kOffBar = kOffComb + kComb;
   static constexpr uint32_t kOffPrefix = kOffBar + (2 * kStages + 2 * kJoins) * 8;
-  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 4u * (batch + 1) + 1024; }
+  static constexpr uint32_t bytes(int batch) { return kOffPrefix + kPerSequence * (batch + 1) + 1024; }
 };
 
 struct TreeStreamParams {
@@ -145,6 +147,7 @@ struct TreeStreamParams {
   float2* part_ml;     // [2 grid][RP]
   int4* part_slots;    // [2 grid]: see ts_write_slot
   PagedView pg;        // PAGED: the block table; the stores are a pool's, capacity = M * S
+  int seg;             // PAGED: kTsSegment
   int box_log2;        // PAGED: positions that one copy brings, a power of two >= 16 that divides the page and the tile
 };
 
@@ -351,12 +354,22 @@ __device__ __forceinline__ int ts_first_tile(int n, int c, int g) {
   return static_cast<int>(static_cast<long long>(n) * c / g);
 }
 
+// PAGED: P_b and the end of every sequence, behind the prefix in shared memory (read from global memory, they were
+// a latency at the start of every segment).
+__device__ __forceinline__ int2* ts_lengths(const TreeStreamParams& p, int* prefix) {
+  return reinterpret_cast<int2*>(prefix + (p.batch + 2) / 2 * 2);
+}
+
 // The tiles before every sequence, into prefix[0 .. B]; all threads of the block.
 template <bool PAGED = false>
 __device__ __forceinline__ void ts_prefix(const TreeStreamParams& p, int units, int tile, int* prefix) {
   for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
-    int tiles = (ts_visible<PAGED>(p, b) + tile - 1) / tile;
-    if constexpr (PAGED) tiles = max(tiles, 1);  // a sequence of nothing but padding: one that nobody sees
+    const int vis = ts_visible<PAGED>(p, b);
+    int tiles = (vis + tile - 1) / tile;
+    if constexpr (PAGED) {
+      tiles = max(tiles, 1);  // a sequence of nothing but padding: one that nobody sees
+      ts_lengths(p, prefix)[b] = make_int2(ts_past(p, b), vis);
+    }
     prefix[b + 1] = tiles * units;
   }
   __syncthreads();
@@ -379,6 +392,29 @@ __device__ __forceinline__ void ts_prefix(const TreeStreamParams& p, int units, 
   __syncthreads();
 }
 
+// PAGED: the line is cut by weight instead, a segment counting as kTsSegment tiles
+// beside its own, so that a CTA with many short units is not the last to end.
+// On the weighted line a unit takes kTsSegment places and then one a tile; tile t
+// belongs to the CTA that holds its place.
+__device__ __forceinline__ int ts_places(const TreeStreamParams& p, const int* prefix, int units) {
+  return prefix[p.batch] + p.seg * units * p.batch;
+}
+// First tile (on the line of tiles) of CTA c of g.
+__device__ __forceinline__ int ts_first_tile_weighted(const TreeStreamParams& p, const int* prefix, int units, int c,
+                                                      int g) {
+  const int x = ts_first_tile(ts_places(p, prefix, units), c, g);
+  if (c == g) return prefix[p.batch];
+  int lo = 0, hi = p.batch - 1;  // the last sequence that begins at or before x
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] + p.seg * units * mid <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  const int nt = (prefix[lo + 1] - prefix[lo]) / units, within = x - prefix[lo] - p.seg * units * lo;
+  const int u = within / (nt + p.seg), o = within % (nt + p.seg);
+  return prefix[lo] + u * nt + max(0, o - p.seg);
+}
+
 // CTA (of g over n tiles, CTA c owning [c n / g, (c + 1) n / g)) that holds tile x.
 __device__ __forceinline__ int ts_cta_of(int x, int n, int g) {
   return static_cast<int>(((static_cast<long long>(x) + 1) * g - 1) / n);
@@ -386,11 +422,14 @@ __device__ __forceinline__ int ts_cta_of(int x, int n, int g) {
 
 // What a slot of partials holds: the unit and its CTAs, where the slot is the
 // first part of a unit that several CTAs share; unit -1 otherwise.
+template <bool PAGED = false>
 __device__ __forceinline__ void ts_write_slot(const TreeStreamParams& p, int n_tiles, int G, int cta, int x0,
                                               const TsWalk& w) {
   const bool first = w.x == x0;
   const bool starts = w.t0 == 0 && w.t1 < w.nt;  // the unit's first part, more to come
-  const int last = ts_cta_of(w.x - w.t0 + w.nt - 1, n_tiles, G);
+  int end = w.x - w.t0 + w.nt - 1;               // the unit's last tile
+  if constexpr (PAGED) end += p.seg * (w.units * w.b + w.u + 1);  // its place; n_tiles: places
+  const int last = ts_cta_of(end, n_tiles, G);
   p.part_slots[2 * cta + (first ? 0 : 1)] =
       starts ? make_int4(w.b, w.u, cta, last) : make_int4(-1, 0, 0, 0);
 }
@@ -449,13 +488,13 @@ struct TsBoxes {
     const int page = paged_page(p.pg, b, pos);
     return page < 0 ? -1 : (page * p.kv_heads + kvh) * p.pg.page_size + pos % p.pg.page_size;
   }
-  __device__ void begin(const TreeStreamParams& p, int b_, int kvh_, int t, int t1, int lane) {
+  __device__ void begin(const TreeStreamParams& p, int b_, int kvh_, int vis_, int t, int t1, int lane) {
     box_log2 = p.box_log2;
     per_log2 = (TILE == 64 ? 6 : 7) - box_log2;
     tiles = 32 >> per_log2;
     b = b_;
     kvh = kvh_;
-    vis = ts_visible<true>(p, b);
+    vis = vis_;
     t0 = t;
     t_end = t1;
     cur = look(p, t, lane);
@@ -501,7 +540,7 @@ template <int D, int FMT, int NG, int NW, int SL, bool PAGED = false>
 __global__ void __launch_bounds__((NW + 4) * 32, 1)
     tree_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const TreeStreamParams p) {
-  using Cfg = TsCfg<D, FMT, NG, NW, SL>;
+  using Cfg = TsCfg<D, FMT, NG, NW, SL, kTsTile<FMT>, PAGED>;
   constexpr int KS = D / 16;  // MMA steps of K Q^T, 16-element row blocks of O^T
   constexpr bool kQuant = FMT != kKvFmtBf16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -554,13 +593,14 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   // Nothing of global memory before this: the launch may overlap the kernel ahead.
   pdl_wait();
   ts_prefix<PAGED>(p, units, kTsTile<FMT>, prefix);
-  const int n_tiles = prefix[p.batch];
+  const int n_tiles = PAGED ? ts_places(p, prefix, units) : prefix[p.batch];
   // With fewer tiles than CTAs only the first n_tiles CTAs take part, so that
   // every CTA between a unit's first and last holds one of its tiles.
   const int G = min(n_tiles, p.grid);
   if (threadIdx.x < 2) p.part_slots[2 * cta + threadIdx.x] = make_int4(-1, 0, 0, 0);
   if (cta >= G) return;
-  const int x0 = ts_first_tile(n_tiles, cta, G), x1 = ts_first_tile(n_tiles, cta + 1, G);
+  const int x0 = PAGED ? ts_first_tile_weighted(p, prefix, units, cta, G) : ts_first_tile(n_tiles, cta, G);
+  const int x1 = PAGED ? ts_first_tile_weighted(p, prefix, units, cta + 1, G) : ts_first_tile(n_tiles, cta + 1, G);
   __syncthreads();
 
   if (warp >= NW + 2) {
@@ -575,7 +615,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       [[maybe_unused]] const int tokens = ts_tokens<PAGED>(p, w.b);
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
-      if (!whole && warp == NW + 2 && lane == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
+      if (!whole && warp == NW + 2 && lane == 0) ts_write_slot<PAGED>(p, n_tiles, G, cta, x0, w);
       if (!__all_sync(kFull, ts_wait(&join_full[buf], phase, &s_bad))) return;
       const float *so = join_o(buf), *sm_m = join_m(buf), *sm_l = sm_m + NW * Cfg::kRows;
       for (int r = warp - NW - 2; r < rows; r += 2) {
@@ -632,7 +672,7 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
     bool ok = true;
     while (more && ok) {
       const int64_t row0 = (static_cast<int64_t>(w.b) * p.kv_heads + w.u / p.passes) * p.capacity;
-      if constexpr (PAGED) at.begin(p, w.b, w.u / p.passes, w.t0, w.t1, lane);
+      if constexpr (PAGED) at.begin(p, w.b, w.u / p.passes, ts_lengths(p, prefix)[w.b].y, w.t0, w.t1, lane);
       for (int t = w.t0; t < w.t1; ++t) {
         ok = filled < Cfg::kStages || ts_wait(&empty[stage], phase ^ 1u, &s_bad);
         if constexpr (PAGED) ok = __all_sync(kFull, ok);
@@ -714,7 +754,8 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   uint32_t phase = 0;
   while (more) {
     const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes;
-    const int past = ts_past(p, b), vis = ts_visible<PAGED>(p, b);
+    const int past = PAGED ? ts_lengths(p, prefix)[b].x : ts_past(p, b);
+    const int vis = PAGED ? ts_lengths(p, prefix)[b].y : ts_visible(p, b);
     const int n0 = pass * p.rows_per_pass + rc * Cfg::kRows;  // this warp's first query row
     // Query row n = t * group + j; global row of q and ctx:
     auto q_row = [&](int n) -> int64_t {
@@ -783,10 +824,10 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       p_unit[j][0] = p_unit[j][1] = kTsPScale / kTsMinUnit;
     }
 
-    // SL slices of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile); `gone`: those (bits)
-    // whose page is not there.
-    auto slice = [&](auto edge_tag, const uint8_t* st, int r0, int pos0, [[maybe_unused]] unsigned gone) {
+    // SL slices of 16 positions of the tile in `st`, first position pos0 (row r0 of the tile).
+    auto slice = [&](auto edge_tag, auto slices_tag, const uint8_t* st, int r0, int pos0) {
       constexpr bool EDGE = decltype(edge_tag)::value;
+      constexpr int SL = decltype(slices_tag)::value;
       const uint8_t *kt = st, *vt = st + Cfg::kOffV;
       // ---- S^T = K Q^T of one slice; score rows: its positions g and 8 + g
       auto scores = [&](int r0, float (&s)[NG][2][4]) {  // two accumulators, alternate steps
@@ -904,7 +945,6 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
               const int pos = pos0 + 16 * z + g + (i >> 1) * 8, u = pos - past;
               const int t = tok[j][i & 1];
               bool ok = t >= 0 && pos < vis;
-              if constexpr (PAGED) ok &= (gone >> z & 1u) == 0u;
               if (ok && u >= 0)
                 ok = p.mask ? p.mask[b * p.mask_stride + static_cast<int64_t>(t) * p.tokens + u] != 0 : u <= t;
               sees[z][j][i] = ok;
@@ -1105,13 +1145,13 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
         if constexpr (FMT == kKvFmtE4m3) {
 #pragma unroll
           for (int i = 0; i < BYTES / 4; ++i) {
-            uint32_t d[4][2];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ts_e4m3x4(c[e][i], d[e][0], d[e][1]);
+            // Two positions' codes of an element side by side before they are decoded: half of the permutations.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              uint32_t a[4] = {__byte_perm(d[0][h], d[1][h], 0x5410), __byte_perm(d[0][h], d[1][h], 0x7632),
-                               __byte_perm(d[2][h], d[3][h], 0x5410), __byte_perm(d[2][h], d[3][h], 0x7632)};
+              const uint32_t sel = h ? 0x7362 : 0x5140;
+              uint32_t a[4];
+              ts_e4m3x4(__byte_perm(c[0][i], c[1][i], sel), a[0], a[1]);
+              ts_e4m3x4(__byte_perm(c[2][i], c[3][i], sel), a[2], a[3]);
               pv(2 * i + h, a);
             }
           }
@@ -1128,16 +1168,19 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             }
 #pragma unroll
           for (int i = 0; i < BYTES / 4; ++i) {
-            uint32_t d[4][4];
+            // Two positions' codes of an element side by side before they are decoded; even and odd elements.
+            uint32_t d[2][2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) e2m1x8_to_f16x2x4(c[e][i], d[e]);
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t x = c[2 * e][i], y = c[2 * e + 1][i];
+              e2m1x8_to_f16x2x4((x & 0x0f0f0f0fu) | (y << 4 & 0xf0f0f0f0u), d[e][0]);
+              e2m1x8_to_f16x2x4((x >> 4 & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), d[e][1]);
+            }
             const uint32_t b0 = bs[i * NB / (BYTES / 4)][0], b1 = bs[i * NB / (BYTES / 4)][1];
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-              uint32_t a[4] = {ts_hmul2(__byte_perm(d[0][h], d[1][h], 0x5410), b0),
-                               ts_hmul2(__byte_perm(d[0][h], d[1][h], 0x7632), b0),
-                               ts_hmul2(__byte_perm(d[2][h], d[3][h], 0x5410), b1),
-                               ts_hmul2(__byte_perm(d[2][h], d[3][h], 0x7632), b1)};
+              uint32_t a[4] = {ts_hmul2(d[0][0][h], b0), ts_hmul2(d[0][1][h], b0), ts_hmul2(d[1][0][h], b1),
+                               ts_hmul2(d[1][1][h], b1)};
               pv(4 * i + h, a);
             }
           }
@@ -1186,10 +1229,18 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
           const int r0 = (turn0 + i) * 16 * SL;
           const int pos0 = t * kTsTile<FMT> + r0;
           if (pos0 >= vis) break;
-          const unsigned gone = absent >> (r0 / 16) & ((1u << SL) - 1u);
-          if (PAGED && gone == (1u << SL) - 1u) continue;
-          if (pos0 + 16 * SL <= past && !gone) slice(std::false_type{}, st, r0, pos0, gone);
-          else slice(std::true_type{}, st, r0, pos0, gone);
+          const unsigned gone = absent >> (r0 / 16) & ((1u << SL) - 1u);  // slices whose page is not there
+          using Slices = std::integral_constant<int, SL>;
+          if (pos0 + 16 * SL <= past && !gone) {
+            slice(std::false_type{}, Slices{}, st, r0, pos0);
+          } else if constexpr (PAGED) {  // one at a time: half of the code that a segment's end has to fetch
+#pragma unroll 1
+            for (int z = 0; z < SL; ++z)
+              if (pos0 + 16 * z < vis && !(gone >> z & 1u))
+                slice(std::true_type{}, std::integral_constant<int, 1>{}, st, r0 + 16 * z, pos0 + 16 * z);
+          } else {
+            slice(std::true_type{}, Slices{}, st, r0, pos0);
+          }
         }
         __syncwarp();
         if (lane == 0) ts_arrive(&empty[stage]);
