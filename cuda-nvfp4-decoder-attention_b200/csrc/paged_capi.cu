@@ -4,7 +4,7 @@
 // Declarations: include/nvfp4_decoder_attention.h.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
+
 
 #include "host_util.cuh"
 #include "kv_host.cuh"
@@ -250,6 +250,7 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
   const PagedView pg = {block_table, static_cast<int>(c->batch), static_cast<int>(max_pages),
                         static_cast<int>(c->capacity), counts};
   if (pl.stream) {
+    const int64_t tile = c->format == NVFP4DA_KV_BF16 ? kTsTile<kKvFmtBf16> : kTsTile<kKvFmtE4m3>;
     CUtensorMap tk, tv;
     if (!tree_map(&tk, *c, c->k_codes, pl.box) || !tree_map(&tv, *c, c->v_codes, pl.box))
       return fail(NVFP4DA_ERR_CUDA, "tensor map encoding failed for the paged attention");
@@ -276,7 +277,8 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
     t.pg = pg;
-    t.seg = atoi(getenv("SEG"));
+    t.seg = c->format == NVFP4DA_KV_BF16 ? kTsSegment<kKvFmtBf16> : kTsSegment<kKvFmtE4m3>;
+    t.loaders = pl.box < tile ? 4 : 2;
     while (2 << t.box_log2 <= pl.box) ++t.box_log2;
     cudaError_t e = c->format == NVFP4DA_KV_BF16
                         ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, pl.wide, tk, tv, t, s)

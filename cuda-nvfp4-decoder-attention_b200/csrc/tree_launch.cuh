@@ -43,6 +43,13 @@ cudaError_t launch_tree_stream(const CUtensorMap& tk, const CUtensorMap& tv, con
   auto* kern = tree_stream_kernel<D, FMT, NG, NW, SL, PAGED>;
   using Cfg = TsCfg<D, FMT, NG, NW, SL, kTsTile<FMT>, PAGED>;
   const uint32_t smem = Cfg::bytes(p.batch);
+  if constexpr (PAGED) {  // the warps' register shares are drawn from what the block is launched with
+    static const int regs = [&] {
+      cudaFuncAttributes a{};
+      return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs * Cfg::kThreads < (kTsPagedRegs * NW + kTsPagedOtherRegs * 8) * 32) return cudaErrorLaunchOutOfResources;
+  }
   cudaError_t e = ensure_smem(kern, smem);
   if (e != cudaSuccess) return e;
   e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(Cfg::kThreads), smem, s, true, tk, tv, p);

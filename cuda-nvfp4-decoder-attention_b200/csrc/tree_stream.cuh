@@ -81,6 +81,12 @@ static __device__ unsigned g_tree_errors;  // of the translation unit's kernels
 // thirds of the HBM rate even with nothing else to do.
 template <int FMT>
 constexpr int kTsTile = FMT == kKvFmtBf16 ? 64 : 128;
+// PAGED: what a segment costs beside its tiles, in tiles.  us for 0, 2, 4, 6 of them, 24 query heads over 6 KV heads:
+// 64 sequences of 10 to 2,000 positions BF16 76, 63, 63, 64, E4M3 86, 55, 49, 49, NVFP4 89, 61, 57, 54; of 1,024 to
+// 8,191 E4M3 113, 109, 111, 114; 16 of 100 to 30,000 NVFP4 90, 80, 78, 78.
+template <int FMT>
+constexpr int kTsSegment = FMT == kKvFmtBf16 ? 3 : 4;
+constexpr int kTsPagedRegs = 176, kTsPagedOtherRegs = 80;  // 256 * 176 + 256 * 80 = 512 * 128
 constexpr int kTsMaxBatch = 1024;  // sequences whose prefix shared memory holds
 // A score may pass the reference m by kTsSlack (log2), and m moves to kTsLift
 // above the score that passed it.  Over codes p_j <= 1 then, so that p_j gamma_j
@@ -97,7 +103,9 @@ constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 template <int D, int FMT, int NG, int NW, int SL, int TILE = kTsTile<FMT>, bool PAGED = false>
 struct TsCfg {
   static_assert(D == 64 || D == 128 || D == 256, "head_dim 64, 128 or 256");
-  static constexpr int kThreads = (NW + 4) * 32;  // consumers, two loading and two joining warps
+  // Consumers, two loading and two joining warps; PAGED: four loading ones, and two that make up a warpgroup.
+  static constexpr int kLoaders = PAGED ? 4 : 2;
+  static constexpr int kThreads = (NW + (PAGED ? 8 : 4)) * 32;
   static constexpr int kRowBytes = FMT == kKvFmtBf16 ? 2 * D : (FMT == kKvFmtE4m3 ? D : D / 2);
   static constexpr uint32_t kCodes = TILE * kRowBytes;  // one of K, V
   static constexpr uint32_t kBlockScales = FMT == kKvFmtNvfp4 ? TILE * (D / 16) : 0;
@@ -148,6 +156,7 @@ struct TreeStreamParams {
   int4* part_slots;    // [2 grid]: see ts_write_slot
   PagedView pg;        // PAGED: the block table; the stores are a pool's, capacity = M * S
   int seg;             // PAGED: kTsSegment
+  int loaders;         // PAGED: warps that copy K and V, 2 or 4 (a tile then has two boxes at least)
   int box_log2;        // PAGED: positions that one copy brings, a power of two >= 16 that divides the page and the tile
 };
 
@@ -537,7 +546,7 @@ __device__ __forceinline__ void ts_load_scales_paged(uint8_t* blocks, uint8_t* r
 // tile's copy would bring it; 16-position slices of pages that are not there (their
 // boxes come in as zeros) are left out.
 template <int D, int FMT, int NG, int NW, int SL, bool PAGED = false>
-__global__ void __launch_bounds__((NW + 4) * 32, 1)
+__global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
     tree_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const TreeStreamParams p) {
   using Cfg = TsCfg<D, FMT, NG, NW, SL, kTsTile<FMT>, PAGED>;
@@ -578,7 +587,8 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   pdl_launch_dependents();  // the join waits for this kernel's memory itself
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(&full[s], !kQuant ? 2 : PAGED ? 66 : 34);  // K's and V's bytes, and the lanes that copy scales
+      // K's and V's bytes, and the lanes that copy scales (PAGED: of K and of V by warps of their own)
+      mbar_init(&full[s], (PAGED && p.loaders == 4 ? 4 : 2) + (!kQuant ? 0 : PAGED ? 64 : 32));
       mbar_init(&empty[s], pw_n >= kTurns ? kTurns * rc_n : NW);
     }
     for (int i = 0; i < Cfg::kJoins; ++i) {
@@ -603,7 +613,14 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
   const int x1 = PAGED ? ts_first_tile_weighted(p, prefix, units, cta + 1, G) : ts_first_tile(n_tiles, cta + 1, G);
   __syncthreads();
 
-  if (warp >= NW + 2) {
+  // 128 registers a thread at launch: the consumers take what the others give.
+  if constexpr (PAGED) {
+    if (warp < NW) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTsPagedRegs));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTsPagedOtherRegs));
+    if (warp >= NW + Cfg::kLoaders + 2) return;
+  }
+
+  if (warp >= NW + Cfg::kLoaders) {
     // ---------------------------------------------------------------- joins: every other row of a segment
     TsWalk w;
     bool more = w.begin(prefix, p.batch, units, x0, x1);
@@ -615,10 +632,10 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
       [[maybe_unused]] const int tokens = ts_tokens<PAGED>(p, w.b);
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
-      if (!whole && warp == NW + 2 && lane == 0) ts_write_slot<PAGED>(p, n_tiles, G, cta, x0, w);
+      if (!whole && warp == NW + Cfg::kLoaders && lane == 0) ts_write_slot<PAGED>(p, n_tiles, G, cta, x0, w);
       if (!__all_sync(kFull, ts_wait(&join_full[buf], phase, &s_bad))) return;
       const float *so = join_o(buf), *sm_m = join_m(buf), *sm_l = sm_m + NW * Cfg::kRows;
-      for (int r = warp - NW - 2; r < rows; r += 2) {
+      for (int r = warp - NW - Cfg::kLoaders; r < rows; r += 2) {
         // Position warp `lane` of the row's chunk: its factor.
         const int chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
         const int at = (lane * rc_n + chunk) * Cfg::kRows + rr;
@@ -658,9 +675,13 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
 
   if (warp >= NW) {
     // ---------------------------------------------------------------- loads: warp NW K, the next one V and scales
+    // (PAGED: two warps K, two V)
     // Scales go by 16-byte copies of a whole warp: a bulk copy takes one thread over a hundred cycles to
     // issue, and four of them per tile held E4M3 and NVFP4 caches at 0.8 and 0.4 of the HBM rate.
-    const bool is_v = warp > NW;
+    const bool is_v = PAGED ? warp >= NW + 2 : warp > NW;
+    // PAGED: with four loaders this warp's every other box, the scales for the second; with two all of it.
+    [[maybe_unused]] const int split = PAGED && p.loaders == 4 ? 1 : 0, half = (warp - NW) & 1;
+    if (PAGED && half > split) return;
     if (!PAGED && lane != 0 && !(is_v && kQuant)) return;
     TsWalk w;
     bool more = w.begin(prefix, p.batch, units, x0, x1);
@@ -681,15 +702,15 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
         const int64_t row = row0 + static_cast<int64_t>(t) * kTsTile<FMT>;
         if constexpr (PAGED) {
           at.advance(p, t, lane);
-          // Lane i's box, and lane i's 16-position slice.
-          const int mine = at.row(t, lane << p.box_log2), of_slice = at.row(t, lane * 16);
+          const int of_slice = at.row(t, lane * 16);  // lane i's 16-position slice
           const unsigned absent = __ballot_sync(kFull, lane < kTsTile<FMT> / 16 && of_slice < 0);
-          if (lane == 0) {
-            if (!is_v) s_absent[stage] = absent;
-            mbar_arrive_expect_tx(&full[stage], Cfg::kCodes);
-          }
+          if (lane == 0 && !is_v && !half) s_absent[stage] = absent;
+          // Lane i's box, of this warp's.  A thread takes some 200 cycles to issue a copy, whatever its size: with
+          // one warp each for K and V pages of 16 held E4M3 at 111 us where whole tiles took 102 (NVFP4 111, 94).
+          const int box = (lane << split) + half, mine = at.row(t, box << p.box_log2);
+          if (lane == 0) mbar_arrive_expect_tx(&full[stage], Cfg::kCodes >> split);
           __syncwarp();
-          if (lane < 1 << at.per_log2) {
+          if (box < 1 << at.per_log2) {
             // Behind the pool's last row: zeros.
             const int from = mine >= 0 ? mine : p.pg.pages * p.kv_heads * p.pg.page_size;
             uint8_t* dst = st + (is_v ? Cfg::kOffV : 0);
@@ -697,9 +718,9 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
             if constexpr (!kQuant) {
 #pragma unroll
               for (int bx = 0; bx < D / 64; ++bx)
-                ts_tma_2d(dst + bx * (kTsTile<FMT> * 128) + (lane << p.box_log2) * 128, map, bx * 64, from, &full[stage]);
+                ts_tma_2d(dst + bx * (kTsTile<FMT> * 128) + (box << p.box_log2) * 128, map, bx * 64, from, &full[stage]);
             } else {  // rows stand in groups of 16
-              ts_tma_2d(dst + (lane << p.box_log2) * Cfg::kRowBytes, map, 0, from / 16 * (16 * Cfg::kRowBytes / 128),
+              ts_tma_2d(dst + (box << p.box_log2) * Cfg::kRowBytes, map, 0, from / 16 * (16 * Cfg::kRowBytes / 128),
                         &full[stage]);
             }
           }
@@ -717,10 +738,12 @@ __global__ void __launch_bounds__((NW + 4) * 32, 1)
           }
         }
         if constexpr (kQuant && PAGED) {
-          ts_load_scales_paged<D, FMT, Cfg, kTsTile<FMT>>(st + (is_v ? Cfg::kOffVb : Cfg::kOffKb),
-                                                          st + (is_v ? Cfg::kOffVr : Cfg::kOffKr), is_v ? p.v : p.k, at, t,
-                                                          lane);
-          ts_copy_arrive(&full[stage]);
+          if (half == split) {
+            ts_load_scales_paged<D, FMT, Cfg, kTsTile<FMT>>(st + (is_v ? Cfg::kOffVb : Cfg::kOffKb),
+                                                            st + (is_v ? Cfg::kOffVr : Cfg::kOffKr), is_v ? p.v : p.k, at,
+                                                            t, lane);
+            ts_copy_arrive(&full[stage]);
+          }
         } else if constexpr (kQuant) {
           if (is_v) {
             ts_load_scales<D, FMT, Cfg, kTsTile<FMT>>(st, p, row, all_rows, lane);
