@@ -44,7 +44,7 @@ int check_table(const nvfp4da_page_table* t, PageTableParams& p) {
 // Plan of the paged attention.
 struct PagedPlan {
   bool stream;  // tree_stream_kernel, else the general kernel
-  int wide, row_chunks, rows_per_pass, passes, box;
+  int row_chunks, rows_per_pass, passes, box;
   int splits;   // general kernel
   int64_t split_len;
   size_t bytes;
@@ -79,10 +79,9 @@ int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int6
   pl.stream = (d == 64 || d == 128 || d == 256) && batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
               product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
   if (pl.stream) {
-    pl.wide = nq > 8 && (d == 64 || (d == 128 && c->format == NVFP4DA_KV_BF16)) ? 2 : 1;
     pl.row_chunks = 1;
-    while (pl.row_chunks < kTsWarps && 8 * pl.wide * pl.row_chunks < nq) pl.row_chunks *= 2;
-    pl.rows_per_pass = 8 * pl.wide * pl.row_chunks;
+    while (pl.row_chunks < kTsWarps && 8 * pl.row_chunks < nq) pl.row_chunks *= 2;
+    pl.rows_per_pass = 8 * pl.row_chunks;
     pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
     pl.box = static_cast<int>(std::min(tile, c->capacity & -c->capacity));
     // Tiles and their order are 32-bit in the kernel.
@@ -281,10 +280,10 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     t.loaders = pl.box < tile ? 4 : 2;
     while (2 << t.box_log2 <= pl.box) ++t.box_log2;
     cudaError_t e = c->format == NVFP4DA_KV_BF16
-                        ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, pl.wide, tk, tv, t, s)
+                        ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, 1, tk, tv, t, s)
                     : c->format == NVFP4DA_KV_E4M3
-                        ? launch_tree_stream_d<kKvFmtE4m3, true>(c->head_dim, pl.wide, tk, tv, t, s)
-                        : launch_tree_stream_d<kKvFmtNvfp4, true>(c->head_dim, pl.wide, tk, tv, t, s);
+                        ? launch_tree_stream_d<kKvFmtE4m3, true>(c->head_dim, 1, tk, tv, t, s)
+                        : launch_tree_stream_d<kKvFmtNvfp4, true>(c->head_dim, 1, tk, tv, t, s);
     return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "streaming paged attention launch");
   }
   TreeAttnParams p{};
