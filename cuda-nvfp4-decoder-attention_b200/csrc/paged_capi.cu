@@ -41,10 +41,25 @@ int check_table(const nvfp4da_page_table* t, PageTableParams& p) {
   return NVFP4DA_OK;
 }
 
+// Query rows per KV head from which tree_tc_kernel runs.  Streaming / tcgen05, us, 6 KV heads (64 rows: 4), 8 sequences
+// of 200 to 400 positions, 32 of 100 to 4,000, 8 of 8,000 to 12,000, pages of 32; head_dim 128:
+//          8 rows                   12 rows                  20 rows                  64 rows
+//   BF16   23/24   61/62   73/75    24/24   65/62   75/75    28/24   85/62   85/74    40/23  124/52  124/60
+//   E4M3   24/30   46/77   52/77    26/30   54/79   60/77    30/30   79/77   88/83    46/30  110/64  120/69
+//   NVFP4  24/32   46/77   48/75    26/32   60/79   67/75    32/30   89/73   99/75    46/30  120/61  134/67
+// and head_dim 64:
+//   BF16   19/22   44/50   48/54    19/22   50/50   50/54    24/22   67/50   65/54    32/22  101/42   91/46
+//   E4M3   22/26   36/67   36/63    22/26   44/67   46/64    26/26   60/65   67/67    36/26   83/54   89/56
+//   NVFP4  22/26   36/65   38/62    23/26   46/67   50/62    26/26   67/64   75/66    38/26   89/54   97/54
+constexpr int64_t paged_tc_min_rows(int64_t head_dim, int format) {
+  return format == NVFP4DA_KV_BF16 ? (head_dim == 64 ? 17 : 9) : format == NVFP4DA_KV_E4M3 && head_dim == 64 ? 33 : 17;
+}
+
 // Plan of the paged attention.
 struct PagedPlan {
-  bool stream;  // tree_stream_kernel, else the general kernel
-  int row_chunks, rows_per_pass, passes, box;
+  bool stream;  // tree_stream_kernel (or tc: tree_tc_kernel), else the general kernel
+  bool tc;
+  int row_chunks, rows_per_pass, passes, tile, box;
   int splits;   // general kernel
   int64_t split_len;
   size_t bytes;
@@ -73,21 +88,26 @@ int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int6
   if (!product_within(group, tokens, 65535) || !product_within(batch * q_heads, tokens, kI32Max))
     return fail(NVFP4DA_ERR_UNSUPPORTED, "too many query rows: (Hq/Hkv)*T must be at most 65535 and B*T*Hq below 2^31");
   const int64_t visible = max_past + tokens, d = c->head_dim, nq = group * tokens;
-  // The streaming kernel: tensor-core tiles for these head dimensions; the tile
-  // line, the pool's 128-byte lines and the prefix of the batch have to fit.
-  const int64_t tile = c->format == NVFP4DA_KV_BF16 ? kTsTile<kKvFmtBf16> : kTsTile<kKvFmtE4m3>;
+  // The streaming kernel: tensor-core tiles for these head dimensions; the pool's
+  // 128-byte lines and the prefix of the batch have to fit.
   pl.stream = (d == 64 || d == 128 || d == 256) && batch <= kTsMaxBatch && tensor_map_encoder() != nullptr &&
               product_within(c->batch * c->kv_heads * c->capacity, 2, kI32Max);
+  pl.tc = pl.stream && d <= 128 && nq >= paged_tc_min_rows(d, c->format);
+  // Places of tiles and their order are 32-bit in the kernels.
+  if (!product_within(batch * c->kv_heads * (ceil_div(capacity, kTtKeys) + kTtSegment), ceil_div(nq, 8), kI32Max))
+    pl.stream = pl.tc = false;
   if (pl.stream) {
-    pl.row_chunks = 1;
-    while (pl.row_chunks < kTsWarps && 8 * pl.row_chunks < nq) pl.row_chunks *= 2;
-    pl.rows_per_pass = 8 * pl.row_chunks;
-    pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
-    pl.box = static_cast<int>(std::min(tile, c->capacity & -c->capacity));
-    // Tiles and their order are 32-bit in the kernel.
-    pl.stream = product_within(batch * c->kv_heads * ceil_div(capacity, tile), pl.passes, kI32Max);
-  }
-  if (pl.stream) {
+    if (pl.tc) {
+      pl.passes = static_cast<int>(ceil_div(nq, 2 * kTtRows));
+      pl.rows_per_pass = static_cast<int>(ceil_div(nq, pl.passes));
+    } else {
+      pl.row_chunks = 1;
+      while (pl.row_chunks < kTsWarps && 8 * pl.row_chunks < nq) pl.row_chunks *= 2;
+      pl.rows_per_pass = 8 * pl.row_chunks;
+      pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
+    }
+    pl.tile = pl.tc ? kTtKeys : c->format == NVFP4DA_KV_BF16 ? kTsTile<kKvFmtBf16> : kTsTile<kKvFmtE4m3>;
+    pl.box = static_cast<int>(std::min<int64_t>(pl.tile, c->capacity & -c->capacity));
     pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * (pl.rows_per_pass * (d * 4 + 8) + 16), 256);
     return NVFP4DA_OK;
   }
@@ -249,7 +269,6 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
   const PagedView pg = {block_table, static_cast<int>(c->batch), static_cast<int>(max_pages),
                         static_cast<int>(c->capacity), counts};
   if (pl.stream) {
-    const int64_t tile = c->format == NVFP4DA_KV_BF16 ? kTsTile<kKvFmtBf16> : kTsTile<kKvFmtE4m3>;
     CUtensorMap tk, tv;
     if (!tree_map(&tk, *c, c->k_codes, pl.box) || !tree_map(&tv, *c, c->v_codes, pl.box))
       return fail(NVFP4DA_ERR_CUDA, "tensor map encoding failed for the paged attention");
@@ -276,9 +295,18 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
     t.pg = pg;
-    t.seg = c->format == NVFP4DA_KV_BF16 ? kTsSegment<kKvFmtBf16> : kTsSegment<kKvFmtE4m3>;
-    t.loaders = pl.box < tile ? 4 : 2;
+    t.seg = pl.tc ? kTtSegment : c->format == NVFP4DA_KV_BF16 ? kTsSegment<kKvFmtBf16> : kTsSegment<kKvFmtE4m3>;
+    t.loaders = pl.box < pl.tile ? 4 : 2;
     while (2 << t.box_log2 <= pl.box) ++t.box_log2;
+    if (pl.tc) {
+      const bool split = pl.rows_per_pass > kTtRows;
+      cudaError_t e = c->format == NVFP4DA_KV_BF16
+                          ? launch_tree_tc_d<kKvFmtBf16, true>(c->head_dim, split, tk, tv, t, s)
+                      : c->format == NVFP4DA_KV_E4M3
+                          ? launch_tree_tc_d<kKvFmtE4m3, true>(c->head_dim, split, tk, tv, t, s)
+                          : launch_tree_tc_d<kKvFmtNvfp4, true>(c->head_dim, split, tk, tv, t, s);
+      return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "tensor-core paged attention launch");
+    }
     cudaError_t e = c->format == NVFP4DA_KV_BF16
                         ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, 1, tk, tv, t, s)
                     : c->format == NVFP4DA_KV_E4M3

@@ -1,9 +1,10 @@
-// Launches of the streaming tree attention and its joins, over caches of whole
+// Launches of the streaming and the tensor-core tree attention and their joins, over caches of whole
 // sequences and (PAGED) over pools of pages.
 #pragma once
 
 #include "kv_host.cuh"
 #include "tree_stream.cuh"
+#include "tree_tc.cuh"
 
 namespace nvfp4da {
 
@@ -78,6 +79,49 @@ cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& 
       return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
     default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
   }
+}
+
+// Query rows per KV head from which tree_tc_kernel runs.  The streaming kernel
+// decodes codes in registers for the rows of one warp, this one once for all
+// rows.  Both, 8 sequences x 6 KV heads x 4 query heads each, us streaming /
+// tcgen05 after 300, 2,000 and 12,000 positions, head_dim 128:
+//          8 rows (2 tokens)        12 rows                  20 rows                  64 rows
+//   BF16   20/27  23/28  58/69      25/26  30/29   65/69     29/28  37/31   78/72     66/27  78/33  151/75
+//   E4M3   20/26  23/33  41/74      22/26  39/32  131/74     26/27  46/35  146/77     47/30  88/38  211/84
+//   NVFP4  20/27  24/33  40/72      22/26  38/33  118/72     26/28  45/36  131/77     47/30  87/38  192/82
+// and head_dim 64, where a tile is half the bytes and the decoding, but the
+// tcgen05 kernel's warps take as long for it:
+//          12 rows                  24 rows                  32 rows                  64 rows
+//   BF16   27/27  26/28  38/57      22/26  27/26  56/58      27/27  31/26  60/59      41/21  48/27   96/62
+//   E4M3   20/23  23/29  45/65      21/24  30/30  62/66      21/24  33/30  66/67      29/25  52/32  106/73
+//   NVFP4  20/24  23/30  43/68      20/24  30/31  61/70      21/25  34/31  64/71      29/26  52/32  107/76
+constexpr int64_t tc_min_rows(int64_t head_dim, bool bf16) { return head_dim == 64 ? 33 : bf16 ? 13 : 9; }
+
+template <int D, int FMT, bool SPLIT, bool PAGED = false>
+cudaError_t launch_tree_tc(const CUtensorMap& tk, const CUtensorMap& tv, const TreeStreamParams& p, cudaStream_t s) {
+  auto* kern = tree_tc_kernel<D, FMT, SPLIT, PAGED>;
+  const uint32_t smem = TtCfg<D, FMT, SPLIT>::template bytes<PAGED>(p.batch);
+  // The warps' register shares are drawn from what the block is launched with.
+  static const int regs = [&] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs * kTtThreads < (kTtSoftmaxRegs * kTtSoftmaxWarps + kTtOtherRegs * (kTtThreads / 32 - kTtSoftmaxWarps)) * 32)
+    return cudaErrorLaunchOutOfResources;
+  cudaError_t e = ensure_smem(kern, smem);
+  if (e != cudaSuccess) return e;
+  e = launch(kern, dim3(static_cast<unsigned>(p.grid)), dim3(kTtThreads), smem, s, true, tk, tv, p);
+  return e != cudaSuccess ? e : launch_tree_combine<D, PAGED>(p, s);
+}
+
+template <int FMT, bool PAGED = false>
+cudaError_t launch_tree_tc_d(int64_t head_dim, bool split, const CUtensorMap& tk, const CUtensorMap& tv,
+                             const TreeStreamParams& p, cudaStream_t s) {
+  if (head_dim == 64)
+    return split ? launch_tree_tc<64, FMT, true, PAGED>(tk, tv, p, s)
+                 : launch_tree_tc<64, FMT, false, PAGED>(tk, tv, p, s);
+  return split ? launch_tree_tc<128, FMT, true, PAGED>(tk, tv, p, s)
+               : launch_tree_tc<128, FMT, false, PAGED>(tk, tv, p, s);
 }
 
 // The tensor map of K or V: BF16 rows in 64-element boxes, codes as 128-byte lines.

@@ -171,6 +171,11 @@ __device__ __forceinline__ void ts_tma_2d(void* dst, const CUtensorMap* map, int
 __device__ __forceinline__ void ts_copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+// The same, zeros where there is nothing to copy (`src` is valid all the same).
+__device__ __forceinline__ void ts_copy16_or_zeros(void* dst, const void* src, bool copy) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(copy ? 16 : 0)
+               : "memory");
+}
 __device__ __forceinline__ void ts_copy_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -520,7 +525,8 @@ struct TsBoxes {
   __device__ int row(int t, int r) const { return __shfl_sync(kFull, cur, ((t - t0) << per_log2) + ((r & (TILE - 1)) >> box_log2)); }
 };
 
-// ts_load_scales of K or of V (`from`, to `blocks` and `rows`) for a tile whose boxes stand apart.
+// ts_load_scales of K or of V (`from`, to `blocks` and `rows`) for a tile whose boxes stand apart; zeros where there is
+// none.
 template <int D, int FMT, typename Cfg, int TILE>
 __device__ __forceinline__ void ts_load_scales_paged(uint8_t* blocks, uint8_t* rows, const KvStore& from,
                                                      const TsBoxes<TILE>& at, int t, int lane) {
@@ -530,14 +536,15 @@ __device__ __forceinline__ void ts_load_scales_paged(uint8_t* blocks, uint8_t* r
     for (uint32_t i = 0; i < Cfg::kBlockScales; i += 512) {
       const uint32_t o = i + lane * 16;
       const int r = o / (D / 16), row = at.row(t, r);
-      if (o < Cfg::kBlockScales && row >= 0)
-        ts_copy16(blocks + o, from.block_scales + static_cast<int64_t>(row + (r & in_box)) * (D / 16));
+      if (o < Cfg::kBlockScales)
+        ts_copy16_or_zeros(blocks + o, from.block_scales + static_cast<int64_t>(max(row, 0) + (r & in_box)) * (D / 16),
+                           row >= 0);
     }
   }
 #pragma unroll
   for (int i = 0; i < TILE; i += 128) {
     const int r = i + lane * 4, row = at.row(t, r);
-    if (r < TILE && row >= 0) ts_copy16(rows + r * 4, from.row_scales + row + (r & in_box));
+    if (r < TILE) ts_copy16_or_zeros(rows + r * 4, from.row_scales + max(row, 0) + (r & in_box), row >= 0);
   }
 }
 
@@ -1251,7 +1258,7 @@ __global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
         for (int i = 0; i < turns; ++i) {
           const int r0 = (turn0 + i) * 16 * SL;
           const int pos0 = t * kTsTile<FMT> + r0;
-          if (pos0 >= vis) break;
+          if (pos0 >= vis || (PAGED && n0 >= nq)) break;
           const unsigned gone = absent >> (r0 / 16) & ((1u << SL) - 1u);  // slices whose page is not there
           using Slices = std::integral_constant<int, SL>;
           if (pos0 + 16 * SL <= past && !gone) {

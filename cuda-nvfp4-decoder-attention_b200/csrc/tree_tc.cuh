@@ -103,8 +103,14 @@ struct TtCfg {
   static constexpr uint32_t kOffPrefix = kOffUnits + kUnits;
   // Stream 1's o of up to 64 rows overlays Q when the streams are joined.
   static_assert(kPanels * kQPanel >= 64u * D * 4, "room to join the streams");
-  static constexpr uint32_t bytes(int batch) { return kOffPrefix + 4u * (batch + 1) + 1024; }
+  template <bool PAGED = false>
+  static constexpr uint32_t bytes(int batch) { return kOffPrefix + (PAGED ? 12u : 4u) * (batch + 1) + 1024; }
 };
+
+// PAGED: what a segment costs beside its tiles, in tiles (see kTsSegment).  us for 0, 4, 8, 12, 16 of them: 64 rows of 32
+// sequences of 100 to 4,000 positions, head_dim 128, BF16 91, 56, 52, 52, 52, NVFP4 120, 75, 64, 61, 62.
+constexpr int kTtSegment = 12;
+constexpr int kTtGoneSlots = 16;  // tiles whose missing pages are kept: more than the loads are ahead of the softmax
 
 // ---------------------------------------------------------------- tcgen05
 // Shared-memory operand descriptors, 128-byte swizzle: start address >> 4
@@ -258,7 +264,10 @@ __device__ __forceinline__ float tt_v_global(const KvStore& v, int64_t row, int 
   return ((d & 1) ? pair.y : pair.x) * f16x2_to_f32x2(e4m3x2_to_f16x2(v.block_scales[row * (D / 16) + d / 16])).x;
 }
 
-template <int D, int FMT, bool SPLIT>
+// PAGED: a tile's boxes come from the pages that the block table names, K's by the loading warp and V's by the one
+// that copies scales; boxes of pages that are not there, and their scales, come in as zeros, and the softmax leaves
+// their keys out.
+template <int D, int FMT, bool SPLIT, bool PAGED = false>
 __global__ void __launch_bounds__(kTtThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const TreeStreamParams p) {
@@ -274,6 +283,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile unsigned s_bad;    // a wait gave up
   __shared__ volatile unsigned s_wild;   // an infinity or NaN was taken out of V
+  [[maybe_unused]] __shared__ unsigned s_gone[PAGED ? kTtGoneSlots : 1];  // of a tile, 16-key slices that are not there
+  [[maybe_unused]] __shared__ int s_range[PAGED ? 4 : 1];                 // places, G, first tile, end
   __shared__ float4 join[2][kTtRows];    // a stream's m, l and the unit of its o, where the two are joined
   int* prefix = reinterpret_cast<int*>(smem + C::kOffPrefix);
   float* units_kv = reinterpret_cast<float*>(smem + C::kOffUnits);  // [slot][kUnitFloats]
@@ -292,7 +303,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&ring_full[i], 33);  // the codes' bytes, and the lanes that copy scales
+      mbar_init(&ring_full[i], PAGED ? 34 : 33);  // the codes' bytes, and the lanes that copy scales
       mbar_init(&ring_free[i], kTtPrepWarps);
       mbar_init(&k_full[i], kQuant ? kTtPrepWarps / 2 : 1);
       mbar_init(&k_free[i], SPLIT ? 2 : 1);  // each stream that reads the tile
@@ -322,7 +333,17 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   pdl_wait();
   if (tid < 2) p.part_slots[2 * cta + tid] = make_int4(-1, 0, 0, 0);
   tt_fence_before();
-  ts_prefix(p, units, kTtKeys, prefix);
+  ts_prefix<PAGED>(p, units, kTtKeys, prefix);
+  if constexpr (PAGED) {
+    if (tid == 0) {
+      const int places = ts_places(p, prefix, units), g = min(places, p.grid);
+      s_range[0] = places;
+      s_range[1] = g;
+      s_range[2] = cta < g ? ts_first_tile_weighted(p, prefix, units, cta, g) : 0;
+      s_range[3] = cta < g ? ts_first_tile_weighted(p, prefix, units, cta + 1, g) : 0;
+    }
+    __syncthreads();
+  }
   tt_fence_after();
   const uint32_t tmem = tmem_slot;
   // Tensor memory columns: scores [stream][buffer][64], then o [stream][D].
@@ -332,6 +353,12 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   // Each role walks the CTA's range itself (kept apart, so that no role holds
   // another's registers).
   auto range = [&](int& n_tiles, int& G, int& x0) {
+    if constexpr (PAGED) {
+      n_tiles = s_range[0];
+      G = s_range[1];
+      x0 = s_range[2];
+      return s_range[3];
+    }
     n_tiles = prefix[p.batch];
     G = min(n_tiles, p.grid);
     x0 = cta < G ? ts_first_tile(n_tiles, cta, G) : 0;
@@ -352,7 +379,61 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTtOtherRegs));
     TsWalk w;
     bool more = begin(w);
-    if (kQuant && warp == kTtLoadWarp + 2) {
+    if (PAGED && (warp == kTtLoadWarp || warp == kTtLoadWarp + 2)) {
+      // ---------------------------------------------------------------- pages: K, or V and the scales of both
+      const bool is_v = warp != kTtLoadWarp;
+      constexpr int kRing = kQuant ? (C::kStages ? C::kStages : 1) : C::kK;
+      static_assert(kQuant || C::kK == C::kV, "one ring each of the same length");
+      uint64_t* full = kQuant ? ring_full : is_v ? v_raw : k_full;
+      uint64_t* empty = kQuant ? ring_free : is_v ? v_free : k_free;
+      TsBoxes<kTtKeys> at;
+      TtRing<kRing> r;
+      int filled = 0;
+      bool ok = true;
+      for (; more && ok; more = w.next()) {
+        at.begin(p, w.b, w.u / p.passes, ts_lengths(p, prefix)[w.b].y, w.t0, w.t1, lane);
+        for (int t = w.t0; t < w.t1; ++t) {
+          ok = __all_sync(kFull, ts_wait(&empty[r.i], r.phase ^ 1u, &s_bad));
+          if (!ok) break;
+          at.advance(p, t, lane);
+          const int mine = at.row(t, lane << p.box_log2), of_slice = at.row(t, lane * 16);
+          const unsigned gone = __ballot_sync(kFull, lane < kTtKeys / 16 && of_slice < 0);
+          if (lane == 0) {
+            if (!is_v) s_gone[filled & (kTtGoneSlots - 1)] = gone;
+            mbar_arrive_expect_tx(&full[r.i], kQuant ? Codes::kCodes : C::kOperand);
+          }
+          __syncwarp();
+          uint8_t* st = smem + (kQuant ? C::kOffRing + r.i * Codes::kStage
+                                       : (is_v ? C::kOffV : C::kOffK) + r.i * C::kOperand);
+          if (lane < 1 << at.per_log2) {
+            // Behind the pool's last row: zeros.
+            const int from = mine >= 0 ? mine : p.pg.pages * p.kv_heads * p.pg.page_size;
+            const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+            if constexpr (kQuant) {  // rows stand in groups of 16
+              ts_tma_2d(st + (is_v ? Codes::kOffV : 0) + (lane << p.box_log2) * Codes::kRowBytes, map, 0,
+                        from / 16 * (16 * Codes::kRowBytes / 128), &full[r.i]);
+            } else {
+#pragma unroll
+              for (int pn = 0; pn < C::kPanels; ++pn)
+                ts_tma_2d(st + pn * (kTtKeys * 128) + (lane << p.box_log2) * 128, map, pn * 64, from, &full[r.i]);
+            }
+          }
+          __syncwarp();
+          if constexpr (kQuant) {
+            if (is_v) {
+              ts_load_scales_paged<D, FMT, Codes, kTtKeys>(st + Codes::kOffKb, st + Codes::kOffKr, p.k, at, t, lane);
+              ts_load_scales_paged<D, FMT, Codes, kTtKeys>(st + Codes::kOffVb, st + Codes::kOffVr, p.v, at, t, lane);
+              ts_copy_arrive(&full[r.i]);
+            }
+          }
+          ++filled;
+          r.next();
+        }
+      }
+      if constexpr (kQuant) ts_copies_landed();
+      if (lane == 0) ts_all_landed<kRing>(full, filled);
+      __syncwarp();
+    } else if (kQuant && warp == kTtLoadWarp + 2) {
       // ---------------------------------------------------------------- scales (see ts_load_scales)
       const int64_t all_rows = static_cast<int64_t>(p.batch) * p.kv_heads * p.capacity;
       TtRing<C::kStages ? C::kStages : 1> rk;
@@ -528,7 +609,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       int slot = 0;
       bool ok = true;
       for (; more && ok; more = w.next()) {
-        const int past = ts_past(p, w.b), vis = ts_visible(p, w.b);
+        const int past = PAGED ? ts_lengths(p, prefix)[w.b].x : ts_past(p, w.b);
+        const int vis = PAGED ? ts_lengths(p, prefix)[w.b].y : ts_visible(p, w.b);
         for (int t = w.t0; t < w.t1; ++t) {
           const int key0 = t * kTtKeys;
           const bool edge = key0 + kTtKeys > past;
@@ -645,6 +727,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     uint32_t s_count = 0, o_count = 0, end_phase = 0, o_end_phase = 0;  // scores seen, P tiles given, segments ended
     bool first_segment = true;
     int slot0 = 0;  // unit slot of the segment's first tile
+    [[maybe_unused]] int tile0 = 0;  // the CTA's tiles before the segment
     bool ok = true;
     // Row of Q and of the context of row n of a pass of unit u.
     auto q_row = [&](int64_t b, int u, int n) {
@@ -653,7 +736,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     };
     for (; more && ok; more = w.next()) {
       const int b = w.b, kvh = w.u / p.passes, pass = w.u % p.passes, tiles = w.t1 - w.t0;
-      const int past = ts_past(p, b), vis = ts_visible(p, b);
+      const int past = PAGED ? ts_lengths(p, prefix)[b].x : ts_past(p, b);
+      const int vis = PAGED ? ts_lengths(p, prefix)[b].y : ts_visible(p, b);
       const int n_first = pass * p.rows_per_pass, rows = min(p.rows_per_pass, nq - n_first);
       const bool shifted = upper;
       const int half = (rows + 1) / 2;
@@ -740,7 +824,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         const int key0 = (w.t0 + i) * kTtKeys;
         // Keys of the tile this row sees, one bit each.  With a mask, a lane per key and a vote per token: a byte at a
         // time per row, it took a fifth of a one-tile segment's time.
-        const bool edge = key0 + kTtKeys > past;
+        bool edge = key0 + kTtKeys > past;
         unsigned long long seen = ~0ull;
         if (edge) {
           if (!p.mask) {
@@ -768,6 +852,15 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         ok = ts_wait(&s_full[s][buf], (s_count >> 1) & 1, &s_bad);
         if (!(ok = __all_sync(kFull, ok))) break;
         tt_fence_after();
+        if constexpr (PAGED) {
+          const unsigned gone = s_gone[(tile0 + i) & (kTtGoneSlots - 1)];
+          if (gone) {
+            edge = true;
+#pragma unroll
+            for (int z = 0; z < kTtKeys / 16; ++z)
+              if (gone >> z & 1u) seen &= ~(0xffffull << (16 * z));
+          }
+        }
         ++s_count;
         const uint32_t s_at = s_col(s, buf) + lanes;
         const float* unit = units_kv + ((slot0 + i) & (kTtUnitSlots - 1)) * C::kUnitFloats;
@@ -941,6 +1034,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         else tile(std::false_type{});
       }
       slot0 = (slot0 + tiles) & (kTtUnitSlots - 1);
+      if constexpr (PAGED) tile0 += tiles;
       // Every P V of the segment.  (Waiting on o_done here could miss it: it may be one or two phases on.)
       ok = ok && ts_wait(&o_end[s], o_end_phase, &s_bad);
       ok = __all_sync(kFull, ok);
@@ -1006,7 +1100,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         int n_tiles, G, x0;
         range(n_tiles, G, x0);
         const int64_t slot = 2 * static_cast<int64_t>(cta) + (w.x == x0 ? 0 : 1);
-        if (!whole && tid == 0) ts_write_slot(p, n_tiles, G, cta, x0, w);
+        if (!whole && tid == 0) ts_write_slot<PAGED>(p, n_tiles, G, cta, x0, w);
+        const bool padding = PAGED && tok >= ts_tokens<PAGED>(p, b);
+        if (padding) lj = f_own = f_other = 0.0f;
         const float inv = lj == 0.0f ? 0.0f : __fdiv_rn(1.0f, lj);
         const int64_t v_row = (b * p.kv_heads + kvh) * p.capacity;
         // Infinities and NaN of V that were taken out, for the rows that see them: 16 columns.  They were taken out of
@@ -1015,9 +1111,15 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           const int first = max(past / kTtKeys * kTtKeys, w.t0 * kTtKeys), last = min(vis, w.t1 * kTtKeys);
           for (int pos = first; pos < last; ++pos) {
             if (!tree_sees(mask_row, tok, pos - past)) continue;
+            int64_t row = v_row + pos;
+            if constexpr (PAGED) {
+              const int page = paged_page(p.pg, b, pos);
+              if (page < 0) continue;
+              row = (static_cast<int64_t>(page) * p.kv_heads + kvh) * p.pg.page_size + pos % p.pg.page_size;
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float x = tt_v_global<D, FMT>(p.v, v_row + pos, c + e);
+              const float x = tt_v_global<D, FMT>(p.v, row, c + e);
               if (!isfinite(x)) o[e] += x;
             }
           }
@@ -1100,7 +1202,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               o[e] = (f_own == 0.0f ? 0.0f : o[e] * f_own) + (f_other == 0.0f ? 0.0f : o1[e] * f_other);
-            if (s_wild) add_wild(c, o);
+            if (s_wild && !padding) add_wild(c, o);
             if (whole) {
               uint4* dst = reinterpret_cast<uint4*>(p.ctx + q_row_own * D + c);
 #pragma unroll

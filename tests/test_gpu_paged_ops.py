@@ -294,6 +294,48 @@ def test_padded_batches_and_pages_that_are_gone(cp, format, d, size):
 
 
 @pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [8, 9, 12, 13, 32, 33, 64, 65, 128, 129, 256, 257, 600])
+def test_rows_on_both_sides_of_every_kernel_rule(cp, format, d, rows):
+    """Ragged sequences, one of them padding, pages that are gone, trees; every number of query rows a rule looks at."""
+    group = next(g for g in (4, 3, 2, 1) if rows % g == 0) if rows != 600 else 8
+    t, pasts, size = rows // group, [0, 333, 64, 201], {64: 32, 128: 16}[d]
+    cache, table = sequences(cp, format, pasts, t, 2, size, d, rows)
+    counts = torch.tensor([t, t, 0, max(1, t // 2)])
+    table[1, 2], table[1, 5], table[3, 0] = -1, cache.pages, -7
+    mask = draft_reference.random_tree(4, t, rows)[0]
+    q = randn((4, t, 2 * group, d), 3)
+    q[2], q[3, counts[3]:] = float("nan"), float("inf")
+    got = cp.cuda_paged_attention(q.cuda(), cache, table.cuda(), past_lengths=torch.tensor(pasts).cuda(),
+                                  max_past_length=333, counts=counts.cuda(), tree_mask=mask.cuda())
+    check_context(got, *ref.attention(q.nan_to_num(0, 0, 0), cache, table, pasts, mask, counts))
+    assert (got[2] == 0).all() and (got[3, counts[3]:] == 0).all()
+
+
+@pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
+@pytest.mark.parametrize("t", [1, 8, 40])
+def test_infinities_in_rows_that_are_seen(cp, format, t):
+    """Rows of V with an infinity or NaN reach the queries that see them, and no other."""
+    pasts, size, d = [100, 70], 16, 128
+    cache, table = sequences(cp, format, pasts, t, 1, size, d, 41)
+    rows = randn((2, 1, 1, d), 9).cuda()
+    rows[0, 0, 0, 5] = float("inf")
+    wild = torch.tensor([[int(table[0, 37 // size]) * size + 37 % size],
+                         [int(table[1, (70 + t - 1) // size]) * size + (70 + t - 1) % size]])
+    cp.cuda_paged_kv_append_(cache, randn((2, 1, 1, d), 8).cuda(), rows, wild.cuda())
+    q = randn((2, t, 4, d), 3)
+    got = cp.cuda_paged_attention(q.cuda(), cache, table.cuda(), past_lengths=torch.tensor(pasts).cuda(),
+                                  max_past_length=100)
+    bad = ~torch.isfinite(got)
+    assert bad[0, :, :, 5].all() and not bad[1].any()
+    if format == "bf16":  # a quantised row with an infinity is NaN throughout
+        bad[0, :, :, 5] = False
+        assert not bad.any()
+    else:
+        assert bad[0].all()
+
+
+@pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
 def test_masks_that_leave_a_row_empty(cp, format):
     cache, table = sequences(cp, format, [0, 0], 3, 2, 16, 64, 5)
     mask = torch.tensor([[[0, 0, 0], [1, 1, 0], [0, 0, 0]], [[1, 0, 0], [0, 0, 0], [0, 0, 1]]]).bool()
