@@ -69,15 +69,16 @@ cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& 
       case 128: return launch_tree_stream<128, FMT, 1, true>(tk, tv, p, s);
       default: return launch_tree_stream<256, FMT, 1, true>(tk, tv, p, s);
     }
-  }
-  switch (head_dim) {
-    case 64:
-      return wide == 2 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
-    case 128:
-      if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
-        if (wide == 2) return launch_tree_stream<128, FMT, 2>(tk, tv, p, s);
-      return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
-    default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
+  } else {
+    switch (head_dim) {
+      case 64:
+        return wide == 2 ? launch_tree_stream<64, FMT, 2>(tk, tv, p, s) : launch_tree_stream<64, FMT, 1>(tk, tv, p, s);
+      case 128:
+        if constexpr (FMT == kKvFmtBf16)  // codes: tcgen05 from 9 rows on
+          if (wide == 2) return launch_tree_stream<128, FMT, 2>(tk, tv, p, s);
+        return launch_tree_stream<128, FMT, 1>(tk, tv, p, s);
+      default: return launch_tree_stream<256, FMT, 1>(tk, tv, p, s);
+    }
   }
 }
 
