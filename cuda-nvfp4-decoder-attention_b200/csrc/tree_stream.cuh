@@ -103,9 +103,9 @@ constexpr float kTsMinUnit = 7.88860905e-31f;  // 2^-100
 template <int D, int FMT, int NG, int NW, int SL, int TILE = kTsTile<FMT>, bool PAGED = false>
 struct TsCfg {
   static_assert(D == 64 || D == 128 || D == 256, "head_dim 64, 128 or 256");
-  // Consumers, two loading and two joining warps; PAGED: four loading ones, and two that make up a warpgroup.
-  static constexpr int kLoaders = PAGED ? 4 : 2;
-  static constexpr int kThreads = (NW + (PAGED ? 8 : 4)) * 32;
+  // Consumers, two loading and two joining warps; PAGED: four of each.
+  static constexpr int kLoaders = PAGED ? 4 : 2, kJoiners = PAGED ? 4 : 2;
+  static constexpr int kThreads = (NW + kLoaders + kJoiners) * 32;
   static constexpr int kRowBytes = FMT == kKvFmtBf16 ? 2 * D : (FMT == kKvFmtE4m3 ? D : D / 2);
   static constexpr uint32_t kCodes = TILE * kRowBytes;  // one of K, V
   static constexpr uint32_t kBlockScales = FMT == kKvFmtNvfp4 ? TILE * (D / 16) : 0;
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
     }
     for (int i = 0; i < Cfg::kJoins; ++i) {
       mbar_init(&join_full[i], NW);
-      mbar_init(&join_free[i], 2);
+      mbar_init(&join_free[i], Cfg::kJoiners);
     }
     fence_mbar_init();
     s_bad = 0u;
@@ -624,11 +624,10 @@ __global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
   if constexpr (PAGED) {
     if (warp < NW) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTsPagedRegs));
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTsPagedOtherRegs));
-    if (warp >= NW + Cfg::kLoaders + 2) return;
   }
 
   if (warp >= NW + Cfg::kLoaders) {
-    // ---------------------------------------------------------------- joins: every other row of a segment
+    // ---------------------------------------------------------------- joins: every kJoiners-th row of a segment
     TsWalk w;
     bool more = w.begin(prefix, p.batch, units, x0, x1);
     int buf = 0;
@@ -642,7 +641,7 @@ __global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
       if (!whole && warp == NW + Cfg::kLoaders && lane == 0) ts_write_slot<PAGED>(p, n_tiles, G, cta, x0, w);
       if (!__all_sync(kFull, ts_wait(&join_full[buf], phase, &s_bad))) return;
       const float *so = join_o(buf), *sm_m = join_m(buf), *sm_l = sm_m + NW * Cfg::kRows;
-      for (int r = warp - NW - Cfg::kLoaders; r < rows; r += 2) {
+      for (int r = warp - NW - Cfg::kLoaders; r < rows; r += Cfg::kJoiners) {
         // Position warp `lane` of the row's chunk: its factor.
         const int chunk = r / Cfg::kRows, rr = r % Cfg::kRows;
         const int at = (lane * rc_n + chunk) * Cfg::kRows + rr;
