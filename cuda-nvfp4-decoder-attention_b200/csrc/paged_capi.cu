@@ -55,10 +55,18 @@ constexpr int64_t paged_tc_min_rows(int64_t head_dim, int format) {
   return format == NVFP4DA_KV_BF16 ? (head_dim == 64 ? 17 : 9) : format == NVFP4DA_KV_E4M3 && head_dim == 64 ? 33 : 17;
 }
 
+// Groups of 8 query rows that a warp of the streaming kernel holds.  Wider warps decode codes fewer times, but have less
+// of a tile each: us for 1, 2, 3 groups, E4M3, head_dim 64, 8 KV heads, 37 sequences of 90 to 6,003 positions: 12 rows 61,
+// 62, 75; 20 rows 90, 84, 78; 32 rows 94, 88, 113.  20 rows of 8 sequences of 8,000 to 12,000 at head_dim 128: 106, 113.
+int paged_width(int64_t head_dim, int format, int64_t rows) {
+  return head_dim != 64 || format != NVFP4DA_KV_E4M3 || rows <= 16 ? 1 : rows <= 24 ? 3 : 2;
+}
+
 // Plan of the paged attention.
 struct PagedPlan {
   bool stream;  // tree_stream_kernel (or tc: tree_tc_kernel), else the general kernel
   bool tc;
+  int wide;  // groups of 8 query rows per warp
   int row_chunks, rows_per_pass, passes, tile, box;
   int splits;   // general kernel
   int64_t split_len;
@@ -102,8 +110,9 @@ int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int6
       pl.rows_per_pass = static_cast<int>(ceil_div(nq, pl.passes));
     } else {
       pl.row_chunks = 1;
-      while (pl.row_chunks < kTsWarps && 8 * pl.row_chunks < nq) pl.row_chunks *= 2;
-      pl.rows_per_pass = 8 * pl.row_chunks;
+      pl.wide = paged_width(d, c->format, nq);
+      while (pl.row_chunks < kTsWarps && 8 * pl.wide * pl.row_chunks < nq) pl.row_chunks *= 2;
+      pl.rows_per_pass = 8 * pl.wide * pl.row_chunks;
       pl.passes = static_cast<int>(ceil_div(nq, pl.rows_per_pass));
     }
     pl.tile = pl.tc ? kTtKeys : c->format == NVFP4DA_KV_BF16 ? kTsTile<kKvFmtBf16> : kTsTile<kKvFmtE4m3>;
@@ -295,7 +304,9 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     t.part_o = reinterpret_cast<float*>(t.part_slots + 2 * t.grid);
     t.part_ml = reinterpret_cast<float2*>(t.part_o + static_cast<size_t>(2 * t.grid) * pl.rows_per_pass * c->head_dim);
     t.pg = pg;
-    t.seg = pl.tc ? kTtSegment : c->format == NVFP4DA_KV_BF16 ? kTsSegment<kKvFmtBf16> : kTsSegment<kKvFmtE4m3>;
+    t.seg = pl.tc                               ? kTtSegment
+            : c->format == NVFP4DA_KV_BF16 ? kTsSegment<kKvFmtBf16>
+                                           : kTsSegment<kKvFmtE4m3> + pl.wide - 1;
     t.loaders = pl.box < pl.tile ? 4 : 2;
     while (2 << t.box_log2 <= pl.box) ++t.box_log2;
     if (pl.tc) {
@@ -308,10 +319,10 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
       return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "tensor-core paged attention launch");
     }
     cudaError_t e = c->format == NVFP4DA_KV_BF16
-                        ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, 1, tk, tv, t, s)
+                        ? launch_tree_stream_d<kKvFmtBf16, true>(c->head_dim, pl.wide, tk, tv, t, s)
                     : c->format == NVFP4DA_KV_E4M3
-                        ? launch_tree_stream_d<kKvFmtE4m3, true>(c->head_dim, 1, tk, tv, t, s)
-                        : launch_tree_stream_d<kKvFmtNvfp4, true>(c->head_dim, 1, tk, tv, t, s);
+                        ? launch_tree_stream_d<kKvFmtE4m3, true>(c->head_dim, pl.wide, tk, tv, t, s)
+                        : launch_tree_stream_d<kKvFmtNvfp4, true>(c->head_dim, pl.wide, tk, tv, t, s);
     return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "streaming paged attention launch");
   }
   TreeAttnParams p{};

@@ -61,11 +61,13 @@ template <int FMT, bool PAGED = false>
 cudaError_t launch_tree_stream_d(int64_t head_dim, int wide, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const TreeStreamParams& p, cudaStream_t s) {
   if constexpr (PAGED) {
-    // One width: wider warps have fewer of them at a tile, and what they save in decoding they lose.  us for 1, 2, 3
-    // groups of 8 rows a warp, 8 x 8 KV heads, 8,000 to 12,000 positions: 20 rows of E4M3, head_dim 64, 80, 75, 70 (300
-    // positions 26, 27, 29), 64 rows 88, 88, 106; head_dim 128 20 rows 106, 113, BF16 105, 102.
     switch (head_dim) {
-      case 64: return launch_tree_stream<64, FMT, 1, true>(tk, tv, p, s);
+      case 64:
+        if constexpr (FMT == kKvFmtE4m3) {  // the others: tcgen05 from 17 rows on
+          if (wide == 3) return launch_tree_stream<64, FMT, 3, true>(tk, tv, p, s);
+          if (wide == 2) return launch_tree_stream<64, FMT, 2, true>(tk, tv, p, s);
+        }
+        return launch_tree_stream<64, FMT, 1, true>(tk, tv, p, s);
       case 128: return launch_tree_stream<128, FMT, 1, true>(tk, tv, p, s);
       default: return launch_tree_stream<256, FMT, 1, true>(tk, tv, p, s);
     }

@@ -295,7 +295,7 @@ def test_padded_batches_and_pages_that_are_gone(cp, format, d, size):
 
 @pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("rows", [8, 9, 12, 13, 32, 33, 64, 65, 128, 129, 256, 257, 600])
+@pytest.mark.parametrize("rows", [8, 9, 12, 13, 16, 17, 24, 25, 32, 33, 64, 65, 128, 129, 256, 257, 600])
 def test_rows_on_both_sides_of_every_kernel_rule(cp, format, d, rows):
     """Ragged sequences, one of them padding, pages that are gone, trees; every number of query rows a rule looks at."""
     group = next(g for g in (4, 3, 2, 1) if rows % g == 0) if rows != 600 else 8
@@ -310,6 +310,17 @@ def test_rows_on_both_sides_of_every_kernel_rule(cp, format, d, rows):
                                   max_past_length=333, counts=counts.cuda(), tree_mask=mask.cuda())
     check_context(got, *ref.attention(q.nan_to_num(0, 0, 0), cache, table, pasts, mask, counts))
     assert (got[2] == 0).all() and (got[3, counts[3]:] == 0).all()
+
+
+@pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
+@pytest.mark.parametrize("t", [2, 5, 40])
+def test_many_rows_of_wide_heads(cp, format, t):
+    """Head dimension 256 keeps the streaming kernel, whatever the rows."""
+    cache, table = sequences(cp, format, [70, 5], t, 2, 16, 256, 51)
+    q = randn((2, t, 16, 256), 3)
+    got = cp.cuda_paged_attention(q.cuda(), cache, table.cuda(), past_lengths=torch.tensor([70, 5]).cuda(),
+                                  max_past_length=70)
+    check_context(got, *ref.attention(q, cache, table, [70, 5]))
 
 
 @pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
