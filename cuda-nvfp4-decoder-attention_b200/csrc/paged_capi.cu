@@ -396,14 +396,15 @@ int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, c
   p.next = next_tokens;
   p.pieces = static_cast<int>(ceil_div(ceil_div(vocab, kVerifyPiece), kVerifyMaxSegments));
   p.segments = static_cast<int>(ceil_div(vocab, static_cast<int64_t>(kVerifyPiece) * p.pieces));
-  // CTAs a sequence, a power of two: as many as have a segment for every warp and as fit the GPU two to an SM with
-  // the rest of the batch.  us for 1, 2, 4, 8 CTAs: one sequence of 128,000 tokens 37, 27, 20, 16; 8 of them 74, 46,
-  // 33, 25; 64 of them 105, 68, 57, 63; 128 of 32,000 24, 25, 31, 47.
-  const int64_t most = std::min<int64_t>(2LL * sm_count() / batch, ceil_div(p.segments, kVerifyWarps));
+  // CTAs a sequence, a power of two: as many as have a segment for every warp and as fit the GPU four to an SM with the
+  // rest of the batch.  Twice as many warps a CTA: 48 given trees 23 -> 25 us, 64 trees over 128,000 tokens 53 -> 57, 256
+  // over 32,000 43 -> 53.
+  const int64_t most = std::min<int64_t>(4LL * sm_count() / batch, ceil_div(p.segments, kVerifyWarps));
   unsigned ctas = 1;
   while (ctas < kVerifyMaxCluster && 2 * ctas <= most) ctas *= 2;
   const size_t smem = verify_smem(p.nodes, p.segments);
   cudaError_t e = ensure_smem(verify_drafted_kernel, static_cast<uint32_t>(smem));
+  if (e == cudaSuccess && ctas > 8) e = ensure_big_clusters(verify_drafted_kernel);
   if (e == cudaSuccess)
     e = launch_cluster(verify_drafted_kernel, dim3(static_cast<unsigned>(batch) * ctas), dim3(kVerifyThreads), smem,
                        static_cast<cudaStream_t>(stream), true, ctas, p);

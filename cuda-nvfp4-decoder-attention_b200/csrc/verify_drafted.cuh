@@ -36,8 +36,8 @@
 
 namespace nvfp4da {
 
-constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
-constexpr int kVerifyMaxNodes = 1024, kVerifyMaxCluster = 8;
+constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyMaxNodes = 1024, kVerifyMaxCluster = 16;
 constexpr int kVerifyPiece = 512;  // elements a warp has in flight
 constexpr int kVerifyMaxSegments = 1024;
 
