@@ -371,6 +371,41 @@ def test_many_ragged_sequences(cp, format):
     check_context(got, *ref.attention(q, cache, table, pasts))
 
 
+@pytest.mark.parametrize("format,b", [("bf16", 1024), ("nvfp4", 1024), ("fp8", 1025)])
+def test_as_many_sequences_as_the_streaming_kernel_takes_and_one_more(cp, format, b):
+    g = torch.Generator().manual_seed(b)
+    pasts = torch.randint(0, 60, (b,), generator=g).tolist()
+    cache, table = sequences(cp, format, pasts, 1, 1, 16, 64, 61)
+    q = randn((b, 1, 2, 64), 3)
+    got = cp.cuda_paged_attention(q.cuda(), cache, table.cuda(), past_lengths=torch.tensor(pasts).cuda(),
+                                  max_past_length=60)
+    check_context(got, *ref.attention(q, cache, table, pasts))
+
+
+@pytest.mark.parametrize("format", ["bf16", "fp8"])
+def test_offsets_past_32_bits(cp, format):
+    """A pool of more than 2^31 elements; the sequence lives on its last pages."""
+    pages, hkv, size, d, n = 17000, 8, 64, 256, 150
+    cache = cp.PagedKVCache.allocate(pages, hkv, size, d, format)
+    assert cache.k_codes.numel() > 1 << 31
+    table = torch.tensor([[pages - 1, pages - 3, pages - 2]], dtype=torch.int32)
+    at = torch.arange(n)
+    slots = (table[0, at // size].long() * size + at % size)[None].cuda()
+    k, v = (randn((1, n, hkv, d), s).cuda() for s in (1, 2))
+    cp.cuda_paged_kv_append_(cache, k, v, slots)
+    got = cp.cuda_paged_kv_read(cache, slots)
+    tail = cp.PagedKVCache(format, d, *(getattr(cache, f"{n}_{f}")[-3:].clone() if getattr(cache, f"{n}_{f}") is not None
+                                        else None for f in ("codes", "row_scales", "block_scales") for n in "kv"))
+    tail_table = table - (pages - 3)
+    want = cp.cuda_paged_kv_read(tail, (tail_table[0, at // size].long() * size + at % size)[None].cuda())
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and (got[0] != 0).any()
+    for rows in (1, 3):  # the streaming kernel, and with a head dimension of 256 many rows of it
+        q = randn((1, rows, 4 * hkv, d), 3)
+        past = torch.tensor([n - rows]).cuda()
+        got = cp.cuda_paged_attention(q.cuda(), cache, table.cuda(), past_lengths=past, max_past_length=n)
+        check_context(got, *ref.attention(q, tail, tail_table, [n - rows]))
+
+
 @pytest.mark.parametrize("format", ["bf16", "fp8", "nvfp4"])
 @pytest.mark.parametrize("t", [1, 5])
 def test_paged_is_the_whole_cache_s_attention(cp, format, t):

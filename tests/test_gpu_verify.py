@@ -173,6 +173,24 @@ def test_repeated_and_captured_calls_agree(cp):
     assert all(x.tolist() == y for x, y in zip(out, want))
 
 
+def test_offsets_past_32_bits_and_the_longest_chain(cp):
+    """More than 2^31 probabilities: one-hot rows lead down a chain of 1,024 nodes."""
+    b, t, v = 2, 1024, (1 << 20) + 4
+    target = torch.zeros((b, t, v), device="cuda")
+    tokens = torch.randint(0, v, (b, t), generator=torch.Generator().manual_seed(1)).cuda()
+    node = torch.arange(t - 1).cuda()
+    for i in range(b):
+        target[i, node, tokens[i, 1:]] = 1.0
+        target[i, t - 1, v - 1 - i] = 0.25
+    u = torch.full((b, t), 0.9).cuda()
+    path, counts, nexts = cp.cuda_verify_drafted(target, tokens, u)
+    assert counts.tolist() == [t, t] and nexts.tolist() == [v - 1, v - 2]
+    assert torch.equal(path, torch.arange(t).cuda().expand(b, t))
+    tokens[1, 700] = (tokens[1, 700] + 1) % v  # a candidate that has no probability: the row's own token is drawn
+    path, counts, nexts = cp.cuda_verify_drafted(target, tokens, u)
+    assert counts.tolist() == [t, 700] and nexts[1] == (tokens[1, 700] - 1) % v and (path[1, 700:] == -1).all()
+
+
 def test_refusals(cp):
     target, draft, tokens, parents, u = (x.cuda() for x in problem(2, 3, 10, True, 1))
 
