@@ -57,6 +57,27 @@
 // 12 or 16 consumer warps, for which registers suffice with one slice at a time,
 // were no faster.
 //
+// PAGED (paged_kv.cuh): the cache is a pool of pages, position j of sequence b row
+// j % S of page table[b, j / S].
+//   tiles     come in boxes of 2^k positions (the largest that divides the page and
+//             the tile), each a TMA copy of its own; with more than one a tile, two
+//             warps copy K and two V, since a thread takes some 200 cycles to issue
+//             a copy.  Copied 16 bytes a lane instead, E4M3 in pages of 16 took 176
+//             us where the TMA unit took 111.  A warp looks 32 boxes up at once.
+//   pages     that the table does not name, and padding (counts): the loading warp
+//             marks a tile's 16-position slices that are not there, consumers leave
+//             them out; a padding row's context is zeros.
+//   the line  is cut by weight, a segment counting kTsSegment tiles beside its own:
+//             64 E4M3 sequences of 10 to 2,000 positions 99 us unweighted, 61 so.
+//   a segment's start and end: lengths stand in shared memory, four warps join its
+//             rows, and its last slices are taken one at a time, half of the code to
+//             fetch (a segment had missed the instruction cache at every third
+//             request).
+// 64 sequences x 6 heads, 1,024 to 8,191 positions, one token: BF16 142 us, 6.3
+// TB/s, 0.96 of a copy; E4M3 in pages of 16 94 us, 4.9 TB/s (no arithmetic at all:
+// 10 us less); 8 x 32,768 of NVFP4 78 us: the ALU pipe's decoding (64 conversions
+// and 36 unpackings a slice), 45 % of the issue slots.
+//
 // Waits are bounded: one that lasts a second records kErrBarrierTimeout in
 // g_tree_errors, and every role of the CTA leaves (its results are then garbage;
 // the GPU stays usable).  The loading warps leave only when what they copy into

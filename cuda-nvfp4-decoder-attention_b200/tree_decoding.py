@@ -11,6 +11,7 @@ slots after the P_b committed positions, tree attention, the O projection.
     y, k, v = cuda_decoder_attention_tree_forward_(
         x, g_in, wq, wk, wv, g_q, g_k, wo, cache, depths=depths, tree_mask=mask, inv_freq=inv_freq,
         attention_factor=factor, past_lengths=past, max_past_length=bound)
+    path, counts, token = cuda_verify_drafted(target, drafted, uniforms, draft_probs=draft, parents=parents)
     accept_drafted_(cache, k, v, path, past_lengths=past, counts=counts)   # path: int64 [B, n]
     past += counts
 
