@@ -9,6 +9,7 @@
 #include "host_util.cuh"
 #include "kv_host.cuh"
 #include "page_table.cuh"
+#include "paged_general.cuh"
 #include "paged_kv.cuh"
 #include "tree_attention.cuh"
 #include "tree_launch.cuh"
@@ -62,13 +63,31 @@ int paged_width(int64_t head_dim, int format, int64_t rows) {
   return head_dim != 64 || format != NVFP4DA_KV_E4M3 || rows <= 16 ? 1 : rows <= 24 ? 3 : 2;
 }
 
+// CTAs an SM of paged_attn_general_kernel that the splits of the cache's length are to give.
+constexpr int64_t kPgenPerSm = 8;
+
+template <int FMT, int KS>
+cudaError_t launch_paged_general(dim3 grid, const TreeAttnParams& p, const PagedView& pg, cudaStream_t s) {
+  auto* kern = paged_attn_general_kernel<FMT, KS>;
+  cudaError_t e = ensure_smem(kern, pgen_smem<KS>());
+  return e != cudaSuccess ? e : launch(kern, grid, dim3(kPgenThreads), pgen_smem<KS>(), s, true, p, pg);
+}
+
+template <int FMT, int KS = 16>
+cudaError_t launch_paged_general_d(int64_t head_dim, dim3 grid, const TreeAttnParams& p, const PagedView& pg,
+                                   cudaStream_t s) {
+  if (head_dim == 16 * KS) return launch_paged_general<FMT, KS>(grid, p, pg, s);
+  if constexpr (KS > 1) return launch_paged_general_d<FMT, KS - 1>(head_dim, grid, p, pg, s);
+  return cudaErrorInvalidValue;
+}
+
 // Plan of the paged attention.
 struct PagedPlan {
-  bool stream;  // tree_stream_kernel (or tc: tree_tc_kernel), else the general kernel
+  bool stream;  // tree_stream_kernel (or tc: tree_tc_kernel), else paged_attn_general_kernel
   bool tc;
   int wide;  // groups of 8 query rows per warp
   int row_chunks, rows_per_pass, passes, tile, box;
-  int splits;   // general kernel
+  int splits;  // general kernel
   int64_t split_len;
   size_t bytes;
 };
@@ -120,10 +139,10 @@ int plan_paged(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages, int6
     pl.bytes = align_up(static_cast<size_t>(2 * sm_count()) * (pl.rows_per_pass * (d * 4 + 8) + 16), 256);
     return NVFP4DA_OK;
   }
-  const int64_t base = batch * c->kv_heads * ceil_div(group * tokens, kTreeWarps);
-  int64_t splits = std::min(ceil_div(8LL * sm_count(), base), ceil_div(visible, 128));
+  const int64_t base = batch * c->kv_heads * ceil_div(nq, kPgenRows);
+  int64_t splits = std::min(ceil_div(kPgenPerSm * sm_count(), base), ceil_div(visible, 2 * kPgenTile));
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, 1024));
-  pl.split_len = ceil_div(ceil_div(visible, splits), 32) * 32;
+  pl.split_len = ceil_div(ceil_div(visible, splits), kPgenTile) * kPgenTile;
   pl.splits = static_cast<int>(ceil_div(visible, pl.split_len));
   const size_t rows = static_cast<size_t>(batch * tokens * q_heads);
   pl.bytes = align_up(pl.splits > 1 ? rows * pl.splits * (c->head_dim + 2) * 4 : 16, 256);
@@ -326,7 +345,6 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
     return e == cudaSuccess ? NVFP4DA_OK : cuda_fail(e, "streaming paged attention launch");
   }
   TreeAttnParams p{};
-  p.pg = pg;
   p.q = q;
   p.k = k_store(*c);
   p.v = v_store(*c);
@@ -344,16 +362,13 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
   p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c->head_dim)));
   p.splits = pl.splits;
   p.split_len = pl.split_len;
-  p.lanes = std::max(2, lanes_per_row(c->head_dim, 8));
-  const int64_t group = q_heads / c->kv_heads;
-  const dim3 grid(static_cast<unsigned>(pl.splits), static_cast<unsigned>(ceil_div(group * tokens, kTreeWarps)),
+  const dim3 grid(static_cast<unsigned>(pl.splits),
+                  static_cast<unsigned>(ceil_div(q_heads / c->kv_heads * tokens, kPgenRows)),
                   static_cast<unsigned>(batch * c->kv_heads));
-  switch (c->format) {
-    case NVFP4DA_KV_BF16: tree_attn_general_kernel<kKvFmtBf16, true><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
-    case NVFP4DA_KV_E4M3: tree_attn_general_kernel<kKvFmtE4m3, true><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
-    default: tree_attn_general_kernel<kKvFmtNvfp4, true><<<grid, kTreeWarps * 32, 0, s>>>(p); break;
-  }
-  NVFP4DA_CHECK_LAUNCH("paged attention launch");
+  cudaError_t e = c->format == NVFP4DA_KV_BF16   ? launch_paged_general_d<kKvFmtBf16>(c->head_dim, grid, p, pg, s)
+                  : c->format == NVFP4DA_KV_E4M3 ? launch_paged_general_d<kKvFmtE4m3>(c->head_dim, grid, p, pg, s)
+                                                 : launch_paged_general_d<kKvFmtNvfp4>(c->head_dim, grid, p, pg, s);
+  if (e != cudaSuccess) return cuda_fail(e, "paged attention launch");
   if (pl.splits > 1) {
     const int64_t rows = batch * tokens * q_heads;
     tree_combine_kernel<<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, s>>>(p);

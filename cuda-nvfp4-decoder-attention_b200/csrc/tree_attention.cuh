@@ -20,7 +20,6 @@
 
 #include "common.cuh"
 #include "kv_quant.cuh"
-#include "paged_kv.cuh"
 
 namespace nvfp4da {
 
@@ -39,7 +38,6 @@ struct TreeAttnParams {
   int splits;
   int64_t split_len;
   int lanes;  // lanes per key (power of two >= D / 8)
-  PagedView pg;  // PAGED: the block table; the stores are a pool's, capacity = M * S
 };
 
 // P_b clamped so that the drafted slots lie in the cache.
@@ -73,10 +71,7 @@ constexpr int kTreeWarps = 4;
 // split, `lanes` lanes per key, 32 / lanes keys at a time, every lane 8
 // elements of the head.  Every row reads the keys again (from L2): this kernel
 // serves the head dimensions the streaming kernel does not.
-//
-// PAGED: position j of the sequence is row j % S of the page that the block table
-// names (paged_kv.cuh); positions of pages that it does not name are not seen.
-template <int FMT, bool PAGED = false>
+template <int FMT>
 __global__ void __launch_bounds__(kTreeWarps * 32) tree_attn_general_kernel(const TreeAttnParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = p.q_heads / p.kv_heads;
@@ -87,9 +82,7 @@ __global__ void __launch_bounds__(kTreeWarps * 32) tree_attn_general_kernel(cons
   const int sub = lane & (p.lanes - 1), d0 = sub * 8;
   const bool has = d0 < p.head_dim;
   const int64_t past = tree_past(p.past_lengths, p.past_length, b, p.capacity);
-  int tokens = p.tokens;
-  if constexpr (PAGED) tokens = paged_count(p.pg, b, p.tokens);
-  const int64_t end = PAGED && tokens == 0 ? 0 : min(past + tokens, p.capacity);
+  const int64_t end = min(past + p.tokens, p.capacity);
   const int64_t j0 = blockIdx.x * p.split_len, j1 = min(j0 + p.split_len, end);
   const uint8_t* mask_row = p.mask ? p.mask + b * p.mask_stride + static_cast<int64_t>(t) * p.tokens : nullptr;
   const int64_t out_row = (static_cast<int64_t>(b) * p.tokens + t) * p.q_heads + h;
@@ -109,17 +102,11 @@ __global__ void __launch_bounds__(kTreeWarps * 32) tree_attn_general_kernel(cons
   const int step = 32 / p.lanes;
   for (int64_t base = j0; base < j1; base += step) {
     const int64_t j = base + lane / p.lanes;
-    bool sees = j < j1 && tree_sees(mask_row, t, j - past);
-    int64_t row = row0 + j;
-    if constexpr (PAGED) {
-      const int page = sees && t < tokens ? paged_page(p.pg, b, static_cast<int>(j)) : -1;
-      sees = page >= 0;
-      row = (static_cast<int64_t>(page) * p.kv_heads + kvh) * p.pg.page_size + j % p.pg.page_size;
-    }
+    const bool sees = j < j1 && tree_sees(mask_row, t, j - past);
     float k[8] = {}, v[8] = {};
     if (sees && has) {
-      tree_load8<FMT>(p.k, row, d0, p.head_dim, k);
-      tree_load8<FMT>(p.v, row, d0, p.head_dim, v);
+      tree_load8<FMT>(p.k, row0 + j, d0, p.head_dim, k);
+      tree_load8<FMT>(p.v, row0 + j, d0, p.head_dim, v);
     }
     float s = 0.0f;
 #pragma unroll
