@@ -178,6 +178,8 @@ int nvfp4da_reserve_pages(const nvfp4da_page_table* table, const int64_t* past_l
   p.lengths = past_lengths;
   p.counts = counts;
   p.tokens = static_cast<int>(tokens);
+  p.by_tokens = page_divisor(static_cast<uint32_t>(tokens));
+  p.by_size = page_divisor(static_cast<uint32_t>(p.page_size));
   p.slots = slots;
   p.granted = granted;
   cudaError_t e = launch_cluster(reserve_pages_kernel, dim3(kPageCtas), dim3(kPageThreads), 0,

@@ -242,7 +242,7 @@ def cuda_paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, *, p
 
     Position j of sequence b is row ``j % S`` of page ``block_table[b, j // S]``;
     token t of q ``[B, T, Hq, D]`` sees positions below P_b (``past_lengths`` CUDA
-    int64 ``[B]``, ``max_past_length`` a host bound on them) and ``P_b + u`` where
+    int64 ``[B]``; ``max_past_length``, a host bound, plans the work) and ``P_b + u`` where
     ``tree_mask[b, t, u]`` (without one ``u <= t``).  Positions whose entry names no
     page are not seen.  Tokens ``t >= counts[b]`` (CUDA int64 ``[B]``) are padding
     and give zeros.  T = 1 is single-token decode.

@@ -405,7 +405,8 @@ int nvfp4da_paged_kv_read(const nvfp4da_kv_cache* pool, const int64_t* slots, in
 /* nvfp4da_tree_attention through a block table [B, M]: position j of sequence b is
  * row j % S of page block_table[b * M + j / S].  Positions whose entry names no page
  * are not seen.  counts (device int64 [B], optional): tokens t >= counts[b] are
- * padding; their context is zeros.  T = 1 is decode.  The flags of
+ * padding; their context is zeros.  T = 1 is decode.  max_past_length is what the
+ * work is planned for (lengths past it are right, but may be slow).  The flags of
  * nvfp4da_tree_attention_sync_status are these kernels' too. */
 size_t nvfp4da_paged_attention_workspace_size(const nvfp4da_kv_cache* pool, int64_t batch, int64_t max_pages,
                                               int64_t tokens, int64_t q_heads, int64_t max_past_length);

@@ -432,6 +432,17 @@ def test_paged_is_the_whole_cache_s_attention(cp, format, t):
     assert ((got.float() - want.float()).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("d", [96, 128])
+@pytest.mark.parametrize("bound", [0, 100])
+def test_lengths_past_the_bound_that_a_call_is_planned_for(cp, d, bound):
+    pasts = [1500, 90]
+    cache, table = sequences(cp, "fp8", pasts, 1, 2, 16, d, 71)
+    q = randn((2, 1, 4, d), 3)
+    got = cp.cuda_paged_attention(q.cuda(), cache, table.cuda(), past_lengths=torch.tensor(pasts).cuda(),
+                                  max_past_length=bound)
+    check_context(got, *ref.attention(q, cache, table, pasts))
+
+
 def test_attention_refusals(cp):
     cache, q = cp.PagedKVCache.allocate(3, 2, 16, 64, "fp8"), randn((2, 1, 4, 64), 1).cuda()
     table, past = torch.zeros((2, 2), dtype=torch.int32).cuda(), torch.zeros((2,), dtype=torch.int64).cuda()
