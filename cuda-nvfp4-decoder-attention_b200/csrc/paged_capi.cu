@@ -5,7 +5,6 @@
 #include <algorithm>
 #include <cmath>
 
-
 #include "host_util.cuh"
 #include "kv_host.cuh"
 #include "page_table.cuh"
