@@ -389,7 +389,7 @@ int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, c
   if (nodes > kVerifyMaxNodes)
     return fail(NVFP4DA_ERR_UNSUPPORTED, "verify_drafted: at most %d nodes a tree, got %lld", kVerifyMaxNodes,
                 static_cast<long long>(nodes));
-  if (vocab > kI32Max - 65536 || batch > kI32Max / kVerifyMaxCluster)
+  if (vocab > (1 << 30) || batch > kI32Max / kVerifyMaxCluster)
     return fail(NVFP4DA_ERR_UNSUPPORTED, "verify_drafted: vocabulary or batch too large");
   VerifyParams p{};
   p.target = target;
@@ -418,7 +418,8 @@ int nvfp4da_verify_drafted(const float* target, const int64_t* target_strides, c
   const int64_t most = std::min<int64_t>(4LL * sm_count() / batch, ceil_div(p.segments, kVerifyWarps));
   unsigned ctas = 1;
   while (ctas < kVerifyMaxCluster && 2 * ctas <= most) ctas *= 2;
-  const size_t smem = verify_smem(p.nodes, p.segments);
+  p.per_cta = static_cast<int>(ceil_div(p.segments, ctas));
+  const size_t smem = verify_smem(p.nodes, p.per_cta);
   cudaError_t e = ensure_smem(verify_drafted_kernel, static_cast<uint32_t>(smem));
   if (e == cudaSuccess && ctas > 8) e = ensure_big_clusters(verify_drafted_kernel);
   if (e == cudaSuccess)

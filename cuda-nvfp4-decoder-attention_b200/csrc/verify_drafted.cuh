@@ -24,15 +24,16 @@
 //
 // A cluster of CTAs takes a sequence.  Every CTA gathers the children's p(x) and
 // q(x) first, so that the walk reads shared memory, and walks by itself.  A row is
-// cut into segments, dealt to the cluster's warps in turn; a warp has all of a
-// segment (16 elements a lane) in flight at once.  All CTAs exchange the segments'
-// sums and add them in the same order (the same bits everywhere), and one warp
-// looks for the border of u_0 in the segment that holds it.
+// cut into segments, a run of them to each CTA; a warp has all of a segment (16
+// elements a lane) in flight at once.  The CTAs exchange the sums of their runs and
+// add them in the same order (the same bits everywhere), and one warp looks for the
+// border of u_0 in the segment that holds it.  (Every segment's sum to every CTA: 64
+// trees over 128,000 tokens 51 us for 48.)
 //
 // What bounds it: the sequence with the most rejections, one after another (a sum
-// needs the one before it).  64 trees of 8 over 128,000 tokens: 53 us, 1.5 sums a
+// needs the one before it).  64 trees of 8 over 128,000 tokens: 46 us, 1.5 sums a
 // sequence and five at most, the first of which read 64 MB from HBM; 48 trees of 13
-// given candidates over 49,999 tokens 19 us, one sum a node (one a rejection: 72
+// given candidates over 49,999 tokens 17 us, one sum a node (one a rejection: 72
 // us); one chain over 32,000 tokens 8.4 us.  Per element two conversions to FP64 and
 // three FP64 operations; elements are checked with an integer maximum a piece, and
 // cleaned one by one only where that finds one (all of them cleaned: 68 us for 57).
@@ -61,15 +62,16 @@ struct VerifyParams {
   int nodes, vocab;       // T, V
   int vec;                // rows are 16-byte aligned
   int pieces, segments;   // of kVerifyPiece elements a segment; segments of a row
+  int per_cta;            // segments of a CTA
   int64_t* path;          // [B, T]
   int64_t* accepted;      // [B]
   int64_t* next;          // [B]
 };
 
-// Shared memory: two sets of the segments' sums, then of the nodes p(x), q(x), u, token, parent, path, and the
-// tokens of a node's given children.
+// Shared memory: two sets of the CTAs' sums, those of the CTA's segments, then of the nodes the sum of p(x) of the
+// siblings behind them, p(x), q(x), u, token, parent, path, and the tokens of a node's given children.
 constexpr size_t verify_smem(int nodes, int segments) {
-  return static_cast<size_t>(segments) * 16 + static_cast<size_t>(nodes) * 28;
+  return 2 * kVerifyMaxCluster * 8 + static_cast<size_t>(segments) * 8 + static_cast<size_t>(nodes) * 36;
 }
 
 __device__ __forceinline__ double verify_clean(float x) {
@@ -83,8 +85,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
   pdl_wait();  // nothing of global memory before this: the launch may overlap the kernel ahead
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   extern __shared__ __align__(16) uint8_t verify_raw[];
-  double* s_part = reinterpret_cast<double*>(verify_raw);  // [2][segments]
-  float* s_p = reinterpret_cast<float*>(s_part + 2 * p.segments);
+  double* s_total = reinterpret_cast<double*>(verify_raw);  // [2][kVerifyMaxCluster]
+  double* s_part = s_total + 2 * kVerifyMaxCluster;         // [per_cta]
+  double* s_behind = s_part + p.per_cta;
+  float* s_p = reinterpret_cast<float*>(s_behind + p.nodes);
   float* s_q = s_p + p.nodes;
   float* s_u = s_q + p.nodes;
   int* s_token = reinterpret_cast<int*>(s_u + p.nodes);  // -1: no child
@@ -164,23 +168,32 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
       r[3] = e == 3 ? 0.0 : r[3];
     }
   };
-  int buf = 0;  // s_part's other half holds the last row's sums
+  const int seg0 = rank * p.per_cta, seg1 = min(seg0 + p.per_cta, p.segments);
+  int buf = 0;  // s_total's other half holds the last row's sums
   // Sum of what is left.  All threads of the cluster.
   auto sum_left = [&](const Left& l) -> double {
-    double* part = s_part + buf * p.segments;
 #pragma unroll 1
-    for (int seg = rank * kVerifyWarps + warp; seg < p.segments; seg += ctas * kVerifyWarps) {
+    for (int seg = seg0 + warp; seg < seg1; seg += kVerifyWarps) {
       double sum = 0.0;
 #pragma unroll 1
       for (int k = 0; k < p.pieces; ++k) {
         const int y = (seg * p.pieces + k) * kVerifyPiece;
         if (y >= p.vocab) break;
         float4 x[4], z[4] = {};
+        if (p.vec && y + kVerifyPiece <= p.vocab) {  // no branch between the loads: 53 us for 51
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = fetch4(l.p, y + 128 * i + 4 * lane);
-        if (l.q) {
+          for (int i = 0; i < 4; ++i) x[i] = __ldg(reinterpret_cast<const float4*>(l.p + y + 128 * i + 4 * lane));
+          if (l.q) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) z[i] = fetch4(l.q, y + 128 * i + 4 * lane);
+            for (int i = 0; i < 4; ++i) z[i] = __ldg(reinterpret_cast<const float4*>(l.q + y + 128 * i + 4 * lane));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = fetch4(l.p, y + 128 * i + 4 * lane);
+          if (l.q) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = fetch4(l.q, y + 128 * i + 4 * lane);
+          }
         }
         // Elements as they should be, no negative ones, infinities or NaN: below the bits of infinity.
         uint32_t top = 0u;
@@ -234,13 +247,19 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
         }
       }
       sum = warp_sum_f64(sum);
-      if (lane < ctas) cluster.map_shared_rank(part, lane)[seg] = sum;
+      if (lane == 0) s_part[seg - seg0] = sum;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      double own = 0.0;
+      for (int i = lane; i < seg1 - seg0; i += 32) own += s_part[i];
+      own = warp_sum_f64(own);
+      if (lane < ctas) cluster.map_shared_rank(s_total, lane)[buf * kVerifyMaxCluster + rank] = own;
     }
     sync();
+    const double all = warp_sum_f64(lane < ctas ? s_total[buf * kVerifyMaxCluster + lane] : 0.0);
     buf ^= 1;
-    double all = 0.0;
-    for (int i = lane; i < p.segments; i += 32) all += part[i];
-    return warp_sum_f64(all);
+    return all;
   };
 
   // ---- the walk: the same in every thread of the cluster
@@ -284,15 +303,27 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
           n += __popc(votes);
         }
         left.given = n;
+        if (warp == 0) {  // from the last node on; nothing is subtracted, so that the smallest p(x) stay
+          double carry = 0.0;
+          for (int base = nodes - 1; base >= t; base -= 32) {
+            const int i = base - lane;
+            double behind = i >= t && i + 1 < nodes && s_parent[i + 1] == node ? verify_clean(s_p[i + 1]) : 0.0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double x = __shfl_up_sync(kFull, behind, o);
+              if (lane >= o) behind += x;
+            }
+            behind += carry;
+            if (i >= t) s_behind[i] = behind;
+            carry = __shfl_sync(kFull, behind, 31);
+          }
+        }
         __syncthreads();
         total = sum_left(left);
         summed = true;
       }
       // s: what is left without the children so far, those to come still in it
-      double more = 0.0;
-      for (int i = t + 1 + lane; i < nodes; i += 32)
-        if (s_parent[i] == node) more += verify_clean(s_p[i]);
-      scale = total + warp_sum_f64(more);
+      scale = total + s_behind[t];
     }
     if (scale == 0.0) {
       open = false;
@@ -301,7 +332,6 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
     }
   }
   if (!summed) total = sum_left(left);
-  const double* part = s_part + (buf ^ 1) * p.segments;
   __syncthreads();
   if (rank == 0) {
     for (int t = threadIdx.x; t < p.nodes; t += kVerifyThreads)
@@ -315,32 +345,47 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
 
   // ---- the next token: the first segment whose end passes u_0 sum r, else the last with anything in it
   const double border = static_cast<double>(s_u[0]) * total;
-  const int per_lane = (p.segments + 31) / 32, i0 = lane * per_lane, i1 = min(i0 + per_lane, p.segments);
-  double own = 0.0;
-  for (int i = i0; i < i1; ++i) own += part[i];
-  double upto = own;
+  // The sums before `own` of the lanes, to which the first one belongs whose end passes the border.
+  auto before_of = [&](double own) {
+    double upto = __shfl_up_sync(kFull, own, 1);
+    if (lane == 0) upto = 0.0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double u = __shfl_up_sync(kFull, upto, o);
-    if (lane >= o) upto += u;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const double u = __shfl_up_sync(kFull, upto, o);
+      if (lane >= o) upto += u;
+    }
+    return upto;
+  };
+  const double cta = lane < ctas ? s_total[(buf ^ 1) * kVerifyMaxCluster + lane] : 0.0;
+  double before = before_of(cta);
+  unsigned holders = __ballot_sync(kFull, before + cta > border && cta > 0.0);
+  const unsigned filled = __ballot_sync(kFull, cta > 0.0);
+  bool found = holders != 0;
+  const int of = found ? __ffs(holders) - 1 : 31 - __clz(filled);
+  if (of != rank) return;
+  before = __shfl_sync(kFull, before, of);
+  const int per_lane = (seg1 - seg0 + 31) / 32, i0 = min(lane * per_lane, seg1 - seg0);
+  const int i1 = min(i0 + per_lane, seg1 - seg0);
+  double own = 0.0;
+  for (int i = i0; i < i1; ++i) own += s_part[i];
   int holder = -1, last = -1;
-  double before = 0.0, run_up = upto - own;
+  double run_up = before + before_of(own);
   for (int i = i0; i < i1; ++i) {
-    if (part[i] > 0.0) last = i;
-    if (holder < 0 && run_up + part[i] > border) {
+    if (s_part[i] > 0.0) last = i;
+    if (found && holder < 0 && s_part[i] > 0.0 && run_up + s_part[i] > border) {
       holder = i;
       before = run_up;
     }
-    run_up += part[i];
+    run_up += s_part[i];
   }
-  const unsigned holders = __ballot_sync(kFull, holder >= 0), lasts = __ballot_sync(kFull, last >= 0);
-  holder = __shfl_sync(kFull, holder, holders ? __ffs(holders) - 1 : 0);
-  before = __shfl_sync(kFull, before, holders ? __ffs(holders) - 1 : 0);
+  holders = __ballot_sync(kFull, holder >= 0);
+  const unsigned lasts = __ballot_sync(kFull, last >= 0);
+  found = holders != 0;
+  holder = __shfl_sync(kFull, holder, found ? __ffs(holders) - 1 : 0);
+  before = __shfl_sync(kFull, before, found ? __ffs(holders) - 1 : 0);
   last = __shfl_sync(kFull, last, lasts ? 31 - __clz(lasts) : 0);
-  const bool found = holder >= 0;
-  const int seg = found ? holder : last;
-  if (seg % (ctas * kVerifyWarps) != rank * kVerifyWarps + warp) return;
+  const int local = found ? holder : last, seg = seg0 + local;
+  if (local % kVerifyWarps != warp) return;
   int best = -1;  // the last element so far that is left
 #pragma unroll 1
   for (int y = seg * p.pieces * kVerifyPiece; y < min((seg + 1) * p.pieces * kVerifyPiece, p.vocab); y += 128) {

@@ -132,6 +132,26 @@ def test_candidates_that_repeat_or_are_none(cp, sampled):
     check(cp, target, tokens, u, draft if sampled else None, parents)
 
 
+def test_siblings_that_hold_all_of_a_row(cp):
+    """Given siblings of probabilities 2^-1, 2^-2, ...: what the last ones hold decides, however little it is.  In exact
+    arithmetic s is below twice a sibling's own p, which the one half of a row does not round away."""
+    for n in (2, 31, 33, 64, 65, 120):
+        v = 700
+        target = torch.zeros((3, n + 1, v))
+        target[:, 0, :n] = 2.0 ** -torch.arange(1.0, n + 1)
+        target[:, 1:, 9] = 1.0
+        tokens = torch.arange(-1, n).repeat(3, 1)
+        tokens[:, 0] = 0
+        parents = torch.zeros(n + 1, dtype=torch.int64)
+        u = torch.full((3, n + 1), 0.75)
+        u[:, 0] = 0.7
+        u[1, n] = 2.0  # none is left: the row stands again
+        u[2, 1:] = 0.75 * (torch.arange(n) < n // 2)
+        path, counts, nexts = check(cp, target, tokens, u, None, parents)
+        assert counts.tolist() == [2, 1, 2] and path[:, 1].tolist() == [n, -1, n // 2 + 1]
+        assert nexts.tolist() == [9, 1, 9]
+
+
 @pytest.mark.parametrize("sampled", [True, False])
 def test_tokens_follow_the_target(cp, sampled):
     """The first new token of 40,000 trees: within 5 standard deviations of the target's row everywhere."""
