@@ -184,7 +184,9 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PageT
   __shared__ int s_keep[kPageThreads], s_held[kPageThreads], s_back[kPageThreads], s_upto[kPageThreads];
   const int free_count = pages_clamp(*p.free_count, p.pages);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int pushed = 0;
+  // Places on the stack are unsigned: a table may name a page in all of its 2^31 entries, and the free ones come on top.
+  const unsigned room_on_stack = p.pages;
+  unsigned pushed = 0;
   for (int base = (p.batch - 1) / kPageThreads * kPageThreads; base >= 0; base -= kPageThreads) {
     const int chunk = min(kPageThreads, p.batch - base);
     if (static_cast<int>(threadIdx.x) < chunk) {
@@ -225,25 +227,25 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PageT
     if (static_cast<int>(threadIdx.x) < chunk) s_upto[chunk - 1 - threadIdx.x] = upto;
     __syncthreads();
     if (few > 0) {
-      int to = free_count + pushed + s_upto[i_own] - 1;  // of the first page that goes back
+      unsigned to = free_count + pushed + s_upto[i_own] - 1;  // of the first page that goes back
 #pragma unroll
       for (int k = 0; k < kPageFew; ++k) {
         if (k < few) *entry(i_own, s_keep[i_own] + k) = -1;
         if (named(own[k])) {
-          if (to < p.pages) p.free_pages[to] = own[k];
+          if (to < room_on_stack) p.free_pages[to] = own[k];
           --to;
         }
       }
     }
     for (int i = warp; i < chunk; i += kPageThreads / 32) {
       if (s_held[i] - s_keep[i] <= kPageFew) continue;
-      int to = free_count + pushed + s_upto[i] - 1;
+      unsigned to = free_count + pushed + s_upto[i] - 1;
       for (int k = s_keep[i] + lane; k - lane < s_held[i]; k += 32) {
         const int page = k < s_held[i] ? *entry(i, k) : -1;
         const bool back = named(page);
         const unsigned votes = __ballot_sync(kFull, back);
-        const int at = to - __popc(votes & ((1u << lane) - 1u));
-        if (back && at < p.pages) p.free_pages[at] = page;
+        const unsigned at = to - __popc(votes & ((1u << lane) - 1u));
+        if (back && at < room_on_stack) p.free_pages[at] = page;
         if (k < s_held[i]) *entry(i, k) = -1;
         to -= __popc(votes);
       }
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PageT
     pushed += total;
     __syncthreads();
   }
-  if (threadIdx.x == 0) *p.free_count = min(free_count + pushed, p.pages);
+  if (threadIdx.x == 0) *p.free_count = min(free_count + pushed, room_on_stack);
 }
 
 }  // namespace nvfp4da
