@@ -24,11 +24,13 @@
 //
 // A cluster of CTAs takes a sequence.  Every CTA gathers the children's p(x) and
 // q(x) first, so that the walk reads shared memory, and walks by itself.  A row is
-// cut into segments, a run of them to each CTA; a warp has all of a segment (16
-// elements a lane) in flight at once.  The CTAs exchange the sums of their runs and
-// add them in the same order (the same bits everywhere), and one warp looks for the
-// border of u_0 in the segment that holds it.  (Every segment's sum to every CTA: 64
-// trees over 128,000 tokens 51 us for 48.)
+// cut into segments and these into sixteen runs, each CTA having as many runs as
+// another; a warp has all of a segment (16 elements a lane) in flight at once.  The
+// CTAs exchange the sums of their runs, and one warp looks for the border of u_0 in
+// the segment that holds it.  (Every segment's sum to every CTA: 64 trees over
+// 128,000 tokens 51 us for 48.)  Which elements make a sum, and in which order,
+// follows from the vocabulary alone: the same bits whatever the number of CTAs,
+// which follows from the batch and the GPU.
 //
 // What bounds it: the sequence with the most rejections, one after another (a sum
 // needs the one before it).  64 trees of 8 over 128,000 tokens: 46 us, 1.5 sums a
@@ -47,6 +49,7 @@ namespace nvfp4da {
 
 constexpr int kVerifyThreads = 256, kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyMaxNodes = 1024, kVerifyMaxCluster = 16;
+constexpr int kVerifyRuns = kVerifyMaxCluster;  // of a row's segments
 constexpr int kVerifyPiece = 512;  // elements a warp has in flight
 constexpr int kVerifyMaxSegments = 1024;
 
@@ -62,16 +65,16 @@ struct VerifyParams {
   int nodes, vocab;       // T, V
   int vec;                // rows are 16-byte aligned
   int pieces, segments;   // of kVerifyPiece elements a segment; segments of a row
-  int per_cta;            // segments of a CTA
+  int per_cta;            // segments of a CTA at most
   int64_t* path;          // [B, T]
   int64_t* accepted;      // [B]
   int64_t* next;          // [B]
 };
 
-// Shared memory: two sets of the CTAs' sums, those of the CTA's segments, then of the nodes the sum of p(x) of the
+// Shared memory: two sets of the runs' sums, those of the CTA's segments, then of the nodes the sum of p(x) of the
 // siblings behind them, p(x), q(x), u, token, parent, path, and the tokens of a node's given children.
 constexpr size_t verify_smem(int nodes, int segments) {
-  return 2 * kVerifyMaxCluster * 8 + static_cast<size_t>(segments) * 8 + static_cast<size_t>(nodes) * 36;
+  return 2 * kVerifyRuns * 8 + static_cast<size_t>(segments) * 8 + static_cast<size_t>(nodes) * 36;
 }
 
 __device__ __forceinline__ double verify_clean(float x) {
@@ -85,8 +88,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
   pdl_wait();  // nothing of global memory before this: the launch may overlap the kernel ahead
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   extern __shared__ __align__(16) uint8_t verify_raw[];
-  double* s_total = reinterpret_cast<double*>(verify_raw);  // [2][kVerifyMaxCluster]
-  double* s_part = s_total + 2 * kVerifyMaxCluster;         // [per_cta]
+  double* s_total = reinterpret_cast<double*>(verify_raw);  // [2][kVerifyRuns]
+  double* s_part = s_total + 2 * kVerifyRuns;               // [per_cta]
   double* s_behind = s_part + p.per_cta;
   float* s_p = reinterpret_cast<float*>(s_behind + p.nodes);
   float* s_q = s_p + p.nodes;
@@ -168,7 +171,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
       r[3] = e == 3 ? 0.0 : r[3];
     }
   };
-  const int seg0 = rank * p.per_cta, seg1 = min(seg0 + p.per_cta, p.segments);
+  const int runs = kVerifyRuns / ctas, run0 = rank * runs;  // this CTA's
+  auto first_of = [&](int run) { return run * p.segments / kVerifyRuns; };
+  const int seg0 = first_of(run0), seg1 = first_of(run0 + runs);
   int buf = 0;  // s_total's other half holds the last row's sums
   // Sum of what is left.  All threads of the cluster.
   auto sum_left = [&](const Left& l) -> double {
@@ -250,14 +255,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
       if (lane == 0) s_part[seg - seg0] = sum;
     }
     __syncthreads();
-    if (warp == 0) {
+    for (int run = run0 + warp; run < run0 + runs; run += kVerifyWarps) {
       double own = 0.0;
-      for (int i = lane; i < seg1 - seg0; i += 32) own += s_part[i];
+      for (int i = first_of(run) + lane; i < first_of(run + 1); i += 32) own += s_part[i - seg0];
       own = warp_sum_f64(own);
-      if (lane < ctas) cluster.map_shared_rank(s_total, lane)[buf * kVerifyMaxCluster + rank] = own;
+      if (lane < ctas) cluster.map_shared_rank(s_total, lane)[buf * kVerifyRuns + run] = own;
     }
     sync();
-    const double all = warp_sum_f64(lane < ctas ? s_total[buf * kVerifyMaxCluster + lane] : 0.0);
+    const double all = warp_sum_f64(lane < kVerifyRuns ? s_total[buf * kVerifyRuns + lane] : 0.0);
     buf ^= 1;
     return all;
   };
@@ -356,16 +361,16 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafted_kernel(const Ve
     }
     return upto;
   };
-  const double cta = lane < ctas ? s_total[(buf ^ 1) * kVerifyMaxCluster + lane] : 0.0;
-  double before = before_of(cta);
-  unsigned holders = __ballot_sync(kFull, before + cta > border && cta > 0.0);
-  const unsigned filled = __ballot_sync(kFull, cta > 0.0);
+  const double run_sum = lane < kVerifyRuns ? s_total[(buf ^ 1) * kVerifyRuns + lane] : 0.0;
+  double before = before_of(run_sum);
+  unsigned holders = __ballot_sync(kFull, before + run_sum > border && run_sum > 0.0);
+  const unsigned filled = __ballot_sync(kFull, run_sum > 0.0);
   bool found = holders != 0;
   const int of = found ? __ffs(holders) - 1 : 31 - __clz(filled);
-  if (of != rank) return;
+  if (of < run0 || of >= run0 + runs) return;
   before = __shfl_sync(kFull, before, of);
-  const int per_lane = (seg1 - seg0 + 31) / 32, i0 = min(lane * per_lane, seg1 - seg0);
-  const int i1 = min(i0 + per_lane, seg1 - seg0);
+  const int end = first_of(of + 1) - seg0, per_lane = (first_of(of + 1) - first_of(of) + 31) / 32;
+  const int i0 = min(first_of(of) - seg0 + lane * per_lane, end), i1 = min(i0 + per_lane, end);
   double own = 0.0;
   for (int i = i0; i < i1; ++i) own += s_part[i];
   int holder = -1, last = -1;
