@@ -13,7 +13,8 @@
 // position j = P_b + t, -1 for t >= n_b, in a page that is not there, and for
 // sequences that are not served (granted[b] = 0, their table as it was).
 // Release: sequence b keeps ceil(L_b / S) pages; the others go back, the last
-// sequence's last page first: a release undoes the reserve before it.
+// sequence's last page first: a release undoes the reserve before it.  A page stands
+// once in the table: references are not counted, and what a row names goes back.
 //
 // Reserving is one scan over the batch, which every CTA of a cluster of eight does
 // for itself, 1,024 sequences at a time; the CTAs share the writing of the table

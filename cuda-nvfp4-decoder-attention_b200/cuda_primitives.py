@@ -209,7 +209,9 @@ def cuda_release_pages_(table, lengths: torch.Tensor) -> None:
     """Let sequence b of a ``PageTable`` keep the pages of its first ``lengths[b]`` positions (CUDA int64 ``[B]``).
 
     The others go back on the free stack, the last sequence's last page first, so
-    that a release undoes the reserve before it; length 0 ends a sequence.
+    that a release undoes the reserve before it; length 0 ends a sequence.  Pages are
+    not counted: one that two rows name (or one row twice) would go back though it is
+    still in use, and come back twice, so a page may stand in a ``PageTable`` once.
     """
     _ops.cuda_release_pages_(table.pages, table.held, table.free_pages, table.free_count, table.page_size, lengths)
 

@@ -16,7 +16,9 @@ device: ``pages`` int32 ``[B, M]`` names the pages of each sequence in order, -1
 behind the ``held`` (int64 ``[B]``) that it has; ``free_pages`` int32 ``[N]`` is
 a stack of ``free_count`` (int64 ``[1]``) pages that nobody holds.
 ``cuda_reserve_pages_`` and ``cuda_release_pages_`` change it.  The pools of all
-layers can share one table.
+layers can share one table.  A page stands once in it, in one row or on the stack:
+nothing counts references, so sequences that share pages name them in a block table
+of their own for the attention, and one row of the ``PageTable`` holds them.
 """
 
 from __future__ import annotations

@@ -385,7 +385,9 @@ int nvfp4da_reserve_pages(const nvfp4da_page_table* table, const int64_t* past_l
                           int64_t tokens, int64_t* slots, int64_t* granted, void* stream);
 /* Sequence b keeps ceil(lengths[b] / S) of its pages (none for a length below 1);
  * the others go back on the stack, the last sequence's last page first, and their
- * entries become -1: a release undoes the reserve before it. */
+ * entries become -1: a release undoes the reserve before it.  References are not
+ * counted: a page may stand once in the table, else it goes back while another row
+ * names it, and comes back twice. */
 int nvfp4da_release_pages(const nvfp4da_page_table* table, const int64_t* lengths, void* stream);
 
 /* Rows of new_k, new_v [B, T, Hkv, D] (BF16, by element strides of batch, token
