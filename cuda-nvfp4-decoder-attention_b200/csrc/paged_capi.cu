@@ -273,7 +273,7 @@ int nvfp4da_paged_kv_read(const nvfp4da_kv_cache* c, const int64_t* slots, int64
 
 size_t nvfp4da_paged_attention_workspace_size(const nvfp4da_kv_cache* c, int64_t batch, int64_t max_pages,
                                               int64_t tokens, int64_t q_heads, int64_t max_past_length) {
-  PagedPlan pl;
+  PagedPlan pl{};
   return plan_paged(c, batch, max_pages, tokens, q_heads, max_past_length, pl) ? 0 : pl.bytes;
 }
 
@@ -281,7 +281,7 @@ int nvfp4da_paged_attention(const uint16_t* q, const nvfp4da_kv_cache* c, const 
                             int64_t max_pages, const uint8_t* tree_mask, int64_t mask_batch_stride, uint16_t* context,
                             int64_t tokens, int64_t q_heads, const int64_t* past_lengths, int64_t max_past_length,
                             const int64_t* counts, void* ws, size_t ws_bytes, void* stream) {
-  PagedPlan pl;
+  PagedPlan pl{};
   int r = plan_paged(c, batch, max_pages, tokens, q_heads, max_past_length, pl);
   if (r) return r;
   if (!q || !context || !block_table || !past_lengths)

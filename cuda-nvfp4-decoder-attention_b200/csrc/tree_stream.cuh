@@ -573,11 +573,11 @@ __device__ __forceinline__ void ts_load_scales_paged(uint8_t* blocks, uint8_t* r
 // PAGED: a tile comes in boxes, each from its own page, to the places that a whole
 // tile's copy would bring it; 16-position slices of pages that are not there (their
 // boxes come in as zeros) are left out.
-template <int D, int FMT, int NG, int NW, int SL, bool PAGED = false>
+template <int D, int FMT, int NG, int NW, int SLICES, bool PAGED = false>
 __global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
     tree_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const TreeStreamParams p) {
-  using Cfg = TsCfg<D, FMT, NG, NW, SL, kTsTile<FMT>, PAGED>;
+  using Cfg = TsCfg<D, FMT, NG, NW, SLICES, kTsTile<FMT>, PAGED>;
   constexpr int KS = D / 16;  // MMA steps of K Q^T, 16-element row blocks of O^T
   constexpr bool kQuant = FMT != kKvFmtBf16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -1276,16 +1276,16 @@ __global__ void __launch_bounds__((NW + (PAGED ? 8 : 4)) * 32, 1)
         unsigned absent = 0u;
         if constexpr (PAGED) absent = s_absent[stage];
         for (int i = 0; i < turns; ++i) {
-          const int r0 = (turn0 + i) * 16 * SL;
+          const int r0 = (turn0 + i) * 16 * SLICES;
           const int pos0 = t * kTsTile<FMT> + r0;
           if (pos0 >= vis || (PAGED && n0 >= nq)) break;
-          const unsigned gone = absent >> (r0 / 16) & ((1u << SL) - 1u);  // slices whose page is not there
-          using Slices = std::integral_constant<int, SL>;
-          if (pos0 + 16 * SL <= past && !gone) {
+          const unsigned gone = absent >> (r0 / 16) & ((1u << SLICES) - 1u);  // slices whose page is not there
+          using Slices = std::integral_constant<int, SLICES>;
+          if (pos0 + 16 * SLICES <= past && !gone) {
             slice(std::false_type{}, Slices{}, st, r0, pos0);
           } else if constexpr (PAGED) {  // one at a time: half of the code that a segment's end has to fetch
 #pragma unroll 1
-            for (int z = 0; z < SL; ++z)
+            for (int z = 0; z < SLICES; ++z)
               if (pos0 + 16 * z < vis && !(gone >> z & 1u))
                 slice(std::true_type{}, std::integral_constant<int, 1>{}, st, r0 + 16 * z, pos0 + 16 * z);
           } else {
