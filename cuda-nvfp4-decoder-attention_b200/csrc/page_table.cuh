@@ -22,7 +22,7 @@
 // them.  Releasing is one CTA's: most steps give back a page or none a sequence.
 //
 // Latency bounds both: reserving for eight sequences of one token and releasing
-// take 11.7 us, two launches; 64 prompts of 2,048 tokens (1 MB of slots, 8,000
+// take 12 to 13 us, two launches; 64 prompts of 2,048 tokens (1 MB of slots, 8,000
 // pages) 18 us, where one CTA for the slots took 71 and divisions by the compiler 20.
 // Four slots in a row a thread, with one division for them, were no faster.
 #pragma once

@@ -56,13 +56,22 @@ constexpr int64_t paged_tc_min_rows(int64_t head_dim, int format) {
 }
 
 // Groups of 8 query rows that a warp of the streaming kernel holds.  Wider warps decode codes fewer times, but have less
-// of a tile each: us for 1, 2, 3 groups, E4M3, head_dim 64, 8 KV heads, 37 sequences of 90 to 6,003 positions: 12 rows 61,
-// 62, 75; 20 rows 90, 84, 78; 32 rows 94, 88, 113.  20 rows of 8 sequences of 8,000 to 12,000 at head_dim 128: 106, 113.
+// of a tile each: us for 1, 2, 3 groups, E4M3, head_dim 64, 8 KV heads, the best of 17 to 24 rows and of 25 to 32 where
+// decoding counts, some 2 to 6 us slower where a segment is a few tiles:
+//                                       12 rows          20 rows          24 rows          32 rows
+//   37 sequences of 90 to 6,003         64, 64, 76       94, 90, 80       96, 92, 82       98, 94, 119
+//   64 of 2,000 to 3,000                88, 88, 107      133, 125, 111    133, 125, 115    137, 129, 168
+//   4 of 30,000 to 32,000               66, 64, 74       98, 92, 78       100, 92, 80      102, 94, 119
+//   32 of 10 to 300                     25, 27, 33       31, 29, 35       31, 31, 35       33, 31, 41
+//   8 of 50 to 600                      21, 21, 24       23, 23, 25       23, 25, 27       25, 25, 29
+// 20 rows of 8 sequences of 8,000 to 12,000 at head_dim 128: 106, 113.
 int paged_width(int64_t head_dim, int format, int64_t rows) {
   return head_dim != 64 || format != NVFP4DA_KV_E4M3 || rows <= 16 ? 1 : rows <= 24 ? 3 : 2;
 }
 
-// CTAs an SM of paged_attn_general_kernel that the splits of the cache's length are to give.
+// CTAs an SM of paged_attn_general_kernel that the splits of the cache's length are to give.  us for 4, 8, 16: 64
+// sequences of 1,024 to 8,191 positions, head_dim 96, BF16 249, 260, 240, E4M3 228, 237, 223; 8 x 26,000 E4M3 180, 162, 197; 16 of
+// 3,000 to 5,000, head_dim 192, BF16 135, 119, 148; 16 of 100 to 4,000, head_dim 80, 32 rows of NVFP4 49, 57, 80.
 constexpr int64_t kPgenPerSm = 8;
 
 template <int FMT, int KS>

@@ -18,7 +18,7 @@
 // at the end for the queries that do.
 //
 // 64 sequences x 6 heads, 1,024 to 8,191 positions, head_dim 96, one token x 4 heads:
-// BF16 254 us, E4M3 227, NVFP4 207 (floors 102, 53, 31; a warp per query row with
+// BF16 247 us, E4M3 225, NVFP4 212 (floors 106, 55, 32; a warp per query row with
 // scalar products, as over whole caches, took 1.2 ms for a smaller call).  Bound by
 // instructions and the latency between them: a quarter of a tile's 16 query rows is
 // in use, issue slots 42 %.
@@ -124,7 +124,10 @@ __device__ __forceinline__ bool pgen_finite(uint32_t& w) {
 }
 
 // Four CTAs an SM up to head_dim 128 (8 x 26,000 positions, head_dim 96: E4M3 206 -> 185 us, NVFP4 192 -> 165); with
-// five, or three of larger heads of codes, registers spill.  BF16 at head_dim 192: three 529 us, two 689.
+// five, or three of larger heads of codes, registers spill.  At 112 and 128 four spill too (bytes stored a thread: BF16
+// 360 and 436, E4M3 76 and 72, NVFP4 0 and 28), which costs BF16 and E4M3 at 112 dearly: 64 sequences of 1,024 to 8,191
+// positions, head_dim 96 / 112, BF16 247 / 611 us, E4M3 225 / 452, NVFP4 212 / 251.  Three there were not tried.  BF16
+// at head_dim 192: three 529 us, two 689.
 template <int FMT, int KS>
 __global__ void __launch_bounds__(kPgenThreads, KS <= 8 ? 4 : FMT == kKvFmtBf16 ? 3 : 1) paged_attn_general_kernel(const TreeAttnParams p, const PagedView pg) {
   constexpr int D = 16 * KS, kStride = D + 8;  // elements: rows 4 banks apart, modulo 8
@@ -150,8 +153,9 @@ __global__ void __launch_bounds__(kPgenThreads, KS <= 8 ? 4 : FMT == kKvFmtBf16 
   // The last split takes what is left, also past the host's bound.
   const int j1 = static_cast<int>(blockIdx.x + 1 == gridDim.x ? end : min(j0 + p.split_len, static_cast<int64_t>(end)));
 
-  // ---- Q, and where this thread's two rows of scores (g and g + 8) stand.  Over codes Q goes to FP16 by a power of
-  // two that brings the row's largest element to [2^14, 2^15): exact down to 2^-39 of it.
+  // ---- Q, and where this thread's two rows of scores (g and g + 8) stand.  Over codes Q goes to FP16 by the power of
+  // two (2^100 at most) that brings the row's largest element to [2^14, 2^15): 8 bits are exact from 2^-31 of that
+  // element on, smaller elements are off by 2^-25 of the scaled row at most (FP16's steps end at 2^-24).
   for (int r = warp; r < kPgenRows; r += kPgenWarps) {
     const int n = n0 + r;
     const uint16_t* src = p.q + ((static_cast<int64_t>(b) * p.tokens + n / group) * p.q_heads + kvh * group + n % group) * D;

@@ -28,8 +28,10 @@
 // registers; nothing is written back to shared memory.
 //
 // Numerics.  Codes (times the NVFP4 block scale) are exact in FP16; the query
-// row is scaled by a power of two to FP16 (exact down to 2^-39 of its largest
-// element); the row scale of K multiplies the FP32 score.  P goes to FP16 as
+// row is scaled to FP16 by the power of two that brings its largest element to
+// [2^14, 2^15), 2^100 at most: its 8 bits are exact from 2^-31 of that element on,
+// smaller ones are off by 2^-25 of the scaled row (2^-39 of it) at most; the row
+// scale of K multiplies the FP32 score.  P goes to FP16 as
 // p_j gamma_j / G 2^5, where G follows the largest contribution p_j gamma_j that
 // the query has met (>= 2^-100): 11 significant bits down to 2^-19 of that
 // contribution, absolute steps of 2^-29 of it below.  (With the largest gamma_j
@@ -68,7 +70,8 @@
 //             marks a tile's 16-position slices that are not there, consumers leave
 //             them out; a padding row's context is zeros.
 //   the line  is cut by weight, a segment counting kTsSegment tiles beside its own:
-//             64 E4M3 sequences of 10 to 2,000 positions 99 us unweighted, 61 so.
+//             64 E4M3 sequences of 10 to 2,000 positions, pages of 16, 59 us unweighted,
+//             47 so.
 //   a segment's start and end: lengths stand in shared memory, four warps join its
 //             rows, and its last slices are taken one at a time, half of the code to
 //             fetch (a segment had missed the instruction cache at every third
@@ -76,7 +79,9 @@
 // 64 sequences x 6 heads, 1,024 to 8,191 positions, one token: BF16 142 us, 6.3
 // TB/s, 0.96 of a copy; E4M3 in pages of 16 94 us, 4.9 TB/s (no arithmetic at all:
 // 10 us less); 8 x 32,768 of NVFP4 78 us: the ALU pipe's decoding (64 conversions
-// and 36 unpackings a slice), 45 % of the issue slots.
+// and 36 unpackings a slice), 45 % of the issue slots.  Head dimension 256 (1,024 to
+// 8,191 positions): BF16 290 us, 0.98 of a copy, E4M3 171, NVFP4 166; its instances
+// spill 80 to 132 bytes a thread, that of three groups of E4M3 at 64 44 bytes.
 //
 // Waits are bounded: one that lasts a second records kErrBarrierTimeout in
 // g_tree_errors, and every role of the CTA leaves (its results are then garbage;
@@ -103,7 +108,8 @@ static __device__ unsigned g_tree_errors;  // of the translation unit's kernels
 template <int FMT>
 constexpr int kTsTile = FMT == kKvFmtBf16 ? 64 : 128;
 // PAGED: what a segment costs beside its tiles, in tiles.  us for 0, 2, 4, 6 of them, 24 query heads over 6 KV heads:
-// 64 sequences of 10 to 2,000 positions BF16 76, 63, 63, 64, E4M3 86, 55, 49, 49, NVFP4 89, 61, 57, 54; of 1,024 to
+// 64 sequences of 10 to 2,000 positions, pages of 32, BF16 76, 63, 63, 64, E4M3 86, 55, 49, 49, NVFP4 89, 61, 57, 54 (as
+// the kernel was when this was chosen; with the last slices taken one at a time 0 costs less, see above); of 1,024 to
 // 8,191 E4M3 113, 109, 111, 114; 16 of 100 to 30,000 NVFP4 90, 80, 78, 78.
 template <int FMT>
 constexpr int kTsSegment = FMT == kKvFmtBf16 ? 3 : 4;
