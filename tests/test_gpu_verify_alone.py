@@ -9,6 +9,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_verify import check, problem
+
 pytestmark = pytest.mark.gpu
 
 
@@ -68,3 +70,16 @@ def test_a_sequence_alone_and_in_a_batch(cp, sampled):
     for n in (kinds, 3 * kinds, batch):
         rows = torch.arange(n) % kinds
         assert all(torch.equal(x, y[rows]) for x, y in zip(call(rows), alone))
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("v", [4097, 5000, 7680, 8191, 8193, 9000, 16385, 70001])
+def test_rows_of_fewer_segments_than_runs_and_a_few_more(cp, sampled, v):
+    """Runs that hold no segment, one, or one more than others: the definition's paths and tokens."""
+    target, draft, tokens, parents, u = problem(6, 7, v, True, v, near=1.5)
+    check(cp, target, tokens, u, draft if sampled else None, parents)
+    one = torch.zeros((6, 7, v))  # all of a row in one element: of the first, a middle or the last segment
+    for i, y in enumerate((0, 511, 512, v // 2, v - 512, v - 1)):
+        one[i, :, y] = 0.75
+    path, counts, nexts = check(cp, one, tokens, u, draft if sampled else None, parents)
+    assert sorted(set(nexts.tolist())) == sorted({0, 511, 512, v // 2, v - 512, v - 1})
