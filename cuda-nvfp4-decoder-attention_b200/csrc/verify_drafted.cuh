@@ -33,10 +33,10 @@
 // which follows from the batch and the GPU.
 //
 // What bounds it: the sequence with the most rejections, one after another (a sum
-// needs the one before it).  64 trees of 8 over 128,000 tokens: 46 us, 1.5 sums a
-// sequence and five at most, the first of which read 64 MB from HBM; 48 trees of 13
-// given candidates over 49,999 tokens 18 to 19 us, one sum a node (one a rejection: 72
-// us); one chain over 32,000 tokens 8.4 us.  Per element two conversions to FP64 and
+// needs the one before it).  64 trees of 8 over 128,000 tokens: 42 to 49 us by the
+// numbers drawn, 1.5 sums a sequence and five at most, the first of which read 64 MB
+// from HBM; 48 trees of 13 given candidates over 49,999 tokens 17 to 19.5 us, one sum a
+// node (one a rejection: 72 us); one chain over 32,000 tokens 8.2 us.  Per element two conversions to FP64 and
 // three FP64 operations; elements are checked with an integer maximum a piece, and
 // cleaned one by one only where that finds one (all of them cleaned: 68 us for 57).
 #pragma once
