@@ -56,8 +56,8 @@ constexpr int64_t paged_tc_min_rows(int64_t head_dim, int format) {
 }
 
 // Groups of 8 query rows that a warp of the streaming kernel holds.  Wider warps decode codes fewer times, but have less
-// of a tile each: us for 1, 2, 3 groups, E4M3, head_dim 64, 8 KV heads, the best of 17 to 24 rows and of 25 to 32 where
-// decoding counts, some 2 to 6 us slower where a segment is a few tiles:
+// of a tile each.  Three groups for 17 to 24 rows and two for 25 to 32 are the fastest where decoding counts; where a
+// segment is a few tiles, three cost 2 to 4 us more than one.  us for 1, 2, 3 groups, E4M3, head_dim 64, 8 KV heads:
 //                                       12 rows          20 rows          24 rows          32 rows
 //   37 sequences of 90 to 6,003         64, 64, 76       94, 90, 80       96, 92, 82       98, 94, 119
 //   64 of 2,000 to 3,000                88, 88, 107      133, 125, 111    133, 125, 115    137, 129, 168
@@ -70,8 +70,8 @@ int paged_width(int64_t head_dim, int format, int64_t rows) {
 }
 
 // CTAs an SM of paged_attn_general_kernel that the splits of the cache's length are to give.  us for 4, 8, 16: 64
-// sequences of 1,024 to 8,191 positions, head_dim 96, BF16 249, 260, 240, E4M3 228, 237, 223; 8 x 26,000 E4M3 180, 162, 197; 16 of
-// 3,000 to 5,000, head_dim 192, BF16 135, 119, 148; 16 of 100 to 4,000, head_dim 80, 32 rows of NVFP4 49, 57, 80.
+// sequences of 1,024 to 8,191 positions, head_dim 96, BF16 249, 260, 240, E4M3 228, 237, 223; 8 x 26,000 E4M3 180, 162,
+// 197; 16 of 3,000 to 5,000, head_dim 192, BF16 135, 119, 148; 16 of 100 to 4,000, head_dim 80, 32 rows of NVFP4 49, 57, 80.
 constexpr int64_t kPgenPerSm = 8;
 
 template <int FMT, int KS>
